@@ -567,6 +567,84 @@ int dl_rkl_marginalised_compact_ws(const void* logits, int logits_dtype, int64_t
 
 
 /*
+ * Generalised Jensen-Shannon divergence against a sparse (top-K) teacher with the rest of the vocabulary as one more outcome,
+ * loss and gradient in one sweep.  Where dl_div_topk renormalises the teacher over its K entries, the outcomes here are the K
+ * listed ids and "the rest", all columns that are not listed: what a student gives to tokens its teacher did not store counts.
+ *   P  exp(t_val) on the listed ids (log-probs of the whole vocabulary, as dl_teacher_topk stores them); the rest has
+ *      max(1 - their sum, rest_min); all divided by their sum
+ *   Q  softmax(logits * inv_T), the rest's columns added up
+ *   beta = 0: KL(P|Q);   beta = 1: KL(Q|P);   0 < beta < 1: beta KL(P|M) + (1 - beta) KL(Q|M), M = beta P + (1 - beta) Q
+ * logits, row_map, t_val, t_idx, t_cnt, row_loss, grad, grad_scale as for dl_div_topk (stored log-probs are taken at the
+ * temperature they were stored at: the tempered mass of what was not stored is not known).  0 <= K <= DL_MAX_TOPK.
+ * rest_min   in (0, 1): storage rounds log-probs (fp16: 1 - sum is uncertain by some 1e-4), and where the top K hold all of the
+ *            teacher's mass a rest of 0 would make KL(Q|P) infinite.
+ * Entries that do not count, as for dl_div_topk: ids outside [0, V), stored log-probs of -inf, entries from t_cnt on; their
+ * columns belong to the rest.  An id that is listed again has its masses added up.  Where no column outside the list has an
+ * unmasked logit (-inf, or a masked value: below -2^31 after scaling, two-byte logits -2^20) the rest is no outcome.  A row
+ * without any unmasked logit, or without both entries and rest, counts for nothing: loss 0, gradient 0.
+ * grad must not overlap the logits (parts of wide rows read listed logits that belong to each other).
+ * workspace  dl_div_topk_rest_workspace_bytes(...) bytes (0 for rows of up to 65536 two-byte / 32768 four-byte columns), 16-byte
+ *            aligned, contents irrelevant; two launches that may overlap in time must not share it.
+ * flags      DL_TOPK_NO_WAIT (test hook, as for dl_div_topk).
+ * V up to 524288 two-byte / 262144 four-byte columns; any element-aligned pointers and strides.  beta, rest_min or inv_T out of
+ * range: DL_ERR_SHAPE.  Losses, sums and the K outcomes are fp32; two-byte logits hold the rest's powers as pre-scaled fp16
+ * between the sweeps, as dl_div_topk does.
+ */
+int64_t dl_div_topk_rest_workspace_bytes(int dtype, int64_t n_rows, int64_t V);
+int dl_div_topk_rest(float beta, const void* logits, int logits_dtype, int64_t row_stride, int64_t n_rows, int64_t V,
+                     const int32_t* row_map, const void* t_val, int t_val_dtype, const void* t_idx, int t_idx_itype, int K,
+                     int64_t n_teacher_rows, const int32_t* t_cnt, float inv_T, float rest_min, float grad_scale,
+                     float* row_loss, void* grad, int64_t grad_stride, void* workspace, int64_t workspace_bytes, int flags,
+                     void* stream);
+
+/*
+ * Sampling: one token per row of logits [n_rows, V] from one given random number per row, `u` fp32 in [0, 1) (24 bits count;
+ * values outside are brought in).
+ * The tokens of a row are ordered by descending logit, equal logits by index.  With every fp32 operation rounded by itself,
+ *   t_i = (x_i - max x) * (log2(e) / T),  W_i = floor(2^31 2^t_i)  (2^t: rint(t) and a polynomial of degree 5 in what is left)
+ * are the weights; sums of them are exact, and so is every choice below.
+ *   top_k > 0   keeps the first top_k tokens (with a weight);
+ *   top_p < 1   of those the tokens with less than max(1, floor(mass * floor(2^24 top_p) / 2^24)) ahead of them;
+ *   min_p > 0   what comes ahead of the first token with W < floor(2^31 min_p);
+ *   token       the kept token in whose stretch floor(kept mass * floor(2^24 u) / 2^24) falls.
+ * T <= 0 (or NaN): the first maximum.  An infinite logit shares the mass with those equal to it.  NaN and -inf logits have no
+ * weight; a row with nothing else gives token -1, logp -inf, kept 0.
+ * temperature, top_k, top_p, min_p: one entry per row, or NULL and the `_all` value counts for every row.
+ * token int64 [n_rows]; logp fp32 (optional): log-probability of the token under softmax(logits / T) before the filters; kept
+ * int32 (optional): how many tokens the filters kept.
+ * V up to 4194304 (DL_ERR_LIMIT); any element-aligned logits and row stride.
+ */
+int dl_sample_rows(const void* logits, int dtype, int64_t row_stride, int64_t n_rows, int64_t V, const float* u,
+                   const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                   float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* token, float* logp,
+                   int32_t* kept, void* stream);
+
+/*
+ * Embedding: rows of a table by token id, scaled.
+ *   out[n, :] = round(scale * table[tokens[n], :])
+ * table [vocab, width] (row stride `table_stride`) and out [n_tokens, width] (`out_stride`) of one dtype; tokens int32 or
+ * int64.  A token outside [0, vocab) is padding: its row is zero.  The product is fp32, rounded once to the dtype.
+ * Any element-aligned pointers and strides.
+ */
+int dl_embed_rows(const void* table, int dtype, int64_t table_stride, int64_t vocab, int64_t width, const void* tokens, int itype,
+                  int64_t n_tokens, float scale, void* out, int64_t out_stride, void* stream);
+
+/*
+ * The gradient of dl_embed_rows by its table, dense:
+ *   grad[v, :] = round(scale * sum over {n : tokens[n] == v} of g[n, :]  (+ grad[v, :] if `accumulate`))
+ * g [n_tokens, width] (row stride `g_stride`) of `dtype`, grad [vocab, width] (`grad_stride`) of the same dtype or fp32.
+ * Without `accumulate` every row of grad is written (zeros where no token names it); with it only rows that some token names.
+ * Tokens outside [0, vocab) are left out.  The rows of a token are summed in fp32 in ascending order of n (in runs of 32
+ * sorted tokens, the runs' sums then in order): no atomics, the same bits on every call.
+ * workspace  at least dl_embed_grad_workspace_bytes(...) bytes on a 256-byte boundary, contents irrelevant; two calls that may
+ *            overlap in time must not share it.  About 16 bytes per token + width / 4 bytes per token.
+ */
+int64_t dl_embed_grad_workspace_bytes(int64_t n_tokens, int64_t width);
+int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t n_tokens, int64_t width, const void* tokens, int itype,
+                  float scale, int accumulate, void* grad, int grad_dtype, int64_t grad_stride, int64_t vocab, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/*
  * Deterministic sum of n fp32 values times `scale` into out[0] (fixed reduction tree,
  * double accumulation).  Replaces the `.mean()` of utils/finetuning_utils.py:54 /
  * the `+=` accumulation of classes/losses.py:43-47.

@@ -1,0 +1,542 @@
+// Sampling: one token per row of logits, from a given random number, with temperature, top-k, top-p and min-p.
+//
+// The tokens of a row go in descending order of their logits, equal logits by their index.  Their weights are whole numbers,
+//   W_i = floor(2^31 2^t_i),   t_i = (x_i - max x) log2(e) / T   (fp32, every operation rounded by itself),
+// the power from a polynomial whose products and sums are rounded one by one.  Sums of whole numbers are exact, so the
+// choice depends neither on the order of any additions nor on how a row is dealt to threads and workgroups: the same
+// logits and the same random number give the same token on any launch, and on any machine with IEEE arithmetic.  (What is
+// lost of a row's mass: below 2^-31 of the largest weight per token; the random number itself has 24 bits.)
+//   top-k  the first k tokens;  top-p  tokens with less than floor(p * mass of those) ahead of them;  min-p  up to the
+//   first token whose weight is below min_p * 2^31.  All three cut the ordered list behind some token, so what is kept is
+//   a prefix, and the token is the one in whose stretch of the prefix's mass floor(u * mass) falls.
+// So a row needs three look-ups in its ordered weights, not a sort: a histogram of (mass, count) over 1024 bins, a 32nd of a
+// power of two wide, says in which bin each answer lies, and only the bins up to there (usually a few dozen tokens), or
+// just that bin, are collected and sorted in LDS.  A bin that holds more than the list (equal logits, flat rows) is
+// narrowed by eight bits of the logits' order at a time; what remains after 32 bits are equal logits, whose weights are
+// equal too.
+#include "distill_common.hpp"
+#include "distill_hip.h"
+
+#include <algorithm>
+
+namespace dl {
+
+typedef unsigned long long u64;
+
+constexpr int SAMPLE_BINS = 1024, SAMPLE_CAP = 2048;
+constexpr int64_t SAMPLE_MAX_V = 1 << 22;      // a row's mass stays below 2^53
+
+struct SampleParams {
+  const void* logits; int64_t row_stride, n_rows, V;
+  const float* u;
+  const float* T; const int32_t* k; const float* p; const float* m;      // one per row, or NULL: the ones below for all rows
+  float T0, p0, m0; int k0;
+  int64_t* token; float* logp; int32_t* kept;
+};
+
+// What the weights of a row are relative to.  `peak`: the limit in which only the maximum has any (T <= 0, an infinite maximum).
+struct RowScale { float top, rate; bool peak; };
+
+__device__ __forceinline__ RowScale row_scale(float top, float T) {
+  RowScale s;
+  s.top = top;
+  s.rate = LOG2E / T;
+  s.peak = !(T > 0.f) || s.rate == INFINITY || top == INFINITY;
+  return s;
+}
+// t of a logit, at least -64 (NaN as well)
+__device__ __forceinline__ float sample_t(const RowScale& s, float x) {
+#pragma clang fp contract(off)
+  if (s.peak) return x == s.top ? 0.f : -64.f;
+  const float d = x - s.top;
+  return fmaxf(d * s.rate, -64.f);
+}
+// 2^(t + 31), every operation rounded by itself
+__device__ __forceinline__ float sample_power(float t) {
+#pragma clang fp contract(off)
+  const float n = rintf(t), f = t - n;
+  float p = 0x1.5bba14p-10f;
+  p = p * f + 0x1.3cea88p-7f;
+  p = p * f + 0x1.c6b752p-5f;
+  p = p * f + 0x1.ebf9bcp-3f;
+  p = p * f + 0x1.62e42ap-1f;
+  p = p * f + 1.f;
+  return __builtin_amdgcn_ldexpf(p, (int)n + 31);
+}
+__device__ __forceinline__ unsigned sample_weight(float t) { return (unsigned)sample_power(t); }
+__device__ __forceinline__ int sample_bin(float t) { return min((int)(t * -32.f), SAMPLE_BINS - 1); }      // rounded towards 0
+// Ascending with the logit; -0 counts as 0.
+__device__ __forceinline__ unsigned order_of(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float logit_of(unsigned order) { return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ u64 sample_word(float x, int column) { return ((u64)~order_of(x) << 32) | (unsigned)column; }
+__device__ __forceinline__ float word_logit(u64 w) { return logit_of(~(unsigned)(w >> 32)); }
+// floor(mass * part / 2^24)
+__device__ __forceinline__ u64 share_of(u64 mass, unsigned part) { return (mass >> 24) * part + (((mass & 0xffffffu) * part) >> 24); }
+
+// f(logit, column) for every column of [lo, hi) of a row, on any element boundary; four loads in flight per thread.
+template <class Tag, int NT, class F>
+__device__ __forceinline__ void each_logit(const char* row, int64_t lo, int64_t hi, F f) {
+  using C = Chunk<Tag>;
+  const char* at = row + lo * Tag::bytes;
+  const int n = (int)(hi - lo), whole = n / C::N;
+  constexpr int UN = 4;
+  for (int c0 = threadIdx.x; c0 < whole; c0 += NT * UN) {
+    u32x4 v[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (c0 + i * NT < whole) v[i] = load16_unaligned(at + (int64_t)(c0 + i * NT) * 16);
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (c0 + i * NT >= whole) break;
+      float x[C::N];
+      C::unpack(v[i], x);
+#pragma unroll
+      for (int e = 0; e < C::N; ++e) f(x[e], (int)lo + (c0 + i * NT) * C::N + e);
+    }
+  }
+  const int col = whole * C::N + (int)threadIdx.x;
+  if (col < n) f(load_as_float(at, Tag::id, col), (int)lo + col);
+}
+
+// A list of tokens in order with their masses: those of some bins, or some of one bin's.
+struct SampleLds {
+  u64 mass[SAMPLE_BINS + 1];                 // of a bin; then of all bins ahead of it
+  u64 word[SAMPLE_CAP], upto[SAMPLE_CAP];    // the list; the mass up to and with each of its tokens
+  u64 wave_mass[32], hit_mass;
+  unsigned count[SAMPLE_BINS + 1], wave_count[32];
+  unsigned n, hit;
+  float red[16];
+};
+
+template <int NT>
+struct Sampler {
+  static constexpr int NW = NT / WAVE;
+  SampleLds& s;
+  const char* row;
+  int64_t V;
+  RowScale sc;
+  // the list in LDS: bins [lo_bin, hi_bin] whole (hi_bin < 0: none), tokens and mass ahead of it
+  int lo_bin = 0, hi_bin = -1, n = 0;
+  unsigned ahead = 0;
+  u64 ahead_mass = 0;
+
+  __device__ Sampler(SampleLds& lds, const char* r, int64_t v, const RowScale& scale) : s(lds), row(r), V(v), sc(scale) {}
+
+  // Sums over the workgroup of a pair; the result in every thread.
+  __device__ void sum(u64& mass, unsigned& count) {
+    const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+#pragma unroll
+    for (int o = WAVE / 2; o > 0; o >>= 1) {
+      mass += __shfl_xor(mass, o, WAVE);
+      count += __shfl_xor(count, o, WAVE);
+    }
+    __syncthreads();
+    if (lane == 0) { s.wave_mass[w] = mass; s.wave_count[w] = count; }
+    __syncthreads();
+    mass = 0;
+    count = 0;
+    for (int i = 0; i < NW; ++i) { mass += s.wave_mass[i]; count += s.wave_count[i]; }
+  }
+  // Exclusive sums over the workgroup's threads, in order.
+  __device__ void scan(u64& mass, unsigned& count) {
+    const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+    const u64 m0 = mass;
+    const unsigned c0 = count;
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) {
+      const u64 a = __shfl_up(mass, o, WAVE);
+      const unsigned b = __shfl_up(count, o, WAVE);
+      if (lane >= o) { mass += a; count += b; }
+    }
+    __syncthreads();
+    if (lane == WAVE - 1) { s.wave_mass[w] = mass; s.wave_count[w] = count; }
+    __syncthreads();
+    mass -= m0;
+    count -= c0;
+    for (int i = 0; i < w; ++i) { mass += s.wave_mass[i]; count += s.wave_count[i]; }
+  }
+  // Masses and counts of bins -> of all bins ahead; entry `bins` gets the totals.
+  template <int BINS>
+  __device__ void scan_bins(u64* mass, unsigned* count) {
+    constexpr int EACH = (BINS + NT - 1) / NT;
+    u64 m[EACH], mm = 0;
+    unsigned c[EACH], cc = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int b = threadIdx.x * EACH + j;
+      m[j] = b < BINS ? mass[b] : 0;
+      c[j] = b < BINS ? count[b] : 0;
+      mm += m[j];
+      cc += c[j];
+    }
+    scan(mm, cc);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int b = threadIdx.x * EACH + j;
+      if (b < BINS) { mass[b] = mm; count[b] = cc; }
+      mm += m[j];
+      cc += c[j];
+      if (b == BINS - 1) { mass[BINS] = mm; count[BINS] = cc; }
+    }
+    __syncthreads();
+  }
+  // The one index b < bins for which test(b) holds, in every thread.
+  template <class Test>
+  __device__ int find(int bins, Test test) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += NT)
+      if (test(b)) s.hit = (unsigned)b;
+    __syncthreads();
+    return (int)s.hit;
+  }
+  __device__ int bin_of_count(unsigned q) { return find(SAMPLE_BINS, [&](int b) { return s.count[b] < q && s.count[b + 1] >= q; }); }
+  __device__ int bin_reaching(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] < m && s.mass[b + 1] >= m; }); }
+  __device__ int bin_passing(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] <= m && s.mass[b + 1] > m; }); }
+
+  // Tokens for which in(t, x) holds (and that have a weight) into the list, in order, with their masses behind `mass`.
+  template <class Tag, class In>
+  __device__ void collect(unsigned before, u64 mass, In in) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    each_logit<Tag, NT>(row, 0, V, [&](float x, int col) {
+      const float t = sample_t(sc, x);
+      if (in(t, x) && sample_weight(t) > 0) {
+        const unsigned at = atomicAdd(&s.n, 1u);
+        if (at < SAMPLE_CAP) s.word[at] = sample_word(x, col);
+      }
+    });
+    __syncthreads();
+    n = min((int)s.n, SAMPLE_CAP);
+    sort();
+    ahead = before;
+    ahead_mass = mass;
+    constexpr int EACH = SAMPLE_CAP / NT;
+    unsigned w[EACH], none = 0;
+    u64 sum_w = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x * EACH + j;
+      w[j] = i < n ? sample_weight(sample_t(sc, word_logit(s.word[i]))) : 0u;
+      sum_w += w[j];
+    }
+    scan(sum_w, none);
+    sum_w += mass;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x * EACH + j;
+      sum_w += w[j];
+      if (i < n) s.upto[i] = sum_w;
+    }
+    __syncthreads();
+  }
+  // The list's words ascending.  Up to 256: every word's place is the number of words below it (all are different).
+  __device__ void sort() {
+    const int tid = threadIdx.x;
+    if (n <= 256) {
+      u64 mine = 0;
+      int place = 0;
+      if (tid < n) {
+        mine = s.word[tid];
+        for (int j = 0; j < n; ++j) place += s.word[j] < mine;
+      }
+      __syncthreads();
+      if (tid < n) s.word[place] = mine;
+    } else if (n <= NT) {
+      sort_in_registers<1>();
+    } else {
+      sort_in_registers<SAMPLE_CAP / NT>();
+    }
+    __syncthreads();
+  }
+  template <int EACH>
+  __device__ void sort_in_registers() {
+    u64 w[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) w[j] = (int)threadIdx.x * EACH + j < n ? s.word[threadIdx.x * EACH + j] : ~0ull;
+    __syncthreads();
+    block_sort<u64, NT, EACH>(w, s.word);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) s.word[threadIdx.x * EACH + j] = w[j];
+  }
+  template <class Tag>
+  __device__ void collect_bins(int lo, int hi) {
+    const float above = -(float)lo * 0.03125f, below = -(float)(hi + 1) * 0.03125f;      // bin lo .. hi: below < t <= above
+    const bool last = hi == SAMPLE_BINS - 1;
+    collect<Tag>(s.count[lo], s.mass[lo], [&](float t, float) { return t <= above && (last || t > below); });
+    lo_bin = lo;
+    hi_bin = hi;
+  }
+
+  // Equal logits too many for the list, after narrow(): the order of their logit, tokens and mass ahead of them.
+  bool ties = false;
+  unsigned tie_order = 0, tie_weight = 0;
+
+  // Makes the list hold the part of `bin` in which tokens-ahead-of-it <= target < ... (by_count), or the mass does, or sets `ties`.
+  template <class Tag>
+  __device__ void narrow(int bin, bool by_count, u64 target) {
+    u64* mass = s.word;                                       // 257 of each, in the list's place
+    unsigned* count = reinterpret_cast<unsigned*>(s.upto);
+    unsigned prefix = 0, before = s.count[bin];
+    u64 before_mass = s.mass[bin];
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      __syncthreads();
+      for (int i = threadIdx.x; i <= 256; i += NT) { mass[i] = 0; count[i] = 0; }
+      __syncthreads();
+      each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+        const float t = sample_t(sc, x);
+        if (sample_bin(t) != bin) return;
+        const unsigned o = order_of(x), w = sample_weight(t);
+        if (w == 0 || (shift < 24 && (o >> (shift + 8)) != prefix)) return;
+        const int slot = 255 - (int)((o >> shift) & 255u);
+        atomicAdd(&mass[slot], (u64)w);
+        atomicAdd(&count[slot], 1u);
+      });
+      __syncthreads();
+      scan_bins<256>(mass, count);
+      const u64 m0 = before_mass;
+      const unsigned c0 = before;
+      const int slot = find(256, [&](int b) {
+        return by_count ? c0 + count[b] <= target && target < c0 + count[b + 1] : m0 + mass[b] <= target && target < m0 + mass[b + 1];
+      });
+      const unsigned inside = count[slot + 1] - count[slot];
+      const u64 inside_mass = mass[slot + 1] - mass[slot];
+      before = c0 + count[slot];
+      before_mass = m0 + mass[slot];
+      prefix = (prefix << 8) | (unsigned)(255 - slot);
+      if (inside <= SAMPLE_CAP) {
+        const unsigned want = prefix;
+        const int sh = shift;
+        collect<Tag>(before, before_mass, [&](float t, float x) { return sample_bin(t) == bin && (order_of(x) >> sh) == want; });
+        lo_bin = 0;
+        hi_bin = -1;                                          // part of a bin: of no use to other look-ups
+        return;
+      }
+      if (shift == 0) {
+        ties = true;
+        tie_order = prefix;
+        tie_weight = (unsigned)(inside_mass / inside);
+        ahead = before;
+        ahead_mass = before_mass;
+        lo_bin = 0;
+        hi_bin = -1;
+      }
+    }
+  }
+  // The list (or `ties`) so that it holds the target of bin `bin`.
+  template <class Tag>
+  __device__ void reach(int bin, bool by_count, u64 target) {
+    ties = false;
+    if (bin >= lo_bin && bin <= hi_bin) return;
+    if (s.count[bin + 1] - s.count[bin] <= SAMPLE_CAP) collect_bins<Tag>(bin, bin);
+    else narrow<Tag>(bin, by_count, target);
+  }
+  // Mass of the first q tokens.
+  template <class Tag>
+  __device__ u64 mass_of_first(unsigned q, int bin) {
+    reach<Tag>(bin, true, q - 1);
+    if (ties) return ahead_mass + (u64)(q - ahead) * tie_weight;
+    return s.upto[q - ahead - 1];
+  }
+  // The number of tokens, and their mass, up to the first one at which the mass reaches m.
+  template <class Tag>
+  __device__ void first_reaching(u64 m, int bin, unsigned& tokens, u64& mass) {
+    reach<Tag>(bin, false, m - 1);
+    if (ties) {
+      const u64 q = (m - ahead_mass + tie_weight - 1) / tie_weight;
+      tokens = ahead + (unsigned)q;
+      mass = ahead_mass + q * tie_weight;
+      return;
+    }
+    const int i = find(n, [&](int j) { return s.upto[j] >= m && (j == 0 ? ahead_mass : s.upto[j - 1]) < m; });
+    tokens = ahead + (unsigned)i + 1;
+    mass = s.upto[i];
+  }
+  // The token in whose stretch m falls, and its t.
+  template <class Tag>
+  __device__ int token_at(u64 m, int bin, float& t) {
+    reach<Tag>(bin, false, m);
+    if (ties) {
+      const unsigned j = (unsigned)((m - ahead_mass) / tie_weight);
+      t = sample_t(sc, logit_of(tie_order));
+      return equal_logit<Tag>(j);
+    }
+    const int i = find(n, [&](int k) { return s.upto[k] > m && (k == 0 ? ahead_mass : s.upto[k - 1]) <= m; });
+    t = sample_t(sc, word_logit(s.word[i]));
+    return (int)(unsigned)s.word[i];
+  }
+  // The column of the j-th logit of order `tie_order`: every wave counts those of a stretch of columns, then the one that
+  // holds the j-th walks its stretch again.
+  template <class Tag>
+  __device__ int equal_logit(unsigned j) {
+    const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+    const int64_t each = (V + NW - 1) / NW, lo = min(V, w * each), hi = min(V, lo + each);
+    unsigned mine = 0;
+    for (int64_t c = lo + lane; c < hi; c += WAVE) mine += order_of(load_as_float(row, Tag::id, c)) == tie_order;
+#pragma unroll
+    for (int o = WAVE / 2; o > 0; o >>= 1) mine += __shfl_xor(mine, o, WAVE);
+    __syncthreads();
+    if (lane == 0) s.wave_count[w] = mine;
+    __syncthreads();
+    unsigned before = 0;
+    for (int i = 0; i < w; ++i) before += s.wave_count[i];
+    if (j >= before && j < before + mine) {
+      for (int64_t c0 = lo; c0 < hi; c0 += WAVE) {
+        const bool is = c0 + lane < hi && order_of(load_as_float(row, Tag::id, c0 + lane)) == tie_order;
+        const u64 all = __ballot(is);
+        if (is && before + __popcll(all & ((1ull << lane) - 1ull)) == j) s.hit = (unsigned)(c0 + lane);
+        before += __popcll(all);
+        if (before > j) break;
+      }
+    }
+    __syncthreads();
+    return (int)s.hit;
+  }
+  // The number of tokens ahead of the first whose weight is below `least`, and their mass, if that comes before `tokens`.
+  template <class Tag>
+  __device__ void cut_below(unsigned least, unsigned& tokens, u64& mass) {
+    // bins ahead of the threshold's, less one for what rounding does to it, hold no such token; from two behind it on, all are
+    const int behind = min((int)((31.f - log2f((float)least)) * 32.f) + 2, SAMPLE_BINS - 1);
+    if (hi_bin < 0 || lo_bin > 0) {
+      if (s.count[behind + 1] <= SAMPLE_CAP) collect_bins<Tag>(0, behind);
+    }
+    if (hi_bin >= 0 && lo_bin == 0 && (hi_bin >= behind || tokens <= (unsigned)n)) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.hit = min(tokens, (unsigned)n);      // (tokens behind the list are all below)
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += NT)
+        if (s.upto[i] - (i == 0 ? 0 : s.upto[i - 1]) < least) atomicMin(&s.hit, (unsigned)i);
+      __syncthreads();
+      const unsigned q = s.hit;
+      if (q < tokens) {
+        tokens = q;
+        mass = s.upto[q - 1];
+      }
+      return;
+    }
+    // Too many for the list: the largest logit with too small a weight, then what lies above it.
+    unsigned worst = 0;
+    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+      const unsigned w = sample_weight(sample_t(sc, x));
+      if (w > 0 && w < least) worst = max(worst, order_of(x));
+    });
+    worst = wave_max(worst);
+    __syncthreads();
+    if ((threadIdx.x & (WAVE - 1)) == 0) s.wave_count[threadIdx.x / WAVE] = worst;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) worst = max(worst, s.wave_count[i]);
+    u64 m = 0;
+    unsigned c = 0;
+    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+      const unsigned w = sample_weight(sample_t(sc, x));
+      if (w > 0 && order_of(x) > worst) { m += w; ++c; }
+    });
+    sum(m, c);
+    if (c < tokens) {
+      tokens = c;
+      mass = m;
+    }
+  }
+};
+
+// From the histogram in LDS (sums ahead of each bin) to the row's outputs.
+template <class Tag, int NT>
+__device__ void sample_finish(const SampleParams& p, SampleLds& s, int64_t r, const char* row, const RowScale& sc, float powers) {
+  Sampler<NT> a(s, row, p.V, sc);
+  const float T = p.T ? p.T[r] : p.T0, top_p = p.p ? p.p[r] : p.p0, min_p = p.m ? p.m[r] : p.m0;
+  const int k = T > 0.f ? (p.k ? p.k[r] : p.k0) : 1;
+  unsigned tokens = s.count[SAMPLE_BINS];
+  u64 mass = s.mass[SAMPLE_BINS];
+  if (k > 0 && (unsigned)k < tokens) {
+    const int bin = a.bin_of_count(k);
+    if (s.count[bin + 1] <= SAMPLE_CAP) a.template collect_bins<Tag>(0, bin);      // holds whatever is asked below
+    mass = a.template mass_of_first<Tag>(k, bin);
+    tokens = k;
+  }
+  if (top_p < 1.f) {
+    const u64 part = share_of(mass, (unsigned)(fmaxf(top_p, 0.f) * 0x1p24f)), want = part > 0 ? part : 1;
+    const int bin = a.bin_reaching(want);
+    if (a.hi_bin < 0 && s.count[bin + 1] <= SAMPLE_CAP) a.template collect_bins<Tag>(0, bin);
+    a.template first_reaching<Tag>(want, bin, tokens, mass);
+  }
+  const unsigned least = min_p > 0.f ? (unsigned)(fminf(min_p, 1.f) * 0x1p31f) : 0u;
+  if (least > 0) a.template cut_below<Tag>(least, tokens, mass);
+  const unsigned u = (unsigned)fminf(fmaxf(p.u[r], 0.f) * 0x1p24f, 0x1p24f - 1.f);
+  const u64 want = share_of(mass, u);
+  float t;
+  const int token = a.template token_at<Tag>(want, a.bin_passing(want), t);
+  if (threadIdx.x == 0) {
+    p.token[r] = token;
+    if (p.logp) p.logp[r] = (t - log2f(powers * 0x1p-31f)) * LN2;
+    if (p.kept) p.kept[r] = (int)tokens;
+  }
+}
+
+template <class Tag, int NT>
+__global__ __launch_bounds__(NT) void sample_row_kernel(const SampleParams p) {
+  __shared__ SampleLds s;
+  const int64_t r = blockIdx.x;
+  const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
+  for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) { s.mass[b] = 0; s.count[b] = 0; }
+  float top = -INFINITY;
+  each_logit<Tag, NT>(row, 0, p.V, [&](float x, int) { top = fmaxf(top, x); });
+  top = block_max<NT>(top, s.red);
+  if (top == -INFINITY) {                    // nothing to draw from
+    if (threadIdx.x == 0) {
+      p.token[r] = -1;
+      if (p.logp) p.logp[r] = -INFINITY;
+      if (p.kept) p.kept[r] = 0;
+    }
+    return;
+  }
+  const RowScale sc = row_scale(top, p.T ? p.T[r] : p.T0);
+  float powers = 0.f;
+  each_logit<Tag, NT>(row, 0, p.V, [&](float x, int) {
+    const float t = sample_t(sc, x), e = sample_power(t);
+    powers += e;
+    const unsigned w = (unsigned)e;
+    if (w > 0) {
+      const int b = sample_bin(t);
+      atomicAdd(&s.mass[b], (u64)w);
+      atomicAdd(&s.count[b], 1u);
+    }
+  });
+  powers = block_sum<NT>(powers, s.red);
+  Sampler<NT>(s, row, p.V, sc).template scan_bins<SAMPLE_BINS>(s.mass, s.count);
+  sample_finish<Tag, NT>(p, s, r, row, sc, powers);
+}
+
+template <class Tag>
+static int launch_sample(const SampleParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((sample_row_kernel<Tag, 512>), dim3((unsigned)p.n_rows), dim3(512), 0, st, p);
+  return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH;
+}
+
+}  // namespace dl
+
+extern "C" int dl_sample_rows(const void* logits, int dtype, int64_t row_stride, int64_t n_rows, int64_t V, const float* u,
+                              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                              float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* token, float* logp,
+                              int32_t* kept, void* stream) {
+  using namespace dl;
+  if ((unsigned)dtype > DL_F16) return DL_ERR_DTYPE;
+  if (n_rows < 0 || V <= 0 || row_stride < V) return DL_ERR_SHAPE;
+  if (n_rows == 0) return DL_OK;
+  if (!logits || !u || !token) return DL_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(token) % 8 ||
+      (reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) |
+       reinterpret_cast<uintptr_t>(top_p) | reinterpret_cast<uintptr_t>(min_p) | reinterpret_cast<uintptr_t>(logp) |
+       reinterpret_cast<uintptr_t>(kept)) % 4)
+    return DL_ERR_ALIGN;
+  if (V > SAMPLE_MAX_V || n_rows > 0x7fffffffLL) return DL_ERR_LIMIT;
+  SampleParams p{logits, row_stride, n_rows, V, u, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all,
+                 token, logp, kept};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == DL_F32) return launch_sample<TagF32>(p, st);
+  if (dtype == DL_BF16) return launch_sample<TagBF16>(p, st);
+  return launch_sample<TagF16>(p, st);
+}

@@ -1,0 +1,417 @@
+// Generalised Jensen-Shannon divergence against a top-K teacher with the rest of the vocabulary as one more outcome.
+//
+// Outcomes: the K listed ids and "the rest", every column that is not listed.
+//   P  the teacher: exp(t_val) on the listed ids; the rest has what they leave of 1, at least rest_min; divided by their sum
+//   Q  the student: softmax(x / T), the rest's columns added up
+//   beta = 0: KL(P|Q);  beta = 1: KL(Q|P);  between: beta KL(P|M) + (1 - beta) KL(Q|M) with M = beta P + (1 - beta) Q
+// Gradient: with s_j = q_j dL/dq_j (beta = 0: -p_j; 1: q_j log(q_j / p_j); between: (1 - beta) q_j log(q_j / m_j)) and S their sum,
+//   dL/dz_k = s_k - q_k S on a listed id, and softmax over the rest's columns times (s_rest - q_rest S) on those:
+// the rest's columns need one number per row, so the row is read once, written once and costs two exponentials' worth of
+// vector work per column.  Bound by HBM traffic, 2 V bytes x the element size per row.
+//
+// Layout as in the forward-KL kernels: a row, or one column part of it, sits in its workgroup's registers; parts exchange
+// (max, sum) of the rest's columns through records in a workspace, with a bounded wait and a second launch for parts
+// that gave up.  Listed columns are taken out of the registers (-inf in their place) before the row's statistics, so
+// that the rest's mass is a sum of what it consists of and not 1 minus the listed mass: a confident student leaves it
+// 1e-8, which that difference would lose.  Every part works out all K outcomes itself (some ten microseconds of one
+// workgroup against exchanging K values): listed logits of other parts are fetched straight from memory, behind the
+// part's own loads, when the line is on its way to another part of the XCD anyway.
+#include "topk_div.hpp"
+#include "distill_hip.h"
+
+namespace dl {
+
+struct RestParams {
+  const void* logits; int64_t row_stride, n_rows, V;
+  const int32_t* row_map;
+  const void* t_val; int t_val_dtype; const void* t_idx; int t_idx_itype; int K;
+  int64_t n_trows; const int32_t* t_cnt;
+  float beta, inv_T, rest_min, grad_scale;
+  float* row_loss; void* grad; int64_t grad_stride;
+  void* workspace; int parts; int spin_limit;
+};
+
+// Lists of the row's entries by the 16-byte chunk of their column (chunks that share a head share a list).
+struct RestLds {
+  int *idx, *next, *head;
+  float *lp, *z, *val, *red, *xm, *xs;
+  int* xok;
+  unsigned* own;
+  __device__ RestLds(unsigned char* base, int K) {
+    const int Kp = (K + 3) & ~3;
+    idx = reinterpret_cast<int*>(base);
+    next = idx + Kp;
+    lp = reinterpret_cast<float*>(next + Kp);
+    z = lp + Kp;
+    val = z + Kp;
+    red = val + Kp;
+    xm = red + 64;
+    xs = xm + MAX_PARTS;
+    xok = reinterpret_cast<int*>(xs + MAX_PARTS);
+    head = xok + MAX_PARTS;
+    own = reinterpret_cast<unsigned*>(head + CORRECTION_HEADS);
+  }
+  static size_t bytes(int K, int threads) { return (size_t)(5 * ((K + 3) & ~3) + 64 + 3 * MAX_PARTS + CORRECTION_HEADS + threads) * 4; }
+};
+
+// One outcome's part of the loss, and s = q dL/dq.  The logarithm of the mixture goes through log1p / expm1 on the side
+// where the exponential is at most 1, so that it neither overflows nor loses a student close to the teacher.
+__device__ __forceinline__ void rest_outcome(float lp, float lq, float beta, float& loss, float& slope) {
+  const float p = expf(lp), q = expf(lq), r = lp - lq;
+  if (beta == 0.f) {
+    loss += p * r;
+    slope = -p;
+  } else if (beta == 1.f) {
+    slope = q == 0.f ? 0.f : -q * r;
+    loss += slope;
+  } else {
+    float over_p, over_q;                // log(m / p), log(m / q)
+    if (r > 0.f) {
+      over_p = log1pf((1.f - beta) * expm1f(-r));
+      over_q = r + over_p;
+    } else {
+      over_q = log1pf(beta * expm1f(r));
+      over_p = over_q - r;
+    }
+    slope = q == 0.f ? 0.f : -(1.f - beta) * q * over_q;
+    loss += slope - beta * p * over_p;
+  }
+}
+
+// `RETRY`: the part is finished by the second launch; every record of the row is there.
+template <class Tag, int NT, int NCH, bool SPLIT, bool RETRY>
+__device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s, int64_t r, int h) {
+  using C = Chunk<Tag>;
+  using M = ChunkMap<NT, NCH>;
+  const int tid = threadIdx.x, P = SPLIT ? p.parts : 1;
+  const int64_t lo = (int64_t)h * NT * NCH * C::N;
+  const int n_cols = (int)min(p.V - lo, (int64_t)NT * NCH * C::N), nch = n_cols / C::N, tail = n_cols - nch * C::N;
+  char* gpart = p.grad ? reinterpret_cast<char*>(p.grad) + (r * p.grad_stride + lo) * Tag::bytes : nullptr;
+  const auto leave = [&]() {             // a row that counts for nothing
+    if (gpart) zero_row_any<Tag, NT>(gpart, n_cols);
+    if (tid == 0 && h == 0 && p.row_loss) p.row_loss[r] = 0.f;
+  };
+  const int64_t trow = teacher_row(p.row_map, r, p.n_trows);
+  if (trow < 0) return leave();
+  const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
+  const char* rpart = row + lo * Tag::bytes;
+
+  correction_clear<NT>(s.head, s.own);
+  u32x4 reg[NCH];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = M::chunk(i, tid);
+    reg[i] = C::neg_inf();
+    if (c < nch) reg[i] = load16_unaligned(rpart + (int64_t)c * 16);
+    else if (c == nch && tail) reg[i] = load_chunk_elementwise<Tag>(rpart, c, n_cols);
+  }
+  __syncthreads();
+  const int cnt = p.t_cnt ? min(p.K, max(p.t_cnt[trow], 0)) : p.K;
+  for (int k = tid; k < p.K; k += NT) {
+    const int64_t id = k < cnt ? load_index(p.t_idx, p.t_idx_itype, trow * p.K + k) : -1;
+    const float lp = k < cnt ? load_as_float(p.t_val, p.t_val_dtype, trow * p.K + k) : -INFINITY;
+    const bool counts = id >= 0 && id < p.V && lp != -INFINITY;
+    s.idx[k] = counts ? (int)id : -1;
+    s.lp[k] = lp;
+    if (counts) {
+      s.next[k] = atomicExch(&s.head[(int)(id / C::N) & (CORRECTION_HEADS - 1)], k);
+      if (id >= lo && id < lo + n_cols) {
+        const int c = (int)(id - lo) / C::N;
+        atomicOr(&s.own[M::owner(c)], 1u << M::reg(c));
+      }
+    }
+  }
+  __syncthreads();
+  // An id that is listed again has its masses added up, in the order of its entries, in the first of them; val = -inf
+  // marks the others, and entries that do not count.
+  for (int k = tid; k < p.K; k += NT) {
+    const int id = s.idx[k];
+    float lp = s.lp[k];
+    if (id < 0) {
+      lp = -INFINITY;
+    } else {
+      const int first = s.head[(id / C::N) & (CORRECTION_HEADS - 1)];
+      bool again = false, later = false;
+      for (int j = first; j >= 0; j = s.next[j])
+        if (j != k && s.idx[j] == id) { again = true; later = later || j < k; }
+      if (later) {
+        lp = -INFINITY;
+      } else if (again) {
+        float sum = expf(lp);
+        for (int at = k;;) {
+          int next = p.K;
+          for (int j = first; j >= 0; j = s.next[j])
+            if (j > at && j < next && s.idx[j] == id) next = j;
+          if (next == p.K) break;
+          sum += expf(s.lp[next]);
+          at = next;
+        }
+        lp = logf(sum);
+      }
+      if (SPLIT && (id < lo || id >= lo + n_cols)) s.z[k] = load_as_float(row, Tag::id, id);
+    }
+    s.val[k] = lp;
+  }
+  const unsigned mine = s.own[tid];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    if (mine & (1u << i)) {
+      const int gc = (int)(lo / C::N) + M::chunk(i, tid);
+      float f[C::N];
+      C::unpack(reg[i], f);
+      for (int k = s.head[gc & (CORRECTION_HEADS - 1)]; k >= 0; k = s.next[k]) {
+        const int id = s.idx[k], e = id - gc * C::N;
+        if (e < 0 || e >= C::N) continue;
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::N; ++j) x = j == e ? f[j] : x;
+        s.z[k] = x;
+        if constexpr (Tag::bytes == 4) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) reg[i][j] = j == e ? 0xff800000u : reg[i][j];
+        } else {
+          const unsigned inf = Tag::id == BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j == e / 2) reg[i][j] = (e & 1) ? (reg[i][j] & 0xffffu) | (inf << 16) : (reg[i][j] & 0xffff0000u) | inf;
+        }
+      }
+    }
+  }
+
+  // the rest's columns: max, sum of 2^(x a - max a); the powers stay in the registers for the gradient
+  const float a = p.inv_T * LOG2E;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    float f[C::N];
+    forget(reg[i]);
+    C::unpack(reg[i], f);
+#pragma unroll
+    for (int e = 0; e < C::N; ++e) mx = fmaxf(mx, f[e]);
+  }
+  mx = block_max<NT>(mx, s.red);
+  constexpr float BIAS = C::stash_bias;
+  float mb = mx * a;
+  // A rest of nothing but masked columns counts as none, whatever they are masked with (distill_common.hpp: MASKED_BELOW; two-byte
+  // logits are thousands apart at -2^20 already).
+  const bool masked = mb < (Tag::bytes == 2 ? -0x1p20f : MASKED_BELOW);
+  if (masked) { mb = 0.f; mx = -INFINITY; }
+  const float mb_own = mb - BIAS;
+  float sm = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    float f[C::N];
+    forget(reg[i]);
+    C::unpack(reg[i], f);
+#pragma unroll
+    for (int e = 0; e < C::N; ++e) {
+      f[e] = fast_exp2(fmaf(f[e], a, -mb_own));
+      sm += f[e];
+    }
+    reg[i] = C::stash(f);
+    forget(reg[i]);
+  }
+  sm = block_sum<NT>(sm * __builtin_exp2f(-BIAS), s.red);
+
+  if (SPLIT) {
+    PartStats* ws = reinterpret_cast<PartStats*>(p.workspace) + r * P;
+    if (tid == 0 && !RETRY) part_publish(ws + h, mx, sm, 0.f);
+    if (tid < P) {
+      float om = mx, os = sm, ob;
+      s.xok[tid] = (tid == h) || part_collect(ws + tid, RETRY ? 0x7fffffff : p.spin_limit, om, os, ob);
+      s.xm[tid] = om; s.xs[tid] = os;
+    }
+    __syncthreads();
+    bool all_ok = true;
+    for (int j = 0; j < P; ++j) all_ok = all_ok && (s.xok[j] != 0);
+    if (!all_ok) {                       // nothing is written yet; the part's own record is out
+      if (tid == 0) {
+        RetryList list(p.workspace, p.n_rows, P);
+        list.entries[atomicAdd(list.count, 1u)] = (unsigned)(r * P + h);
+      }
+      return;
+    }
+    float top = s.xm[0];
+    for (int j = 1; j < P; ++j) top = fmaxf(top, s.xm[j]);
+    float S = 0.f;
+    if (top == -INFINITY) {
+      for (int j = 0; j < P; ++j) S += s.xs[j];                       // 0, or NaN
+    } else {
+      for (int j = 0; j < P; ++j) S += s.xs[j] * fast_exp2((s.xm[j] - top) * a);
+    }
+    mb = top == -INFINITY ? 0.f : top * a;
+    sm = S;
+  }
+  const float b = mb + fast_log2(sm);    // log2 of the rest's sum: -inf where no column outside the list has a finite logit
+
+  // the K outcomes and the rest
+  float zmax = -INFINITY, ps = 0.f;
+  for (int k = tid; k < p.K; k += NT)
+    if (s.val[k] != -INFINITY) {
+      zmax = fmaxf(zmax, s.z[k] * a);
+      ps += expf(s.val[k]);
+    }
+  zmax = fmaxf(block_max<NT>(zmax, s.red), b);
+  float zs = 0.f;
+  for (int k = tid; k < p.K; k += NT)
+    if (s.val[k] != -INFINITY) zs += fast_exp2(s.z[k] * a - zmax);
+  block_sum2<NT>(zs, ps, s.red);
+  const bool rest = !(b == -INFINITY);
+  if (zmax == -INFINITY || (!rest && ps == 0.f)) return leave();      // no finite logit, or nothing to compare
+  const float lse = zmax + fast_log2(zs + (rest ? fast_exp2(b - zmax) : 0.f));
+  const float p0 = rest ? fmaxf(1.f - ps, p.rest_min) : 0.f, lz = logf(ps + p0);
+  float loss = 0.f, slopes = 0.f;
+  for (int k = tid; k < p.K; k += NT)
+    if (s.val[k] != -INFINITY) {
+      float slope;
+      rest_outcome(s.val[k] - lz, (s.z[k] * a - lse) * LN2, p.beta, loss, slope);
+      slopes += slope;
+      s.lp[k] = slope;
+    }
+  block_sum2<NT>(loss, slopes, s.red);
+  float slope0 = 0.f, q0 = 0.f;
+  if (rest) {
+    const float lq0 = (b - lse) * LN2;
+    rest_outcome(logf(p0) - lz, lq0, p.beta, loss, slope0);
+    slopes += slope0;
+    q0 = expf(lq0);
+  }
+  if (tid == 0 && h == 0 && p.row_loss) p.row_loss[r] = loss;
+  if (!gpart) return;
+  const float c = p.inv_T * p.grad_scale;
+  for (int k = tid; k < p.K; k += NT)
+    if (s.val[k] != -INFINITY) s.lp[k] = (s.lp[k] - fast_exp2(s.z[k] * a - lse) * slopes) * c;
+  const float kc = !rest || masked ? 0.f : fast_exp2(mb_own - b) * (slope0 - q0 * slopes) * c;      // stashed power -> gradient
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int ch = M::chunk(i, tid);
+    if (ch < nch || (ch == nch && tail)) {
+      float f[C::N];
+      forget(reg[i]);
+      C::unstash(reg[i], f);
+#pragma unroll
+      for (int e = 0; e < C::N; ++e) f[e] *= kc;
+      if (mine & (1u << i)) {
+        const int gc = (int)(lo / C::N) + ch;
+        for (int k = s.head[gc & (CORRECTION_HEADS - 1)]; k >= 0; k = s.next[k]) {
+          const int e = s.idx[k] - gc * C::N;
+          if (e < 0 || e >= C::N || s.val[k] == -INFINITY) continue;
+          const float v = s.lp[k];
+#pragma unroll
+          for (int j = 0; j < C::N; ++j) f[j] = j == e ? v : f[j];
+        }
+      }
+      if (ch < nch) store16_stream_any(gpart + (int64_t)ch * 16, C::pack(f));
+      else store_chunk_elementwise<Tag>(gpart, ch, n_cols, C::pack(f));
+    }
+  }
+}
+
+template <class Tag, int NT, int NCH, bool SPLIT>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void rest_kernel(const RestParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const RestLds s(smem, p.K);
+  const int P = SPLIT ? p.parts : 1;
+  const unsigned grp = SPLIT ? blockIdx.x / (8u * P) : 0u, t_in = SPLIT ? blockIdx.x % (8u * P) : 0u;
+  const int64_t r = SPLIT ? (int64_t)grp * 8 + (t_in & 7u) : xcd_banded_row(blockIdx.x);
+  if (r >= p.n_rows) return;
+  rest_part<Tag, NT, NCH, SPLIT, false>(p, s, r, SPLIT ? (int)(t_in >> 3) : 0);
+}
+
+template <class Tag, int NT, int NCH>
+__device__ __attribute__((noinline)) void rest_part_again(const RestParams& p, const RestLds& s, unsigned at) {
+  rest_part<Tag, NT, NCH, true, true>(p, s, (int64_t)(at / (unsigned)p.parts), (int)(at % (unsigned)p.parts));
+}
+template <class Tag, int NT, int NCH>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void rest_retry_kernel(const RestParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const RestLds s(smem, p.K);
+  const RetryList list(p.workspace, p.n_rows, p.parts);
+  const unsigned n = *list.count;
+#pragma unroll 1
+  for (unsigned e = blockIdx.x; e < n; e += gridDim.x) {
+    rest_part_again<Tag, NT, NCH>(p, s, list.entries[e]);
+    __syncthreads();
+  }
+}
+
+// Threads and chunks per thread of a workgroup, parts per row, for rows of `nch` chunks (parts == 0: too wide).
+struct RestShape { int NT, NCH, parts; };
+static RestShape rest_shape(int64_t nch) {
+  if (nch <= 256 * 4) return {256, 4, 1};
+  if (nch <= 256 * 8) return {256, 8, 1};
+  if (nch <= 512 * 8) return {512, 8, 1};
+  if (nch <= 512 * 13) return {512, 13, 1};
+  if (nch <= 512 * 16) return {512, 16, 1};
+  const int64_t parts = (nch + 256 * 16 - 1) / (256 * 16);
+  if (parts > MAX_PARTS) return {0, 0, 0};
+  const int64_t per_thread = (nch + parts * 256 - 1) / (parts * 256);
+  return {256, per_thread <= 13 ? 13 : per_thread <= 14 ? 14 : 16, (int)parts};
+}
+
+template <class Tag, int NT, int NCH>
+static void launch_rest_row(const RestParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, false>), dim3(xcd_banded_grid(p.n_rows)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
+}
+template <class Tag, int NT, int NCH>
+static void launch_rest_parts(const RestParams& p, hipStream_t st) {
+  const int64_t n16 = split_clear_words(p.n_rows, p.parts);
+  hipLaunchKernelGGL(clear_workspace_kernel<256>, dim3((unsigned)((n16 + 255) / 256)), dim3(256), 0, st, reinterpret_cast<u32x4*>(p.workspace), n16);
+  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, true>), dim3((unsigned)((p.n_rows + 7) / 8 * 8 * p.parts)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
+  hipLaunchKernelGGL((rest_retry_kernel<Tag, NT, NCH>), dim3((unsigned)std::min<int64_t>(p.n_rows * p.parts, 256)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
+}
+
+template <class Tag>
+static int launch_rest(const RestParams& p, const RestShape& sh, hipStream_t st) {
+  if (sh.parts == 1) {
+    if (sh.NT == 256) sh.NCH == 4 ? launch_rest_row<Tag, 256, 4>(p, st) : launch_rest_row<Tag, 256, 8>(p, st);
+    else if (sh.NCH == 8) launch_rest_row<Tag, 512, 8>(p, st);
+    else if (sh.NCH == 13) launch_rest_row<Tag, 512, 13>(p, st);
+    else launch_rest_row<Tag, 512, 16>(p, st);
+  } else {
+    if (sh.NCH == 13) launch_rest_parts<Tag, 256, 13>(p, st);
+    else if (sh.NCH == 14) launch_rest_parts<Tag, 256, 14>(p, st);
+    else launch_rest_parts<Tag, 256, 16>(p, st);
+  }
+  return launch_status();
+}
+
+static int64_t rest_chunks(int dtype, int64_t V) { return dtype == DL_F32 ? (V + 3) / 4 : (V + 7) / 8; }
+
+}  // namespace dl
+
+extern "C" int64_t dl_div_topk_rest_workspace_bytes(int dtype, int64_t n_rows, int64_t V) {
+  using namespace dl;
+  if ((unsigned)dtype > DL_F16 || n_rows <= 0 || V <= 0) return 0;
+  const RestShape sh = rest_shape(rest_chunks(dtype, V));
+  return sh.parts > 1 ? RetryList::bytes(n_rows, sh.parts) : 0;
+}
+
+extern "C" int dl_div_topk_rest(float beta, const void* logits, int logits_dtype, int64_t row_stride, int64_t n_rows, int64_t V,
+                                const int32_t* row_map, const void* t_val, int t_val_dtype, const void* t_idx, int t_idx_itype, int K,
+                                int64_t n_teacher_rows, const int32_t* t_cnt, float inv_T, float rest_min, float grad_scale,
+                                float* row_loss, void* grad, int64_t grad_stride, void* workspace, int64_t workspace_bytes, int flags,
+                                void* stream) {
+  using namespace dl;
+  if ((unsigned)logits_dtype > DL_F16 || (unsigned)t_val_dtype > DL_F16 || (unsigned)t_idx_itype > DL_I64) return DL_ERR_DTYPE;
+  if (n_rows < 0 || V <= 0 || K < 0 || n_teacher_rows < 0 || row_stride < V || (grad && grad_stride < V)) return DL_ERR_SHAPE;
+  if (!(beta >= 0.f && beta <= 1.f) || !(rest_min > 0.f && rest_min < 1.f) || !(inv_T > 0.f)) return DL_ERR_SHAPE;
+  if (n_rows == 0) return DL_OK;
+  if (!logits || (n_teacher_rows > 0 && K > 0 && (!t_val || !t_idx)) || (!row_loss && !grad)) return DL_ERR_NULL;
+  if (K > DL_MAX_TOPK) return DL_ERR_LIMIT;
+  const uintptr_t eb = logits_dtype == DL_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % eb || reinterpret_cast<uintptr_t>(grad) % eb || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      reinterpret_cast<uintptr_t>(t_val) % (t_val_dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(t_idx) % (t_idx_itype == DL_I64 ? 8 : 4))
+    return DL_ERR_ALIGN;
+  const RestShape sh = rest_shape(rest_chunks(logits_dtype, V));
+  if (sh.parts == 0 || (n_rows + 64) * sh.parts > 0x7fffffffLL) return DL_ERR_LIMIT;
+  if (sh.parts > 1 && (!workspace || workspace_bytes < RetryList::bytes(n_rows, sh.parts))) return DL_ERR_WORKSPACE;
+  RestParams p{logits, row_stride, n_rows, V, row_map, t_val, t_val_dtype, t_idx, t_idx_itype, K, n_teacher_rows, t_cnt, beta, inv_T, rest_min,
+               grad_scale, row_loss, grad, grad_stride, workspace, sh.parts, (flags & DL_TOPK_NO_WAIT) ? 0 : SPIN_LIMIT};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (logits_dtype == DL_F32) return launch_rest<TagF32>(p, sh, st);
+  if (logits_dtype == DL_BF16) return launch_rest<TagBF16>(p, sh, st);
+  return launch_rest<TagF16>(p, sh, st);
+}

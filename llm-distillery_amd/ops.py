@@ -153,6 +153,75 @@ def div_topk(kind: str, logits: torch.Tensor, t_val: torch.Tensor, t_idx: torch.
     return row_loss, grad
 
 
+def div_topk_rest(beta: float, logits: torch.Tensor, t_val: torch.Tensor, t_idx: torch.Tensor, *, row_map: torch.Tensor | None = None,
+                  t_cnt: torch.Tensor | None = None, T: float = 1.0, rest_min: float = 2.0 ** -14, grad_scale: float = 1.0,
+                  want_grad: bool = True, grad_out: torch.Tensor | None = None, no_wait: bool = False):
+    """Per-token generalised Jensen-Shannon divergence against a top-K teacher, with the rest of the vocabulary as one more outcome,
+    and in the same launch d(sum of row losses)/d(logits) * grad_scale.
+
+    `beta` = 0 is KL(teacher | student), 1 is KL(student | teacher), between them beta KL(P | M) + (1 - beta) KL(Q | M) with
+    M = beta P + (1 - beta) Q.  The teacher's rest has what its stored log-probs (of the whole vocabulary) leave of 1, at least
+    `rest_min`; the student's is the mass of all columns that are not listed.  For losses on what the student itself wrote, where a
+    student can leave the teacher's top K: `div_topk`, which renormalises over the K entries, does not see that.
+    Tensors as for `div_topk`, but `grad_out` must not share memory with the logits.  `no_wait` is the library's test hook
+    (DL_TOPK_NO_WAIT).  Returns (row_loss fp32 [rows], grad like logits or None)."""
+    _dev(logits, "logits")
+    x = _rows_2d(logits)
+    R, V = x.shape
+    dev = x.device
+    _dev(t_val, "t_val", dev), _dev(t_idx, "t_idx", dev)
+    if x.dtype not in _DT or t_val.dtype not in _DT or t_idx.dtype not in _IT:
+        raise RuntimeError("unsupported dtype")
+    if t_val.dim() != 2 or t_val.shape != t_idx.shape:
+        raise RuntimeError("t_val and t_idx must both be [N, K]")
+    if not 0.0 <= beta <= 1.0:
+        raise ValueError("beta must lie in [0, 1]")
+    if not 0.0 < rest_min < 1.0:
+        raise ValueError("rest_min must lie in (0, 1)")
+    if not T > 0.0:
+        raise ValueError("the temperature must be positive")
+    if R == 1 and x.stride(0) < V:
+        x = x.as_strided((1, V), (V, 1))                      # a single row's stride means nothing
+    t_val, t_idx = t_val.contiguous(), t_idx.contiguous()
+    N, K = t_val.shape
+    if row_map is None and N < R:
+        raise RuntimeError(f"{R} logits rows but only {N} teacher rows and no row_map")
+    _, rm_ptr = _opt_i32(row_map, R, "row_map", dev)
+    _, cnt_ptr = _opt_i32(t_cnt, N, "t_cnt", dev)
+    row_loss = torch.empty(R, dtype=torch.float32, device=dev)
+    grad, g_ptr, g_stride = None, 0, V
+    if want_grad:
+        grad = _grad_target(grad_out, R, V, x.dtype, dev, like=x)
+        if grad_out is not None and _share_memory(grad_out, x):
+            raise RuntimeError("grad_out must not share memory with the logits")
+        g_ptr, g_stride = grad.data_ptr(), _row_pitch(grad)
+    lib = _lib.load()
+    ws_bytes = lib.dl_div_topk_rest_workspace_bytes(_DT[x.dtype], R, V)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _on(dev):
+        st = lib.dl_div_topk_rest(beta, x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, rm_ptr, t_val.data_ptr(), _DT[t_val.dtype],
+                                  t_idx.data_ptr(), _IT[t_idx.dtype], K, N, cnt_ptr, 1.0 / T, rest_min, grad_scale,
+                                  row_loss.data_ptr(), g_ptr, g_stride, ws.data_ptr() if ws is not None else 0, ws_bytes,
+                                  _lib.DL_TOPK_NO_WAIT if no_wait else 0, _stream_ptr(dev))
+    _lib.check(st, "dl_div_topk_rest")
+    if grad is not None and logits.dim() != 2 and grad_out is None:
+        grad = grad.view(logits.shape)
+    return row_loss, grad
+
+
+def _row_pitch(t: torch.Tensor) -> int:
+    """The row stride of a matrix that is dense along its rows; its width where it has a single row (whose stride means nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two matrices, dense along their rows, overlap."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _row_pitch(t) + t.shape[1]) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
 def div_topk_static(kind: str, logits: torch.Tensor, t_val: torch.Tensor, t_idx: torch.Tensor, row_loss: torch.Tensor,
                     grad: torch.Tensor | None, *, row_map: torch.Tensor | None = None, t_cnt: torch.Tensor | None = None,
                     T: float = 1.0, teacher_T: float | None = None, grad_scale: float = 1.0, unique_ids: bool = False,
