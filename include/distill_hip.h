@@ -598,6 +598,28 @@ int dl_div_topk_rest(float beta, const void* logits, int logits_dtype, int64_t r
                      void* stream);
 
 /*
+ * 8-bit floating point (e4m3) with a scale for every block of 128 columns, and the product of two such matrices.
+ *
+ * dl_quantize_blocks: x [rows, cols] -> codes [rows, whole blocks] (zeros behind the last column), scales.  block_rows 1: a scale for
+ * every 128 values of a row, scales[r, kb]; 128: for every 128 x 128 values, scales[r / 128, kb] (element r * scale_row_stride + kb *
+ * scale_block_stride either way).  scale = max(largest magnitude / 448, 2^-100); code = x / scale, rounded to even.  NaN stays NaN; an
+ * infinity makes its block's scale infinite and itself NaN.
+ *
+ * dl_matmul_blocks: out[m, n] = sum over kb of a_scale[m, kb] * b_scale[n / 128, kb] * sum over the block's 128 columns of a[m, k] b[n, k],
+ * out [M, N] of out_dtype, rounded once.  K columns, in whole blocks whose tails hold zeros.  A block's products are summed inside the
+ * matrix unit, where the sum of 128 products is off by up to 2^-12 of the sum of their magnitudes (products far smaller than the
+ * largest are cut off); block sums are scaled and added in fp32.  Up to 64 rows take a kernel that reads the weights once.
+ *
+ * codes, a and b: 16-byte aligned, strides of whole 16 bytes, at least the whole blocks (DL_ERR_ALIGN, DL_ERR_SHAPE); x and out: any
+ * element-aligned address and stride.  Scale strides in elements, not negative.
+ */
+int dl_quantize_blocks(const void* x, int dtype, int64_t row_stride, int64_t rows, int64_t cols, int block_rows, void* codes,
+                       int64_t code_stride, float* scales, int64_t scale_row_stride, int64_t scale_block_stride, void* stream);
+int dl_matmul_blocks(const void* a, int64_t a_stride, const float* a_scale, int64_t a_scale_row, int64_t a_scale_block, int64_t M,
+                     const void* b, int64_t b_stride, const float* b_scale, int64_t b_scale_row, int64_t b_scale_block, int64_t N,
+                     int64_t K, void* out, int out_dtype, int64_t out_stride, void* stream);
+
+/*
  * Sampling: one token per row of logits [n_rows, V] from one given random number per row, `u` fp32 in [0, 1) (24 bits count;
  * values outside are brought in).
  * The tokens of a row are ordered by descending logit, equal logits by index.  With every fp32 operation rounded by itself,

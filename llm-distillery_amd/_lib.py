@@ -85,6 +85,9 @@ _SIGNATURES = {
     "dl_div_topk_rest_workspace_bytes": (c_int64, [c_int, c_int64, c_int64]),
     "dl_div_topk_rest": (c_int, [c_float, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int, _P, c_int, c_int, c_int64, _P,
                                  c_float, c_float, c_float, _P, _P, c_int64, _P, c_int64, c_int, _P]),
+    "dl_quantize_blocks": (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, c_int64, _P]),
+    "dl_matmul_blocks": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int64, _P,
+                                 c_int, c_int64, _P]),
     "dl_sample_rows": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, _P, _P, _P, c_float, c_int, c_float, c_float, _P, _P,
                                _P, _P]),
     "dl_embed_rows": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int, c_int64, c_float, _P, c_int64, _P]),

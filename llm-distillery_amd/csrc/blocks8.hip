@@ -1,0 +1,385 @@
+// Matrix product in 8-bit floating point (e4m3) with a scale for every block of 128, and what makes its operands.
+//
+//   out[m, n] = sum over blocks kb of  sa[m, kb] * sb[n / 128, kb] * sum over the 128 columns k of kb of a[m, k] * b[n, k]
+//
+// a: one scale for every 128 values of a row (activations, quantised on the way); b: one for every 128 x 128 weights.
+// One matrix instruction sums a whole block: v_mfma_f32_16x16x128_f8f6f4 takes 16 x 128 by 128 x 16 values, so a block's sum
+// leaves the matrix unit once and is scaled and added in fp32 on the vector unit, four multiply-adds per lane beside 32
+// cycles of the matrix unit.  The operands are passed with b first: a lane then holds four neighbouring columns n of one
+// row m, one scale product serves all four, and the result is stored in pieces of four.
+// Any order of the 128 values will do as long as both operands have the same one: a lane's 32 bytes are two 16-byte
+// pieces, 64 bytes apart, so that every load instruction covers 64 contiguous bytes of a row.
+#include "distill_common.hpp"
+#include "distill_hip.h"
+
+#include <algorithm>
+
+namespace dl {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int QB = 128;                       // values that share a scale; bytes of a block of a row
+constexpr float QMAX = 448.f, QSCALE_MIN = 0x1p-100f;
+
+// ---- quantise ---------------------------------------------------------------------------------------
+// scale = max(largest magnitude / 448, 2^-100), code = x / scale rounded to e4m3 (ties to even): both divisions are IEEE ones.
+// Columns behind the last one are zeros, up to the end of the block.  NaN stays NaN; a block with an infinity has an infinite
+// scale and NaN in the infinity's place.
+template <class Tag>
+__device__ __forceinline__ void load_eight(const char* row, int64_t col, int64_t cols, float* f) {
+  if (col + 8 <= cols) {
+    if constexpr (Tag::bytes == 2) {
+      Chunk<Tag>::unpack(load16_unaligned(row + col * 2), f);
+    } else {
+      Chunk<Tag>::unpack(load16_unaligned(row + col * 4), f);
+      Chunk<Tag>::unpack(load16_unaligned(row + col * 4 + 16), f + 4);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = col + e < cols ? load_as_float(row, Tag::id, col + e) : 0.f;
+  }
+}
+__device__ __forceinline__ float largest_of_eight(const float* f) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
+  return m;
+}
+__device__ __forceinline__ u32x2 code_eight(const float* f, float scale) {
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = f[e] / scale;
+  u32x2 c;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], v, true);
+    c[i] = (unsigned)v;
+  }
+  return c;
+}
+struct QuantParams {
+  const char* x; int64_t row_stride, rows, cols, blocks;
+  unsigned char* codes; int64_t code_stride;
+  float* scales; int64_t scale_row, scale_block;
+};
+// One scale per row and block: 16 threads a block, one workgroup sixteen blocks of a row.
+template <class Tag>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantParams p) {
+  const int64_t r = blockIdx.y, kb = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int t = threadIdx.x % 16;
+  if (kb >= p.blocks) return;
+  const int64_t col = kb * QB + t * 8;
+  for (int64_t row = r; row < p.rows; row += gridDim.y) {
+    float f[8];
+    load_eight<Tag>(p.x + row * p.row_stride * Tag::bytes, col, p.cols, f);
+    float m = largest_of_eight(f);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
+    const float scale = fmaxf(m / QMAX, QSCALE_MIN);
+    *reinterpret_cast<u32x2*>(p.codes + row * p.code_stride + col) = code_eight(f, scale);
+    if (t == 0) p.scales[row * p.scale_row + kb * p.scale_block] = scale;
+  }
+}
+// One scale per 128 x 128: a workgroup a block, the values in its registers between the maximum and the codes.
+template <class Tag>
+__global__ __launch_bounds__(256) void quantize_squares_kernel(const QuantParams p) {
+  __shared__ float red[4];
+  const int64_t kb = blockIdx.x, row0 = (int64_t)blockIdx.y * QB, col = kb * QB + (threadIdx.x % 16) * 8;
+  float f[8][8], m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = row0 + i * 16 + threadIdx.x / 16;
+    if (row < p.rows) load_eight<Tag>(p.x + row * p.row_stride * Tag::bytes, col, p.cols, f[i]);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+    m = fmaxf(m, largest_of_eight(f[i]));
+  }
+  m = block_max<256>(m, red);
+  const float scale = fmaxf(m / QMAX, QSCALE_MIN);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = row0 + i * 16 + threadIdx.x / 16;
+    if (row < p.rows) *reinterpret_cast<u32x2*>(p.codes + row * p.code_stride + col) = code_eight(f[i], scale);
+  }
+  if (threadIdx.x == 0) p.scales[blockIdx.y * p.scale_row + kb * p.scale_block] = scale;
+}
+
+// ---- product ----------------------------------------------------------------------------------------
+struct BlocksParams {
+  const unsigned char* a; int64_t a_stride; const float* sa; int64_t sa_row, sa_block; int64_t M;
+  const unsigned char* b; int64_t b_stride; const float* sb; int64_t sb_row, sb_block; int64_t N;
+  int blocks;
+  char* out; int64_t out_stride;
+};
+__device__ __forceinline__ f32x4 block_product(const i32x8& b, const i32x8& a) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);      // e4m3 both, unscaled
+}
+__device__ __forceinline__ i32x8 join_pieces(const u32x4& lo, const u32x4& hi) {
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+// Four neighbouring columns of a row, as far as it reaches.
+template <class Tag>
+__device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, const f32x4& v) {
+  if (n + 4 <= N) {
+    if constexpr (Tag::bytes == 4) {
+      store16_unaligned(row + n * 4, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+    } else {
+      const float f[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+      const u32x4 c = Chunk<Tag>::pack(f);
+      const u32x2 two = {c[0], c[1]};
+      __builtin_memcpy(row + n * 2, &two, 8);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < N) store_from_float(row, Tag::id, n + i, v[i]);
+  }
+}
+
+// Few rows: the weights stream from memory straight into the matrix instructions' operands.  A workgroup's four waves
+// take every fourth block of the same 16 * NT columns (together they read 512 contiguous bytes of each row) and add up in LDS, in
+// the order of the waves.  MT tiles of 16 rows; rows behind the last are read as the last and not stored.
+template <class Tag, int MT, int NT>
+__global__ __launch_bounds__(256) void few_rows_kernel(const BlocksParams p) {
+  __shared__ float part[4][MT * 16][NT * 16 + 1];
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, g = lane / 16;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+  const unsigned char* bp[NT];
+  const float* sbp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    bp[j] = p.b + min(n0 + j * 16 + i16, p.N - 1) * p.b_stride + g * 16;
+    sbp[j] = p.sb + min(n0 + j * 16, p.N - 1) / QB * p.sb_row;
+  }
+  const unsigned char* ap[MT];
+  const float* sap[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = min((int64_t)i * 16 + i16, p.M - 1);
+    ap[i] = p.a + m * p.a_stride + g * 16;
+    sap[i] = p.sa + m * p.sa_row;
+  }
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int kb = w; kb < p.blocks; kb += 4) {
+    i32x8 b[NT], a[MT];
+    float sb[NT], sa[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      b[j] = join_pieces(load16_stream(bp[j] + (int64_t)kb * QB), load16_stream(bp[j] + (int64_t)kb * QB + 64));
+      sb[j] = sbp[j][kb * p.sb_block];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      a[i] = join_pieces(*reinterpret_cast<const u32x4*>(ap[i] + (int64_t)kb * QB), *reinterpret_cast<const u32x4*>(ap[i] + (int64_t)kb * QB + 64));
+      sa[i] = sap[i][kb * p.sa_block];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const f32x4 v = block_product(b[j], a[i]);
+        const float s = sa[i] * sb[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(v[e], s, acc[i][j][e]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[w][i * 16 + i16][j * 16 + g * 4 + e] = acc[i][j][e];
+  __syncthreads();
+  constexpr int QUADS = NT * 4;
+  for (int q = threadIdx.x; q < MT * 16 * QUADS; q += 256) {
+    const int m = q / QUADS, n = q % QUADS * 4;
+    if (m >= p.M) break;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = part[0][m][n + e] + part[1][m][n + e] + part[2][m][n + e] + part[3][m][n + e];
+    if (n0 + n < p.N) store_four<Tag>(p.out + (int64_t)m * p.out_stride * Tag::bytes, n0 + n, p.N, v);
+  }
+}
+
+// Many rows: tiles of BM x BN, a wave WM x WN of it; one block of 128 columns per step, fetched into LDS by loads that bypass the
+// registers while the step before is computed.  A row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted by
+// piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS
+// in lane order, so it is their source addresses that are permuted.)
+typedef const unsigned __attribute__((address_space(1))) * global_words;
+typedef unsigned __attribute__((address_space(3))) * lds_words;
+template <int ROWS, int WAVES>
+__device__ __forceinline__ void fetch_tile(const unsigned char* base, int64_t stride, int64_t row0, int64_t rows, int64_t byte0, unsigned char* lds) {
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+#pragma unroll
+  for (int i = 0; i < ROWS / 8 / WAVES; ++i) {
+    const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+    const unsigned char* src = base + min(row0 + row, rows - 1) * stride + byte0 + piece * 16;
+    __builtin_amdgcn_global_load_lds((global_words)src, (lds_words)(lds + (i * WAVES + w) * 1024), 16, 0, 0);
+  }
+}
+__device__ __forceinline__ i32x8 tile_operand(const unsigned char* lds, int row0) {
+  const int lane = threadIdx.x & (WAVE - 1), row = row0 + lane % 16, at = row * QB + ((lane / 16) ^ ((row >> 1) & 7)) * 16;
+  return join_pieces(*reinterpret_cast<const u32x4*>(lds + at), *reinterpret_cast<const u32x4*>(lds + (at ^ 64)));
+}
+
+template <class Tag, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(const BlocksParams p, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16;
+  static_assert(WN <= QB && QB % WN == 0, "a wave's columns share their scales");
+  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows) of 128 bytes
+  constexpr int STEP = (BM + BN) * QB;
+  // Consecutive workgroups go round the 8 XCDs: each takes a contiguous eighth of the tiles, in bands of 8 rows of tiles, so
+  // that the tiles an XCD works on at a time share their operands in its L2.
+  const unsigned total = tiles_m * tiles_n, b = blockIdx.x;
+  const unsigned t = (b & 7u) * (gridDim.x >> 3) + (b >> 3);
+  if (t >= total) return;
+  const unsigned band = t / (8u * tiles_n), high = min(8u, tiles_m - band * 8u), in = t - band * 8u * tiles_n;
+  const int64_t m0 = (int64_t)(band * 8u + in % high) * BM, n0 = (int64_t)(in / high) * BN;
+
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, g = lane / 16;
+  const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
+  const float* sbp = p.sb + min(n0 + wn, p.N - 1) / QB * p.sb_row;
+  const float* sap[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sap[i] = p.sa + min(m0 + wm + i * 16 + i16, p.M - 1) * p.sa_row;
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  fetch_tile<BM, WAVES>(p.a, p.a_stride, m0, p.M, 0, lds);
+  fetch_tile<BN, WAVES>(p.b, p.b_stride, n0, p.N, 0, lds + BM * QB);
+  float sa[TM], sb = sbp[0];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sa[i] = sap[i][0];
+  for (int kb = 0; kb < p.blocks; ++kb) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                                          // the step's tiles are there, and everyone is done with the other's
+    const unsigned char* at = lds + (kb & 1) * STEP;
+    float s[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) s[i] = sa[i] * sb;
+    if (kb + 1 < p.blocks) {
+      unsigned char* next = lds + ((kb + 1) & 1) * STEP;
+      fetch_tile<BM, WAVES>(p.a, p.a_stride, m0, p.M, (int64_t)(kb + 1) * QB, next);
+      fetch_tile<BN, WAVES>(p.b, p.b_stride, n0, p.N, (int64_t)(kb + 1) * QB, next + BM * QB);
+      sb = sbp[(kb + 1) * p.sb_block];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) sa[i] = sap[i][(kb + 1) * p.sa_block];
+    }
+    i32x8 bf[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) bf[j] = tile_operand(at + BM * QB, wn + j * 16);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const i32x8 af = tile_operand(at, wm + i * 16);
+      f32x4 v[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) v[j] = block_product(bf[j], af);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(v[j][e], s[i], acc[i][j][e]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t m = m0 + wm + i * 16 + i16;
+    if (m >= p.M) continue;
+    char* row = p.out + m * p.out_stride * Tag::bytes;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int64_t n = n0 + wn + j * 16 + g * 4;
+      if (n < p.N) store_four<Tag>(row, n, p.N, acc[i][j]);
+    }
+  }
+}
+
+static int blocks_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH; }
+
+template <class Tag, int BM, int BN, int WM, int WN>
+static int launch_tiles(const BlocksParams& p, hipStream_t st) {
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * (BM + BN) * QB;
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+  if (tm * tn > 0x7ffffff0LL) return DL_ERR_LIMIT;
+  if (bytes > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&tile_kernel<Tag, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return DL_ERR_LAUNCH;
+  hipLaunchKernelGGL((tile_kernel<Tag, BM, BN, WM, WN>), dim3((unsigned)((tm * tn + 7) / 8 * 8)), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
+  return blocks_status();
+}
+
+template <class Tag>
+static int launch_blocks(const BlocksParams& p, hipStream_t st) {
+  if (p.M <= 64) {
+    const dim3 grid((unsigned)((p.N + 31) / 32)), nt(256);
+    if (p.M <= 16) hipLaunchKernelGGL((few_rows_kernel<Tag, 1, 2>), grid, nt, 0, st, p);
+    else if (p.M <= 32) hipLaunchKernelGGL((few_rows_kernel<Tag, 2, 2>), grid, nt, 0, st, p);
+    else hipLaunchKernelGGL((few_rows_kernel<Tag, 4, 2>), grid, nt, 0, st, p);
+    return blocks_status();
+  }
+  if ((p.M + 255) / 256 * ((p.N + 255) / 256) >= 256) return launch_tiles<Tag, 256, 256, 128, 64>(p, st);
+  if ((p.M + 127) / 128 * ((p.N + 127) / 128) >= 256) return launch_tiles<Tag, 128, 128, 64, 64>(p, st);
+  return launch_tiles<Tag, 64, 64, 32, 32>(p, st);
+}
+
+}  // namespace dl
+
+extern "C" int dl_quantize_blocks(const void* x, int dtype, int64_t row_stride, int64_t rows, int64_t cols, int block_rows, void* codes,
+                                  int64_t code_stride, float* scales, int64_t scale_row_stride, int64_t scale_block_stride, void* stream) {
+  using namespace dl;
+  if ((unsigned)dtype > DL_F16) return DL_ERR_DTYPE;
+  const int64_t blocks = (cols + QB - 1) / QB;
+  if (rows < 0 || cols < 0 || row_stride < cols || code_stride < blocks * QB || (block_rows != 1 && block_rows != QB) || scale_row_stride < 0 ||
+      scale_block_stride < 0)
+    return DL_ERR_SHAPE;
+  if (rows == 0 || cols == 0) return DL_OK;
+  if (!x || !codes || !scales) return DL_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(codes) % 16 || code_stride % 16 ||
+      reinterpret_cast<uintptr_t>(scales) % 4)
+    return DL_ERR_ALIGN;
+  if (blocks > 0x7fffffffLL || (block_rows == QB && (rows + QB - 1) / QB > 65535)) return DL_ERR_LIMIT;
+  const QuantParams p{reinterpret_cast<const char*>(x), row_stride, rows, cols, blocks, reinterpret_cast<unsigned char*>(codes), code_stride,
+                      scales, scale_row_stride, scale_block_stride};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 rows_grid((unsigned)((blocks + 15) / 16), (unsigned)std::min<int64_t>(rows, 65535)), squares_grid((unsigned)blocks, (unsigned)((rows + QB - 1) / QB));
+#define DL_QUANTIZE(TAG)                                                                              \
+  if (block_rows == 1) hipLaunchKernelGGL(quantize_rows_kernel<TAG>, rows_grid, dim3(256), 0, st, p); \
+  else hipLaunchKernelGGL(quantize_squares_kernel<TAG>, squares_grid, dim3(256), 0, st, p);
+  if (dtype == DL_F32) { DL_QUANTIZE(TagF32) } else if (dtype == DL_BF16) { DL_QUANTIZE(TagBF16) } else { DL_QUANTIZE(TagF16) }
+#undef DL_QUANTIZE
+  return blocks_status();
+}
+
+extern "C" int dl_matmul_blocks(const void* a, int64_t a_stride, const float* a_scale, int64_t a_scale_row, int64_t a_scale_block, int64_t M,
+                                const void* b, int64_t b_stride, const float* b_scale, int64_t b_scale_row, int64_t b_scale_block, int64_t N,
+                                int64_t K, void* out, int out_dtype, int64_t out_stride, void* stream) {
+  using namespace dl;
+  if ((unsigned)out_dtype > DL_F16) return DL_ERR_DTYPE;
+  const int64_t blocks = (K + QB - 1) / QB;
+  if (M < 0 || N < 0 || K <= 0 || a_stride < blocks * QB || b_stride < blocks * QB || out_stride < N || a_scale_row < 0 || a_scale_block < 0 ||
+      b_scale_row < 0 || b_scale_block < 0)
+    return DL_ERR_SHAPE;
+  if (M == 0 || N == 0) return DL_OK;
+  if (!a || !b || !a_scale || !b_scale || !out) return DL_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 16 || a_stride % 16 || b_stride % 16 ||
+      (reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) % 4 || reinterpret_cast<uintptr_t>(out) % (out_dtype == DL_F32 ? 4 : 2))
+    return DL_ERR_ALIGN;
+  if (blocks > 0xffffff || (N + 31) / 32 > 0x7fffffffLL) return DL_ERR_LIMIT;
+  const BlocksParams p{reinterpret_cast<const unsigned char*>(a), a_stride, a_scale, a_scale_row, a_scale_block, M,
+                       reinterpret_cast<const unsigned char*>(b), b_stride, b_scale, b_scale_row, b_scale_block, N, (int)blocks,
+                       reinterpret_cast<char*>(out), out_stride};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (out_dtype == DL_F32) return launch_blocks<TagF32>(p, st);
+  if (out_dtype == DL_BF16) return launch_blocks<TagBF16>(p, st);
+  return launch_blocks<TagF16>(p, st);
+}

@@ -69,3 +69,86 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[flo
     _lib.check(st, "dl_sample_rows")
     shape = logits.shape[:-1]
     return tokens.view(shape), logp.view(shape), kept.view(shape)
+
+
+class BlockQuantized(NamedTuple):
+    """A matrix [rows, width] held in 8-bit floating point (e4m3): `codes` [rows, width rounded up to whole blocks of 128] with zeros
+    behind the last column, and `scales` fp32 [rows or row blocks of 128, column blocks]; an element is its code times its scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    width: int
+
+    def dequantize(self) -> torch.Tensor:
+        """The matrix in fp32 (plain torch; for looking at it)."""
+        rows = self.codes.shape[0]
+        s = self.scales if self.scales.shape[0] == rows else self.scales.repeat_interleave(128, 0)[:rows]
+        return (self.codes.float() * s.repeat_interleave(128, 1))[:, :self.width]
+
+
+def _blocks(n: int) -> int:
+    return -(-n // 128)
+
+
+def quantize_blocks(x: torch.Tensor, *, rows: int = 1) -> BlockQuantized:
+    """x [..., width] (bf16/fp16/fp32, rows evenly strided) in 8-bit floating point with one scale for every 128 values of a row
+    (`rows` = 1: activations) or for every 128 x 128 values (`rows` = 128: weights, laid out once).
+
+    A block's scale is its largest magnitude / 448, at least 2^-100; codes are the values over the scale, rounded to even."""
+    _dev(x, "x")
+    if rows not in (1, 128):
+        raise ValueError("rows must be 1 or 128")
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    v = _rows_2d(x)
+    if v.dtype not in _DT:
+        raise RuntimeError("unsupported dtype")
+    R, W = v.shape
+    dev = v.device
+    kb = _blocks(W)
+    codes = torch.empty((R, kb * 128), dtype=torch.float8_e4m3fn, device=dev)
+    if rows == 1:
+        scales = torch.empty((kb, R), dtype=torch.float32, device=dev).t()      # the scales of a block of columns side by side
+    else:
+        scales = torch.empty((_blocks(R), kb), dtype=torch.float32, device=dev)
+    if R and W:
+        with _on(dev):
+            st = _lib.load().dl_quantize_blocks(v.data_ptr(), _DT[v.dtype], _row_pitch(v), R, W, rows, codes.data_ptr(), kb * 128,
+                                                scales.data_ptr(), scales.stride(0), scales.stride(1), _stream_ptr(dev))
+        _lib.check(st, "dl_quantize_blocks")
+    return BlockQuantized(codes, scales, W)
+
+
+def _check_blocks(q: BlockQuantized, name: str, groups: int, dev: torch.device) -> None:
+    _dev(q.codes, f"{name}.codes", dev), _dev(q.scales, f"{name}.scales", dev)
+    if q.codes.dtype != torch.float8_e4m3fn or q.codes.dim() != 2 or q.codes.shape[1] != _blocks(q.width) * 128 or \
+            (q.codes.numel() and (q.codes.stride(1) != 1 or q.codes.shape[0] > 1 and q.codes.stride(0) < q.codes.shape[1])):
+        raise RuntimeError(f"{name}.codes must be a float8_e4m3fn matrix of whole blocks of 128 columns, dense along its rows")
+    if q.scales.dtype != torch.float32 or tuple(q.scales.shape) != (groups, _blocks(q.width)):
+        raise RuntimeError(f"{name}.scales must be fp32 [{groups}, {_blocks(q.width)}], not {tuple(q.scales.shape)}")
+
+
+def matmul_blocks(a: BlockQuantized, b: BlockQuantized, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [M, width] times the transpose of b [N, width], both in 8-bit floating point: [M, N] in `dtype` (bf16/fp16/fp32).
+
+    `a` has a scale for every 128 values of a row, `b` for every 128 x 128 (`quantize_blocks` with rows = 1 and 128).  A block's
+    128 products are summed by the matrix unit, the scaled sums of the blocks in fp32, and the result is rounded once.  For up to 64
+    rows the weights stream through the card once; their result does not depend on what other rows there are."""
+    dev = a.codes.device
+    if dtype not in _DT:
+        raise RuntimeError("unsupported dtype")
+    M, N = a.codes.shape[0], b.codes.shape[0]
+    if a.width != b.width:
+        raise RuntimeError(f"a has {a.width} columns, b {b.width}")
+    _dev(a.codes, "a.codes")
+    _check_blocks(a, "a", M, dev)
+    _check_blocks(b, "b", _blocks(N), dev)
+    if a.width == 0:
+        raise RuntimeError("the rows have no columns")
+    out = torch.empty((M, N), dtype=dtype, device=dev)
+    if M and N:
+        with _on(dev):
+            st = _lib.load().dl_matmul_blocks(a.codes.data_ptr(), _row_pitch(a.codes), a.scales.data_ptr(), a.scales.stride(0), a.scales.stride(1), M,
+                                              b.codes.data_ptr(), _row_pitch(b.codes), b.scales.data_ptr(), b.scales.stride(0), b.scales.stride(1), N,
+                                              a.width, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
+        _lib.check(st, "dl_matmul_blocks")
+    return out
