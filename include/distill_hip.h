@@ -602,7 +602,8 @@ int dl_div_topk_rest(float beta, const void* logits, int logits_dtype, int64_t r
  *
  * dl_quantize_blocks: x [rows, cols] -> codes [rows, whole blocks] (zeros behind the last column), scales.  block_rows 1: a scale for
  * every 128 values of a row, scales[r, kb]; 128: for every 128 x 128 values, scales[r / 128, kb] (element r * scale_row_stride + kb *
- * scale_block_stride either way).  scale = max(largest magnitude / 448, 2^-100); code = x / scale, rounded to even.  NaN stays NaN; an
+ * scale_block_stride either way).  scale = max(largest magnitude * r, 2^-100) with r = 1 / 448 in
+ * fp32; code = x / scale, rounded to even.  NaN stays NaN; an
  * infinity makes its block's scale infinite and itself NaN.
  *
  * dl_matmul_blocks: out[m, n] = sum over kb of a_scale[m, kb] * b_scale[n / 128, kb] * sum over the block's 128 columns of a[m, k] b[n, k],

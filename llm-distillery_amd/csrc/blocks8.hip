@@ -20,10 +20,10 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int QB = 128;                       // values that share a scale; bytes of a block of a row
-constexpr float QMAX = 448.f, QSCALE_MIN = 0x1p-100f;
+constexpr float QSCALE = 1.f / 448.f, QSCALE_MIN = 0x1p-100f;
 
 // ---- quantise ---------------------------------------------------------------------------------------
-// scale = max(largest magnitude / 448, 2^-100), code = x / scale rounded to e4m3 (ties to even): both divisions are IEEE ones.
+// scale = max(largest magnitude * (1 / 448 in fp32), 2^-100), code = x / scale (an IEEE division) rounded to e4m3, ties to even.
 // Columns behind the last one are zeros, up to the end of the block.  NaN stays NaN; a block with an infinity has an infinite
 // scale and NaN in the infinity's place.
 template <class Tag>
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantParams p)
     float m = largest_of_eight(f);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
-    const float scale = fmaxf(m / QMAX, QSCALE_MIN);
+    const float scale = fmaxf(m * QSCALE, QSCALE_MIN);
     *reinterpret_cast<u32x2*>(p.codes + row * p.code_stride + col) = code_eight(f, scale);
     if (t == 0) p.scales[row * p.scale_row + kb * p.scale_block] = scale;
   }
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void quantize_squares_kernel(const QuantParams
     m = fmaxf(m, largest_of_eight(f[i]));
   }
   m = block_max<256>(m, red);
-  const float scale = fmaxf(m / QMAX, QSCALE_MIN);
+  const float scale = fmaxf(m * QSCALE, QSCALE_MIN);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = row0 + i * 16 + threadIdx.x / 16;

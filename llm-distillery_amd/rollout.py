@@ -93,7 +93,7 @@ def quantize_blocks(x: torch.Tensor, *, rows: int = 1) -> BlockQuantized:
     """x [..., width] (bf16/fp16/fp32, rows evenly strided) in 8-bit floating point with one scale for every 128 values of a row
     (`rows` = 1: activations) or for every 128 x 128 values (`rows` = 128: weights, laid out once).
 
-    A block's scale is its largest magnitude / 448, at least 2^-100; codes are the values over the scale, rounded to even."""
+    A block's scale is its largest magnitude times 1 / 448 (in fp32), at least 2^-100; codes are the values over the scale, rounded to even."""
     _dev(x, "x")
     if rows not in (1, 128):
         raise ValueError("rows must be 1 or 128")

@@ -30,7 +30,7 @@ def quantised(x, rows):
     full = torch.zeros(g * rows, kb * 128)
     full[:R, :W] = x.float()
     t = full.view(g, rows, kb, 128)
-    scales = torch.maximum(t.abs().amax((1, 3)) / torch.tensor(448.0), torch.tensor(2.0 ** -100))
+    scales = torch.maximum(t.abs().amax((1, 3)) * (torch.tensor(1.0) / torch.tensor(448.0)), torch.tensor(2.0 ** -100))
     return e4m3(t / scales[:, None, :, None]).view(g * rows, kb * 128)[:R], scales
 
 
