@@ -657,10 +657,10 @@ int dl_embed_rows(const void* table, int dtype, int64_t table_stride, int64_t vo
  *   grad[v, :] = round(scale * sum over {n : tokens[n] == v} of g[n, :]  (+ grad[v, :] if `accumulate`))
  * g [n_tokens, width] (row stride `g_stride`) of `dtype`, grad [vocab, width] (`grad_stride`) of the same dtype or fp32.
  * Without `accumulate` every row of grad is written (zeros where no token names it); with it only rows that some token names.
- * Tokens outside [0, vocab) are left out.  The rows of a token are summed in fp32 in ascending order of n (in runs of 32
- * sorted tokens, the runs' sums then in order): no atomics, the same bits on every call.
+ * Tokens outside [0, vocab) are left out.  The rows of a token are summed in fp32 in ascending order of n (in runs of 4 to
+ * 32 sorted tokens, the runs' sums then in order): no atomics, the same bits on every call.
  * workspace  at least dl_embed_grad_workspace_bytes(...) bytes on a 256-byte boundary, contents irrelevant; two calls that may
- *            overlap in time must not share it.  About 16 bytes per token + width / 4 bytes per token.
+ *            overlap in time must not share it.  16 bytes per token, 256 KiB, and width / 4 bytes per token (up to 2 * width for few tokens).
  */
 int64_t dl_embed_grad_workspace_bytes(int64_t n_tokens, int64_t width);
 int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t n_tokens, int64_t width, const void* tokens, int itype,

@@ -90,20 +90,21 @@ __device__ __forceinline__ unsigned long long token_word(const void* tokens, int
 }
 
 constexpr int SORT_SMALL = 1024;      // tokens one workgroup sorts in registers
-__global__ __launch_bounds__(1024) void embed_sort_small_kernel(const void* __restrict__ tokens, int itype, int n, int64_t vocab,
-                                                                unsigned long long* __restrict__ sorted, ZeroShare z) {
+template <int NT>
+__global__ __launch_bounds__(NT) void embed_sort_small_kernel(const void* __restrict__ tokens, int itype, int n, int64_t vocab,
+                                                              unsigned long long* __restrict__ sorted, ZeroShare z) {
   if (blockIdx.x > 0) return zero_rows(z, blockIdx.x - 1);
-  __shared__ unsigned long long xch[SORT_SMALL];
+  __shared__ unsigned long long xch[NT];
   unsigned long long w[1] = {~0ull};
   if ((int)threadIdx.x < n) w[0] = token_word(tokens, itype, threadIdx.x, vocab);
-  block_sort<unsigned long long, 1024, 1>(w, xch);
+  block_sort<unsigned long long, NT, 1>(w, xch);
   if ((int)threadIdx.x < n) sorted[threadIdx.x] = w[0];
 }
 
 // Longer lists: a stable sort by digits of `bits` bits, lowest first (two of them up to a million ids).  A pass counts
 // each workgroup's digits in one launch and deals its words out in the next, where every workgroup adds up the counts
 // ahead of it itself: at most SORT_BLOCKS of them.
-constexpr int SORT_NT = 256, SORT_WAVES = SORT_NT / WAVE, SORT_BINS = 1024, SORT_BLOCKS = 64;
+constexpr int SORT_NT = 256, SORT_WAVES = SORT_NT / WAVE, SORT_BINS = 1024, SORT_BLOCKS = 64, SORT_LEAST = 512;      // words a workgroup has at least
 struct SortPass {
   const void* tokens; int itype; int64_t vocab;      // the first pass makes its words from the tokens
   const unsigned long long* in;                      // the later ones read them (NULL: the first)
@@ -134,24 +135,29 @@ __global__ __launch_bounds__(SORT_NT) void embed_sort_deal_kernel(const SortPass
   __shared__ unsigned place[SORT_WAVES][SORT_BINS];      // counts, then the next free place, of a wave's words with a digit
   __shared__ unsigned wave_total[SORT_WAVES];
   const int bins = 1 << s.bits, tid = threadIdx.x, lane = tid & (WAVE - 1), w = tid / WAVE;
-  constexpr int EACH = SORT_BINS / SORT_NT;
+  constexpr int EACH = SORT_BINS / SORT_NT;              // (4: a pass has at least that many bins)
+  static_assert(EACH == 4, "one 16-byte load per workgroup's counts");
   // this thread's digits tid * EACH ..: words of all workgroups, words of the workgroups ahead
   unsigned all[EACH], ahead[EACH], mine = 0u;
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
     all[j] = ahead[j] = 0u;
-    const int d = tid * EACH + j;
-    if (d < bins)
-      for (unsigned b = 0; b < s.blocks; ++b) {
-        const unsigned c = s.counts[(int64_t)b * bins + d];
-        all[j] += c;
-        if (b < blockIdx.x) ahead[j] += c;
-      }
-    mine += all[j];
 #pragma unroll
-    for (int k = 0; k < SORT_WAVES; ++k)
-      if (d < SORT_BINS) place[k][d] = 0u;
+    for (int k = 0; k < SORT_WAVES; ++k) place[k][tid * EACH + j] = 0u;
   }
+  if (tid * EACH < bins) {
+#pragma unroll 8
+    for (unsigned b = 0; b < s.blocks; ++b) {
+      const u32x4 c = *reinterpret_cast<const u32x4*>(s.counts + (int64_t)b * bins + tid * EACH);
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        all[j] += c[j];
+        ahead[j] += b < blockIdx.x ? c[j] : 0u;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) mine += all[j];
   unsigned before = mine;                                // exclusive sum over the threads
 #pragma unroll
   for (int o = 1; o < WAVE; o <<= 1) {
@@ -199,82 +205,101 @@ __global__ __launch_bounds__(SORT_NT) void embed_sort_deal_kernel(const SortPass
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------
-constexpr int SUM_NT = 256, SUM_TILE = 32, SUM_AHEAD = 8;
+// Sorted words are cut into tiles of 32, or as few as 4 where that would leave most of the card idle (the depth of a tile is a chain
+// of dependent memory round trips: 131 tokens x 1024 columns take 5 us with tiles of 4, 17 with 32).
+constexpr int SUM_NT = 128, SUM_TILE_MOST = 32, SUM_TILE_LEAST = 4, SUM_AHEAD = 8;
+static int sum_tile(int64_t n, int64_t width) {
+  int tile = SUM_TILE_MOST;
+  while (tile > SUM_TILE_LEAST && n * width < (int64_t)tile << 20) tile /= 2;
+  return tile;
+}
 struct SumParams {
   const unsigned long long* sorted; int64_t n, vocab, width;
   const char* g; int64_t g_stride;
   char* grad; int64_t grad_stride;
   float* partial;                  // [tiles][2][width]: the sum of a tile's first token (if it began earlier), of its last (if it goes on)
-  float scale; unsigned slices;
+  float scale; unsigned slices; int tile;
 };
 __device__ __forceinline__ unsigned word_token(unsigned long long w) { return (unsigned)(w >> 32); }
 
+// n of the Chunk<Tag>::N columns from `col` on, zeros behind.
 template <class Tag>
-__device__ __forceinline__ void load_columns(const char* row, int64_t col, int n, float* f) {      // n of Chunk<Tag>::N columns, zeros behind
+__device__ __forceinline__ u32x4 load_columns(const char* row, int64_t col, int n) {
+  const char* at = row + col * Tag::bytes;
+  if (n == Chunk<Tag>::N) return load16_unaligned(at);
+  u32x4 v{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < Chunk<Tag>::N; ++e)
+    if (e < n) {
+      if constexpr (Tag::bytes == 4) v[e] = reinterpret_cast<const unsigned*>(at)[e];
+      else v[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(at)[e] << (16 * (e & 1));
+    }
+  return v;
+}
+template <class Tag>
+__device__ __forceinline__ void store_columns(char* row, int64_t col, int n, const float* f) {
   if (n == Chunk<Tag>::N) {
-    Chunk<Tag>::unpack(load16_unaligned(row + col * Tag::bytes), f);
+    store16_stream_any(row + col * Tag::bytes, Chunk<Tag>::pack(f));
   } else {
 #pragma unroll
-    for (int e = 0; e < Chunk<Tag>::N; ++e) f[e] = e < n ? load_as_float(row, Tag::id, col + e) : 0.f;
-  }
-}
-// The N sums of columns [col, col + n) to the gradient's row, `scale` times, onto what it holds where ADD.
-template <class TagO, int N, bool ADD>
-__device__ __forceinline__ void store_sum(char* row, int64_t col, int n, float scale, const float* sum) {
-  using C = Chunk<TagO>;
-#pragma unroll
-  for (int k = 0; k < N / C::N; ++k) {
-    const int have = min(max(n - k * C::N, 0), C::N);
-    float old[C::N], f[C::N];
-    if (ADD) load_columns<TagO>(row, col + k * C::N, have, old);
-#pragma unroll
-    for (int e = 0; e < C::N; ++e) f[e] = ADD ? fmaf(scale, sum[k * C::N + e], old[e]) : scale * sum[k * C::N + e];
-    if (have == C::N) {
-      store16_stream_any(row + (col + k * C::N) * TagO::bytes, C::pack(f));
-    } else {
-#pragma unroll
-      for (int e = 0; e < C::N; ++e)
-        if (e < have) store_from_float(row, TagO::id, col + k * C::N + e, f[e]);
-    }
+    for (int e = 0; e < Chunk<Tag>::N; ++e)
+      if (e < n) store_from_float(row, Tag::id, col + e, f[e]);
   }
 }
 
 template <class Tag, class TagO, bool ADD>
 __global__ __launch_bounds__(SUM_NT) void embed_sum_kernel(const SumParams p) {
   using C = Chunk<Tag>;
-  const int64_t tile = blockIdx.x / p.slices, t0 = tile * SUM_TILE;
+  using O = Chunk<TagO>;
+  constexpr int PIECES = C::N / O::N;                          // 16-byte pieces of the gradient beside one of g
+  const int64_t tile = blockIdx.x / p.slices, t0 = tile * p.tile;
   const int64_t col = ((int64_t)(blockIdx.x % p.slices) * SUM_NT + threadIdx.x) * C::N;
   const int cols = (int)min((int64_t)C::N, p.width - col);
-  __shared__ unsigned long long word[SUM_TILE + 2];      // the tile's, and one on either side (~0: none)
-  if (threadIdx.x < SUM_TILE + 2) {
+  __shared__ unsigned long long word[SUM_TILE_MOST + 2];      // the tile's, and one on either side (~0: none)
+  if ((int)threadIdx.x < p.tile + 2) {
     const int64_t i = t0 - 1 + threadIdx.x;
     word[threadIdx.x] = i >= 0 && i < p.n ? p.sorted[i] : ~0ull;
   }
   __syncthreads();
   if (cols <= 0) return;
-  const int count = (int)min((int64_t)SUM_TILE, p.n - t0);
+  const int count = (int)min((int64_t)p.tile, p.n - t0);
+  const auto grad_row = [&](unsigned v) { return p.grad + (int64_t)v * p.grad_stride * TagO::bytes; };
   float sum[C::N];
 #pragma unroll
   for (int e = 0; e < C::N; ++e) sum[e] = 0.f;
   bool open = word_token(word[0]) == word_token(word[1]);      // the running token began in an earlier tile
   for (int i0 = 0; i0 < count; i0 += SUM_AHEAD) {
-    float f[SUM_AHEAD][C::N];
+    u32x4 x[SUM_AHEAD], old[ADD ? SUM_AHEAD : 1][PIECES];
 #pragma unroll
-    for (int j = 0; j < SUM_AHEAD; ++j)
-      if (i0 + j < count && word_token(word[1 + i0 + j]) < p.vocab)
-        load_columns<Tag>(p.g + (int64_t)(unsigned)word[1 + i0 + j] * p.g_stride * Tag::bytes, col, cols, f[j]);
+    for (int j = 0; j < SUM_AHEAD; ++j) {
+      const unsigned v = i0 + j < count ? word_token(word[1 + i0 + j]) : (unsigned)p.vocab;
+      if (v >= p.vocab) continue;
+      x[j] = load_columns<Tag>(p.g + (int64_t)(unsigned)word[1 + i0 + j] * p.g_stride * Tag::bytes, col, cols);
+      if (ADD && word_token(word[2 + i0 + j]) != v)
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) old[ADD ? j : 0][k] = load_columns<TagO>(grad_row(v), col + k * O::N, min(max(cols - k * O::N, 0), O::N));
+    }
 #pragma unroll
     for (int j = 0; j < SUM_AHEAD; ++j) {
       const int i = i0 + j;
       if (i >= count) break;
       const unsigned v = word_token(word[1 + i]);
       if (v >= p.vocab) return;                                // padding: behind all tokens
+      float f[C::N];
+      C::unpack(x[j], f);
 #pragma unroll
-      for (int e = 0; e < C::N; ++e) sum[e] += f[j][e];
+      for (int e = 0; e < C::N; ++e) sum[e] += f[e];
       const bool same = word_token(word[2 + i]) == v;
       if (same && i + 1 < count) continue;
       if (!open && !same) {
-        store_sum<TagO, C::N, ADD>(p.grad + (int64_t)v * p.grad_stride * TagO::bytes, col, cols, p.scale, sum);
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          float to[O::N];
+          if (ADD) O::unpack(old[ADD ? j : 0][k], to);
+#pragma unroll
+          for (int e = 0; e < O::N; ++e) to[e] = ADD ? fmaf(p.scale, sum[k * O::N + e], to[e]) : p.scale * sum[k * O::N + e];
+          store_columns<TagO>(grad_row(v), col + k * O::N, min(max(cols - k * O::N, 0), O::N), to);
+        }
       } else {
         float* part = p.partial + (tile * 2 + (open ? 0 : 1)) * p.width + col;
 #pragma unroll
@@ -288,37 +313,88 @@ __global__ __launch_bounds__(SUM_NT) void embed_sum_kernel(const SumParams p) {
   }
 }
 
-// The tokens that cross tiles: the tile in which one begins adds up its partial sums in order.
+// The tokens that cross tiles: the tile in which one begins adds up its partial sums in order, 8 loads in flight per thread; a
+// token that crosses more than 64 tiles is dealt to the workgroup's waves, a contiguous stretch of tiles each, whose sums then meet
+// in LDS in order.
+constexpr int JOIN_NT = 256, JOIN_COLS = 4, JOIN_AHEAD = 8, JOIN_DEALT = 64;
+__device__ __forceinline__ void add_partials(const SumParams& p, int64_t from, int64_t to, int64_t col, int cols, float* sum) {      // tiles [from, to)
+  if (cols == JOIN_COLS) {
+    for (int64_t t = from; t < to; t += JOIN_AHEAD) {
+      u32x4 x[JOIN_AHEAD];
+#pragma unroll
+      for (int j = 0; j < JOIN_AHEAD; ++j)
+        if (t + j < to) x[j] = load16_unaligned(p.partial + (t + j) * 2 * p.width + col);
+#pragma unroll
+      for (int j = 0; j < JOIN_AHEAD; ++j)
+        if (t + j < to)
+#pragma unroll
+          for (int e = 0; e < JOIN_COLS; ++e) sum[e] += __uint_as_float(x[j][e]);
+    }
+  } else {
+    for (int64_t t = from; t < to; ++t)
+#pragma unroll
+      for (int e = 0; e < JOIN_COLS; ++e)
+        if (e < cols) sum[e] += p.partial[t * 2 * p.width + col + e];
+  }
+}
 template <class TagO, bool ADD>
-__global__ __launch_bounds__(SUM_NT) void embed_join_kernel(const SumParams p) {
-  const int64_t tile = blockIdx.x / p.slices, t0 = tile * SUM_TILE, t1 = t0 + SUM_TILE;
+__global__ __launch_bounds__(JOIN_NT) void embed_join_kernel(const SumParams p) {
+  __shared__ float met[JOIN_NT / WAVE][WAVE * JOIN_COLS];
+  const int64_t tile = blockIdx.x / p.slices, t0 = tile * p.tile, t1 = t0 + p.tile;
   if (t1 >= p.n) return;
   const unsigned v = word_token(p.sorted[t1 - 1]);
   if (v >= p.vocab || word_token(p.sorted[t1]) != v) return;                                     // ends with the tile
   if (word_token(p.sorted[t0]) == v && t0 > 0 && word_token(p.sorted[t0 - 1]) == v) return;      // began in an earlier one
-  // how many further tiles it reaches: the first place behind it, by bisection
-  int64_t lo = t1, hi = p.n;                             // sorted[lo] is the token, sorted[hi] is not
+  int64_t lo = t1, hi = p.n;                             // where it ends, by bisection: sorted[lo] is the token, sorted[hi] is not
   while (hi - lo > 1) {
     const int64_t mid = (lo + hi) / 2;
     (word_token(p.sorted[mid]) == v ? lo : hi) = mid;
   }
-  const int64_t last = lo / SUM_TILE;
-  constexpr int N = 4;
-  const int64_t per = (int64_t)p.slices * SUM_NT * N;
-  for (int64_t col = ((int64_t)(blockIdx.x % p.slices) * SUM_NT + threadIdx.x) * N; col < p.width; col += per) {
-    const int cols = (int)min((int64_t)N, p.width - col);
-    float sum[N];
+  const int64_t end = lo / p.tile + 1, span = end - tile - 1;
+  char* row = p.grad + (int64_t)v * p.grad_stride * TagO::bytes;
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
+  constexpr int NW = JOIN_NT / WAVE;
+  const auto finish = [&](const float* sum, int64_t col, int cols) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e] = e < cols ? p.partial[(tile * 2 + 1) * p.width + col + e] : 0.f;
-#pragma unroll 4
-    for (int64_t t = tile + 1; t <= last; ++t)
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e < cols) sum[e] += p.partial[t * 2 * p.width + col + e];
-    char* row = p.grad + (int64_t)v * p.grad_stride * TagO::bytes;
-#pragma unroll
-    for (int e = 0; e < N; ++e)
+    for (int e = 0; e < JOIN_COLS; ++e)
       if (e < cols) store_from_float(row, TagO::id, col + e, ADD ? fmaf(p.scale, sum[e], load_as_float(row, TagO::id, col + e)) : p.scale * sum[e]);
+  };
+  const int64_t slice0 = (int64_t)(blockIdx.x % p.slices) * JOIN_NT * JOIN_COLS;
+  if (span <= JOIN_DEALT) {
+    const int64_t col = slice0 + threadIdx.x * JOIN_COLS;
+    const int cols = (int)min((int64_t)JOIN_COLS, p.width - col);
+    if (cols <= 0) return;
+    float sum[JOIN_COLS];
+#pragma unroll
+    for (int e = 0; e < JOIN_COLS; ++e) sum[e] = e < cols ? p.partial[(tile * 2 + 1) * p.width + col + e] : 0.f;
+    add_partials(p, tile + 1, end, col, cols, sum);
+    finish(sum, col, cols);
+    return;
+  }
+  const int64_t each = (span + NW - 1) / NW, from = min(end, tile + 1 + w * each), to = min(end, from + each);
+  for (int q = 0; q < NW; ++q) {
+    const int64_t col = slice0 + (q * WAVE + lane) * JOIN_COLS;
+    const int cols = (int)min((int64_t)JOIN_COLS, p.width - col);
+    float sum[JOIN_COLS] = {0.f, 0.f, 0.f, 0.f};
+    if (cols > 0) {
+      if (w == 0)
+#pragma unroll
+        for (int e = 0; e < JOIN_COLS; ++e)
+          if (e < cols) sum[e] = p.partial[(tile * 2 + 1) * p.width + col + e];
+      add_partials(p, from, to, col, cols, sum);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < JOIN_COLS; ++e) met[w][lane * JOIN_COLS + e] = sum[e];
+    __syncthreads();
+    if (w == q && cols > 0) {
+#pragma unroll
+      for (int e = 0; e < JOIN_COLS; ++e) {
+        sum[e] = met[0][lane * JOIN_COLS + e];
+        for (int k = 1; k < NW; ++k) sum[e] += met[k][lane * JOIN_COLS + e];
+      }
+      finish(sum, col, cols);
+    }
   }
 }
 
@@ -326,16 +402,17 @@ static int embed_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_
 
 template <class Tag, class TagO>
 static int launch_sums(const SumParams& s, bool add, hipStream_t st) {
-  SumParams p = s;
-  const int64_t tiles = (p.n + SUM_TILE - 1) / SUM_TILE;
+  SumParams p = s, j = s;
+  const int64_t tiles = (p.n + p.tile - 1) / p.tile;
   p.slices = (unsigned)((p.width + SUM_NT * Chunk<Tag>::N - 1) / (SUM_NT * Chunk<Tag>::N));
-  const dim3 grid((unsigned)(tiles * p.slices)), nt(SUM_NT);
+  j.slices = (unsigned)((p.width + JOIN_NT * JOIN_COLS - 1) / (JOIN_NT * JOIN_COLS));
+  const dim3 grid((unsigned)(tiles * p.slices)), joins((unsigned)((tiles - 1) * j.slices));      // (the last tile is no token's first)
   if (add) {
-    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, true>), grid, nt, 0, st, p);
-    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, true>), grid, nt, 0, st, p);
+    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, true>), grid, dim3(SUM_NT), 0, st, p);
+    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, true>), joins, dim3(JOIN_NT), 0, st, j);
   } else {
-    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, false>), grid, nt, 0, st, p);
-    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, false>), grid, nt, 0, st, p);
+    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, false>), grid, dim3(SUM_NT), 0, st, p);
+    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, false>), joins, dim3(JOIN_NT), 0, st, j);
   }
   return embed_status();
 }
@@ -343,11 +420,13 @@ static int launch_sums(const SumParams& s, bool add, hipStream_t st) {
 // Places of the workspace, each on a 256-byte boundary: two lists of words, the digit counts, the partial sums.
 struct EmbedSpace {
   int64_t words, counts, partial, total;
+  int tile;
   EmbedSpace(int64_t n, int64_t width) {
     const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
     words = up(n * 8);
     counts = n > SORT_SMALL ? up((int64_t)SORT_BLOCKS * SORT_BINS * 4) : 0;
-    partial = up((n + SUM_TILE - 1) / SUM_TILE * 2 * width * 4);
+    tile = sum_tile(n, width);
+    partial = up((n + tile - 1) / tile * 2 * width * 4);
     total = 2 * words + counts + partial;
   }
 };
@@ -397,7 +476,7 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
       reinterpret_cast<uintptr_t>(workspace) % 256)
     return DL_ERR_ALIGN;
   const int64_t slices = (width + SUM_NT * 4 - 1) / (SUM_NT * 4);
-  if (n_tokens > 0x7fffffffLL || vocab > 0x7ffffffeLL || (n_tokens / SUM_TILE + 1) * slices > 0x7fffffffLL) return DL_ERR_LIMIT;
+  if (n_tokens > 0x7fffffffLL || vocab > 0x7ffffffeLL || (n_tokens / SUM_TILE_LEAST + 1) * slices > 0x7fffffffLL) return DL_ERR_LIMIT;
   const EmbedSpace sp(n_tokens, width);
   if (n_tokens > 0 && (!workspace || workspace_bytes < sp.total)) return DL_ERR_WORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -424,10 +503,11 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
   const unsigned long long* sorted = words[0];
   if (passes == 0) {
     const ZeroShare z = share();
-    hipLaunchKernelGGL(embed_sort_small_kernel, dim3(1 + z.blocks), dim3(1024), 0, st, tokens, itype, (int)n_tokens, vocab, words[0], z);
+    if (n_tokens <= 256) hipLaunchKernelGGL(embed_sort_small_kernel<256>, dim3(1 + z.blocks), dim3(256), 0, st, tokens, itype, (int)n_tokens, vocab, words[0], z);
+    else hipLaunchKernelGGL(embed_sort_small_kernel<1024>, dim3(1 + z.blocks), dim3(1024), 0, st, tokens, itype, (int)n_tokens, vocab, words[0], z);
   } else {
-    const int64_t per = std::max<int64_t>(2048, ((n_tokens + SORT_BLOCKS - 1) / SORT_BLOCKS + SORT_NT - 1) / SORT_NT * SORT_NT);
-    SortPass s{tokens, itype, vocab, nullptr, words[0], reinterpret_cast<unsigned*>(ws + 2 * sp.words), n_tokens, per, 0, (digits + passes - 1) / passes,
+    const int64_t per = std::max<int64_t>(SORT_LEAST, ((n_tokens + SORT_BLOCKS - 1) / SORT_BLOCKS + SORT_NT - 1) / SORT_NT * SORT_NT);
+    SortPass s{tokens, itype, vocab, nullptr, words[0], reinterpret_cast<unsigned*>(ws + 2 * sp.words), n_tokens, per, 0, std::max(2, (digits + passes - 1) / passes),
                (unsigned)((n_tokens + per - 1) / per)};
     for (int k = 0; k < passes; ++k) {
       const ZeroShare a = share();
@@ -442,7 +522,7 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
   }
   if (n_tokens == 0) return embed_status();
   SumParams p{sorted, n_tokens, vocab, width, reinterpret_cast<const char*>(g), g_stride, reinterpret_cast<char*>(grad), grad_stride,
-              reinterpret_cast<float*>(ws + 2 * sp.words + sp.counts), scale, 0};
+              reinterpret_cast<float*>(ws + 2 * sp.words + sp.counts), scale, 0, sp.tile};
   if (dtype == DL_F32) return launch_sums<TagF32, TagF32>(p, accumulate != 0, st);
   if (dtype == DL_BF16) return grad_dtype == DL_F32 ? launch_sums<TagBF16, TagF32>(p, accumulate != 0, st) : launch_sums<TagBF16, TagBF16>(p, accumulate != 0, st);
   return grad_dtype == DL_F32 ? launch_sums<TagF16, TagF32>(p, accumulate != 0, st) : launch_sums<TagF16, TagF16>(p, accumulate != 0, st);

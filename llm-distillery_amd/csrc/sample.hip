@@ -34,20 +34,14 @@ struct SampleParams {
   int64_t* token; float* logp; int32_t* kept;
 };
 
-// What the weights of a row are relative to.  `peak`: the limit in which only the maximum has any (T <= 0, an infinite maximum).
-struct RowScale { float top, rate; bool peak; };
+// What the weights of a row are relative to.
+struct RowScale { float top, rate; };
 
-__device__ __forceinline__ RowScale row_scale(float top, float T) {
-  RowScale s;
-  s.top = top;
-  s.rate = LOG2E / T;
-  s.peak = !(T > 0.f) || s.rate == INFINITY || top == INFINITY;
-  return s;
-}
+// Rows in which only the maximum has a weight: T <= 0 (or NaN), T so small that 1 / T is infinite, an infinite maximum.
+__device__ __forceinline__ bool only_the_maximum(float top, float T) { return !(T > 0.f) || LOG2E / T == INFINITY || top == INFINITY; }
 // t of a logit, at least -64 (NaN as well)
 __device__ __forceinline__ float sample_t(const RowScale& s, float x) {
 #pragma clang fp contract(off)
-  if (s.peak) return x == s.top ? 0.f : -64.f;
   const float d = x - s.top;
   return fmaxf(d * s.rate, -64.f);
 }
@@ -76,18 +70,22 @@ __device__ __forceinline__ float word_logit(u64 w) { return logit_of(~(unsigned)
 // floor(mass * part / 2^24)
 __device__ __forceinline__ u64 share_of(u64 mass, unsigned part) { return (mass >> 24) * part + (((mass & 0xffffffu) * part) >> 24); }
 
-// f(logit, column) for every column of [lo, hi) of a row, on any element boundary; four loads in flight per thread.
+// f(logit, column) for every column of [lo, hi) of a row, on any element boundary; eight loads in flight per thread.
 template <class Tag, int NT, class F>
 __device__ __forceinline__ void each_logit(const char* row, int64_t lo, int64_t hi, F f) {
   using C = Chunk<Tag>;
   const char* at = row + lo * Tag::bytes;
   const int n = (int)(hi - lo), whole = n / C::N;
   constexpr int UN = 4;
-  for (int c0 = threadIdx.x; c0 < whole; c0 += NT * UN) {
-    u32x4 v[UN];
+  u32x4 v[UN], ahead[UN];
+  const auto fetch = [&](int c0, u32x4* to) {
 #pragma unroll
     for (int i = 0; i < UN; ++i)
-      if (c0 + i * NT < whole) v[i] = load16_unaligned(at + (int64_t)(c0 + i * NT) * 16);
+      if (c0 + i * NT < whole) to[i] = load16_unaligned(at + (int64_t)(c0 + i * NT) * 16);
+  };
+  fetch(threadIdx.x, v);
+  for (int c0 = threadIdx.x; c0 < whole; c0 += NT * UN) {
+    fetch(c0 + NT * UN, ahead);                  // the next four are on their way while these are worked on
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       if (c0 + i * NT >= whole) break;
@@ -96,10 +94,15 @@ __device__ __forceinline__ void each_logit(const char* row, int64_t lo, int64_t 
 #pragma unroll
       for (int e = 0; e < C::N; ++e) f(x[e], (int)lo + (c0 + i * NT) * C::N + e);
     }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) v[i] = ahead[i];
   }
   const int col = whole * C::N + (int)threadIdx.x;
   if (col < n) f(load_as_float(at, Tag::id, col), (int)lo + col);
 }
+
+// A bin behind which every token has less weight than `least`: the threshold's, and two more for what rounding does to it.
+__device__ __forceinline__ int bin_behind(unsigned least) { return min((int)((31.f - log2f((float)least)) * 32.f) + 2, SAMPLE_BINS - 1); }
 
 // A list of tokens in order with their masses: those of some bins, or some of one bin's.
 struct SampleLds {
@@ -122,6 +125,7 @@ struct Sampler {
   int lo_bin = 0, hi_bin = -1, n = 0;
   unsigned ahead = 0;
   u64 ahead_mass = 0;
+  bool overflow = false;                     // more tokens than the list holds
 
   __device__ Sampler(SampleLds& lds, const char* r, int64_t v, const RowScale& scale) : s(lds), row(r), V(v), sc(scale) {}
 
@@ -196,13 +200,18 @@ struct Sampler {
   __device__ int bin_reaching(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] < m && s.mass[b + 1] >= m; }); }
   __device__ int bin_passing(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] <= m && s.mass[b + 1] > m; }); }
 
-  // Tokens for which in(t, x) holds (and that have a weight) into the list, in order, with their masses behind `mass`.
+  // Tokens for which in(t, x) holds (and that have a weight; only t > below is asked) into the list, in order, with their masses
+  // behind `mass`.  Most of a row is far below: one comparison of the logit itself, with room for what rounding does to t, is
+  // all that it costs.
   template <class Tag, class In>
-  __device__ void collect(unsigned before, u64 mass, In in) {
+  __device__ void collect(unsigned before, u64 mass, float below, In in) {
+    const float far = sc.top + fmaxf(below, -33.f) / sc.rate;
+    const float least = far - 1e-5f * (fabsf(far) + fabsf(sc.top));
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
     each_logit<Tag, NT>(row, 0, V, [&](float x, int col) {
+      if (!(x >= least)) return;
       const float t = sample_t(sc, x);
       if (in(t, x) && sample_weight(t) > 0) {
         const unsigned at = atomicAdd(&s.n, 1u);
@@ -210,6 +219,7 @@ struct Sampler {
       }
     });
     __syncthreads();
+    overflow = s.n > SAMPLE_CAP;
     n = min((int)s.n, SAMPLE_CAP);
     sort();
     ahead = before;
@@ -263,13 +273,45 @@ struct Sampler {
 #pragma unroll
     for (int j = 0; j < EACH; ++j) s.word[threadIdx.x * EACH + j] = w[j];
   }
+  // (The tokens ahead are counted on the way: the counts of the bins may be estimates.)
   template <class Tag>
   __device__ void collect_bins(int lo, int hi) {
-    const float above = -(float)lo * 0.03125f, below = -(float)(hi + 1) * 0.03125f;      // bin lo .. hi: below < t <= above
-    const bool last = hi == SAMPLE_BINS - 1;
-    collect<Tag>(s.count[lo], s.mass[lo], [&](float t, float) { return t <= above && (last || t > below); });
+    const float above = -(float)lo * 0.03125f, below = hi == SAMPLE_BINS - 1 ? -65.f : -(float)(hi + 1) * 0.03125f;      // bin lo .. hi: below < t <= above
+    unsigned before = 0;
+    collect<Tag>(0, s.mass[lo], below, [&](float t, float) {
+      before += t > above;
+      return t <= above && t > below;
+    });
+    u64 none = 0;
+    if (lo > 0) sum(none, before);
+    ahead = before;
     lo_bin = lo;
     hi_bin = hi;
+  }
+  // Look-ups in the list as it is.
+  __device__ void in_list_reaching(u64 m, unsigned& tokens, u64& mass) {
+    const int i = find(n, [&](int j) { return s.upto[j] >= m && (j == 0 ? ahead_mass : s.upto[j - 1]) < m; });
+    tokens = ahead + (unsigned)i + 1;
+    mass = s.upto[i];
+  }
+  __device__ int in_list_token(u64 m, float& t) {
+    const int i = find(n, [&](int k) { return s.upto[k] > m && (k == 0 ? ahead_mass : s.upto[k - 1]) <= m; });
+    t = sample_t(sc, word_logit(s.word[i]));
+    return (int)(unsigned)s.word[i];
+  }
+  // (a list from the first token on, and all tokens behind it below `least` or `tokens` within it)
+  __device__ void in_list_below(unsigned least, unsigned& tokens, u64& mass) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.hit = min(tokens, (unsigned)n);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT)
+      if (s.upto[i] - (i == 0 ? 0 : s.upto[i - 1]) < least) atomicMin(&s.hit, (unsigned)i);
+    __syncthreads();
+    const unsigned q = s.hit;
+    if (q < tokens) {
+      tokens = q;
+      mass = s.upto[q - 1];
+    }
   }
 
   // Equal logits too many for the list, after narrow(): the order of their logit, tokens and mass ahead of them.
@@ -311,7 +353,7 @@ struct Sampler {
       if (inside <= SAMPLE_CAP) {
         const unsigned want = prefix;
         const int sh = shift;
-        collect<Tag>(before, before_mass, [&](float t, float x) { return sample_bin(t) == bin && (order_of(x) >> sh) == want; });
+        collect<Tag>(before, before_mass, -65.f, [&](float t, float x) { return sample_bin(t) == bin && (order_of(x) >> sh) == want; });
         lo_bin = 0;
         hi_bin = -1;                                          // part of a bin: of no use to other look-ups
         return;
@@ -352,9 +394,7 @@ struct Sampler {
       mass = ahead_mass + q * tie_weight;
       return;
     }
-    const int i = find(n, [&](int j) { return s.upto[j] >= m && (j == 0 ? ahead_mass : s.upto[j - 1]) < m; });
-    tokens = ahead + (unsigned)i + 1;
-    mass = s.upto[i];
+    in_list_reaching(m, tokens, mass);
   }
   // The token in whose stretch m falls, and its t.
   template <class Tag>
@@ -365,9 +405,7 @@ struct Sampler {
       t = sample_t(sc, logit_of(tie_order));
       return equal_logit<Tag>(j);
     }
-    const int i = find(n, [&](int k) { return s.upto[k] > m && (k == 0 ? ahead_mass : s.upto[k - 1]) <= m; });
-    t = sample_t(sc, word_logit(s.word[i]));
-    return (int)(unsigned)s.word[i];
+    return in_list_token(m, t);
   }
   // The column of the j-th logit of order `tie_order`: every wave counts those of a stretch of columns, then the one that
   // holds the j-th walks its stretch again.
@@ -399,23 +437,12 @@ struct Sampler {
   // The number of tokens ahead of the first whose weight is below `least`, and their mass, if that comes before `tokens`.
   template <class Tag>
   __device__ void cut_below(unsigned least, unsigned& tokens, u64& mass) {
-    // bins ahead of the threshold's, less one for what rounding does to it, hold no such token; from two behind it on, all are
-    const int behind = min((int)((31.f - log2f((float)least)) * 32.f) + 2, SAMPLE_BINS - 1);
+    const int behind = bin_behind(least);
     if (hi_bin < 0 || lo_bin > 0) {
       if (s.count[behind + 1] <= SAMPLE_CAP) collect_bins<Tag>(0, behind);
     }
     if (hi_bin >= 0 && lo_bin == 0 && (hi_bin >= behind || tokens <= (unsigned)n)) {
-      __syncthreads();
-      if (threadIdx.x == 0) s.hit = min(tokens, (unsigned)n);      // (tokens behind the list are all below)
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += NT)
-        if (s.upto[i] - (i == 0 ? 0 : s.upto[i - 1]) < least) atomicMin(&s.hit, (unsigned)i);
-      __syncthreads();
-      const unsigned q = s.hit;
-      if (q < tokens) {
-        tokens = q;
-        mass = s.upto[q - 1];
-      }
+      in_list_below(least, tokens, mass);
       return;
     }
     // Too many for the list: the largest logit with too small a weight, then what lies above it.
@@ -443,41 +470,175 @@ struct Sampler {
   }
 };
 
-// From the histogram in LDS (sums ahead of each bin) to the row's outputs.
+// The row's settings as whole numbers.
+struct RowCuts { int k; unsigned part, least, u; bool top_p; };      // part, u: of 2^24
+__device__ __forceinline__ RowCuts row_cuts(const SampleParams& p, int64_t r, float T) {
+  const float top_p = p.p ? p.p[r] : p.p0, min_p = p.m ? p.m[r] : p.m0;
+  RowCuts c;
+  c.k = T > 0.f ? (p.k ? p.k[r] : p.k0) : 1;
+  c.top_p = top_p < 1.f;
+  c.part = (unsigned)(fminf(fmaxf(top_p, 0.f), 1.f) * 0x1p24f);
+  c.least = min_p > 0.f ? (unsigned)(fminf(min_p, 1.f) * 0x1p31f) : 0u;
+  c.u = (unsigned)fminf(fmaxf(p.u[r], 0.f) * 0x1p24f, 0x1p24f - 1.f);
+  return c;
+}
+__device__ __forceinline__ u64 mass_wanted(u64 mass, unsigned part) {
+  const u64 m = share_of(mass, part);
+  return m > 0 ? m : 1;
+}
+struct RowResult { int token; unsigned kept; float t; };
+
+// Rows whose maxima share the mass: equal weights, in the order of their columns.
 template <class Tag, int NT>
-__device__ void sample_finish(const SampleParams& p, SampleLds& s, int64_t r, const char* row, const RowScale& sc, float powers) {
-  Sampler<NT> a(s, row, p.V, sc);
-  const float T = p.T ? p.T[r] : p.T0, top_p = p.p ? p.p[r] : p.p0, min_p = p.m ? p.m[r] : p.m0;
-  const int k = T > 0.f ? (p.k ? p.k[r] : p.k0) : 1;
+__device__ __attribute__((noinline)) RowResult sample_maximum(SampleLds& s, const char* row, int64_t V, float top, const RowCuts cuts, unsigned& ties) {
+  Sampler<NT> a(s, row, V, RowScale{top, 0.f});
+  u64 none = 0;
+  ties = 0;
+  unsigned first = 0xffffffffu;
+  each_logit<Tag, NT>(row, 0, V, [&](float x, int col) {
+    if (x == top) {
+      ++ties;
+      first = min(first, (unsigned)col);
+    }
+  });
+  a.sum(none, ties);
+  first = wave_min(first);
+  __syncthreads();
+  if ((threadIdx.x & (WAVE - 1)) == 0) s.wave_count[threadIdx.x / WAVE] = first;
+  __syncthreads();
+  for (int i = 0; i < Sampler<NT>::NW; ++i) first = min(first, s.wave_count[i]);
+  unsigned n = cuts.k > 0 ? min(ties, (unsigned)cuts.k) : ties;
+  if (cuts.top_p) n = (unsigned)((mass_wanted((u64)n << 31, cuts.part) + 0x7fffffffull) >> 31);
+  const unsigned j = (unsigned)(share_of((u64)n << 31, cuts.u) >> 31);
+  a.tie_order = order_of(top);
+  return RowResult{j == 0 ? (int)first : a.template equal_logit<Tag>(j), n, 0.f};
+}
+
+// Any row: a histogram of masses and counts, every look-up by the bins.
+template <class Tag, int NT>
+__device__ __attribute__((noinline)) RowResult sample_any(SampleLds& s, const char* row, int64_t V, const RowScale sc, const RowCuts cuts) {
+  Sampler<NT> a(s, row, V, sc);
+  __syncthreads();
+  for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) { s.mass[b] = 0; s.count[b] = 0; }
+  __syncthreads();
+  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+    const float t = sample_t(sc, x);
+    const unsigned w = sample_weight(t);
+    if (w > 0) {
+      const int b = sample_bin(t);
+      atomicAdd(&s.mass[b], (u64)w);
+      atomicAdd(&s.count[b], 1u);
+    }
+  });
+  __syncthreads();
+  a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
   unsigned tokens = s.count[SAMPLE_BINS];
   u64 mass = s.mass[SAMPLE_BINS];
-  if (k > 0 && (unsigned)k < tokens) {
-    const int bin = a.bin_of_count(k);
+  if (cuts.k > 0 && (unsigned)cuts.k < tokens) {
+    const int bin = a.bin_of_count(cuts.k);
     if (s.count[bin + 1] <= SAMPLE_CAP) a.template collect_bins<Tag>(0, bin);      // holds whatever is asked below
-    mass = a.template mass_of_first<Tag>(k, bin);
-    tokens = k;
+    mass = a.template mass_of_first<Tag>(cuts.k, bin);
+    tokens = cuts.k;
   }
-  if (top_p < 1.f) {
-    const u64 part = share_of(mass, (unsigned)(fmaxf(top_p, 0.f) * 0x1p24f)), want = part > 0 ? part : 1;
+  if (cuts.top_p) {
+    const u64 want = mass_wanted(mass, cuts.part);
     const int bin = a.bin_reaching(want);
     if (a.hi_bin < 0 && s.count[bin + 1] <= SAMPLE_CAP) a.template collect_bins<Tag>(0, bin);
     a.template first_reaching<Tag>(want, bin, tokens, mass);
   }
-  const unsigned least = min_p > 0.f ? (unsigned)(fminf(min_p, 1.f) * 0x1p31f) : 0u;
-  if (least > 0) a.template cut_below<Tag>(least, tokens, mass);
-  const unsigned u = (unsigned)fminf(fmaxf(p.u[r], 0.f) * 0x1p24f, 0x1p24f - 1.f);
-  const u64 want = share_of(mass, u);
-  float t;
-  const int token = a.template token_at<Tag>(want, a.bin_passing(want), t);
-  if (threadIdx.x == 0) {
-    p.token[r] = token;
-    if (p.logp) p.logp[r] = (t - log2f(powers * 0x1p-31f)) * LN2;
-    if (p.kept) p.kept[r] = (int)tokens;
+  if (cuts.least > 0) a.template cut_below<Tag>(cuts.least, tokens, mass);
+  const u64 want = share_of(mass, cuts.u);
+  RowResult res;
+  res.token = a.template token_at<Tag>(want, a.bin_passing(want), res.t);
+  res.kept = tokens;
+  return res;
+}
+
+// Rows with top-k whose first k tokens fit the list: counts of tokens per bin, first of those within 2^-16 of the most likely one
+// (few, and with them few additions in LDS), of all if that is not enough.  (A token has a weight from t = -31 on.)
+// False: not decided here.  `powers`: the sum of 2^(t + 31).
+template <class Tag, int NT>
+__device__ __forceinline__ bool sample_top_k(SampleLds& s, const char* row, int64_t V, const RowScale& sc, RowCuts cuts, float& powers, RowResult& res) {
+  Sampler<NT> a(s, row, V, sc);
+  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+    const float t = sample_t(sc, x);
+    powers += fast_exp2(t);
+    if (t > -16.f) atomicAdd(&s.count[sample_bin(t)], 1u);
+  });
+  powers = block_sum<NT>(powers, s.red) * 0x1p31f;
+  a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
+  if (s.count[SAMPLE_BINS] < (unsigned)cuts.k) {
+    __syncthreads();
+    for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) s.count[b] = 0;
+    __syncthreads();
+    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+      const float t = sample_t(sc, x);
+      if (t >= -31.f) atomicAdd(&s.count[sample_bin(t)], 1u);
+    });
+    __syncthreads();
+    a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
+    cuts.k = min(cuts.k, (int)s.count[SAMPLE_BINS]);
   }
+  const int bin = a.bin_of_count(cuts.k);
+  if (s.count[bin + 1] > SAMPLE_CAP) return false;
+  a.template collect_bins<Tag>(0, bin);
+  unsigned tokens = cuts.k;
+  u64 mass = s.upto[tokens - 1];
+  if (cuts.top_p) a.in_list_reaching(mass_wanted(mass, cuts.part), tokens, mass);
+  if (cuts.least > 0) a.in_list_below(cuts.least, tokens, mass);
+  res.token = a.in_list_token(share_of(mass, cuts.u), res.t);
+  res.kept = tokens;
+  return true;
+}
+
+// Rows without top-k: a histogram of masses.  Counts of tokens are only needed to choose between lists; a bin's mass over its
+// middle weight gives them to 1 %, and whether a list held all is known when it is made.
+template <class Tag, int NT>
+__device__ __forceinline__ bool sample_by_mass(SampleLds& s, const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float& powers, RowResult& res) {
+  Sampler<NT> a(s, row, V, sc);
+  unsigned tokens = 0;
+  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+    const float t = sample_t(sc, x), e = sample_power(t);
+    powers += e;
+    const unsigned w = (unsigned)e;
+    if (w > 0) {
+      ++tokens;
+      atomicAdd(&s.mass[sample_bin(t)], (u64)w);
+    }
+  });
+  powers = block_sum<NT>(powers, s.red);
+  for (int b = threadIdx.x; b < SAMPLE_BINS; b += NT)
+    if (s.mass[b] > 0) s.count[b] = (unsigned)((float)s.mass[b] * fast_exp2((float)b * 0.03125f + (0.015625f - 31.f))) + 1u;
+  __syncthreads();
+  a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
+  u64 mass = s.mass[SAMPLE_BINS], none = 0;
+  constexpr unsigned FITS = SAMPLE_CAP - SAMPLE_CAP / 16;
+  a.sum(none, tokens);
+  if (cuts.top_p || cuts.least > 0) {
+    const u64 want = cuts.top_p ? mass_wanted(mass, cuts.part) : mass;
+    const int end_p = cuts.top_p ? a.bin_reaching(want) : SAMPLE_BINS - 1, behind = cuts.least > 0 ? bin_behind(cuts.least) : SAMPLE_BINS - 1;
+    const int end = min(end_p, behind);
+    if (s.count[end + 1] <= FITS) a.template collect_bins<Tag>(0, end);
+    else if (cuts.least == 0 && s.count[end + 1] - s.count[end] <= FITS) a.template collect_bins<Tag>(end, end);
+    else return false;
+    if (a.overflow) return false;
+    if (cuts.top_p && end_p <= behind) a.in_list_reaching(want, tokens, mass);
+    if (cuts.least > 0) a.in_list_below(cuts.least, tokens, mass);
+  }
+  const u64 want = share_of(mass, cuts.u);
+  const int bin = a.bin_passing(want);
+  if (bin < a.lo_bin || bin > a.hi_bin) {
+    if (s.count[bin + 1] - s.count[bin] > FITS) return false;
+    a.template collect_bins<Tag>(bin, bin);
+    if (a.overflow) return false;
+  }
+  res.token = a.in_list_token(want, res.t);
+  res.kept = tokens;
+  return true;
 }
 
 template <class Tag, int NT>
-__global__ __launch_bounds__(NT) void sample_row_kernel(const SampleParams p) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void sample_row_kernel(const SampleParams p) {
   __shared__ SampleLds s;
   const int64_t r = blockIdx.x;
   const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
@@ -493,26 +654,32 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleParams p) {
     }
     return;
   }
-  const RowScale sc = row_scale(top, p.T ? p.T[r] : p.T0);
-  float powers = 0.f;
-  each_logit<Tag, NT>(row, 0, p.V, [&](float x, int) {
-    const float t = sample_t(sc, x), e = sample_power(t);
-    powers += e;
-    const unsigned w = (unsigned)e;
-    if (w > 0) {
-      const int b = sample_bin(t);
-      atomicAdd(&s.mass[b], (u64)w);
-      atomicAdd(&s.count[b], 1u);
-    }
-  });
-  powers = block_sum<NT>(powers, s.red);
-  Sampler<NT>(s, row, p.V, sc).template scan_bins<SAMPLE_BINS>(s.mass, s.count);
-  sample_finish<Tag, NT>(p, s, r, row, sc, powers);
+  const float T = p.T ? p.T[r] : p.T0;
+  const RowCuts cuts = row_cuts(p, r, T);
+  RowResult res;
+  float logp;
+  if (only_the_maximum(top, T)) {
+    unsigned ties;
+    res = sample_maximum<Tag, NT>(s, row, p.V, top, cuts, ties);
+    logp = -logf((float)ties);
+  } else {
+    const RowScale sc{top, LOG2E / T};
+    float powers = 0.f;
+    const bool done = cuts.k > 0 ? sample_top_k<Tag, NT>(s, row, p.V, sc, cuts, powers, res) : sample_by_mass<Tag, NT>(s, row, p.V, sc, cuts, powers, res);
+    if (!done) res = sample_any<Tag, NT>(s, row, p.V, sc, cuts);
+    logp = (res.t - log2f(powers * 0x1p-31f)) * LN2;
+  }
+  if (threadIdx.x == 0) {
+    p.token[r] = res.token;
+    if (p.logp) p.logp[r] = logp;
+    if (p.kept) p.kept[r] = (int)res.kept;
+  }
 }
 
 template <class Tag>
 static int launch_sample(const SampleParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((sample_row_kernel<Tag, 512>), dim3((unsigned)p.n_rows), dim3(512), 0, st, p);
+  if (p.n_rows <= 256) hipLaunchKernelGGL((sample_row_kernel<Tag, 1024>), dim3((unsigned)p.n_rows), dim3(1024), 0, st, p);
+  else hipLaunchKernelGGL((sample_row_kernel<Tag, 512>), dim3((unsigned)p.n_rows), dim3(512), 0, st, p);
   return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH;
 }
 

@@ -10,15 +10,12 @@ from . import _lib
 from .ops import _DT, _dev, _on, _row_pitch, _rows_2d, _stream_ptr
 
 
-def _setting(value, n: int, dtype: torch.dtype, name: str, dev: torch.device):
-    """(pointer, value for all rows, what keeps the memory alive) of a setting: a number, or a vector with one entry per row."""
-    if not isinstance(value, torch.Tensor):
-        return 0, value, None
-    _dev(value, name, dev)
-    if value.dtype != dtype or value.numel() != n:
-        raise RuntimeError(f"{name} must be a number or a {dtype} tensor with one entry for each of the {n} rows")
-    v = value.reshape(-1).contiguous()
-    return v.data_ptr(), 0, v
+def _row_vector(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, dev: torch.device) -> torch.Tensor:
+    """`t`, one entry per row, as a contiguous vector."""
+    if t.device != dev or t.dtype != dtype or t.numel() != n:
+        _dev(t, name, dev)
+        raise RuntimeError(f"{name} must be a {dtype} tensor with one entry for each of the {n} rows")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[float, torch.Tensor] = 1.0,
@@ -47,28 +44,35 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature: Union[flo
     dev = x.device
     if x.dtype not in _DT:
         raise RuntimeError("unsupported dtype")
-    _dev(u, "u", dev)
-    if u.dtype != torch.float32 or u.numel() != R:
-        raise RuntimeError(f"u must be an fp32 tensor with one entry for each of the {R} rows")
-    u = u.reshape(-1).contiguous()
     if V == 0:
         raise RuntimeError("the rows have no columns")
-    T, T0, keep_T = _setting(temperature, R, torch.float32, "temperature", dev)
-    k, k0, keep_k = _setting(top_k, R, torch.int32, "top_k", dev)
-    p, p0, keep_p = _setting(top_p, R, torch.float32, "top_p", dev)
-    m, m0, keep_m = _setting(min_p, R, torch.float32, "min_p", dev)
-    k0 = int(k0)
-    if not 0 <= k0 <= 0x7fffffff:
+    u = _row_vector(u, R, torch.float32, "u", dev)
+    T, k, p, m = temperature, top_k, top_p, min_p
+    T_ptr = k_ptr = p_ptr = m_ptr = 0
+    if isinstance(T, torch.Tensor):
+        T = _row_vector(T, R, torch.float32, "temperature", dev)
+        T_ptr = T.data_ptr()
+    if isinstance(k, torch.Tensor):
+        k = _row_vector(k, R, torch.int32, "top_k", dev)
+        k_ptr = k.data_ptr()
+    elif not 0 <= k <= 0x7fffffff:
         raise ValueError("top_k must not be negative")
-    tokens = torch.empty(R, dtype=torch.int64, device=dev)
-    logp = torch.empty(R, dtype=torch.float32, device=dev)
-    kept = torch.empty(R, dtype=torch.int32, device=dev)
-    with _on(dev):
-        st = _lib.load().dl_sample_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, u.data_ptr(), T, k, p, m, float(T0), k0, float(p0),
-                                        float(m0), tokens.data_ptr(), logp.data_ptr(), kept.data_ptr(), _stream_ptr(dev))
-    _lib.check(st, "dl_sample_rows")
+    if isinstance(p, torch.Tensor):
+        p = _row_vector(p, R, torch.float32, "top_p", dev)
+        p_ptr = p.data_ptr()
+    if isinstance(m, torch.Tensor):
+        m = _row_vector(m, R, torch.float32, "min_p", dev)
+        m_ptr = m.data_ptr()
     shape = logits.shape[:-1]
-    return tokens.view(shape), logp.view(shape), kept.view(shape)
+    tokens = torch.empty(shape, dtype=torch.int64, device=dev)
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    kept = torch.empty(shape, dtype=torch.int32, device=dev)
+    with _on(dev):
+        st = _lib.load().dl_sample_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, u.data_ptr(), T_ptr, k_ptr, p_ptr, m_ptr,
+                                        0.0 if T_ptr else float(T), 0 if k_ptr else int(k), 0.0 if p_ptr else float(p), 0.0 if m_ptr else float(m),
+                                        tokens.data_ptr(), logp.data_ptr(), kept.data_ptr(), _stream_ptr(dev))
+    _lib.check(st, "dl_sample_rows")
+    return tokens, logp, kept
 
 
 class BlockQuantized(NamedTuple):
