@@ -209,98 +209,196 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const BlocksParams p) {
   }
 }
 
-// Many rows: tiles of BM x BN, a wave WM x WN of it; one block of 128 columns per step, fetched into LDS by loads that bypass the
-// registers while the step before is computed.  A row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted by
-// piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS
-// in lane order, so it is their source addresses that are permuted.)
+// Many rows: tiles of BM x BN, a wave WM x WN of it, one block of 128 columns per step.  A step's operands are fetched into LDS by loads
+// that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted by
+// piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in
+// lane order, so it is their source addresses that are permuted.)
+// Within a step a wave goes through its WM / 16 rows of tiles: the operand of the next row is read while the matrix unit works on
+// this one, and the products of the row before are scaled and added meanwhile.  The step's one barrier sits ahead of the last row:
+// by then all operands of the step are in registers, so what follows it -- the last row's products, the first operands of the next
+// step, the fetch into the buffer that has just become free -- keeps the matrix unit busy across it.
+// Workgroups stay: each walks its tiles as one sequence of steps, so that the next tile's operands arrive while the last one is stored.
 typedef const unsigned __attribute__((address_space(1))) * global_words;
 typedef unsigned __attribute__((address_space(3))) * lds_words;
-template <int ROWS, int WAVES>
-__device__ __forceinline__ void fetch_tile(const unsigned char* base, int64_t stride, int64_t row0, int64_t rows, int64_t byte0, unsigned char* lds) {
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
-#pragma unroll
-  for (int i = 0; i < ROWS / 8 / WAVES; ++i) {
-    const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
-    const unsigned char* src = base + min(row0 + row, rows - 1) * stride + byte0 + piece * 16;
-    __builtin_amdgcn_global_load_lds((global_words)src, (lds_words)(lds + (i * WAVES + w) * 1024), 16, 0, 0);
+typedef const float __attribute__((address_space(4))) * constant_floats;      // read through the scalar unit: not in the fetches' queue
+
+// The operand that begins `lo` / `hi` bytes into LDS for this lane (its two pieces), `rows` (a constant) rows on.
+__device__ __forceinline__ i32x8 tile_operand(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
+  return join_pieces(*reinterpret_cast<const u32x4*>(lds + lo + rows * QB), *reinterpret_cast<const u32x4*>(lds + hi + rows * QB));
+}
+
+// The tiles of a launch: consecutive workgroups go round the 8 XCDs; each XCD has a contiguous eighth of the tiles, in bands of 8
+// rows of tiles, so that the tiles it works on at a time share their operands in its L2.
+struct TileWalk {
+  unsigned tiles_m, tiles_n, first, step, end;
+  __device__ TileWalk(unsigned tm, unsigned tn) : tiles_m(tm), tiles_n(tn) {
+    const unsigned total = tm * tn, each = (total + 7) / 8, xcd = blockIdx.x & 7u;
+    first = xcd * each + (blockIdx.x >> 3);
+    end = min(total, (xcd + 1) * each);
+    step = gridDim.x >> 3;
   }
-}
-__device__ __forceinline__ i32x8 tile_operand(const unsigned char* lds, int row0) {
-  const int lane = threadIdx.x & (WAVE - 1), row = row0 + lane % 16, at = row * QB + ((lane / 16) ^ ((row >> 1) & 7)) * 16;
-  return join_pieces(*reinterpret_cast<const u32x4*>(lds + at), *reinterpret_cast<const u32x4*>(lds + (at ^ 64)));
-}
+  __device__ void origin(unsigned t, int64_t& m, int64_t& n) const {      // in tiles
+    const unsigned band = t / (8u * tiles_n), high = min(8u, tiles_m - band * 8u), in = t - band * 8u * tiles_n;
+    m = band * 8u + in % high;
+    n = in / high;
+  }
+};
 
 template <class Tag, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(const BlocksParams p, unsigned tiles_m, unsigned tiles_n) {
-  constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16;
+  constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16, NA = BM / 8 / WAVES, NB = BN / 8 / WAVES;
   static_assert(WN <= QB && QB % WN == 0, "a wave's columns share their scales");
-  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows) of 128 bytes
-  constexpr int STEP = (BM + BN) * QB;
-  // Consecutive workgroups go round the 8 XCDs: each takes a contiguous eighth of the tiles, in bands of 8 rows of tiles, so
-  // that the tiles an XCD works on at a time share their operands in its L2.
-  const unsigned total = tiles_m * tiles_n, b = blockIdx.x;
-  const unsigned t = (b & 7u) * (gridDim.x >> 3) + (b >> 3);
-  if (t >= total) return;
-  const unsigned band = t / (8u * tiles_n), high = min(8u, tiles_m - band * 8u), in = t - band * 8u * tiles_n;
-  const int64_t m0 = (int64_t)(band * 8u + in % high) * BM, n0 = (int64_t)(in / high) * BN;
-
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, g = lane / 16;
+  static_assert(TM >= 2 && BM % WAVE == 0 && BM / WAVE <= WAVES, "");
+  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes, a's BM scales)
+  constexpr int STEP = (BM + BN) * QB + BM * 4;
+  const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), i16 = lane % 16;      // (w: known to be the wave's)
   const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
-  const float* sbp = p.sb + min(n0 + wn, p.N - 1) / QB * p.sb_row;
-  const float* sap[TM];
+  const TileWalk walk(tiles_m, tiles_n);
+  if (walk.first >= walk.end) return;
+  const unsigned steps = ((walk.end - walk.first + walk.step - 1) / walk.step) * (unsigned)p.blocks;
+
+  // the fetching side: its tile, its block, this thread's places in them
+  unsigned f_tile = walk.first;
+  int f_kb = 0;
+  const unsigned char *f_a, *f_b;
+  const float* f_s;
+  unsigned f_ao[NA], f_bo[NB];
+  const auto f_begin = [&]() {
+    int64_t m, n;
+    walk.origin(f_tile, m, n);
+    m *= BM;
+    n *= BN;
+    f_a = p.a + m * p.a_stride;
+    f_b = p.b + n * p.b_stride;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sap[i] = p.sa + min(m0 + wm + i * 16 + i16, p.M - 1) * p.sa_row;
+    for (int i = 0; i < NA; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_ao[i] = (unsigned)(min((int64_t)row, p.M - 1 - m) * p.a_stride) + piece * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
+    }
+    f_s = p.sa + min(m + (w * WAVE + lane) % BM, p.M - 1) * p.sa_row;
+  };
+  const auto fetch = [&](unsigned step) {
+    unsigned char* to = lds + (step & 1u) * STEP;
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      __builtin_amdgcn_global_load_lds((global_words)(f_a + f_ao[i]), (lds_words)(to + (i * WAVES + w) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      __builtin_amdgcn_global_load_lds((global_words)(f_b + f_bo[i]), (lds_words)(to + BM * QB + (i * WAVES + w) * 1024), 16, 0, 0);
+    if (w < BM / WAVE) __builtin_amdgcn_global_load_lds((global_words)f_s, (lds_words)(to + (BM + BN) * QB + w * WAVE * 4), 4, 0, 0);
+    f_a += QB;
+    f_b += QB;
+    f_s += p.sa_block;
+    if (++f_kb == p.blocks) {
+      f_kb = 0;
+      f_tile += walk.step;
+      if (f_tile < walk.end) f_begin();
+    }
+  };
+  const auto landed = [&]() {                                  // this wave's fetches are there, its reads done; and everyone's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  f_begin();
+  fetch(0);
+  landed();
+  if (steps > 1) fetch(1);
+  // Products are scaled and added two behind the one that the matrix unit starts: their results are there by then.
+  constexpr int Q = TM * TN, BEHIND = 2, KEEP = BEHIND + 1;
+  // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
+  const unsigned lo = i16 * QB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
+  unsigned a_lo = wm * QB + lo, a_hi = wm * QB + hi, b_lo = (BM + wn) * QB + lo, b_hi = (BM + wn) * QB + hi, s_at = (BM + BN) * QB + (wm + i16) * 4;
+  unsigned flip = STEP;                                        // from a place in this step's buffer to the other's
+  i32x8 bf[TN], af[2];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) bf[j] = tile_operand(lds, b_lo, b_hi, j * 16);
+  af[0] = tile_operand(lds, a_lo, a_hi, 0);
+  unsigned step = 0;
+  for (unsigned tile = walk.first; tile < walk.end; tile += walk.step) {
+  int64_t m0, n0;
+  walk.origin(tile, m0, n0);
+  m0 *= BM;
+  n0 *= BN;
+  const constant_floats sbp = (constant_floats)(p.sb + min(n0 + wn, p.N - 1) / QB * p.sb_row);
+  float sb = *sbp;
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  fetch_tile<BM, WAVES>(p.a, p.a_stride, m0, p.M, 0, lds);
-  fetch_tile<BN, WAVES>(p.b, p.b_stride, n0, p.N, 0, lds + BM * QB);
-  float sa[TM], sb = sbp[0];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sa[i] = sap[i][0];
-  for (int kb = 0; kb < p.blocks; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                                          // the step's tiles are there, and everyone is done with the other's
-    const unsigned char* at = lds + (kb & 1) * STEP;
+#pragma unroll 1
+  for (int kb = 0; kb < p.blocks; ++kb, ++step) {
+    const float sb_next = sbp[min(kb + 1, p.blocks - 1) * p.sb_block];
     float s[TM];
+    f32x4 v[KEEP];
+    const auto add = [&](int q) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) s[i] = sa[i] * sb;
-    if (kb + 1 < p.blocks) {
-      unsigned char* next = lds + ((kb + 1) & 1) * STEP;
-      fetch_tile<BM, WAVES>(p.a, p.a_stride, m0, p.M, (int64_t)(kb + 1) * QB, next);
-      fetch_tile<BN, WAVES>(p.b, p.b_stride, n0, p.N, (int64_t)(kb + 1) * QB, next + BM * QB);
-      sb = sbp[(kb + 1) * p.sb_block];
+      for (int e = 0; e < 4; ++e) acc[q / TN][q % TN][e] = fmaf(v[q % KEEP][e], s[q / TN], acc[q / TN][q % TN][e]);
+      asm volatile("" : "+v"(acc[q / TN][q % TN]));            // (here, and not collected behind the barrier)
+    };
 #pragma unroll
-      for (int i = 0; i < TM; ++i) sa[i] = sap[i][(kb + 1) * p.sa_block];
+    for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(lds + s_at + i * 64);
+#pragma unroll
+    for (int i = 0; i < TM - 1; ++i) {
+      af[(i + 1) & 1] = tile_operand(lds, a_lo, a_hi, (i + 1) * 16);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int q = i * TN + j;
+        v[q % KEEP] = block_product(bf[j], af[i & 1]);
+        if (q == 1) {
+#pragma unroll
+          for (int k = 0; k < TM; ++k) s[k] *= sb;
+        }
+        if (q >= BEHIND) add(q - BEHIND);
+      }
+      // the operand's reads first, then a product and the four multiply-adds of an earlier one in turns
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    i32x8 bf[TN];
+    landed();
+    if (step + 2 < steps) fetch(step);                         // (the buffer of this step: all of it is in registers)
+    a_lo += flip;
+    a_hi += flip;
+    b_lo += flip;
+    b_hi += flip;
+    s_at += flip;
+    flip = 0u - flip;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) bf[j] = tile_operand(at + BM * QB, wn + j * 16);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const i32x8 af = tile_operand(at, wm + i * 16);
-      f32x4 v[TN];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) v[j] = block_product(bf[j], af);
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(v[j][e], s[i], acc[i][j][e]);
+    for (int j = 0; j < TN; ++j) {
+      const int q = (TM - 1) * TN + j;
+      v[q % KEEP] = block_product(bf[j], af[(TM - 1) & 1]);
+      bf[j] = tile_operand(lds, b_lo, b_hi, j * 16);           // (behind the last step: what lies there, unused)
+      add(q - BEHIND);
     }
+    af[0] = tile_operand(lds, a_lo, a_hi, 0);
+    add(Q - 2);
+    add(Q - 1);
+    sb = sb_next;
   }
+  int here = lane;
+  asm volatile("" : "+v"(here));                               // (keeps the stores' addresses out of the steps' registers)
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + wm + i * 16 + i16;
-    if (m >= p.M) continue;
+    const int64_t m = m0 + wm + i * 16 + here % 16;
     char* row = p.out + m * p.out_stride * Tag::bytes;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int64_t n = n0 + wn + j * 16 + g * 4;
-      if (n < p.N) store_four<Tag>(row, n, p.N, acc[i][j]);
+      const int64_t n = n0 + wn + j * 16 + here / 16 * 4;
+      if (m < p.M && n < p.N) store_four<Tag>(row, n, p.N, acc[i][j]);
     }
+  }
   }
 }
 
@@ -308,13 +406,14 @@ static int blocks_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL
 
 template <class Tag, int BM, int BN, int WM, int WN>
 static int launch_tiles(const BlocksParams& p, hipStream_t st) {
-  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * (BM + BN) * QB;
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * ((BM + BN) * QB + BM * 4), per_cu = 160 * 1024 / bytes;
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-  if (tm * tn > 0x7ffffff0LL) return DL_ERR_LIMIT;
+  if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
   if (bytes > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(&tile_kernel<Tag, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
     return DL_ERR_LAUNCH;
-  hipLaunchKernelGGL((tile_kernel<Tag, BM, BN, WM, WN>), dim3((unsigned)((tm * tn + 7) / 8 * 8)), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
+  const unsigned grid = (unsigned)std::min<int64_t>((tm * tn + 7) / 8 * 8, 256 * std::min(per_cu, 2));
+  hipLaunchKernelGGL((tile_kernel<Tag, BM, BN, WM, WN>), dim3(grid), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
   return blocks_status();
 }
 
