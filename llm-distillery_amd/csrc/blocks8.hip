@@ -214,13 +214,14 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const BlocksParams p) {
 // piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in
 // lane order, so it is their source addresses that are permuted.)
 // Within a step a wave goes through its WM / 16 rows of tiles: the operand of the next row is read while the matrix unit works on
-// this one, and the products of the row before are scaled and added meanwhile.  The step's one barrier sits ahead of the last row:
-// by then all operands of the step are in registers, so what follows it -- the last row's products, the first operands of the next
-// step, the fetch into the buffer that has just become free -- keeps the matrix unit busy across it.
+// this one, and the products of the row before are scaled and added meanwhile.  A step's last barrier sits ahead of the last row: by
+// then all operands of the step are in registers, so what follows it -- the last row's products, the first operands of the next step,
+// the fetch into what has just become free -- keeps the matrix unit busy across it.  Another one at half the step frees b's place and
+// half of a's, so that three quarters of the bytes have a step and a half to arrive (what the latency of memory asks for: with
+// one step, waits were a third of the time).
 // Workgroups stay: each walks its tiles as one sequence of steps, so that the next tile's operands arrive while the last one is stored.
 typedef const unsigned __attribute__((address_space(1))) * global_words;
 typedef unsigned __attribute__((address_space(3))) * lds_words;
-typedef const float __attribute__((address_space(4))) * constant_floats;      // read through the scalar unit: not in the fetches' queue
 
 // The operand that begins `lo` / `hi` bytes into LDS for this lane (its two pieces), `rows` (a constant) rows on.
 __device__ __forceinline__ i32x8 tile_operand(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
@@ -248,9 +249,9 @@ template <class Tag, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(const BlocksParams p, unsigned tiles_m, unsigned tiles_n) {
   constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16, NA = BM / 8 / WAVES, NB = BN / 8 / WAVES;
   static_assert(WN <= QB && QB % WN == 0, "a wave's columns share their scales");
-  static_assert(TM >= 2 && BM % WAVE == 0 && BM / WAVE <= WAVES, "");
-  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes, a's BM scales)
-  constexpr int STEP = (BM + BN) * QB + BM * 4;
+  static_assert(TM >= 2 && BM % WAVE == 0 && BN % WAVE == 0 && BM / WAVE < WAVES, "the first waves fetch a's scales, the next one b's");
+  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes, a's BM scales, b's for every BN / 64 columns)
+  constexpr int STEP = (BM + BN) * QB + BM * 4 + WAVE * 4;
   const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), i16 = lane % 16;      // (w: known to be the wave's)
   const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
   const TileWalk walk(tiles_m, tiles_n);
@@ -280,41 +281,63 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
       const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
       f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
     }
-    f_s = p.sa + min(m + (w * WAVE + lane) % BM, p.M - 1) * p.sa_row;
+    f_s = w < BM / WAVE ? p.sa + min(m + w * WAVE + lane, p.M - 1) * p.sa_row : p.sb + min(n + lane * (BN / WAVE), p.N - 1) / QB * p.sb_row;
   };
-  const auto fetch = [&](unsigned step) {
+  // In two parts, by when their places become free: `early` after half a step (b, whose operands are in registers from a step's
+  // beginning on, and of a the rows that the waves go through first), `late` at its end.
+  constexpr bool HALVES = WM / 2 == WAVES * 8;                 // every other fetch of a: those rows
+  constexpr int EARLY = NB + (HALVES ? NA / 2 : 0);
+  const auto fetch_a = [&](unsigned char* to, int i) {
+    __builtin_amdgcn_global_load_lds((global_words)(f_a + f_ao[i]), (lds_words)(to + (i * WAVES + w) * 1024), 16, 0, 0);
+  };
+  const auto fetch_early = [&](unsigned step) {
     unsigned char* to = lds + (step & 1u) * STEP;
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-      __builtin_amdgcn_global_load_lds((global_words)(f_a + f_ao[i]), (lds_words)(to + (i * WAVES + w) * 1024), 16, 0, 0);
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       __builtin_amdgcn_global_load_lds((global_words)(f_b + f_bo[i]), (lds_words)(to + BM * QB + (i * WAVES + w) * 1024), 16, 0, 0);
-    if (w < BM / WAVE) __builtin_amdgcn_global_load_lds((global_words)f_s, (lds_words)(to + (BM + BN) * QB + w * WAVE * 4), 4, 0, 0);
+    if (HALVES)
+#pragma unroll
+      for (int i = 0; i < NA; i += 2) fetch_a(to, i);
+  };
+  const auto fetch_late = [&](unsigned step) {
+    unsigned char* to = lds + (step & 1u) * STEP;
+#pragma unroll
+    for (int i = HALVES ? 1 : 0; i < NA; i += HALVES ? 2 : 1) fetch_a(to, i);
+    if (w <= BM / WAVE) __builtin_amdgcn_global_load_lds((global_words)f_s, (lds_words)(to + (BM + BN) * QB + w * WAVE * 4), 4, 0, 0);
     f_a += QB;
     f_b += QB;
-    f_s += p.sa_block;
+    f_s += w < BM / WAVE ? p.sa_block : p.sb_block;
     if (++f_kb == p.blocks) {
       f_kb = 0;
       f_tile += walk.step;
       if (f_tile < walk.end) f_begin();
     }
   };
-  const auto landed = [&]() {                                  // this wave's fetches are there, its reads done; and everyone's
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  const auto meet = [&]() {                                    // everyone's reads so far are done
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  // This wave's fetches are there but for the last `early` part (loads come back in order; the stores of a tile only add to the count).
+  const auto landed = [&](bool early_under_way) {
+    if (early_under_way) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EARLY) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
 
   f_begin();
-  fetch(0);
-  landed();
-  if (steps > 1) fetch(1);
+  fetch_early(0);
+  fetch_late(0);
+  landed(false);
+  meet();
+  if (steps > 1) {
+    fetch_early(1);
+    fetch_late(1);
+  }
   // Products are scaled and added two behind the one that the matrix unit starts: their results are there by then.
   constexpr int Q = TM * TN, BEHIND = 2, KEEP = BEHIND + 1;
   // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
   const unsigned lo = i16 * QB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
-  unsigned a_lo = wm * QB + lo, a_hi = wm * QB + hi, b_lo = (BM + wn) * QB + lo, b_hi = (BM + wn) * QB + hi, s_at = (BM + BN) * QB + (wm + i16) * 4;
+  unsigned a_lo = wm * QB + lo, a_hi = wm * QB + hi, b_lo = (BM + wn) * QB + lo, b_hi = (BM + wn) * QB + hi, s_at = (BM + BN) * QB + (wm + i16) * 4, sb_at = (BM + BN) * QB + BM * 4 + wn * WAVE / BN * 4;
   unsigned flip = STEP;                                        // from a place in this step's buffer to the other's
   i32x8 bf[TN], af[2];
 #pragma unroll
@@ -326,8 +349,6 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
   walk.origin(tile, m0, n0);
   m0 *= BM;
   n0 *= BN;
-  const constant_floats sbp = (constant_floats)(p.sb + min(n0 + wn, p.N - 1) / QB * p.sb_row);
-  float sb = *sbp;
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -335,7 +356,6 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int kb = 0; kb < p.blocks; ++kb, ++step) {
-    const float sb_next = sbp[min(kb + 1, p.blocks - 1) * p.sb_block];
     float s[TM];
     f32x4 v[KEEP];
     const auto add = [&](int q) {
@@ -345,6 +365,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
     };
 #pragma unroll
     for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(lds + s_at + i * 64);
+    const float sb = *reinterpret_cast<const float*>(lds + sb_at);
 #pragma unroll
     for (int i = 0; i < TM - 1; ++i) {
       af[(i + 1) & 1] = tile_operand(lds, a_lo, a_hi, (i + 1) * 16);
@@ -358,22 +379,28 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
         }
         if (q >= BEHIND) add(q - BEHIND);
       }
-      // the operand's reads first, then a product and the four multiply-adds of an earlier one in turns
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      // a product and the four multiply-adds of an earlier one in turns, the next operand's reads behind the first
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (j == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (i == TM / 2 - 1 && step + 2 < steps) {
+        meet();
+        fetch_early(step);                                     // (into this step's buffer)
+      }
     }
-    landed();
-    if (step + 2 < steps) fetch(step);                         // (the buffer of this step: all of it is in registers)
+    landed(step + 2 < steps);
+    meet();
+    if (step + 2 < steps) fetch_late(step);
     a_lo += flip;
     a_hi += flip;
     b_lo += flip;
     b_hi += flip;
     s_at += flip;
+    sb_at += flip;
     flip = 0u - flip;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -385,7 +412,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
     af[0] = tile_operand(lds, a_lo, a_hi, 0);
     add(Q - 2);
     add(Q - 1);
-    sb = sb_next;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
   }
   int here = lane;
   asm volatile("" : "+v"(here));                               // (keeps the stores' addresses out of the steps' registers)
@@ -406,7 +440,7 @@ static int blocks_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL
 
 template <class Tag, int BM, int BN, int WM, int WN>
 static int launch_tiles(const BlocksParams& p, hipStream_t st) {
-  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * ((BM + BN) * QB + BM * 4), per_cu = 160 * 1024 / bytes;
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * ((BM + BN) * QB + BM * 4 + WAVE * 4), per_cu = 160 * 1024 / bytes;
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
   if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
   if (bytes > 64 * 1024 &&
