@@ -139,74 +139,55 @@ __device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, cons
   }
 }
 
-// Few rows: the weights stream from memory straight into the matrix instructions' operands.  A workgroup's four waves
-// take every fourth block of the same 16 * NT columns (together they read 512 contiguous bytes of each row) and add up in LDS, in
-// the order of the waves.  MT tiles of 16 rows; rows behind the last are read as the last and not stored.
-template <class Tag, int MT, int NT>
+// Up to 16 rows: the weights stream from memory straight into the matrix instructions' operands, a wave 16 columns over all blocks, four
+// blocks ahead of the four it works on (a quarter of a wave reads 64 contiguous bytes of 16 rows; a's few rows come from the caches).
+// Bound by the weights' bytes: 128256 x 4096 in 95 us, 5.5 TB/s.  Rows behind the last are read as the last and not stored.
+// A block's scaled sum is added to those of the blocks before it, here as in the tiles below: a row's result has the same bits
+// whatever rows it comes with.
+constexpr int FEW_ROWS = 16, FEW_AHEAD = 4;
+template <class Tag>
 __global__ __launch_bounds__(256) void few_rows_kernel(const BlocksParams p) {
-  __shared__ float part[4][MT * 16][NT * 16 + 1];
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, g = lane / 16;
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
-  const unsigned char* bp[NT];
-  const float* sbp[NT];
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + w) * 16;
+  if (n0 >= p.N) return;
+  const int64_t m = min((int64_t)i16, p.M - 1);
+  const unsigned char* bp = p.b + min(n0 + i16, p.N - 1) * p.b_stride + g * 16;
+  const unsigned char* ap = p.a + m * p.a_stride + g * 16;
+  const float *sbp = p.sb + n0 / QB * p.sb_row, *sap = p.sa + m * p.sa_row;
+  struct Blocks { i32x8 b[FEW_AHEAD], a[FEW_AHEAD]; float sb[FEW_AHEAD], sa[FEW_AHEAD]; };
+  const auto fetch = [&](int kb0, Blocks& t) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    bp[j] = p.b + min(n0 + j * 16 + i16, p.N - 1) * p.b_stride + g * 16;
-    sbp[j] = p.sb + min(n0 + j * 16, p.N - 1) / QB * p.sb_row;
-  }
-  const unsigned char* ap[MT];
-  const float* sap[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t m = min((int64_t)i * 16 + i16, p.M - 1);
-    ap[i] = p.a + m * p.a_stride + g * 16;
-    sap[i] = p.sa + m * p.sa_row;
-  }
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int kb = w; kb < p.blocks; kb += 4) {
-    i32x8 b[NT], a[MT];
-    float sb[NT], sa[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      b[j] = join_pieces(load16_stream(bp[j] + (int64_t)kb * QB), load16_stream(bp[j] + (int64_t)kb * QB + 64));
-      sb[j] = sbp[j][kb * p.sb_block];
+    for (int i = 0; i < FEW_AHEAD; ++i) {
+      const int64_t kb = min(kb0 + i, p.blocks - 1);
+      t.b[i] = join_pieces(load16_stream(bp + kb * QB), load16_stream(bp + kb * QB + 64));
+      t.a[i] = join_pieces(*reinterpret_cast<const u32x4*>(ap + kb * QB), *reinterpret_cast<const u32x4*>(ap + kb * QB + 64));
+      t.sb[i] = sbp[kb * p.sb_block];
+      t.sa[i] = sap[kb * p.sa_block];
     }
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const auto work = [&](int kb0, const Blocks& t) {
+    f32x4 v[FEW_AHEAD];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      a[i] = join_pieces(*reinterpret_cast<const u32x4*>(ap[i] + (int64_t)kb * QB), *reinterpret_cast<const u32x4*>(ap[i] + (int64_t)kb * QB + 64));
-      sa[i] = sap[i][kb * p.sa_block];
+    for (int i = 0; i < FEW_AHEAD; ++i) v[i] = block_product(t.b[i], t.a[i]);
+#pragma unroll
+    for (int i = 0; i < FEW_AHEAD; ++i) {
+      const float s = t.sa[i] * t.sb[i];
+      if (kb0 + i < p.blocks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[i][e], s, acc[e]);
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const f32x4 v = block_product(b[j], a[i]);
-        const float s = sa[i] * sb[j];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(v[e], s, acc[i][j][e]);
-      }
+  };
+  Blocks now, next;
+  fetch(0, now);
+  for (int kb = 0; kb < p.blocks; kb += 2 * FEW_AHEAD) {
+    fetch(kb + FEW_AHEAD, next);
+    work(kb, now);
+    fetch(kb + 2 * FEW_AHEAD, now);
+    work(kb + FEW_AHEAD, next);
   }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[w][i * 16 + i16][j * 16 + g * 4 + e] = acc[i][j][e];
-  __syncthreads();
-  constexpr int QUADS = NT * 4;
-  for (int q = threadIdx.x; q < MT * 16 * QUADS; q += 256) {
-    const int m = q / QUADS, n = q % QUADS * 4;
-    if (m >= p.M) break;
-    f32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = part[0][m][n + e] + part[1][m][n + e] + part[2][m][n + e] + part[3][m][n + e];
-    if (n0 + n < p.N) store_four<Tag>(p.out + (int64_t)m * p.out_stride * Tag::bytes, n0 + n, p.N, v);
-  }
+  const int64_t n = n0 + g * 4;
+  if (i16 < p.M && n < p.N) store_four<Tag>(p.out + i16 * p.out_stride * Tag::bytes, n, p.N, acc);
 }
 
 // Many rows: tiles of BM x BN, a wave WM x WN of it, one block of 128 columns per step.  A step's operands are fetched into LDS by loads
@@ -333,8 +314,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
     fetch_early(1);
     fetch_late(1);
   }
-  // Products are scaled and added two behind the one that the matrix unit starts: their results are there by then.
-  constexpr int Q = TM * TN, BEHIND = 2, KEEP = BEHIND + 1;
+  // Products are scaled and added three behind the one that the matrix unit starts: their results are there by then.
+  constexpr int Q = TM * TN, BEHIND = 3, KEEP = BEHIND + 1;
   // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
   const unsigned lo = i16 * QB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
   unsigned a_lo = wm * QB + lo, a_hi = wm * QB + hi, b_lo = (BM + wn) * QB + lo, b_hi = (BM + wn) * QB + hi, s_at = (BM + BN) * QB + (wm + i16) * 4, sb_at = (BM + BN) * QB + BM * 4 + wn * WAVE / BN * 4;
@@ -410,8 +391,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
       add(q - BEHIND);
     }
     af[0] = tile_operand(lds, a_lo, a_hi, 0);
-    add(Q - 2);
-    add(Q - 1);
+#pragma unroll
+    for (int q = Q - BEHIND; q < Q; ++q) add(q);
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -419,18 +400,43 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
       __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 4 * BEHIND, 0);
   }
+  // The tile's values.  Two-byte results go through 2 KiB of LDS of the wave's own, 16 rows at a time, so that a store writes whole
+  // 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by unit ^ (row % 8).
   int here = lane;
   asm volatile("" : "+v"(here));                               // (keeps the stores' addresses out of the steps' registers)
+  if constexpr (Tag::bytes == 2 && WN == 64) {
+    unsigned char* stage = lds + 2 * STEP + w * 2048;
+    const int row = here % 16, quad = here / 16, r8 = here / 8, unit = here % 8;
+    const int64_t n = n0 + wn + unit * 8;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + wm + i * 16 + here % 16;
-    char* row = p.out + m * p.out_stride * Tag::bytes;
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int64_t n = n0 + wn + j * 16 + here / 16 * 4;
-      if (m < p.M && n < p.N) store_four<Tag>(row, n, p.N, acc[i][j]);
+      for (int j = 0; j < TN; ++j) {
+        const float f[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], 0.f, 0.f, 0.f, 0.f};
+        const u32x4 c = Chunk<Tag>::pack(f);
+        *reinterpret_cast<u32x2*>(stage + row * 128 + ((j * 2 + quad / 2) ^ (row & 7)) * 16 + (quad & 1) * 8) = u32x2{c[0], c[1]};
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int64_t m = m0 + wm + i * 16 + k * 8 + r8;
+        const u32x4 c = *reinterpret_cast<const u32x4*>(stage + (k * 8 + r8) * 128 + (unit ^ r8) * 16);
+        char* to = p.out + (m * p.out_stride + n) * 2;
+        if (m < p.M && n + 8 <= p.N) store16_stream_any(to, c);
+        else if (m < p.M && n < p.N) store_chunk_elementwise<Tag>(to, 0, (int)(p.N - n), c);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + wm + i * 16 + here % 16;
+      char* row = p.out + m * p.out_stride * Tag::bytes;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + wn + j * 16 + here / 16 * 4;
+        if (m < p.M && n < p.N) store_four<Tag>(row, n, p.N, acc[i][j]);
+      }
     }
   }
   }
@@ -440,29 +446,46 @@ static int blocks_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL
 
 template <class Tag, int BM, int BN, int WM, int WN>
 static int launch_tiles(const BlocksParams& p, hipStream_t st) {
-  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * ((BM + BN) * QB + BM * 4 + WAVE * 4), per_cu = 160 * 1024 / bytes;
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * ((BM + BN) * QB + BM * 4 + WAVE * 4) + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
   if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
   if (bytes > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(&tile_kernel<Tag, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
     return DL_ERR_LAUNCH;
-  const unsigned grid = (unsigned)std::min<int64_t>((tm * tn + 7) / 8 * 8, 256 * std::min(per_cu, 2));
+  const unsigned grid = (unsigned)std::min<int64_t>((tm * tn + 7) / 8 * 8, 256 * std::min(per_cu, 4));
   hipLaunchKernelGGL((tile_kernel<Tag, BM, BN, WM, WN>), dim3(grid), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
   return blocks_status();
 }
 
+// The tile of a call: that with the least time by a model of two numbers each, microseconds for a step of a CU -- alone, and what every
+// further tile of the CU adds -- measured over 15 shapes from 64 x 4096 to 4096 x 8000 (64 x 50257 x 2048: 34, 23, 21, 24 us in
+// the order of the list; 128 x 128256 x 4096: 137, 118, 148, 175; 512 x 128256 x 4096: 271, 335, 428, 519; 128 x 8000 x 4096: 51, 34, 21, 18).
+struct TileShape { int bm, bn; float alone, each; };
+constexpr TileShape TILE_SHAPES[] = {{256, 256, 1.55f, 1.55f}, {128, 256, 1.05f, 1.25f}, {64, 128, 0.62f, 0.43f}, {64, 64, 0.50f, 0.26f}};
+static int tile_shape(int64_t M, int64_t N) {
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const TileShape& t = TILE_SHAPES[i];
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const float time = std::max(t.alone, (float)((tiles + 255) / 256) * t.each);
+    if (i == 0 || time < least) { best = i; least = time; }
+  }
+  return best;
+}
+
 template <class Tag>
 static int launch_blocks(const BlocksParams& p, hipStream_t st) {
-  if (p.M <= 64) {
-    const dim3 grid((unsigned)((p.N + 31) / 32)), nt(256);
-    if (p.M <= 16) hipLaunchKernelGGL((few_rows_kernel<Tag, 1, 2>), grid, nt, 0, st, p);
-    else if (p.M <= 32) hipLaunchKernelGGL((few_rows_kernel<Tag, 2, 2>), grid, nt, 0, st, p);
-    else hipLaunchKernelGGL((few_rows_kernel<Tag, 4, 2>), grid, nt, 0, st, p);
+  if (p.M <= FEW_ROWS) {
+    hipLaunchKernelGGL(few_rows_kernel<Tag>, dim3((unsigned)((p.N + 63) / 64)), dim3(256), 0, st, p);
     return blocks_status();
   }
-  if ((p.M + 255) / 256 * ((p.N + 255) / 256) >= 256) return launch_tiles<Tag, 256, 256, 128, 64>(p, st);
-  if ((p.M + 127) / 128 * ((p.N + 127) / 128) >= 256) return launch_tiles<Tag, 128, 128, 64, 64>(p, st);
-  return launch_tiles<Tag, 64, 64, 32, 32>(p, st);
+  switch (tile_shape(p.M, p.N)) {
+    case 0: return launch_tiles<Tag, 256, 256, 128, 64>(p, st);
+    case 1: return launch_tiles<Tag, 128, 256, 64, 64>(p, st);
+    case 2: return launch_tiles<Tag, 64, 128, 32, 64>(p, st);
+    default: return launch_tiles<Tag, 64, 64, 32, 32>(p, st);
+  }
 }
 
 }  // namespace dl

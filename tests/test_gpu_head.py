@@ -121,10 +121,10 @@ def test_exact_where_every_sum_is(D, M):
 
 def test_rows_do_not_depend_on_their_neighbours(D):
     g = torch.Generator().manual_seed(8)
-    x, w = torch.randn(64, 640, generator=g).to(DEV), torch.randn(3000, 640, generator=g).to(DEV)
+    x, w = torch.randn(2000, 1300, generator=g).to(DEV), torch.randn(9001, 1300, generator=g).to(DEV)
     b = D.quantize_blocks(w, rows=128)
     whole = D.matmul_blocks(D.quantize_blocks(x), b, dtype=torch.float32)
-    for lo, hi in ((0, 1), (5, 21), (10, 50)):
+    for lo, hi in ((0, 1), (5, 21), (10, 50), (3, 200), (100, 900), (1000, 1016)):
         assert torch.equal(D.matmul_blocks(D.quantize_blocks(x[lo:hi]), b, dtype=torch.float32), whole[lo:hi])
 
 
