@@ -610,7 +610,7 @@ int dl_div_topk_rest(float beta, const void* logits, int logits_dtype, int64_t r
  * out [M, N] of out_dtype, rounded once.  K columns, in whole blocks whose tails hold zeros.  A block's products are summed inside the
  * matrix unit, where the sum of 128 products is off by up to 2^-12 of the sum of their magnitudes (products far smaller than the
  * largest are cut off); block sums are scaled and added in fp32, one block after
- * the other, whatever M and N: a row's result has the same bits whatever rows it comes with.  Up to 16 rows stream the weights.
+ * the other, whatever M and N: a row's result has the same bits whatever rows it comes with.
  *
  * codes, a and b: 16-byte aligned, strides of whole 16 bytes, at least the whole blocks (DL_ERR_ALIGN, DL_ERR_SHAPE); x and out: any
  * element-aligned address and stride.  Scale strides in elements, not negative.

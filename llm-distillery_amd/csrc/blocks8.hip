@@ -139,58 +139,7 @@ __device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, cons
   }
 }
 
-// Up to 16 rows: the weights stream from memory straight into the matrix instructions' operands, a wave 16 columns over all blocks, four
-// blocks ahead of the four it works on (a quarter of a wave reads 64 contiguous bytes of 16 rows; a's few rows come from the caches).
-// Bound by the weights' bytes: 128256 x 4096 in 95 us, 5.5 TB/s.  Rows behind the last are read as the last and not stored.
-// A block's scaled sum is added to those of the blocks before it, here as in the tiles below: a row's result has the same bits
-// whatever rows it comes with.
-constexpr int FEW_ROWS = 16, FEW_AHEAD = 4;
-template <class Tag>
-__global__ __launch_bounds__(256) void few_rows_kernel(const BlocksParams p) {
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, g = lane / 16;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + w) * 16;
-  if (n0 >= p.N) return;
-  const int64_t m = min((int64_t)i16, p.M - 1);
-  const unsigned char* bp = p.b + min(n0 + i16, p.N - 1) * p.b_stride + g * 16;
-  const unsigned char* ap = p.a + m * p.a_stride + g * 16;
-  const float *sbp = p.sb + n0 / QB * p.sb_row, *sap = p.sa + m * p.sa_row;
-  struct Blocks { i32x8 b[FEW_AHEAD], a[FEW_AHEAD]; float sb[FEW_AHEAD], sa[FEW_AHEAD]; };
-  const auto fetch = [&](int kb0, Blocks& t) {
-#pragma unroll
-    for (int i = 0; i < FEW_AHEAD; ++i) {
-      const int64_t kb = min(kb0 + i, p.blocks - 1);
-      t.b[i] = join_pieces(load16_stream(bp + kb * QB), load16_stream(bp + kb * QB + 64));
-      t.a[i] = join_pieces(*reinterpret_cast<const u32x4*>(ap + kb * QB), *reinterpret_cast<const u32x4*>(ap + kb * QB + 64));
-      t.sb[i] = sbp[kb * p.sb_block];
-      t.sa[i] = sap[kb * p.sa_block];
-    }
-  };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const auto work = [&](int kb0, const Blocks& t) {
-    f32x4 v[FEW_AHEAD];
-#pragma unroll
-    for (int i = 0; i < FEW_AHEAD; ++i) v[i] = block_product(t.b[i], t.a[i]);
-#pragma unroll
-    for (int i = 0; i < FEW_AHEAD; ++i) {
-      const float s = t.sa[i] * t.sb[i];
-      if (kb0 + i < p.blocks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[i][e], s, acc[e]);
-    }
-  };
-  Blocks now, next;
-  fetch(0, now);
-  for (int kb = 0; kb < p.blocks; kb += 2 * FEW_AHEAD) {
-    fetch(kb + FEW_AHEAD, next);
-    work(kb, now);
-    fetch(kb + 2 * FEW_AHEAD, now);
-    work(kb + FEW_AHEAD, next);
-  }
-  const int64_t n = n0 + g * 4;
-  if (i16 < p.M && n < p.N) store_four<Tag>(p.out + i16 * p.out_stride * Tag::bytes, n, p.N, acc);
-}
-
-// Many rows: tiles of BM x BN, a wave WM x WN of it, one block of 128 columns per step.  A step's operands are fetched into LDS by loads
+// Tiles of BM x BN, a wave WM x WN of it, one block of 128 columns per step.  A step's operands are fetched into LDS by loads
 // that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted by
 // piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in
 // lane order, so it is their source addresses that are permuted.)
@@ -476,10 +425,6 @@ static int tile_shape(int64_t M, int64_t N) {
 
 template <class Tag>
 static int launch_blocks(const BlocksParams& p, hipStream_t st) {
-  if (p.M <= FEW_ROWS) {
-    hipLaunchKernelGGL(few_rows_kernel<Tag>, dim3((unsigned)((p.N + 63) / 64)), dim3(256), 0, st, p);
-    return blocks_status();
-  }
   switch (tile_shape(p.M, p.N)) {
     case 0: return launch_tiles<Tag, 256, 256, 128, 64>(p, st);
     case 1: return launch_tiles<Tag, 128, 256, 64, 64>(p, st);
