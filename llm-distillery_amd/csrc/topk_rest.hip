@@ -11,11 +11,11 @@
 //
 // Layout as in the forward-KL kernels: a row, or one column part of it, sits in its workgroup's registers; parts exchange
 // (max, sum) of the rest's columns through records in a workspace, with a bounded wait and a second launch for parts
-// that gave up.  Listed columns are taken out of the registers (-inf in their place) before the row's statistics, so
-// that the rest's mass is a sum of what it consists of and not 1 minus the listed mass: a confident student leaves it
-// 1e-8, which that difference would lose.  Every part works out all K outcomes itself (some ten microseconds of one
-// workgroup against exchanging K values): listed logits of other parts are fetched straight from memory, behind the
-// part's own loads, when the line is on its way to another part of the XCD anyway.
+// that gave up.  Listed columns are taken out of the registers (-inf in their place, by a bit per column in LDS) before the
+// row's statistics, so that the rest's mass is a sum of what it consists of and not 1 minus the listed mass: a confident
+// student leaves it 1e-8, which that difference would lose.  Every thread keeps a few entries in registers: their ids are asked
+// for ahead of the row, their logits (all K of a row, in every part: the lines are on their way to some workgroup of the XCD
+// anyway) behind it, and their maxima and sums travel in the barriers that the row's own need.
 #include "topk_div.hpp"
 #include "distill_hip.h"
 
@@ -31,27 +31,29 @@ struct RestParams {
   void* workspace; int parts; int spin_limit;
 };
 
-// Lists of the row's entries by the 16-byte chunk of their column (chunks that share a head share a list).
+// Lists of the row's entries by the 16-byte chunk of their column (chunks that share a head share a list), and a byte per
+// chunk of the part: which of its columns are listed.
 struct RestLds {
   int *idx, *next, *head;
-  float *lp, *z, *val, *red, *xm, *xs;
+  float *lp, *red, *xm, *xs;
   int* xok;
-  unsigned* own;
-  __device__ RestLds(unsigned char* base, int K) {
+  unsigned *own, *mask;
+  __device__ RestLds(unsigned char* base, int K, int threads) {
     const int Kp = (K + 3) & ~3;
     idx = reinterpret_cast<int*>(base);
     next = idx + Kp;
     lp = reinterpret_cast<float*>(next + Kp);
-    z = lp + Kp;
-    val = z + Kp;
-    red = val + Kp;
+    red = lp + Kp;
     xm = red + 64;
     xs = xm + MAX_PARTS;
     xok = reinterpret_cast<int*>(xs + MAX_PARTS);
     head = xok + MAX_PARTS;
     own = reinterpret_cast<unsigned*>(head + CORRECTION_HEADS);
+    mask = own + threads;
   }
-  static size_t bytes(int K, int threads) { return (size_t)(5 * ((K + 3) & ~3) + 64 + 3 * MAX_PARTS + CORRECTION_HEADS + threads) * 4; }
+  static size_t bytes(int K, int threads, int chunks) {
+    return (size_t)(3 * ((K + 3) & ~3) + 64 + 3 * MAX_PARTS + CORRECTION_HEADS + threads + (threads * chunks + 3) / 4) * 4;
+  }
 };
 
 // One outcome's part of the loss, and s = q dL/dq.  The logarithm of the mixture goes through log1p / expm1 on the side
@@ -78,8 +80,28 @@ __device__ __forceinline__ void rest_outcome(float lp, float lq, float beta, flo
   }
 }
 
-// `RETRY`: the part is finished by the second launch; every record of the row is there.
-template <class Tag, int NT, int NCH, bool SPLIT, bool RETRY>
+// The listed columns of a chunk (`bits`) become -inf.
+template <class Tag>
+__device__ __forceinline__ void take_out(u32x4& c, unsigned bits) {
+  if constexpr (Tag::bytes == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = (bits >> j) & 1u ? 0xff800000u : c[j];
+  } else {
+    constexpr unsigned inf = Tag::id == BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = (bits >> (2 * j)) & 1u ? (c[j] & 0xffff0000u) | inf : c[j];
+      c[j] = (bits >> (2 * j + 1)) & 1u ? (c[j] & 0xffffu) | (inf << 16) : c[j];
+    }
+  }
+}
+
+// Makes the compiler work `v` out here: a sum that is only needed behind a branch is put off to there otherwise, and all that goes into
+// it stays in registers.
+__device__ __forceinline__ void keep(float& v) { asm volatile("" : "+v"(v)); }
+
+// J entries per thread (K <= J * NT).  `RETRY`: the part is finished by the second launch; every record of the row is there.
+template <class Tag, int NT, int NCH, int J, bool SPLIT, bool RETRY>
 __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s, int64_t r, int h) {
   using C = Chunk<Tag>;
   using M = ChunkMap<NT, NCH>;
@@ -96,7 +118,15 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
   const char* rpart = row + lo * Tag::bytes;
 
-  correction_clear<NT>(s.head, s.own);
+  int64_t id[J];
+  float lp[J], z[J];
+  const int cnt = p.t_cnt ? min(p.K, max(p.t_cnt[trow], 0)) : p.K;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int k = j * NT + tid;
+    id[j] = k < cnt ? load_index(p.t_idx, p.t_idx_itype, trow * p.K + k) : -1;
+    lp[j] = k < cnt ? load_as_float(p.t_val, p.t_val_dtype, trow * p.K + k) : -INFINITY;
+  }
   u32x4 reg[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -105,83 +135,66 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
     if (c < nch) reg[i] = load16_unaligned(rpart + (int64_t)c * 16);
     else if (c == nch && tail) reg[i] = load_chunk_elementwise<Tag>(rpart, c, n_cols);
   }
+  correction_clear<NT>(s.head, s.own);
+#pragma unroll
+  for (int i = 0; i < (NCH + 3) / 4; ++i)
+    if (i * NT + tid < (NT * NCH + 3) / 4) s.mask[i * NT + tid] = 0u;
   __syncthreads();
-  const int cnt = p.t_cnt ? min(p.K, max(p.t_cnt[trow], 0)) : p.K;
-  for (int k = tid; k < p.K; k += NT) {
-    const int64_t id = k < cnt ? load_index(p.t_idx, p.t_idx_itype, trow * p.K + k) : -1;
-    const float lp = k < cnt ? load_as_float(p.t_val, p.t_val_dtype, trow * p.K + k) : -INFINITY;
-    const bool counts = id >= 0 && id < p.V && lp != -INFINITY;
-    s.idx[k] = counts ? (int)id : -1;
-    s.lp[k] = lp;
-    if (counts) {
-      s.next[k] = atomicExch(&s.head[(int)(id / C::N) & (CORRECTION_HEADS - 1)], k);
-      if (id >= lo && id < lo + n_cols) {
-        const int c = (int)(id - lo) / C::N;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int k = j * NT + tid;
+    z[j] = -INFINITY;
+    if (!(id[j] >= 0 && id[j] < p.V && lp[j] != -INFINITY)) lp[j] = -INFINITY;      // does not count
+    if (k < p.K) {
+      s.idx[k] = lp[j] != -INFINITY ? (int)id[j] : -1;
+      s.lp[k] = lp[j];
+    }
+    if (lp[j] != -INFINITY) {
+      s.next[k] = atomicExch(&s.head[(int)(id[j] / C::N) & (CORRECTION_HEADS - 1)], k);
+      if (id[j] >= lo && id[j] < lo + n_cols) {
+        const int at = (int)(id[j] - lo), c = at / C::N;
         atomicOr(&s.own[M::owner(c)], 1u << M::reg(c));
+        atomicOr(&s.mask[c / 4], 1u << (8 * (c % 4) + at % C::N));
       }
+      z[j] = load_as_float(row, Tag::id, id[j]);
     }
   }
   __syncthreads();
-  // An id that is listed again has its masses added up, in the order of its entries, in the first of them; val = -inf
-  // marks the others, and entries that do not count.
-  for (int k = tid; k < p.K; k += NT) {
-    const int id = s.idx[k];
-    float lp = s.lp[k];
-    if (id < 0) {
-      lp = -INFINITY;
-    } else {
-      const int first = s.head[(id / C::N) & (CORRECTION_HEADS - 1)];
-      bool again = false, later = false;
-      for (int j = first; j >= 0; j = s.next[j])
-        if (j != k && s.idx[j] == id) { again = true; later = later || j < k; }
-      if (later) {
-        lp = -INFINITY;
-      } else if (again) {
-        float sum = expf(lp);
-        for (int at = k;;) {
-          int next = p.K;
-          for (int j = first; j >= 0; j = s.next[j])
-            if (j > at && j < next && s.idx[j] == id) next = j;
-          if (next == p.K) break;
-          sum += expf(s.lp[next]);
-          at = next;
-        }
-        lp = logf(sum);
+  // An id that is listed again has its masses added up, in the order of its entries, in the first of them; the others no longer count.
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    if (lp[j] == -INFINITY) continue;
+    const int k = j * NT + tid, first = s.head[(int)(id[j] / C::N) & (CORRECTION_HEADS - 1)];
+    bool again = false, later = false;
+    for (int q = first; q >= 0; q = s.next[q])
+      if (q != k && s.idx[q] == (int)id[j]) { again = true; later = later || q < k; }
+    if (later) {
+      lp[j] = -INFINITY;
+    } else if (again) {
+      float sum = expf(lp[j]);
+      for (int at = k;;) {
+        int next = p.K;
+        for (int q = first; q >= 0; q = s.next[q])
+          if (q > at && q < next && s.idx[q] == (int)id[j]) next = q;
+        if (next == p.K) break;
+        sum += expf(s.lp[next]);
+        at = next;
       }
-      if (SPLIT && (id < lo || id >= lo + n_cols)) s.z[k] = load_as_float(row, Tag::id, id);
+      lp[j] = logf(sum);
     }
-    s.val[k] = lp;
   }
   const unsigned mine = s.own[tid];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    if (mine & (1u << i)) {
-      const int gc = (int)(lo / C::N) + M::chunk(i, tid);
-      float f[C::N];
-      C::unpack(reg[i], f);
-      for (int k = s.head[gc & (CORRECTION_HEADS - 1)]; k >= 0; k = s.next[k]) {
-        const int id = s.idx[k], e = id - gc * C::N;
-        if (e < 0 || e >= C::N) continue;
-        float x = 0.f;
-#pragma unroll
-        for (int j = 0; j < C::N; ++j) x = j == e ? f[j] : x;
-        s.z[k] = x;
-        if constexpr (Tag::bytes == 4) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) reg[i][j] = j == e ? 0xff800000u : reg[i][j];
-        } else {
-          const unsigned inf = Tag::id == BF16 ? 0xff80u : 0xfc00u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j == e / 2) reg[i][j] = (e & 1) ? (reg[i][j] & 0xffffu) | (inf << 16) : (reg[i][j] & 0xffff0000u) | inf;
-        }
-      }
-    }
+    forget(reg[i]);                      // (chunk by chunk: no pile-up of masks and halves)
+    if (mine & (1u << i)) take_out<Tag>(reg[i], reinterpret_cast<const unsigned char*>(s.mask)[M::chunk(i, tid)]);
+    forget(reg[i]);
   }
 
-  // the rest's columns: max, sum of 2^(x a - max a); the powers stay in the registers for the gradient
+  // maxima of the rest's columns and of the listed ones; then the sums of the powers over them, and the teacher's mass.  The rest's
+  // powers 2^(x a - max a) stay in the registers for the gradient.
   const float a = p.inv_T * LOG2E;
-  float mx = -INFINITY;
+  float mx = -INFINITY, zmax = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     float f[C::N];
@@ -189,8 +202,14 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
     C::unpack(reg[i], f);
 #pragma unroll
     for (int e = 0; e < C::N; ++e) mx = fmaxf(mx, f[e]);
+    keep(mx);
   }
-  mx = block_max<NT>(mx, s.red);
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    z[j] *= a;
+    if (lp[j] != -INFINITY) zmax = fmaxf(zmax, z[j]);
+  }
+  block_max2<NT>(mx, zmax, s.red);
   constexpr float BIAS = C::stash_bias;
   float mb = mx * a;
   // A rest of nothing but masked columns counts as none, whatever they are masked with (distill_common.hpp: MASKED_BELOW; two-byte
@@ -198,7 +217,7 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   const bool masked = mb < (Tag::bytes == 2 ? -0x1p20f : MASKED_BELOW);
   if (masked) { mb = 0.f; mx = -INFINITY; }
   const float mb_own = mb - BIAS;
-  float sm = 0.f;
+  float sm = 0.f, zs = 0.f, ps = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     float f[C::N];
@@ -209,10 +228,18 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
       f[e] = fast_exp2(fmaf(f[e], a, -mb_own));
       sm += f[e];
     }
+    keep(sm);
     reg[i] = C::stash(f);
     forget(reg[i]);
   }
-  sm = block_sum<NT>(sm * __builtin_exp2f(-BIAS), s.red);
+  sm *= __builtin_exp2f(-BIAS);
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (lp[j] != -INFINITY) {
+      ps += expf(lp[j]);
+      zs += zmax == -INFINITY ? (z[j] == z[j] ? 0.f : z[j]) : fast_exp2(z[j] - zmax);
+    }
+  block_sum3<NT>(sm, zs, ps, s.red);
 
   if (SPLIT) {
     PartStats* ws = reinterpret_cast<PartStats*>(p.workspace) + r * P;
@@ -246,28 +273,18 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   const float b = mb + fast_log2(sm);    // log2 of the rest's sum: -inf where no column outside the list has a finite logit
 
   // the K outcomes and the rest
-  float zmax = -INFINITY, ps = 0.f;
-  for (int k = tid; k < p.K; k += NT)
-    if (s.val[k] != -INFINITY) {
-      zmax = fmaxf(zmax, s.z[k] * a);
-      ps += expf(s.val[k]);
-    }
-  zmax = fmaxf(block_max<NT>(zmax, s.red), b);
-  float zs = 0.f;
-  for (int k = tid; k < p.K; k += NT)
-    if (s.val[k] != -INFINITY) zs += fast_exp2(s.z[k] * a - zmax);
-  block_sum2<NT>(zs, ps, s.red);
   const bool rest = !(b == -INFINITY);
-  if (zmax == -INFINITY || (!rest && ps == 0.f)) return leave();      // no finite logit, or nothing to compare
-  const float lse = zmax + fast_log2(zs + (rest ? fast_exp2(b - zmax) : 0.f));
+  const float top = fmaxf(zmax, b);
+  if (top == -INFINITY && zs == 0.f) return leave();                  // no finite logit
+  if (!rest && ps == 0.f) return leave();                             // nothing to compare
+  const float lse = top + fast_log2((zmax == -INFINITY ? zs : zs * fast_exp2(zmax - top)) + (rest ? fast_exp2(b - top) : 0.f));
   const float p0 = rest ? fmaxf(1.f - ps, p.rest_min) : 0.f, lz = logf(ps + p0);
-  float loss = 0.f, slopes = 0.f;
-  for (int k = tid; k < p.K; k += NT)
-    if (s.val[k] != -INFINITY) {
-      float slope;
-      rest_outcome(s.val[k] - lz, (s.z[k] * a - lse) * LN2, p.beta, loss, slope);
-      slopes += slope;
-      s.lp[k] = slope;
+  float loss = 0.f, slopes = 0.f, slope[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (lp[j] != -INFINITY) {
+      rest_outcome(lp[j] - lz, (z[j] - lse) * LN2, p.beta, loss, slope[j]);
+      slopes += slope[j];
     }
   block_sum2<NT>(loss, slopes, s.red);
   float slope0 = 0.f, q0 = 0.f;
@@ -280,8 +297,12 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   if (tid == 0 && h == 0 && p.row_loss) p.row_loss[r] = loss;
   if (!gpart) return;
   const float c = p.inv_T * p.grad_scale;
-  for (int k = tid; k < p.K; k += NT)
-    if (s.val[k] != -INFINITY) s.lp[k] = (s.lp[k] - fast_exp2(s.z[k] * a - lse) * slopes) * c;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int k = j * NT + tid;
+    if (lp[j] != -INFINITY) s.lp[k] = (slope[j] - fast_exp2(z[j] - lse) * slopes) * c;
+    else if (k < p.K) s.idx[k] = -1;
+  }
   const float kc = !rest || masked ? 0.f : fast_exp2(mb_own - b) * (slope0 - q0 * slopes) * c;      // stashed power -> gradient
   __syncthreads();
 #pragma unroll
@@ -297,7 +318,7 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
         const int gc = (int)(lo / C::N) + ch;
         for (int k = s.head[gc & (CORRECTION_HEADS - 1)]; k >= 0; k = s.next[k]) {
           const int e = s.idx[k] - gc * C::N;
-          if (e < 0 || e >= C::N || s.val[k] == -INFINITY) continue;
+          if (e < 0 || e >= C::N) continue;                           // (entries that do not count: -1)
           const float v = s.lp[k];
 #pragma unroll
           for (int j = 0; j < C::N; ++j) f[j] = j == e ? v : f[j];
@@ -309,30 +330,30 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   }
 }
 
-template <class Tag, int NT, int NCH, bool SPLIT>
+template <class Tag, int NT, int NCH, int J, bool SPLIT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void rest_kernel(const RestParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const RestLds s(smem, p.K);
+  const RestLds s(smem, p.K, NT);
   const int P = SPLIT ? p.parts : 1;
   const unsigned grp = SPLIT ? blockIdx.x / (8u * P) : 0u, t_in = SPLIT ? blockIdx.x % (8u * P) : 0u;
   const int64_t r = SPLIT ? (int64_t)grp * 8 + (t_in & 7u) : xcd_banded_row(blockIdx.x);
   if (r >= p.n_rows) return;
-  rest_part<Tag, NT, NCH, SPLIT, false>(p, s, r, SPLIT ? (int)(t_in >> 3) : 0);
+  rest_part<Tag, NT, NCH, J, SPLIT, false>(p, s, r, SPLIT ? (int)(t_in >> 3) : 0);
 }
 
-template <class Tag, int NT, int NCH>
+template <class Tag, int NT, int NCH, int J>
 __device__ __attribute__((noinline)) void rest_part_again(const RestParams& p, const RestLds& s, unsigned at) {
-  rest_part<Tag, NT, NCH, true, true>(p, s, (int64_t)(at / (unsigned)p.parts), (int)(at % (unsigned)p.parts));
+  rest_part<Tag, NT, NCH, J, true, true>(p, s, (int64_t)(at / (unsigned)p.parts), (int)(at % (unsigned)p.parts));
 }
-template <class Tag, int NT, int NCH>
+template <class Tag, int NT, int NCH, int J>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void rest_retry_kernel(const RestParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const RestLds s(smem, p.K);
+  const RestLds s(smem, p.K, NT);
   const RetryList list(p.workspace, p.n_rows, p.parts);
   const unsigned n = *list.count;
 #pragma unroll 1
   for (unsigned e = blockIdx.x; e < n; e += gridDim.x) {
-    rest_part_again<Tag, NT, NCH>(p, s, list.entries[e]);
+    rest_part_again<Tag, NT, NCH, J>(p, s, list.entries[e]);
     __syncthreads();
   }
 }
@@ -351,16 +372,28 @@ static RestShape rest_shape(int64_t nch) {
   return {256, per_thread <= 13 ? 13 : per_thread <= 14 ? 14 : 16, (int)parts};
 }
 
+// Entries per thread: two, or as many as the most entries ask for.
+template <class Tag, int NT, int NCH, int J>
+static void launch_rest_row_j(const RestParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, J, false>), dim3(xcd_banded_grid(p.n_rows)), dim3(NT), RestLds::bytes(p.K, NT, NCH), st, p);
+}
 template <class Tag, int NT, int NCH>
 static void launch_rest_row(const RestParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, false>), dim3(xcd_banded_grid(p.n_rows)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
+  if (p.K <= 2 * NT) launch_rest_row_j<Tag, NT, NCH, 2>(p, st);
+  else launch_rest_row_j<Tag, NT, NCH, DL_MAX_TOPK / NT>(p, st);
+}
+template <class Tag, int NT, int NCH, int J>
+static void launch_rest_parts_j(const RestParams& p, hipStream_t st) {
+  const size_t lds = RestLds::bytes(p.K, NT, NCH);
+  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, J, true>), dim3((unsigned)((p.n_rows + 7) / 8 * 8 * p.parts)), dim3(NT), lds, st, p);
+  hipLaunchKernelGGL((rest_retry_kernel<Tag, NT, NCH, J>), dim3((unsigned)std::min<int64_t>(p.n_rows * p.parts, 256)), dim3(NT), lds, st, p);
 }
 template <class Tag, int NT, int NCH>
 static void launch_rest_parts(const RestParams& p, hipStream_t st) {
   const int64_t n16 = split_clear_words(p.n_rows, p.parts);
   hipLaunchKernelGGL(clear_workspace_kernel<256>, dim3((unsigned)((n16 + 255) / 256)), dim3(256), 0, st, reinterpret_cast<u32x4*>(p.workspace), n16);
-  hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, true>), dim3((unsigned)((p.n_rows + 7) / 8 * 8 * p.parts)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
-  hipLaunchKernelGGL((rest_retry_kernel<Tag, NT, NCH>), dim3((unsigned)std::min<int64_t>(p.n_rows * p.parts, 256)), dim3(NT), RestLds::bytes(p.K, NT), st, p);
+  if (p.K <= 2 * NT) launch_rest_parts_j<Tag, NT, NCH, 2>(p, st);
+  else launch_rest_parts_j<Tag, NT, NCH, DL_MAX_TOPK / NT>(p, st);
 }
 
 template <class Tag>
