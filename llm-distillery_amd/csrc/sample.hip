@@ -45,17 +45,18 @@ __device__ __forceinline__ float sample_t(const RowScale& s, float x) {
   const float d = x - s.top;
   return fmaxf(d * s.rate, -64.f);
 }
-// 2^(t + 31), every operation rounded by itself
+// 2^(t + 31), every operation rounded by itself.  t plus 1.5 * 2^23 is rint(t) in the lowest bits; the coefficients carry the 2^31 (a
+// power of two changes no rounding), and 2^rint(t) is added to the exponent.
 __device__ __forceinline__ float sample_power(float t) {
 #pragma clang fp contract(off)
-  const float n = rintf(t), f = t - n;
-  float p = 0x1.5bba14p-10f;
-  p = p * f + 0x1.3cea88p-7f;
-  p = p * f + 0x1.c6b752p-5f;
-  p = p * f + 0x1.ebf9bcp-3f;
-  p = p * f + 0x1.62e42ap-1f;
-  p = p * f + 1.f;
-  return __builtin_amdgcn_ldexpf(p, (int)n + 31);
+  const float r = t + 0x1.8p23f, f = t - (r - 0x1.8p23f);
+  float p = 0x1.5bba14p21f;
+  p = p * f + 0x1.3cea88p24f;
+  p = p * f + 0x1.c6b752p26f;
+  p = p * f + 0x1.ebf9bcp28f;
+  p = p * f + 0x1.62e42ap30f;
+  p = p * f + 0x1p31f;
+  return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
 }
 __device__ __forceinline__ unsigned sample_weight(float t) { return (unsigned)sample_power(t); }
 __device__ __forceinline__ int sample_bin(float t) { return min((int)(t * -32.f), SAMPLE_BINS - 1); }      // rounded towards 0
@@ -70,35 +71,48 @@ __device__ __forceinline__ float word_logit(u64 w) { return logit_of(~(unsigned)
 // floor(mass * part / 2^24)
 __device__ __forceinline__ u64 share_of(u64 mass, unsigned part) { return (mass >> 24) * part + (((mass & 0xffffffu) * part) >> 24); }
 
-// f(logit, column) for every column of [lo, hi) of a row, on any element boundary; eight loads in flight per thread.
+// f(logits, n, column) for a row's columns in pieces of n <= 8 (4-byte logits: 4) neighbours, on any element boundary; the pieces of a
+// thread that are whole come eight loads ahead.  Places behind n hold -inf.
 template <class Tag, int NT, class F>
-__device__ __forceinline__ void each_logit(const char* row, int64_t lo, int64_t hi, F f) {
+__device__ __forceinline__ void each_piece(const char* row, int64_t V, F f) {
   using C = Chunk<Tag>;
-  const char* at = row + lo * Tag::bytes;
-  const int n = (int)(hi - lo), whole = n / C::N;
+  const int n = (int)V, whole = n / C::N;
   constexpr int UN = 4;
   u32x4 v[UN], ahead[UN];
   const auto fetch = [&](int c0, u32x4* to) {
 #pragma unroll
     for (int i = 0; i < UN; ++i)
-      if (c0 + i * NT < whole) to[i] = load16_unaligned(at + (int64_t)(c0 + i * NT) * 16);
+      if (c0 + i * NT < whole) to[i] = load16_unaligned(row + (int64_t)(c0 + i * NT) * 16);
   };
+  float x[C::N];
   fetch(threadIdx.x, v);
   for (int c0 = threadIdx.x; c0 < whole; c0 += NT * UN) {
     fetch(c0 + NT * UN, ahead);                  // the next four are on their way while these are worked on
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       if (c0 + i * NT >= whole) break;
-      float x[C::N];
       C::unpack(v[i], x);
-#pragma unroll
-      for (int e = 0; e < C::N; ++e) f(x[e], (int)lo + (c0 + i * NT) * C::N + e);
+      f(x, C::N, (c0 + i * NT) * C::N);
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) v[i] = ahead[i];
   }
   const int col = whole * C::N + (int)threadIdx.x;
-  if (col < n) f(load_as_float(at, Tag::id, col), (int)lo + col);
+  if (col < n) {
+#pragma unroll
+    for (int e = 1; e < C::N; ++e) x[e] = -INFINITY;
+    x[0] = load_as_float(row, Tag::id, col);
+    f(x, 1, col);
+  }
+}
+// f(logit, column) for every column.
+template <class Tag, int NT, class F>
+__device__ __forceinline__ void each_logit(const char* row, int64_t V, F f) {
+  each_piece<Tag, NT>(row, V, [&](const float* x, int n, int col) {
+#pragma unroll
+    for (int e = 0; e < Chunk<Tag>::N; ++e)
+      if (e < n) f(x[e], col + e);
+  });
 }
 
 // A bin behind which every token has less weight than `least`: the threshold's, and two more for what rounding does to it.
@@ -201,29 +215,45 @@ struct Sampler {
   __device__ int bin_passing(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] <= m && s.mass[b + 1] > m; }); }
 
   // Tokens for which in(t, x) holds (and that have a weight; only t > below is asked) into the list, in order, with their masses
-  // behind `mass`.  Most of a row is far below: one comparison of the logit itself, with room for what rounding does to t, is
-  // all that it costs.
+  // behind `mass`.  Most of a row is far below: one comparison for several logits themselves, with room for what rounding
+  // does to t, is all that it costs.
   template <class Tag, class In>
   __device__ void collect(unsigned before, u64 mass, float below, In in) {
+    collect<Tag>(before, mass, below, in, [](float) {});
+  }
+  // (`also` is called with every logit of the row)
+  template <class Tag, class In, class Also>
+  __device__ void collect(unsigned before, u64 mass, float below, In in, Also also) {
     const float far = sc.top + fmaxf(below, -33.f) / sc.rate;
     const float least = far - 1e-5f * (fabsf(far) + fabsf(sc.top));
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each_logit<Tag, NT>(row, 0, V, [&](float x, int col) {
-      if (!(x >= least)) return;
-      const float t = sample_t(sc, x);
-      if (in(t, x) && sample_weight(t) > 0) {
-        const unsigned at = atomicAdd(&s.n, 1u);
-        if (at < SAMPLE_CAP) s.word[at] = sample_word(x, col);
+    each_piece<Tag, NT>(row, V, [&](const float* x, int count, int col) {
+      float most = x[0];
+#pragma unroll
+      for (int e = 0; e < Chunk<Tag>::N; ++e) {
+        if (e < count) also(x[e]);
+        most = fmaxf(most, x[e]);
+      }
+      if (!(most >= least)) return;
+#pragma unroll
+      for (int e = 0; e < Chunk<Tag>::N; ++e) {
+        if (!(x[e] >= least)) continue;
+        const float t = sample_t(sc, x[e]);
+        if (in(t, x[e]) && sample_weight(t) > 0) {
+          const unsigned at = atomicAdd(&s.n, 1u);
+          if (at < SAMPLE_CAP) s.word[at] = sample_word(x[e], col + e);
+        }
       }
     });
     __syncthreads();
     overflow = s.n > SAMPLE_CAP;
     n = min((int)s.n, SAMPLE_CAP);
-    sort();
     ahead = before;
     ahead_mass = mass;
+    if (overflow) return;
+    sort();
     constexpr int EACH = SAMPLE_CAP / NT;
     unsigned w[EACH], none = 0;
     u64 sum_w = 0;
@@ -288,6 +318,23 @@ struct Sampler {
     lo_bin = lo;
     hi_bin = hi;
   }
+  // The likeliest tokens without a histogram of the row: every thread has met some logits while the row's maximum was looked for,
+  // and the q-th largest of the threads' own maxima (`met`) has at least q tokens at or above it, not many more: the last of
+  // the bins that hold them (count: zeros before).  The list then gets those bins, in a sweep in which `also` sees the row.
+  __device__ int likeliest_bins(float met, unsigned q) {
+    const float t = sample_t(sc, met);
+    if (t >= -31.f) atomicAdd(&s.count[sample_bin(t)], 1u);      // (a token has a weight from t = -31 on)
+    __syncthreads();
+    scan_bins<SAMPLE_BINS>(s.mass, s.count);
+    return s.count[SAMPLE_BINS] < q ? SAMPLE_BINS - 1 : bin_of_count(q);
+  }
+  template <class Tag, class Also>
+  __device__ void collect_likeliest(int hi, Also also) {
+    const float below = hi == SAMPLE_BINS - 1 ? -65.f : -(float)(hi + 1) * 0.03125f;
+    collect<Tag>(0, 0, below, [&](float t, float) { return t > below; }, also);
+    lo_bin = 0;
+    hi_bin = hi;
+  }
   // Look-ups in the list as it is.
   __device__ void in_list_reaching(u64 m, unsigned& tokens, u64& mass) {
     const int i = find(n, [&](int j) { return s.upto[j] >= m && (j == 0 ? ahead_mass : s.upto[j - 1]) < m; });
@@ -329,7 +376,7 @@ struct Sampler {
       __syncthreads();
       for (int i = threadIdx.x; i <= 256; i += NT) { mass[i] = 0; count[i] = 0; }
       __syncthreads();
-      each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+      each_logit<Tag, NT>(row, V, [&](float x, int) {
         const float t = sample_t(sc, x);
         if (sample_bin(t) != bin) return;
         const unsigned o = order_of(x), w = sample_weight(t);
@@ -447,7 +494,7 @@ struct Sampler {
     }
     // Too many for the list: the largest logit with too small a weight, then what lies above it.
     unsigned worst = 0;
-    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+    each_logit<Tag, NT>(row, V, [&](float x, int) {
       const unsigned w = sample_weight(sample_t(sc, x));
       if (w > 0 && w < least) worst = max(worst, order_of(x));
     });
@@ -458,7 +505,7 @@ struct Sampler {
     for (int i = 0; i < NW; ++i) worst = max(worst, s.wave_count[i]);
     u64 m = 0;
     unsigned c = 0;
-    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+    each_logit<Tag, NT>(row, V, [&](float x, int) {
       const unsigned w = sample_weight(sample_t(sc, x));
       if (w > 0 && order_of(x) > worst) { m += w; ++c; }
     });
@@ -495,7 +542,7 @@ __device__ __attribute__((noinline)) RowResult sample_maximum(SampleLds& s, cons
   u64 none = 0;
   ties = 0;
   unsigned first = 0xffffffffu;
-  each_logit<Tag, NT>(row, 0, V, [&](float x, int col) {
+  each_logit<Tag, NT>(row, V, [&](float x, int col) {
     if (x == top) {
       ++ties;
       first = min(first, (unsigned)col);
@@ -514,14 +561,18 @@ __device__ __attribute__((noinline)) RowResult sample_maximum(SampleLds& s, cons
   return RowResult{j == 0 ? (int)first : a.template equal_logit<Tag>(j), n, 0.f};
 }
 
+__device__ __forceinline__ void clear_bins(SampleLds& s, int threads) {
+  __syncthreads();
+  for (int b = threadIdx.x; b <= SAMPLE_BINS; b += threads) { s.mass[b] = 0; s.count[b] = 0; }
+  __syncthreads();
+}
+
 // Any row: a histogram of masses and counts, every look-up by the bins.
 template <class Tag, int NT>
 __device__ __attribute__((noinline)) RowResult sample_any(SampleLds& s, const char* row, int64_t V, const RowScale sc, const RowCuts cuts) {
   Sampler<NT> a(s, row, V, sc);
-  __syncthreads();
-  for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) { s.mass[b] = 0; s.count[b] = 0; }
-  __syncthreads();
-  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+  clear_bins(s, NT);
+  each_logit<Tag, NT>(row, V, [&](float x, int) {
     const float t = sample_t(sc, x);
     const unsigned w = sample_weight(t);
     if (w > 0) {
@@ -554,31 +605,73 @@ __device__ __attribute__((noinline)) RowResult sample_any(SampleLds& s, const ch
   return res;
 }
 
-// Rows with top-k whose first k tokens fit the list: counts of tokens per bin, first of those within 2^-16 of the most likely one
-// (few, and with them few additions in LDS), of all if that is not enough.  (A token has a weight from t = -31 on.)
-// False: not decided here.  `powers`: the sum of 2^(t + 31).
+// The usual rows: all that is asked lies among the likeliest tokens.  Two sweeps over the row, this is the second.  False: not
+// decided here.  `powers`: the sum of 2^(t + 31).
 template <class Tag, int NT>
-__device__ __forceinline__ bool sample_top_k(SampleLds& s, const char* row, int64_t V, const RowScale& sc, RowCuts cuts, float& powers, RowResult& res) {
+__device__ __forceinline__ bool sample_likeliest(SampleLds& s, const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float met, float& powers, RowResult& res) {
   Sampler<NT> a(s, row, V, sc);
-  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
-    const float t = sample_t(sc, x);
-    powers += fast_exp2(t);
-    if (t > -16.f) atomicAdd(&s.count[sample_bin(t)], 1u);
-  });
-  powers = block_sum<NT>(powers, s.red) * 0x1p31f;
-  a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
-  if (s.count[SAMPLE_BINS] < (unsigned)cuts.k) {
-    __syncthreads();
-    for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) s.count[b] = 0;
-    __syncthreads();
-    each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+  unsigned tokens = 0, live = 0;
+  u64 mass = 0;
+  if (cuts.k > 0) {
+    a.template collect_likeliest<Tag>(a.likeliest_bins(met, cuts.k), [&](float x) { powers += fast_exp2(sample_t(sc, x)); });
+    powers = block_sum<NT>(powers, s.red) * 0x1p31f;
+    if (a.overflow || (a.n < cuts.k && a.hi_bin < SAMPLE_BINS - 1)) return false;
+    tokens = min(a.n, cuts.k);
+    mass = s.upto[tokens - 1];
+  } else {
+    const int hi = a.likeliest_bins(met, NT / 4);
+    // what lies behind them could outweigh the maximum several times: the histogram at once
+    if (hi < SAMPLE_BINS - 1 && (float)V * fast_exp2(-(float)(hi + 1) * 0.03125f) > 8.f) return false;
+    a.template collect_likeliest<Tag>(hi, [&](float x) {
+      const float e = sample_power(sample_t(sc, x));
+      powers += e;
+      const unsigned w = (unsigned)e;
+      mass += w;
+      live += __popcll(__ballot(w > 0));      // (of the wave: the scalar unit counts)
+    });
+    tokens = (threadIdx.x & (WAVE - 1)) == 0 ? live : 0u;
+    powers = block_sum<NT>(powers, s.red);
+    a.sum(mass, tokens);
+    if (a.overflow) return false;
+  }
+  const u64 listed = s.upto[a.n - 1];
+  if (cuts.top_p) {
+    const u64 want = mass_wanted(mass, cuts.part);
+    if (want > listed) {
+      if (cuts.least == 0 || bin_behind(cuts.least) > a.hi_bin) return false;      // (else min-p cuts ahead of that)
+    } else {
+      a.in_list_reaching(want, tokens, mass);
+    }
+  }
+  if (cuts.least > 0) {
+    if (tokens > (unsigned)a.n && bin_behind(cuts.least) > a.hi_bin) return false;
+    a.in_list_below(cuts.least, tokens, mass);
+  }
+  const u64 want = share_of(mass, cuts.u);
+  if (want >= listed) return false;
+  res.token = a.in_list_token(want, res.t);
+  res.kept = tokens;
+  return true;
+}
+
+// Rows with top-k whose first k tokens fit the list: counts of tokens per bin, first of those within 2^-16 of the most likely one
+// (few, and with them few additions in LDS), of all if that is not enough.  False: not decided here.
+template <class Tag, int NT>
+__device__ __forceinline__ bool sample_top_k(SampleLds& s, const char* row, int64_t V, const RowScale& sc, RowCuts cuts, RowResult& res) {
+  Sampler<NT> a(s, row, V, sc);
+  float least = -16.f;
+  for (;;) {
+    clear_bins(s, NT);
+    each_logit<Tag, NT>(row, V, [&](float x, int) {
       const float t = sample_t(sc, x);
-      if (t >= -31.f) atomicAdd(&s.count[sample_bin(t)], 1u);
+      if (t >= least) atomicAdd(&s.count[sample_bin(t)], 1u);
     });
     __syncthreads();
     a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
-    cuts.k = min(cuts.k, (int)s.count[SAMPLE_BINS]);
+    if (s.count[SAMPLE_BINS] >= (unsigned)cuts.k || least == -31.f) break;
+    least = -31.f;
   }
+  cuts.k = min(cuts.k, (int)s.count[SAMPLE_BINS]);
   const int bin = a.bin_of_count(cuts.k);
   if (s.count[bin + 1] > SAMPLE_CAP) return false;
   a.template collect_bins<Tag>(0, bin);
@@ -597,7 +690,9 @@ template <class Tag, int NT>
 __device__ __forceinline__ bool sample_by_mass(SampleLds& s, const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float& powers, RowResult& res) {
   Sampler<NT> a(s, row, V, sc);
   unsigned tokens = 0;
-  each_logit<Tag, NT>(row, 0, V, [&](float x, int) {
+  powers = 0.f;
+  clear_bins(s, NT);
+  each_logit<Tag, NT>(row, V, [&](float x, int) {
     const float t = sample_t(sc, x), e = sample_power(t);
     powers += e;
     const unsigned w = (unsigned)e;
@@ -643,9 +738,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   const int64_t r = blockIdx.x;
   const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
   for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) { s.mass[b] = 0; s.count[b] = 0; }
-  float top = -INFINITY;
-  each_logit<Tag, NT>(row, 0, p.V, [&](float x, int) { top = fmaxf(top, x); });
-  top = block_max<NT>(top, s.red);
+  float met = -INFINITY;                     // the largest logit that this thread has met
+  each_logit<Tag, NT>(row, p.V, [&](float x, int) { met = fmaxf(met, x); });
+  const float top = block_max<NT>(met, s.red);
   if (top == -INFINITY) {                    // nothing to draw from
     if (threadIdx.x == 0) {
       p.token[r] = -1;
@@ -665,8 +760,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   } else {
     const RowScale sc{top, LOG2E / T};
     float powers = 0.f;
-    const bool done = cuts.k > 0 ? sample_top_k<Tag, NT>(s, row, p.V, sc, cuts, powers, res) : sample_by_mass<Tag, NT>(s, row, p.V, sc, cuts, powers, res);
-    if (!done) res = sample_any<Tag, NT>(s, row, p.V, sc, cuts);
+    if (!sample_likeliest<Tag, NT>(s, row, p.V, sc, cuts, met, powers, res)) {
+      const bool done = cuts.k > 0 ? sample_top_k<Tag, NT>(s, row, p.V, sc, cuts, res) : sample_by_mass<Tag, NT>(s, row, p.V, sc, cuts, powers, res);
+      if (!done) res = sample_any<Tag, NT>(s, row, p.V, sc, cuts);
+    }
     logp = (res.t - log2f(powers * 0x1p-31f)) * LN2;
   }
   if (threadIdx.x == 0) {
