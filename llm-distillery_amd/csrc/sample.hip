@@ -619,7 +619,7 @@ __device__ __forceinline__ bool sample_likeliest(SampleLds& s, const char* row, 
     tokens = min(a.n, cuts.k);
     mass = s.upto[tokens - 1];
   } else {
-    const int hi = a.likeliest_bins(met, NT / 4);
+    const int hi = a.likeliest_bins(met, 128);      // (a list of somewhat more: up to 256 are sorted by counting)
     // what lies behind them could outweigh the maximum several times: the histogram at once
     if (hi < SAMPLE_BINS - 1 && (float)V * fast_exp2(-(float)(hi + 1) * 0.03125f) > 8.f) return false;
     a.template collect_likeliest<Tag>(hi, [&](float x) {
