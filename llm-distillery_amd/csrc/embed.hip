@@ -65,20 +65,42 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const char* __restrict_
 }
 
 // ---- zeroes that ride along ---------------------------------------------------------------------------
-// Bytes [from, to) of a [vocab, width] gradient are zeroed by `blocks` workgroups of a launch.
+// `rows` stretches of `row_bytes` at a pitch (the last one of `last`), zeroed by `blocks` workgroups of a launch.  A dense gradient is cut
+// into stretches of ZERO_PIECE bytes from its first 16-byte boundary on, `head` bytes ahead of that: whole lines whatever the
+// width.  Streaming stores from many short-lived workgroups: 131 MB in 22 us (from 2048 workgroups: 26; ordinary stores: 34).
+constexpr int64_t ZERO_PIECE = 4096, ZERO_BLOCKS = 16384;
 struct ZeroShare {
-  char* base; int64_t pitch_bytes, row_bytes, row0, row1; unsigned blocks;
+  char* base; int64_t pitch, row_bytes, last, rows; int head; unsigned blocks;
 };
-// Workgroup b of z.blocks: whole rows, dealt in turn; 16 bytes per store from the row's first 16-byte boundary on.
+__device__ __forceinline__ void zero_elements(char* at, int bytes) {      // elements of 2 or 4 bytes, fewer than 16 bytes
+  if ((int)threadIdx.x * 2 < bytes) reinterpret_cast<unsigned short*>(at)[threadIdx.x] = 0;
+}
 __device__ __forceinline__ void zero_rows(const ZeroShare& z, unsigned b) {
   const int tid = threadIdx.x, nt = blockDim.x;
-  for (int64_t r = z.row0 + b; r < z.row1; r += z.blocks) {
-    char* row = z.base + r * z.pitch_bytes;
-    const int64_t head = min((int64_t)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15), z.row_bytes), whole = (z.row_bytes - head) / 16;
+  if (b == 0) zero_elements(z.base - z.head, z.head);
+  for (int64_t r = b; r < z.rows; r += z.blocks) {
+    char* row = z.base + r * z.pitch;
+    const int64_t bytes = r + 1 < z.rows ? z.row_bytes : z.last;
+    const int64_t head = min((int64_t)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15), bytes), whole = (bytes - head) / 16;
     for (int64_t c = tid; c < whole; c += nt) store16_stream(row + head + c * 16, u32x4{0u, 0u, 0u, 0u});
-    const int64_t beside = z.row_bytes - whole * 16;          // bytes on either side: whole elements of 2 or 4 bytes
-    for (int64_t i = tid * 2; i < beside; i += nt * 2) *reinterpret_cast<unsigned short*>(row + (i < head ? i : whole * 16 + i)) = 0;
+    zero_elements(row, (int)head);
+    zero_elements(row + head + whole * 16, (int)(bytes - head - whole * 16));
   }
+}
+// Rows [r0, r1) of a gradient with `width` bytes of a row's `pitch`.
+static ZeroShare zero_share(char* grad, int64_t pitch, int64_t width, int64_t r0, int64_t r1) {
+  ZeroShare z{grad + r0 * pitch, pitch, width, width, std::max<int64_t>(r1 - r0, 0), 0, 0};
+  if (pitch == width && z.rows > 0) {
+    int64_t bytes = z.rows * pitch;
+    z.head = (int)std::min<int64_t>((16 - (reinterpret_cast<uintptr_t>(z.base) & 15)) & 15, bytes);
+    z.base += z.head;
+    bytes -= z.head;
+    z.pitch = z.row_bytes = ZERO_PIECE;
+    z.rows = (bytes + ZERO_PIECE - 1) / ZERO_PIECE;
+    z.last = bytes - (z.rows - 1) * ZERO_PIECE;
+  }
+  z.blocks = (unsigned)std::min<int64_t>(std::max<int64_t>(z.rows, z.head > 0), ZERO_BLOCKS);
+  return z;
 }
 
 // ---- sort ---------------------------------------------------------------------------------------------
@@ -490,15 +512,10 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
   int64_t row = 0;
   int launch = 0;
   const auto share = [&]() {
-    ZeroShare z{};
-    z.base = reinterpret_cast<char*>(grad);
-    z.pitch_bytes = grad_stride * (int64_t)ob;
-    z.row_bytes = width * (int64_t)ob;
-    z.row0 = row;
     ++launch;
-    z.row1 = row = accumulate ? 0 : vocab * launch / launches;
-    z.blocks = (unsigned)std::min<int64_t>(z.row1 - z.row0, 2048);
-    return z;
+    const int64_t first = row;
+    row = accumulate ? 0 : vocab * launch / launches;
+    return zero_share(reinterpret_cast<char*>(grad), grad_stride * (int64_t)ob, width * (int64_t)ob, first, row);
   };
   const unsigned long long* sorted = words[0];
   if (passes == 0) {
