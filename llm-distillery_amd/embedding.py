@@ -14,13 +14,15 @@ def _tokens_1d(tokens: torch.Tensor, dev: torch.device) -> torch.Tensor:
     _dev(tokens, "tokens", dev)
     if tokens.dtype not in _IT:
         raise RuntimeError("tokens must be int32 or int64")
-    return tokens.reshape(-1).contiguous()
+    return tokens if tokens.dim() == 1 and tokens.is_contiguous() else tokens.reshape(-1).contiguous()
 
 
 def _matrix(t: torch.Tensor, name: str) -> None:
     if t.dim() != 2 or t.dtype not in _DT:
         raise RuntimeError(f"{name} must be a bf16/fp16/fp32 matrix")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1] or t.shape[1] > 1 and t.stride(1) != 1:
+    rows, width = t.shape
+    pitch, one = t.stride()
+    if rows > 1 and pitch < width or width > 1 and one != 1:
         raise RuntimeError(f"{name} must be dense along its rows")
 
 

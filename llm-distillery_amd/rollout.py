@@ -101,9 +101,7 @@ def quantize_blocks(x: torch.Tensor, *, rows: int = 1) -> BlockQuantized:
     _dev(x, "x")
     if rows not in (1, 128):
         raise ValueError("rows must be 1 or 128")
-    if x.dim() == 1:
-        x = x.unsqueeze(0)
-    v = _rows_2d(x)
+    v = x if x.dim() == 2 and x.stride(1) == 1 else _rows_2d(x if x.dim() > 1 else x.unsqueeze(0))
     if v.dtype not in _DT:
         raise RuntimeError("unsupported dtype")
     R, W = v.shape
@@ -111,7 +109,7 @@ def quantize_blocks(x: torch.Tensor, *, rows: int = 1) -> BlockQuantized:
     kb = _blocks(W)
     codes = torch.empty((R, kb * 128), dtype=torch.float8_e4m3fn, device=dev)
     if rows == 1:
-        scales = torch.empty((kb, R), dtype=torch.float32, device=dev).t()      # the scales of a block of columns side by side
+        scales = torch.empty_strided((R, kb), (1, R), dtype=torch.float32, device=dev)      # the scales of a block of columns side by side
     else:
         scales = torch.empty((_blocks(R), kb), dtype=torch.float32, device=dev)
     if R and W:
@@ -122,13 +120,18 @@ def quantize_blocks(x: torch.Tensor, *, rows: int = 1) -> BlockQuantized:
     return BlockQuantized(codes, scales, W)
 
 
-def _check_blocks(q: BlockQuantized, name: str, groups: int, dev: torch.device) -> None:
-    _dev(q.codes, f"{name}.codes", dev), _dev(q.scales, f"{name}.scales", dev)
-    if q.codes.dtype != torch.float8_e4m3fn or q.codes.dim() != 2 or q.codes.shape[1] != _blocks(q.width) * 128 or \
-            (q.codes.numel() and (q.codes.stride(1) != 1 or q.codes.shape[0] > 1 and q.codes.stride(0) < q.codes.shape[1])):
+def _check_blocks(q: BlockQuantized, name: str, groups: int, blocks: int, dev: torch.device):
+    """(address, row stride) of the codes and (address, strides) of the scales of an operand."""
+    codes, scales = q.codes, q.scales
+    if codes.device != dev or scales.device != dev:
+        _dev(codes, f"{name}.codes", dev), _dev(scales, f"{name}.scales", dev)
+    rows, wide = codes.shape
+    pitch, one = codes.stride()
+    if codes.dtype != torch.float8_e4m3fn or wide != blocks * 128 or rows and (one != 1 or rows > 1 and pitch < wide):
         raise RuntimeError(f"{name}.codes must be a float8_e4m3fn matrix of whole blocks of 128 columns, dense along its rows")
-    if q.scales.dtype != torch.float32 or tuple(q.scales.shape) != (groups, _blocks(q.width)):
-        raise RuntimeError(f"{name}.scales must be fp32 [{groups}, {_blocks(q.width)}], not {tuple(q.scales.shape)}")
+    if scales.dtype != torch.float32 or scales.shape != (groups, blocks):
+        raise RuntimeError(f"{name}.scales must be fp32 [{groups}, {blocks}], not {tuple(scales.shape)}")
+    return codes.data_ptr(), pitch if rows > 1 else wide, scales.data_ptr(), *scales.stride()
 
 
 def matmul_blocks(a: BlockQuantized, b: BlockQuantized, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -140,19 +143,19 @@ def matmul_blocks(a: BlockQuantized, b: BlockQuantized, *, dtype: torch.dtype = 
     dev = a.codes.device
     if dtype not in _DT:
         raise RuntimeError("unsupported dtype")
-    M, N = a.codes.shape[0], b.codes.shape[0]
-    if a.width != b.width:
-        raise RuntimeError(f"a has {a.width} columns, b {b.width}")
-    _dev(a.codes, "a.codes")
-    _check_blocks(a, "a", M, dev)
-    _check_blocks(b, "b", _blocks(N), dev)
-    if a.width == 0:
+    if a.codes.dim() != 2 or b.codes.dim() != 2:
+        raise RuntimeError("codes must be matrices")
+    M, N, W = a.codes.shape[0], b.codes.shape[0], a.width
+    if W != b.width:
+        raise RuntimeError(f"a has {W} columns, b {b.width}")
+    if W == 0:
         raise RuntimeError("the rows have no columns")
+    _dev(a.codes, "a.codes")
+    blocks = _blocks(W)
+    left, right = _check_blocks(a, "a", M, blocks, dev), _check_blocks(b, "b", _blocks(N), blocks, dev)
     out = torch.empty((M, N), dtype=dtype, device=dev)
     if M and N:
         with _on(dev):
-            st = _lib.load().dl_matmul_blocks(a.codes.data_ptr(), _row_pitch(a.codes), a.scales.data_ptr(), a.scales.stride(0), a.scales.stride(1), M,
-                                              b.codes.data_ptr(), _row_pitch(b.codes), b.scales.data_ptr(), b.scales.stride(0), b.scales.stride(1), N,
-                                              a.width, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
+            st = _lib.load().dl_matmul_blocks(*left, M, *right, N, W, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
         _lib.check(st, "dl_matmul_blocks")
     return out
