@@ -73,7 +73,7 @@ __device__ __forceinline__ u64 share_of(u64 mass, unsigned part) { return (mass 
 
 // f(logits, n, column) for a row's columns in pieces of n <= 8 (4-byte logits: 4) neighbours, on any element boundary; the pieces of a
 // thread that are whole come eight loads ahead.  Places behind n hold -inf.
-template <class Tag, int NT, class F>
+template <class Tag, int NT, bool UNROLLED = true, class F>
 __device__ __forceinline__ void each_piece(const char* row, int64_t V, F f) {
   using C = Chunk<Tag>;
   const int n = (int)V, whole = n / C::N;
@@ -88,11 +88,22 @@ __device__ __forceinline__ void each_piece(const char* row, int64_t V, F f) {
   fetch(threadIdx.x, v);
   for (int c0 = threadIdx.x; c0 < whole; c0 += NT * UN) {
     fetch(c0 + NT * UN, ahead);                  // the next four are on their way while these are worked on
+    if constexpr (UNROLLED) {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      if (c0 + i * NT >= whole) break;
-      C::unpack(v[i], x);
-      f(x, C::N, (c0 + i * NT) * C::N);
+      for (int i = 0; i < UN; ++i) {
+        if (c0 + i * NT >= whole) break;
+        C::unpack(v[i], x);
+        f(x, C::N, (c0 + i * NT) * C::N);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < UN; ++i) {
+        if (c0 + i * NT >= whole) break;
+        C::unpack(v[0], x);
+        f(x, C::N, (c0 + i * NT) * C::N);
+#pragma unroll
+        for (int j = 1; j < UN; ++j) v[j - 1] = v[j];
+      }
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) v[i] = ahead[i];
@@ -106,9 +117,9 @@ __device__ __forceinline__ void each_piece(const char* row, int64_t V, F f) {
   }
 }
 // f(logit, column) for every column.
-template <class Tag, int NT, class F>
+template <class Tag, int NT, bool UNROLLED = true, class F>
 __device__ __forceinline__ void each_logit(const char* row, int64_t V, F f) {
-  each_piece<Tag, NT>(row, V, [&](const float* x, int n, int col) {
+  each_piece<Tag, NT, UNROLLED>(row, V, [&](const float* x, int n, int col) {
 #pragma unroll
     for (int e = 0; e < Chunk<Tag>::N; ++e)
       if (e < n) f(x[e], col + e);
@@ -127,11 +138,19 @@ struct SampleLds {
   unsigned n, hit;
   float red[16];
 };
+// (the same for a row, whose address a called function gets without that knowledge)
+__device__ __forceinline__ const char* global_row(const char* row) { return (const char*)(const __attribute__((address_space(1))) char*)row; }
+__device__ __forceinline__ SampleLds& sample_lds() {      // (known as LDS also in functions that are called)
+  __shared__ SampleLds s;
+  return s;
+}
 
-template <int NT>
+// (Every function of it is inlined: the list's bounds stay in registers and what they index is known to be LDS.  Called, they go through
+// scratch memory and generic addresses: FIGURES.  ROLLED: the sweeps' code once and not four times.)
+template <int NT, bool ROLLED = false>
 struct Sampler {
   static constexpr int NW = NT / WAVE;
-  SampleLds& s;
+  SampleLds& s = sample_lds();
   const char* row;
   int64_t V;
   RowScale sc;
@@ -141,10 +160,10 @@ struct Sampler {
   u64 ahead_mass = 0;
   bool overflow = false;                     // more tokens than the list holds
 
-  __device__ Sampler(SampleLds& lds, const char* r, int64_t v, const RowScale& scale) : s(lds), row(r), V(v), sc(scale) {}
+  __device__ __forceinline__ Sampler(const char* r, int64_t v, const RowScale& scale) : row(r), V(v), sc(scale) {}
 
   // Sums over the workgroup of a pair; the result in every thread.
-  __device__ void sum(u64& mass, unsigned& count) {
+  __device__ __forceinline__ void sum(u64& mass, unsigned& count) {
     const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
 #pragma unroll
     for (int o = WAVE / 2; o > 0; o >>= 1) {
@@ -159,7 +178,7 @@ struct Sampler {
     for (int i = 0; i < NW; ++i) { mass += s.wave_mass[i]; count += s.wave_count[i]; }
   }
   // Exclusive sums over the workgroup's threads, in order.
-  __device__ void scan(u64& mass, unsigned& count) {
+  __device__ __forceinline__ void scan(u64& mass, unsigned& count) {
     const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
     const u64 m0 = mass;
     const unsigned c0 = count;
@@ -178,7 +197,7 @@ struct Sampler {
   }
   // Masses and counts of bins -> of all bins ahead; entry `bins` gets the totals.
   template <int BINS>
-  __device__ void scan_bins(u64* mass, unsigned* count) {
+  __device__ __forceinline__ void scan_bins(u64* mass, unsigned* count) {
     constexpr int EACH = (BINS + NT - 1) / NT;
     u64 m[EACH], mm = 0;
     unsigned c[EACH], cc = 0;
@@ -203,33 +222,33 @@ struct Sampler {
   }
   // The one index b < bins for which test(b) holds, in every thread.
   template <class Test>
-  __device__ int find(int bins, Test test) {
+  __device__ __forceinline__ int find(int bins, Test test) {
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += NT)
       if (test(b)) s.hit = (unsigned)b;
     __syncthreads();
     return (int)s.hit;
   }
-  __device__ int bin_of_count(unsigned q) { return find(SAMPLE_BINS, [&](int b) { return s.count[b] < q && s.count[b + 1] >= q; }); }
-  __device__ int bin_reaching(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] < m && s.mass[b + 1] >= m; }); }
-  __device__ int bin_passing(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] <= m && s.mass[b + 1] > m; }); }
+  __device__ __forceinline__ int bin_of_count(unsigned q) { return find(SAMPLE_BINS, [&](int b) { return s.count[b] < q && s.count[b + 1] >= q; }); }
+  __device__ __forceinline__ int bin_reaching(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] < m && s.mass[b + 1] >= m; }); }
+  __device__ __forceinline__ int bin_passing(u64 m) { return find(SAMPLE_BINS, [&](int b) { return s.mass[b] <= m && s.mass[b + 1] > m; }); }
 
   // Tokens for which in(t, x) holds (and that have a weight; only below < t <= above is asked) into the list, in order, with their masses
   // behind `mass`.  Most of a row is far below: one comparison for several logits themselves, with room for what rounding
   // does to t, is all that it costs.
   template <class Tag, class In>
-  __device__ void collect(unsigned before, u64 mass, float above, float below, In in) {
+  __device__ __forceinline__ void collect(unsigned before, u64 mass, float above, float below, In in) {
     collect<Tag>(before, mass, above, below, in, [](float) {});
   }
   // (`also` is called with every logit of the row)
   template <class Tag, class In, class Also>
-  __device__ void collect(unsigned before, u64 mass, float above, float below, In in, Also also) {
+  __device__ __forceinline__ void collect(unsigned before, u64 mass, float above, float below, In in, Also also) {
     const float far = sc.top + fmaxf(below, -33.f) / sc.rate;
     const float least = far - 1e-5f * (fabsf(far) + fabsf(sc.top));
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
-    each_piece<Tag, NT>(row, V, [&](const float* x, int count, int col) {
+    each_piece<Tag, NT, !ROLLED>(row, V, [&](const float* x, int count, int col) {
       float most = x[0];
 #pragma unroll
       for (int e = 0; e < Chunk<Tag>::N; ++e) {
@@ -275,7 +294,7 @@ struct Sampler {
   }
   // The list's words, of tokens above t = `below` and at most t = `above`, ascending.  Up to 256: every word's place is the number of words
   // below it (all are different).
-  __device__ void sort(float above, float below) {
+  __device__ __forceinline__ void sort(float above, float below) {
     const int tid = threadIdx.x;
     if (n <= 256) {
       u64 mine = 0;
@@ -297,7 +316,7 @@ struct Sampler {
   // More: dealt to 1024 bins of t, then every word counts those below it in its bin.  (top_k = 400 of 2048 x 50257
   // rows: 254 us with a bitonic sort through registers, 169 so.  Where a bin holds too many words, equal logits mostly, that sort is
   // what is left: false.)
-  __device__ bool sort_by_bins(float above, float below) {
+  __device__ __forceinline__ bool sort_by_bins(float above, float below) {
     constexpr int BINS = 1024, MOST = 192, EACH = SAMPLE_CAP / NT, PER = BINS / NT;
     unsigned* start = reinterpret_cast<unsigned*>(s.upto);       // free until the masses go there
     const float scale = (float)BINS / (above - fmaxf(below, -32.f));
@@ -354,7 +373,7 @@ struct Sampler {
     return true;
   }
   template <int EACH>
-  __device__ void sort_in_registers() {
+  __device__ __forceinline__ void sort_in_registers() {
     u64 w[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) w[j] = (int)threadIdx.x * EACH + j < n ? s.word[threadIdx.x * EACH + j] : ~0ull;
@@ -366,7 +385,7 @@ struct Sampler {
   }
   // (The tokens ahead are counted on the way: the counts of the bins may be estimates.)
   template <class Tag>
-  __device__ void collect_bins(int lo, int hi) {
+  __device__ __forceinline__ void collect_bins(int lo, int hi) {
     const float above = -(float)lo * 0.03125f, below = hi == SAMPLE_BINS - 1 ? -65.f : -(float)(hi + 1) * 0.03125f;      // bin lo .. hi: below < t <= above
     unsigned before = 0;
     collect<Tag>(0, s.mass[lo], above, below, [&](float t, float) {
@@ -379,10 +398,33 @@ struct Sampler {
     lo_bin = lo;
     hi_bin = hi;
   }
+  // Bins [lo, hi] and, further down, `end`, in one sweep: the list has the tokens of both, their masses those of the row.  (in_list_reaching
+  // is for masses that `end` reaches then, in_list_token for those that [lo, hi] or `end` passes.)
+  template <class Tag>
+  __device__ __forceinline__ void collect_two(int lo, int hi, int end) {
+    const float above = -(float)lo * 0.03125f, below = -(float)(hi + 1) * 0.03125f, above_end = -(float)end * 0.03125f, below_end = end == SAMPLE_BINS - 1 ? -65.f : -(float)(end + 1) * 0.03125f;
+    const u64 gap = s.mass[end] - s.mass[hi + 1];
+    unsigned before = 0, first = 0;
+    collect<Tag>(0, s.mass[lo], above, below_end, [&](float t, float) {
+      before += t > above_end;
+      const bool one = t <= above && t > below, two = t <= above_end && t > below_end;
+      first += one;
+      return one || two;
+    });
+    if (overflow) return;
+    for (int i = threadIdx.x; i < n; i += NT)
+      if (sample_t(sc, word_logit(s.word[i])) <= above_end) s.upto[i] += gap;
+    u64 both = ((u64)first << 32) | before;
+    unsigned none = 0;
+    sum(both, none);
+    ahead = (unsigned)both - (unsigned)(both >> 32);             // of the row's place and the list's, from `end` on
+    lo_bin = lo;
+    hi_bin = hi;
+  }
   // The likeliest tokens without a histogram of the row: every thread has met some logits while the row's maximum was looked for,
   // and the q-th largest of the threads' own maxima (`met`) has at least q tokens at or above it, not many more: the last of
   // the bins that hold them (count: zeros before).  The list then gets those bins, in a sweep in which `also` sees the row.
-  __device__ int likeliest_bins(float met, unsigned q) {
+  __device__ __forceinline__ int likeliest_bins(float met, unsigned q) {
     const float t = sample_t(sc, met);
     if (t >= -31.f) atomicAdd(&s.count[sample_bin(t)], 1u);      // (a token has a weight from t = -31 on)
     __syncthreads();
@@ -390,25 +432,25 @@ struct Sampler {
     return s.count[SAMPLE_BINS] < q ? SAMPLE_BINS - 1 : bin_of_count(q);
   }
   template <class Tag, class Also>
-  __device__ void collect_likeliest(int hi, Also also) {
+  __device__ __forceinline__ void collect_likeliest(int hi, Also also) {
     const float below = hi == SAMPLE_BINS - 1 ? -65.f : -(float)(hi + 1) * 0.03125f;
     collect<Tag>(0, 0, 0.f, below, [&](float t, float) { return t > below; }, also);
     lo_bin = 0;
     hi_bin = hi;
   }
   // Look-ups in the list as it is.
-  __device__ void in_list_reaching(u64 m, unsigned& tokens, u64& mass) {
+  __device__ __forceinline__ void in_list_reaching(u64 m, unsigned& tokens, u64& mass) {
     const int i = find(n, [&](int j) { return s.upto[j] >= m && (j == 0 ? ahead_mass : s.upto[j - 1]) < m; });
     tokens = ahead + (unsigned)i + 1;
     mass = s.upto[i];
   }
-  __device__ int in_list_token(u64 m, float& t) {
+  __device__ __forceinline__ int in_list_token(u64 m, float& t) {
     const int i = find(n, [&](int k) { return s.upto[k] > m && (k == 0 ? ahead_mass : s.upto[k - 1]) <= m; });
     t = sample_t(sc, word_logit(s.word[i]));
     return (int)(unsigned)s.word[i];
   }
   // (a list from the first token on, and all tokens behind it below `least` or `tokens` within it)
-  __device__ void in_list_below(unsigned least, unsigned& tokens, u64& mass) {
+  __device__ __forceinline__ void in_list_below(unsigned least, unsigned& tokens, u64& mass) {
     __syncthreads();
     if (threadIdx.x == 0) s.hit = min(tokens, (unsigned)n);
     __syncthreads();
@@ -428,7 +470,7 @@ struct Sampler {
 
   // Makes the list hold the part of `bin` in which tokens-ahead-of-it <= target < ... (by_count), or the mass does, or sets `ties`.
   template <class Tag>
-  __device__ void narrow(int bin, bool by_count, u64 target) {
+  __device__ __forceinline__ void narrow(int bin, bool by_count, u64 target) {
     u64* mass = s.word;                                       // 257 of each, in the list's place
     unsigned* count = reinterpret_cast<unsigned*>(s.upto);
     unsigned prefix = 0, before = s.count[bin];
@@ -437,7 +479,7 @@ struct Sampler {
       __syncthreads();
       for (int i = threadIdx.x; i <= 256; i += NT) { mass[i] = 0; count[i] = 0; }
       __syncthreads();
-      each_logit<Tag, NT>(row, V, [&](float x, int) {
+      each_logit<Tag, NT, !ROLLED>(row, V, [&](float x, int) {
         const float t = sample_t(sc, x);
         if (sample_bin(t) != bin) return;
         const unsigned o = order_of(x), w = sample_weight(t);
@@ -479,7 +521,7 @@ struct Sampler {
   }
   // The list (or `ties`) so that it holds the target of bin `bin`.
   template <class Tag>
-  __device__ void reach(int bin, bool by_count, u64 target) {
+  __device__ __forceinline__ void reach(int bin, bool by_count, u64 target) {
     ties = false;
     if (bin >= lo_bin && bin <= hi_bin) return;
     if (s.count[bin + 1] - s.count[bin] <= SAMPLE_CAP) collect_bins<Tag>(bin, bin);
@@ -487,14 +529,14 @@ struct Sampler {
   }
   // Mass of the first q tokens.
   template <class Tag>
-  __device__ u64 mass_of_first(unsigned q, int bin) {
+  __device__ __forceinline__ u64 mass_of_first(unsigned q, int bin) {
     reach<Tag>(bin, true, q - 1);
     if (ties) return ahead_mass + (u64)(q - ahead) * tie_weight;
     return s.upto[q - ahead - 1];
   }
   // The number of tokens, and their mass, up to the first one at which the mass reaches m.
   template <class Tag>
-  __device__ void first_reaching(u64 m, int bin, unsigned& tokens, u64& mass) {
+  __device__ __forceinline__ void first_reaching(u64 m, int bin, unsigned& tokens, u64& mass) {
     reach<Tag>(bin, false, m - 1);
     if (ties) {
       const u64 q = (m - ahead_mass + tie_weight - 1) / tie_weight;
@@ -506,7 +548,7 @@ struct Sampler {
   }
   // The token in whose stretch m falls, and its t.
   template <class Tag>
-  __device__ int token_at(u64 m, int bin, float& t) {
+  __device__ __forceinline__ int token_at(u64 m, int bin, float& t) {
     reach<Tag>(bin, false, m);
     if (ties) {
       const unsigned j = (unsigned)((m - ahead_mass) / tie_weight);
@@ -518,7 +560,7 @@ struct Sampler {
   // The column of the j-th logit of order `tie_order`: every wave counts those of a stretch of columns, then the one that
   // holds the j-th walks its stretch again.
   template <class Tag>
-  __device__ int equal_logit(unsigned j) {
+  __device__ __forceinline__ int equal_logit(unsigned j) {
     const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
     const int64_t each = (V + NW - 1) / NW, lo = min(V, w * each), hi = min(V, lo + each);
     unsigned mine = 0;
@@ -544,7 +586,7 @@ struct Sampler {
   }
   // The number of tokens ahead of the first whose weight is below `least`, and their mass, if that comes before `tokens`.
   template <class Tag>
-  __device__ void cut_below(unsigned least, unsigned& tokens, u64& mass) {
+  __device__ __forceinline__ void cut_below(unsigned least, unsigned& tokens, u64& mass) {
     const int behind = bin_behind(least);
     if (hi_bin < 0 || lo_bin > 0) {
       if (s.count[behind + 1] <= SAMPLE_CAP) collect_bins<Tag>(0, behind);
@@ -555,7 +597,7 @@ struct Sampler {
     }
     // Too many for the list: the largest logit with too small a weight, then what lies above it.
     unsigned worst = 0;
-    each_logit<Tag, NT>(row, V, [&](float x, int) {
+    each_logit<Tag, NT, !ROLLED>(row, V, [&](float x, int) {
       const unsigned w = sample_weight(sample_t(sc, x));
       if (w > 0 && w < least) worst = max(worst, order_of(x));
     });
@@ -566,7 +608,7 @@ struct Sampler {
     for (int i = 0; i < NW; ++i) worst = max(worst, s.wave_count[i]);
     u64 m = 0;
     unsigned c = 0;
-    each_logit<Tag, NT>(row, V, [&](float x, int) {
+    each_logit<Tag, NT, !ROLLED>(row, V, [&](float x, int) {
       const unsigned w = sample_weight(sample_t(sc, x));
       if (w > 0 && order_of(x) > worst) { m += w; ++c; }
     });
@@ -598,8 +640,10 @@ struct RowResult { int token; unsigned kept; float t; };
 
 // Rows whose maxima share the mass: equal weights, in the order of their columns.
 template <class Tag, int NT>
-__device__ __attribute__((noinline)) RowResult sample_maximum(SampleLds& s, const char* row, int64_t V, float top, const RowCuts cuts, unsigned& ties) {
-  Sampler<NT> a(s, row, V, RowScale{top, 0.f});
+__device__ __attribute__((noinline)) RowResult sample_maximum(const char* row, int64_t V, float top, const RowCuts cuts, unsigned& ties) {
+  row = global_row(row);
+  SampleLds& s = sample_lds();
+  Sampler<NT> a(row, V, RowScale{top, 0.f});
   u64 none = 0;
   ties = 0;
   unsigned first = 0xffffffffu;
@@ -630,10 +674,12 @@ __device__ __forceinline__ void clear_bins(SampleLds& s, int threads) {
 
 // Any row: a histogram of masses and counts, every look-up by the bins.
 template <class Tag, int NT>
-__device__ __attribute__((noinline)) RowResult sample_any(SampleLds& s, const char* row, int64_t V, const RowScale sc, const RowCuts cuts) {
-  Sampler<NT> a(s, row, V, sc);
+__device__ __attribute__((noinline)) RowResult sample_any(const char* row, int64_t V, const RowScale sc, const RowCuts cuts) {
+  row = global_row(row);
+  SampleLds& s = sample_lds();
+  Sampler<NT, true> a(row, V, sc);
   clear_bins(s, NT);
-  each_logit<Tag, NT>(row, V, [&](float x, int) {
+  each_logit<Tag, NT, false>(row, V, [&](float x, int) {
     const float t = sample_t(sc, x);
     const unsigned w = sample_weight(t);
     if (w > 0) {
@@ -669,8 +715,9 @@ __device__ __attribute__((noinline)) RowResult sample_any(SampleLds& s, const ch
 // The usual rows: all that is asked lies among the likeliest tokens.  Two sweeps over the row, this is the second.  False: not
 // decided here.  `powers`: the sum of 2^(t + 31).
 template <class Tag, int NT>
-__device__ __forceinline__ bool sample_likeliest(SampleLds& s, const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float met, float& powers, RowResult& res) {
-  Sampler<NT> a(s, row, V, sc);
+__device__ __forceinline__ bool sample_likeliest(const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float met, float& powers, RowResult& res) {
+  SampleLds& s = sample_lds();
+  Sampler<NT> a(row, V, sc);
   unsigned tokens = 0, live = 0;
   u64 mass = 0;
   if (cuts.k > 0) {
@@ -718,8 +765,9 @@ __device__ __forceinline__ bool sample_likeliest(SampleLds& s, const char* row, 
 // Rows with top-k whose first k tokens fit the list: counts of tokens per bin, first of those within 2^-16 of the most likely one
 // (few, and with them few additions in LDS), of all if that is not enough.  False: not decided here.
 template <class Tag, int NT>
-__device__ __forceinline__ bool sample_top_k(SampleLds& s, const char* row, int64_t V, const RowScale& sc, RowCuts cuts, RowResult& res) {
-  Sampler<NT> a(s, row, V, sc);
+__device__ __forceinline__ bool sample_top_k(const char* row, int64_t V, const RowScale& sc, RowCuts cuts, RowResult& res) {
+  SampleLds& s = sample_lds();
+  Sampler<NT> a(row, V, sc);
   float least = -16.f;
   for (;;) {
     clear_bins(s, NT);
@@ -748,8 +796,9 @@ __device__ __forceinline__ bool sample_top_k(SampleLds& s, const char* row, int6
 // Rows without top-k: a histogram of masses.  Counts of tokens are only needed to choose between lists; a bin's mass over its
 // middle weight gives them to 1 %, and whether a list held all is known when it is made.
 template <class Tag, int NT>
-__device__ __forceinline__ bool sample_by_mass(SampleLds& s, const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float& powers, RowResult& res) {
-  Sampler<NT> a(s, row, V, sc);
+__device__ __forceinline__ bool sample_by_mass(const char* row, int64_t V, const RowScale& sc, const RowCuts& cuts, float& powers, RowResult& res) {
+  SampleLds& s = sample_lds();
+  Sampler<NT> a(row, V, sc);
   unsigned tokens = 0;
   powers = 0.f;
   clear_bins(s, NT);
@@ -775,8 +824,13 @@ __device__ __forceinline__ bool sample_by_mass(SampleLds& s, const char* row, in
     const int end_p = cuts.top_p ? a.bin_reaching(want) : SAMPLE_BINS - 1, behind = cuts.least > 0 ? bin_behind(cuts.least) : SAMPLE_BINS - 1;
     const int end = min(end_p, behind);
     if (s.count[end + 1] <= FITS) a.template collect_bins<Tag>(0, end);
-    else if (cuts.least == 0 && s.count[end + 1] - s.count[end] <= FITS) a.template collect_bins<Tag>(end, end);
-    else return false;
+    else if (cuts.least == 0 && s.count[end + 1] - s.count[end] <= FITS) {
+      // the token's bin as well: what is kept has a mass between those ahead of and with `end`
+      const int from = a.bin_passing(share_of(s.mass[end], cuts.u)), to = a.bin_passing(share_of(s.mass[end + 1], cuts.u));
+      if (s.count[end + 1] - s.count[min(from, end)] <= FITS) a.template collect_bins<Tag>(min(from, end), end);
+      else if (to < end && s.count[to + 1] - s.count[from] + s.count[end + 1] - s.count[end] <= FITS) a.template collect_two<Tag>(from, to, end);
+      else a.template collect_bins<Tag>(end, end);
+    } else return false;
     if (a.overflow) return false;
     if (cuts.top_p && end_p <= behind) a.in_list_reaching(want, tokens, mass);
     if (cuts.least > 0) a.in_list_below(cuts.least, tokens, mass);
@@ -795,7 +849,7 @@ __device__ __forceinline__ bool sample_by_mass(SampleLds& s, const char* row, in
 
 template <class Tag, int NT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void sample_row_kernel(const SampleParams p) {
-  __shared__ SampleLds s;
+  SampleLds& s = sample_lds();
   const int64_t r = blockIdx.x;
   const char* row = reinterpret_cast<const char*>(p.logits) + r * p.row_stride * Tag::bytes;
   for (int b = threadIdx.x; b <= SAMPLE_BINS; b += NT) { s.mass[b] = 0; s.count[b] = 0; }
@@ -816,14 +870,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   float logp;
   if (only_the_maximum(top, T)) {
     unsigned ties;
-    res = sample_maximum<Tag, NT>(s, row, p.V, top, cuts, ties);
+    res = sample_maximum<Tag, NT>(row, p.V, top, cuts, ties);
     logp = -logf((float)ties);
   } else {
     const RowScale sc{top, LOG2E / T};
     float powers = 0.f;
-    if (!sample_likeliest<Tag, NT>(s, row, p.V, sc, cuts, met, powers, res)) {
-      const bool done = cuts.k > 0 ? sample_top_k<Tag, NT>(s, row, p.V, sc, cuts, res) : sample_by_mass<Tag, NT>(s, row, p.V, sc, cuts, powers, res);
-      if (!done) res = sample_any<Tag, NT>(s, row, p.V, sc, cuts);
+    if (!sample_likeliest<Tag, NT>(row, p.V, sc, cuts, met, powers, res)) {
+      const bool done = cuts.k > 0 ? sample_top_k<Tag, NT>(row, p.V, sc, cuts, res) : sample_by_mass<Tag, NT>(row, p.V, sc, cuts, powers, res);
+      if (!done) res = sample_any<Tag, NT>(row, p.V, sc, cuts);
     }
     logp = (res.t - log2f(powers * 0x1p-31f)) * LN2;
   }
