@@ -150,6 +150,10 @@ __device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, cons
 // half of a's, so that three quarters of the bytes have a step and a half to arrive (what the latency of memory asks for: with
 // one step, waits were a third of the time).
 // Workgroups stay: each walks its tiles as one sequence of steps, so that the next tile's operands arrive while the last one is stored.
+// Measured: 8192 x 128256 x 4096 (bf16 out) 3.80-3.94 ms, 2190-2270 Tflop/s; the matrix units' time alone, at the 1.97 GHz that the card
+// holds under this load, is 2.1 ms, the scaling's multiply-adds share the issue slots with them.  (A library product of the same operands
+// with one scale for all: 3.17 ms.)  Few rows are bound by the weights' bytes: 1 x 128256 x 4096 99-116 us (4.5-5.3 TB/s),
+// 61 x 50257 x 2048 18-19 us (5.5 TB/s).
 typedef const unsigned __attribute__((address_space(1))) * global_words;
 typedef unsigned __attribute__((address_space(3))) * lds_words;
 

@@ -6,8 +6,10 @@
 //   beta = 0: KL(P|Q);  beta = 1: KL(Q|P);  between: beta KL(P|M) + (1 - beta) KL(Q|M) with M = beta P + (1 - beta) Q
 // Gradient: with s_j = q_j dL/dq_j (beta = 0: -p_j; 1: q_j log(q_j / p_j); between: (1 - beta) q_j log(q_j / m_j)) and S their sum,
 //   dL/dz_k = s_k - q_k S on a listed id, and softmax over the rest's columns times (s_rest - q_rest S) on those:
-// the rest's columns need one number per row, so the row is read once, written once and costs two exponentials' worth of
-// vector work per column.  Bound by HBM traffic, 2 V bytes x the element size per row.
+// the rest's columns need one number per row, so the row is read once, written once and costs one exponential per column (two-byte
+// logits: their powers stay in registers as fp16; four-byte ones: as fp32).  Bound by HBM traffic, 2 V bytes x the element size per row:
+// 8192 x 128256 bf16, K = 200: 809-856 us (4.9-5.2 TB/s); 4093 x 50257, K = 100: 185-200 us (a tenth of the rows masked; 50304 columns,
+// whose rows begin on 16 bytes: 15 % less); 131 x 32000 fp32, K = 400: 17 us, the latency of its phases.
 //
 // Layout as in the forward-KL kernels: a row, or one column part of it, sits in its workgroup's registers; parts exchange
 // (max, sum) of the rest's columns through records in a workspace, with a bounded wait and a second launch for parts
@@ -358,7 +360,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
   }
 }
 
-// Threads and chunks per thread of a workgroup, parts per row, for rows of `nch` chunks (parts == 0: too wide).
+// Threads and chunks per thread of a workgroup, parts per row, for rows of `nch` chunks (parts == 0: too wide).  Rows stay whole as far as
+// 512 threads' registers go (us, whole / in parts, K = 200 bf16: 64 x 50304 16.9 / 23.6, 4096 x 50304 174 / 188, 4096 x 50257 201 / 212,
+// 1024 x 65536 59.9 / 67.3).
 struct RestShape { int NT, NCH, parts; };
 static RestShape rest_shape(int64_t nch) {
   if (nch <= 256 * 4) return {256, 4, 1};
@@ -372,7 +376,8 @@ static RestShape rest_shape(int64_t nch) {
   return {256, per_thread <= 13 ? 13 : per_thread <= 14 ? 14 : 16, (int)parts};
 }
 
-// Entries per thread: two, or as many as the most entries ask for.
+// Entries per thread: two, or as many as the most entries ask for (us at K = 200 for 2 / as many: 4096 x 50304 174 / 223,
+// 4096 x 128256 417 / 439).
 template <class Tag, int NT, int NCH, int J>
 static void launch_rest_row_j(const RestParams& p, hipStream_t st) {
   hipLaunchKernelGGL((rest_kernel<Tag, NT, NCH, J, false>), dim3(xcd_banded_grid(p.n_rows)), dim3(NT), RestLds::bytes(p.K, NT, NCH), st, p);
