@@ -213,3 +213,13 @@ def test_refusals(D):
     assert lib.dl_sample_rows(p + 1, 0, 10, 3, 10, p, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, t, 0, 0, 0) == -6
     assert lib.dl_sample_rows(p, 0, 5000000, 3, 5000000, p, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, t, 0, 0, 0) == -4
     assert lib.dl_sample_rows(p, 5, 10, 3, 10, p, 0, 0, 0, 0, 1.0, 0, 1.0, 0.0, t, 0, 0, 0) == -2
+
+
+@pytest.mark.parametrize("R,V,dtype", [(12, 90001, torch.bfloat16), (12, 90001, torch.float32), (270, 20000, torch.float16)])
+def test_cuts_and_tokens_far_down_flat_rows(D, R, V, dtype):
+    """A cut behind many lists' worth of tokens, the token anywhere ahead of it: near the first, in a bin of its own, near the cut."""
+    x, u = rows(R, V, V + 1, dtype=dtype)
+    u = [(0.0, 1.0 - 2.0 ** -24, 0.999, u[r], u[r], u[r])[r % 6] for r in range(R)]
+    T = [(1.2, 1.5, 1.6, 2.5)[r % 4] for r in range(R)]
+    p = [(0.9, 0.98, 0.995)[r % 3] for r in range(R)]
+    check(D, x, u, T, [0] * R, p, [0.0] * R)
