@@ -767,22 +767,24 @@ __device__ __forceinline__ bool sample_likeliest(const char* row, int64_t V, con
 }
 
 // Rows with top-k whose first k tokens fit the list: counts of tokens per bin, first of those within 2^-16 of the most likely one
-// (few, and with them few additions in LDS), of all if that is not enough.  False: not decided here.
+// (few, and with them few additions in LDS), of all if that is not enough.  Bins are counted whole or not at all -- t > -16 is bins 0 to
+// 511, and behind t = -31 no token has a weight -- so a bin holds no more tokens for the list than were counted.  False: not decided here.
 template <class Tag, int NT>
 __device__ __forceinline__ bool sample_top_k(const char* row, int64_t V, const RowScale& sc, RowCuts cuts, RowResult& res) {
   SampleLds& s = sample_lds();
   Sampler<NT> a(row, V, sc);
-  float least = -16.f;
+  constexpr float ALL = -0x1.f00002p4f;      // the number before -31
+  float below = -16.f;
   for (;;) {
     clear_bins(s, NT);
     each_logit<Tag, NT>(row, V, [&](float x, int) {
       const float t = sample_t(sc, x);
-      if (t >= least) atomicAdd(&s.count[sample_bin(t)], 1u);
+      if (t > below) atomicAdd(&s.count[sample_bin(t)], 1u);
     });
     __syncthreads();
     a.template scan_bins<SAMPLE_BINS>(s.mass, s.count);
-    if (s.count[SAMPLE_BINS] >= (unsigned)cuts.k || least == -31.f) break;
-    least = -31.f;
+    if (s.count[SAMPLE_BINS] >= (unsigned)cuts.k || below == ALL) break;
+    below = ALL;
   }
   cuts.k = min(cuts.k, (int)s.count[SAMPLE_BINS]);
   const int bin = a.bin_of_count(cuts.k);

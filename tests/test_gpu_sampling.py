@@ -223,3 +223,18 @@ def test_cuts_and_tokens_far_down_flat_rows(D, R, V, dtype):
     T = [(1.2, 1.5, 1.6, 2.5)[r % 4] for r in range(R)]
     p = [(0.9, 0.98, 0.995)[r % 3] for r in range(R)]
     check(D, x, u, T, [0] * R, p, [0.0] * R)
+
+
+@pytest.mark.parametrize("R", [4, 300])
+@pytest.mark.parametrize("T,dtype,top,edge,behind", [(1.0, torch.float32, 0.0, -11.090355, -11.095), (1.4426950408889634, torch.bfloat16, 20.0, 4.0, 3.984375),
+                                                     (1.4426950408889634, torch.float16, 31.0, 0.0, -0.015625), (1.4426950408889634, torch.float32, 31.0, 15.0, 14.99)])
+def test_top_k_whose_last_token_is_at_the_edge_of_a_bin(D, R, T, dtype, top, edge, behind):
+    """A few tokens at t = -16 or -31 exactly, thousands just behind them (t = -31: without a weight), the k-th among either."""
+    V = 20000
+    x = torch.full((R, V), -30.0)
+    for r in range(R):
+        at = torch.randperm(V, generator=torch.Generator().manual_seed(r))
+        x[r, at[0]], x[r, at[1:11]], x[r, at[11:5011]] = top, edge, behind
+    k = [(5, 11, 12, 4000)[r % 4] for r in range(R)]
+    u = [(1.0 - 2.0 ** -24, 0.0, 0.99999, 0.9999999)[r // 4 % 4] for r in range(R)]
+    check(D, x.to(dtype), u, [T] * R, k, [1.0] * R, [0.0] * R)
