@@ -11,6 +11,7 @@
 // pieces, 64 bytes apart, so that every load instruction covers 64 contiguous bytes of a row.
 #include "distill_common.hpp"
 #include "distill_hip.h"
+#include "product_schedule.hpp"
 
 #include <algorithm>
 
@@ -267,8 +268,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
     fetch_early(1);
     fetch_late(1);
   }
-  // Products are scaled and added three behind the one that the matrix unit starts: their results are there by then.
-  constexpr int Q = TM * TN, BEHIND = 3, KEEP = BEHIND + 1;
+  // Products are scaled and added a few behind the one that the matrix unit starts: their results are there by then.
+  constexpr int Q = TM * TN;
+  using Order = ProductSchedule<Q>;
+  static_assert(Order::sound(), "every product is added once");
   // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
   const unsigned lo = i16 * QB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
   unsigned a_lo = wm * QB + lo, a_hi = wm * QB + hi, b_lo = (BM + wn) * QB + lo, b_hi = (BM + wn) * QB + hi, s_at = (BM + BN) * QB + (wm + i16) * 4, sb_at = (BM + BN) * QB + BM * 4 + wn * WAVE / BN * 4;
@@ -291,11 +294,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
 #pragma unroll 1
   for (int kb = 0; kb < p.blocks; ++kb, ++step) {
     float s[TM];
-    f32x4 v[KEEP];
+    f32x4 v[Order::PLACES];
     const auto add = [&](int q) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[q / TN][q % TN][e] = fmaf(v[q % KEEP][e], s[q / TN], acc[q / TN][q % TN][e]);
+      for (int e = 0; e < 4; ++e) acc[q / TN][q % TN][e] = fmaf(v[Order::place(q)][e], s[q / TN], acc[q / TN][q % TN][e]);
       asm volatile("" : "+v"(acc[q / TN][q % TN]));            // (here, and not collected behind the barrier)
+    };
+    const auto add_in_slot = [&](int slot) {
+      if (Order::added_in(slot) != Order::NONE) add(Order::added_in(slot));
     };
 #pragma unroll
     for (int i = 0; i < TM; ++i) s[i] = *reinterpret_cast<const float*>(lds + s_at + i * 64);
@@ -306,12 +312,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int q = i * TN + j;
-        v[q % KEEP] = block_product(bf[j], af[i & 1]);
+        v[Order::place(q)] = block_product(bf[j], af[i & 1]);
         if (q == 1) {
 #pragma unroll
           for (int k = 0; k < TM; ++k) s[k] *= sb;
         }
-        if (q >= BEHIND) add(q - BEHIND);
+        add_in_slot(q);
       }
       // a product and the four multiply-adds of an earlier one in turns, the next operand's reads behind the first
 #pragma unroll
@@ -339,13 +345,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int q = (TM - 1) * TN + j;
-      v[q % KEEP] = block_product(bf[j], af[(TM - 1) & 1]);
+      v[Order::place(q)] = block_product(bf[j], af[(TM - 1) & 1]);
       bf[j] = tile_operand(lds, b_lo, b_hi, j * 16);           // (behind the last step: what lies there, unused)
-      add(q - BEHIND);
+      add_in_slot(q);
     }
     af[0] = tile_operand(lds, a_lo, a_hi, 0);
 #pragma unroll
-    for (int q = Q - BEHIND; q < Q; ++q) add(q);
+    for (int q = Order::LEFT; q < Q; ++q) add(q);
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -353,7 +359,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(c
       __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, 4 * BEHIND, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 4 * Order::BEHIND, 0);
   }
   // The tile's values.  Two-byte results go through 2 KiB of LDS of the wave's own, 16 rows at a time, so that a store writes whole
   // 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by unit ^ (row % 8).
