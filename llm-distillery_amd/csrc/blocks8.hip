@@ -458,7 +458,7 @@ extern "C" int dl_quantize_blocks(const void* x, int dtype, int64_t row_stride, 
   if (reinterpret_cast<uintptr_t>(x) % (dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(codes) % 16 || code_stride % 16 ||
       reinterpret_cast<uintptr_t>(scales) % 4)
     return DL_ERR_ALIGN;
-  if (blocks > 0x7fffffffLL || (block_rows == QB && (rows + QB - 1) / QB > 65535)) return DL_ERR_LIMIT;
+  if (blocks > LAUNCH_THREADS / 256 || (block_rows == QB && (rows + QB - 1) / QB > 65535)) return DL_ERR_LIMIT;
   const QuantParams p{reinterpret_cast<const char*>(x), row_stride, rows, cols, blocks, reinterpret_cast<unsigned char*>(codes), code_stride,
                       scales, scale_row_stride, scale_block_stride};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

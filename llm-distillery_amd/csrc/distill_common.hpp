@@ -319,6 +319,8 @@ __device__ __forceinline__ int64_t xcd_banded_row(unsigned b) {
 }
 // The other way: every XCD works on a contiguous eighth of the items (`grid` workgroups, a multiple of 8).
 __device__ __forceinline__ unsigned xcd_eighth(unsigned b, unsigned grid) { return (b & 7u) * (grid >> 3) + (b >> 3); }
+// A launch takes fewer than 2^32 threads; of one with more, what is left of their number modulo 2^32 runs, and no error is reported.
+constexpr int64_t LAUNCH_THREADS = (1LL << 32) - 1;
 static inline unsigned xcd_banded_grid(int64_t n_rows) { return (unsigned)((n_rows + 63) / 64 * 64); }
 
 // ---- reductions: fixed order => bit-reproducible ---------------------------------

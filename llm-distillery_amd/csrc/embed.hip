@@ -243,6 +243,7 @@ struct SumParams {
   char* grad; int64_t grad_stride;
   float* partial;                  // [tiles][2][width]: the sum of a tile's first token (if it began earlier), of its last (if it goes on)
   float scale; unsigned slices; int tile;
+  int64_t tile0;                   // the launch's first tile
 };
 __device__ __forceinline__ unsigned word_token(unsigned long long w) { return (unsigned)(w >> 32); }
 
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(SUM_NT) void embed_sum_kernel(const SumParams p) {
   using C = Chunk<Tag>;
   using O = Chunk<TagO>;
   constexpr int PIECES = C::N / O::N;                          // 16-byte pieces of the gradient beside one of g
-  const int64_t tile = blockIdx.x / p.slices, t0 = tile * p.tile;
+  const int64_t tile = p.tile0 + blockIdx.x / p.slices, t0 = tile * p.tile;
   const int64_t col = ((int64_t)(blockIdx.x % p.slices) * SUM_NT + threadIdx.x) * C::N;
   const int cols = (int)min((int64_t)C::N, p.width - col);
   __shared__ unsigned long long word[SUM_TILE_MOST + 2];      // the tile's, and one on either side (~0: none)
@@ -364,7 +365,7 @@ __device__ __forceinline__ void add_partials(const SumParams& p, int64_t from, i
 template <class TagO, bool ADD>
 __global__ __launch_bounds__(JOIN_NT) void embed_join_kernel(const SumParams p) {
   __shared__ float met[JOIN_NT / WAVE][WAVE * JOIN_COLS];
-  const int64_t tile = blockIdx.x / p.slices, t0 = tile * p.tile, t1 = t0 + p.tile;
+  const int64_t tile = p.tile0 + blockIdx.x / p.slices, t0 = tile * p.tile, t1 = t0 + p.tile;
   if (t1 >= p.n) return;
   const unsigned v = word_token(p.sorted[t1 - 1]);
   if (v >= p.vocab || word_token(p.sorted[t1]) != v) return;                                     // ends with the tile
@@ -430,13 +431,17 @@ static int launch_sums(const SumParams& s, bool add, hipStream_t st) {
   const int64_t tiles = (p.n + p.tile - 1) / p.tile;
   p.slices = (unsigned)((p.width + SUM_NT * Chunk<Tag>::N - 1) / (SUM_NT * Chunk<Tag>::N));
   j.slices = (unsigned)((p.width + JOIN_NT * JOIN_COLS - 1) / (JOIN_NT * JOIN_COLS));
-  const dim3 grid((unsigned)(tiles * p.slices)), joins((unsigned)((tiles - 1) * j.slices));      // (the last tile is no token's first)
+  const auto launch = [&](SumParams& q, int64_t end, int threads, auto kernel) {      // tiles [0, end)
+    for (const int64_t most = LAUNCH_THREADS / threads / q.slices; q.tile0 < end; q.tile0 += most)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(std::min(most, end - q.tile0) * q.slices)), dim3(threads), 0, st, q);
+  };
+  // (the last tile is no joined token's first)
   if (add) {
-    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, true>), grid, dim3(SUM_NT), 0, st, p);
-    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, true>), joins, dim3(JOIN_NT), 0, st, j);
+    launch(p, tiles, SUM_NT, embed_sum_kernel<Tag, TagO, true>);
+    launch(j, tiles - 1, JOIN_NT, embed_join_kernel<TagO, true>);
   } else {
-    hipLaunchKernelGGL((embed_sum_kernel<Tag, TagO, false>), grid, dim3(SUM_NT), 0, st, p);
-    if (tiles > 1) hipLaunchKernelGGL((embed_join_kernel<TagO, false>), joins, dim3(JOIN_NT), 0, st, j);
+    launch(p, tiles, SUM_NT, embed_sum_kernel<Tag, TagO, false>);
+    launch(j, tiles - 1, JOIN_NT, embed_join_kernel<TagO, false>);
   }
   return embed_status();
 }
@@ -472,12 +477,18 @@ extern "C" int dl_embed_rows(const void* table, int dtype, int64_t table_stride,
   const char* t = reinterpret_cast<const char*>(table);
   char* o = reinterpret_cast<char*>(out);
   const bool few = n_tokens <= 2048;      // fewer rows than waves: a workgroup each
-#define DL_EMBED(TAG)                                                                                                                        \
-  if (few) hipLaunchKernelGGL((embed_rows_kernel<TAG, 256>), dim3((unsigned)n_tokens), dim3(256), 0, st, t, table_stride, vocab, width,     \
-                              tokens, itype, n_tokens, scale, o, out_stride);                                                                \
-  else hipLaunchKernelGGL((embed_rows_kernel<TAG, 64>), dim3((unsigned)((n_tokens + 3) / 4)), dim3(256), 0, st, t, table_stride, vocab,      \
-                          width, tokens, itype, n_tokens, scale, o, out_stride);
-  if (dtype == DL_F32) { DL_EMBED(TagF32) } else if (dtype == DL_BF16) { DL_EMBED(TagBF16) } else { DL_EMBED(TagF16) }
+  constexpr int64_t MOST = LAUNCH_THREADS / 256 * 4;      // tokens of a launch
+#define DL_EMBED(TAG)                                                                                                                     \
+  if (few) hipLaunchKernelGGL((embed_rows_kernel<TAG, 256>), dim3((unsigned)n), dim3(256), 0, st, t, table_stride, vocab, width, ids,    \
+                              itype, n, scale, to, out_stride);                                                                           \
+  else hipLaunchKernelGGL((embed_rows_kernel<TAG, 64>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, t, table_stride, vocab, width,   \
+                          ids, itype, n, scale, to, out_stride);
+  for (int64_t n0 = 0; n0 < n_tokens; n0 += MOST) {
+    const int64_t n = std::min(MOST, n_tokens - n0);
+    const void* ids = reinterpret_cast<const char*>(tokens) + n0 * (itype == DL_I64 ? 8 : 4);
+    char* to = o + n0 * out_stride * (int64_t)eb;
+    if (dtype == DL_F32) { DL_EMBED(TagF32) } else if (dtype == DL_BF16) { DL_EMBED(TagBF16) } else { DL_EMBED(TagF16) }
+  }
 #undef DL_EMBED
   return embed_status();
 }
@@ -500,7 +511,7 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
       reinterpret_cast<uintptr_t>(workspace) % 256)
     return DL_ERR_ALIGN;
   const int64_t slices = (width + SUM_NT * 4 - 1) / (SUM_NT * 4);
-  if (n_tokens > 0x7fffffffLL || vocab > 0x7ffffffeLL || (n_tokens / SUM_TILE_LEAST + 1) * slices > 0x7fffffffLL) return DL_ERR_LIMIT;
+  if (n_tokens > 0x7fffffffLL || vocab > 0x7ffffffeLL || slices > LAUNCH_THREADS / JOIN_NT) return DL_ERR_LIMIT;
   const EmbedSpace sp(n_tokens, width);
   if (n_tokens > 0 && (!workspace || workspace_bytes < sp.total)) return DL_ERR_WORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -541,7 +552,7 @@ extern "C" int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t
   }
   if (n_tokens == 0) return embed_status();
   SumParams p{sorted, n_tokens, vocab, width, reinterpret_cast<const char*>(g), g_stride, reinterpret_cast<char*>(grad), grad_stride,
-              reinterpret_cast<float*>(ws + 2 * sp.words + sp.counts), scale, 0, sp.tile};
+              reinterpret_cast<float*>(ws + 2 * sp.words + sp.counts), scale, 0, sp.tile, 0};
   if (dtype == DL_F32) return launch_sums<TagF32, TagF32>(p, accumulate != 0, st);
   if (dtype == DL_BF16) return grad_dtype == DL_F32 ? launch_sums<TagBF16, TagF32>(p, accumulate != 0, st) : launch_sums<TagBF16, TagBF16>(p, accumulate != 0, st);
   return grad_dtype == DL_F32 ? launch_sums<TagF16, TagF32>(p, accumulate != 0, st) : launch_sums<TagF16, TagF16>(p, accumulate != 0, st);

@@ -35,6 +35,21 @@ struct SampleParams {
   const float* T; const int32_t* k; const float* p; const float* m;      // one per row, or NULL: the ones below for all rows
   float T0, p0, m0; int k0;
   int64_t* token; float* logp; int32_t* kept;
+  // n rows from row r on
+  SampleParams rows(int64_t r, int64_t n, int bytes) const {
+    SampleParams q = *this;
+    q.logits = reinterpret_cast<const char*>(logits) + r * row_stride * bytes;
+    q.n_rows = n;
+    q.u += r;
+    q.token += r;
+    if (T) q.T += r;
+    if (k) q.k += r;
+    if (this->p) q.p += r;
+    if (m) q.m += r;
+    if (logp) q.logp += r;
+    if (kept) q.kept += r;
+    return q;
+  }
 };
 
 // What the weights of a row are relative to.
@@ -903,7 +918,11 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
 template <class Tag>
 static int launch_sample(const SampleParams& p, hipStream_t st) {
   if (p.n_rows <= 256) hipLaunchKernelGGL((sample_row_kernel<Tag, 1024>), dim3((unsigned)p.n_rows), dim3(1024), 0, st, p);
-  else hipLaunchKernelGGL((sample_row_kernel<Tag, 512>), dim3((unsigned)p.n_rows), dim3(512), 0, st, p);
+  else
+    for (int64_t r = 0, most = LAUNCH_THREADS / 512; r < p.n_rows; r += most) {      // (one launch up to 8388607 rows)
+      const SampleParams q = p.rows(r, std::min(most, p.n_rows - r), Tag::bytes);
+      hipLaunchKernelGGL((sample_row_kernel<Tag, 512>), dim3((unsigned)q.n_rows), dim3(512), 0, st, q);
+    }
   return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH;
 }
 

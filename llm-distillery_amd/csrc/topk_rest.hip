@@ -31,6 +31,23 @@ struct RestParams {
   float beta, inv_T, rest_min, grad_scale;
   float* row_loss; void* grad; int64_t grad_stride;
   void* workspace; int parts; int spin_limit;
+  // n rows from row r on
+  RestParams rows(int64_t r, int64_t n, int bytes) const {
+    RestParams q = *this;
+    q.logits = reinterpret_cast<const char*>(logits) + r * row_stride * bytes;
+    q.n_rows = n;
+    if (row_loss) q.row_loss += r;
+    if (grad) q.grad = reinterpret_cast<char*>(grad) + r * grad_stride * bytes;
+    if (row_map) {
+      q.row_map += r;
+    } else {                             // row r's teacher is row r
+      q.t_val = reinterpret_cast<const char*>(t_val) + r * K * (t_val_dtype == F32 ? 4 : 2);
+      q.t_idx = reinterpret_cast<const char*>(t_idx) + r * K * (t_idx_itype == I64 ? 8 : 4);
+      q.n_trows = n_trows > r ? n_trows - r : 0;
+      if (t_cnt) q.t_cnt += r;
+    }
+    return q;
+  }
 };
 
 // Lists of the row's entries by the 16-byte chunk of their column (chunks that share a head share a list), and a byte per
@@ -402,16 +419,21 @@ static void launch_rest_parts(const RestParams& p, hipStream_t st) {
 }
 
 template <class Tag>
-static int launch_rest(const RestParams& p, const RestShape& sh, hipStream_t st) {
-  if (sh.parts == 1) {
-    if (sh.NT == 256) sh.NCH == 4 ? launch_rest_row<Tag, 256, 4>(p, st) : launch_rest_row<Tag, 256, 8>(p, st);
-    else if (sh.NCH == 8) launch_rest_row<Tag, 512, 8>(p, st);
-    else if (sh.NCH == 13) launch_rest_row<Tag, 512, 13>(p, st);
-    else launch_rest_row<Tag, 512, 16>(p, st);
-  } else {
-    if (sh.NCH == 13) launch_rest_parts<Tag, 256, 13>(p, st);
-    else if (sh.NCH == 14) launch_rest_parts<Tag, 256, 14>(p, st);
-    else launch_rest_parts<Tag, 256, 16>(p, st);
+static int launch_rest(const RestParams& all, const RestShape& sh, hipStream_t st) {
+  // rows of a launch (one launch up to 8388544 rows that stay whole); launches follow each other on the same workspace
+  const int64_t most = LAUNCH_THREADS / (sh.NT * sh.parts) / 64 * 64;
+  for (int64_t r = 0; r < all.n_rows; r += most) {
+    const RestParams p = all.rows(r, std::min(most, all.n_rows - r), Tag::bytes);
+    if (sh.parts == 1) {
+      if (sh.NT == 256) sh.NCH == 4 ? launch_rest_row<Tag, 256, 4>(p, st) : launch_rest_row<Tag, 256, 8>(p, st);
+      else if (sh.NCH == 8) launch_rest_row<Tag, 512, 8>(p, st);
+      else if (sh.NCH == 13) launch_rest_row<Tag, 512, 13>(p, st);
+      else launch_rest_row<Tag, 512, 16>(p, st);
+    } else {
+      if (sh.NCH == 13) launch_rest_parts<Tag, 256, 13>(p, st);
+      else if (sh.NCH == 14) launch_rest_parts<Tag, 256, 14>(p, st);
+      else launch_rest_parts<Tag, 256, 16>(p, st);
+    }
   }
   return launch_status();
 }
