@@ -579,7 +579,8 @@ int dl_rkl_marginalised_compact_ws(const void* logits, int logits_dtype, int64_t
  * rest_min   in (0, 1): storage rounds log-probs (fp16: 1 - sum is uncertain by some 1e-4), and where the top K hold all of the
  *            teacher's mass a rest of 0 would make KL(Q|P) infinite.
  * Entries that do not count, as for dl_div_topk: ids outside [0, V), stored log-probs of -inf, entries from t_cnt on; their
- * columns belong to the rest.  An id that is listed again has its masses added up.  Where no column outside the list has an
+ * columns belong to the rest.  An id that is listed again has its masses added up.  An entry whose mass is 0 in fp32 adds nothing
+ * to KL(P|Q), also where the student rules its id out.  Where no column outside the list has an
  * unmasked logit (-inf, or a masked value: below -2^31 after scaling, two-byte logits -2^20) the rest is no outcome.  A row
  * without any unmasked logit, or without both entries and rest, counts for nothing: loss 0, gradient 0.
  * grad must not overlap the logits (parts of wide rows read listed logits that belong to each other).

@@ -80,7 +80,7 @@ struct RestLds {
 __device__ __forceinline__ void rest_outcome(float lp, float lq, float beta, float& loss, float& slope) {
   const float p = expf(lp), q = expf(lq), r = lp - lq;
   if (beta == 0.f) {
-    loss += p * r;
+    loss += p == 0.f ? 0.f : p * r;      // (an entry without mass adds nothing, where the student has none either: r is infinite)
     slope = -p;
   } else if (beta == 1.f) {
     slope = q == 0.f ? 0.f : -q * r;

@@ -295,3 +295,19 @@ def test_refusals(D):
     assert lib.dl_div_topk_rest(0.5, big.data_ptr(), 1, 600000, 1, 600000, 0, tv.data_ptr(), 2, ti.data_ptr(), 0, 4, 3, 0, 1.0, 0.1, 1.0,
                                 logits.data_ptr(), 0, 0, 0, 0, 0, 0) == -4
     assert lib.dl_div_topk_rest(0.5, 0, 1, 100, 1, 100, 0, tv.data_ptr(), 2, ti.data_ptr(), 0, 4, 3, 0, 1.0, 0.1, 1.0, logits.data_ptr(), 0, 0, 0, 0, 0, 0) == -1
+
+
+@pytest.mark.parametrize("V", [400, 128256])
+@pytest.mark.parametrize("T", [1.0, 2.0])
+@pytest.mark.parametrize("beta", BETAS)
+def test_an_entry_that_both_sides_mask_adds_nothing(D, V, T, beta):
+    """A stored log-prob of fp16's lowest value is an entry without mass; where the student masks its column as well, it adds nothing, as
+    an entry that does not count."""
+    logits, tv, ti = case(3, V, 12, torch.bfloat16, 18)
+    for low in (-math.inf, torch.finfo(torch.bfloat16).min, -1e30):
+        x = logits.clone()
+        for r in range(3):
+            x[r, ti[r, 4 + r].item()] = low
+        got, want = (D.div_topk_rest(beta, x.to(DEV), v.to(DEV), ti.to(DEV), T=T)
+                     for v in (tv.scatter(1, torch.tensor([[4], [5], [6]]), value) for value in (torch.finfo(torch.float16).min, -math.inf)))
+        assert torch.isfinite(want[0]).all() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
