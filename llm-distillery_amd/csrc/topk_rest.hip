@@ -232,8 +232,9 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   constexpr float BIAS = C::stash_bias;
   float mb = mx * a;
   // A rest of nothing but masked columns counts as none, whatever they are masked with (distill_common.hpp: MASKED_BELOW; two-byte
-  // logits are thousands apart at -2^20 already).
-  const bool masked = mb < (Tag::bytes == 2 ? -0x1p20f : MASKED_BELOW);
+  // logits are thousands apart at -2^20 already), and so does a row.
+  constexpr float LOW = Tag::bytes == 2 ? -0x1p20f : MASKED_BELOW;
+  const bool masked = mb < LOW;
   if (masked) { mb = 0.f; mx = -INFINITY; }
   const float mb_own = mb - BIAS;
   float sm = 0.f, zs = 0.f, ps = 0.f;
@@ -294,7 +295,7 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   // the K outcomes and the rest
   const bool rest = !(b == -INFINITY);
   const float top = fmaxf(zmax, b);
-  if (top == -INFINITY && zs == 0.f) return leave();                  // no finite logit
+  if (!rest && zmax < LOW && zs == zs) return leave();                // no unmasked logit (nor NaN)
   if (!rest && ps == 0.f) return leave();                             // nothing to compare
   const float lse = top + fast_log2((zmax == -INFINITY ? zs : zs * fast_exp2(zmax - top)) + (rest ? fast_exp2(b - top) : 0.f));
   const float p0 = rest ? fmaxf(1.f - ps, p.rest_min) : 0.f, lz = logf(ps + p0);

@@ -311,3 +311,17 @@ def test_an_entry_that_both_sides_mask_adds_nothing(D, V, T, beta):
         got, want = (D.div_topk_rest(beta, x.to(DEV), v.to(DEV), ti.to(DEV), T=T)
                      for v in (tv.scatter(1, torch.tensor([[4], [5], [6]]), value) for value in (torch.finfo(torch.float16).min, -math.inf)))
         assert torch.isfinite(want[0]).all() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("V", [400, 128256])
+@pytest.mark.parametrize("dtype,low", [(torch.bfloat16, torch.finfo(torch.bfloat16).min), (torch.bfloat16, -1e30), (torch.float32, -1e10),
+                                       (torch.float32, torch.finfo(torch.float32).min)])
+def test_rows_of_a_low_finite_mask_count_for_nothing(D, V, dtype, low):
+    """Every logit masked with a low value that the scaling leaves finite: the listed ones too."""
+    logits, tv, ti = case(4, V, 10, dtype, 19)
+    logits[1], logits[3] = low, low
+    for T in (1.0, 2.0):
+        for beta in BETAS:
+            loss, grad = D.div_topk_rest(beta, logits.to(DEV), tv.to(DEV), ti.to(DEV), T=T)
+            assert (loss[[1, 3]] == 0).all() and (grad[[1, 3]] == 0).all()
+            assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and (loss[[0, 2]] > 0).all()
