@@ -211,7 +211,9 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   }
 
   // maxima of the rest's columns and of the listed ones; then the sums of the powers over them, and the teacher's mass.  The rest's
-  // powers 2^(x a - max a) stay in the registers for the gradient.
+  // powers 2^(x a - mb), mb the largest one's x a rounded, stay in the registers for the gradient.  Logits are scaled inside fused
+  // multiply-adds and only ever less a maximum: what a power or a log-probability is off by goes with its logit's distance from that
+  // maximum, not with the logit (fp32 logits near 32768 in the middle of a row: losses off by 1e-3 with a product of their own).
   const float a = p.inv_T * LOG2E;
   float mx = -INFINITY, zmax = -INFINITY;
 #pragma unroll
@@ -224,19 +226,19 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
     keep(mx);
   }
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    z[j] *= a;
+  for (int j = 0; j < J; ++j)
     if (lp[j] != -INFINITY) zmax = fmaxf(zmax, z[j]);
-  }
   block_max2<NT>(mx, zmax, s.red);
   constexpr float BIAS = C::stash_bias;
-  float mb = mx * a;
+  float mb_own = mx * a - BIAS, zb = zmax * a;
+  keep(mb_own);                          // (rounded here: what follows has one value for each)
+  keep(zb);
+  float mb = mb_own + BIAS;
   // A rest of nothing but masked columns counts as none, whatever they are masked with (distill_common.hpp: MASKED_BELOW; two-byte
   // logits are thousands apart at -2^20 already), and so does a row.
   constexpr float LOW = Tag::bytes == 2 ? -0x1p20f : MASKED_BELOW;
   const bool masked = mb < LOW;
-  if (masked) { mb = 0.f; mx = -INFINITY; }
-  const float mb_own = mb - BIAS;
+  if (masked) { mb_own = -BIAS; mb = -INFINITY; }
   float sm = 0.f, zs = 0.f, ps = 0.f;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -257,15 +259,15 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
   for (int j = 0; j < J; ++j)
     if (lp[j] != -INFINITY) {
       ps += expf(lp[j]);
-      zs += zmax == -INFINITY ? (z[j] == z[j] ? 0.f : z[j]) : fast_exp2(z[j] - zmax);
+      zs += zb == -INFINITY ? (z[j] == z[j] ? 0.f : z[j]) : fast_exp2(fmaf(z[j], a, -zb));
     }
   block_sum3<NT>(sm, zs, ps, s.red);
 
   if (SPLIT) {
     PartStats* ws = reinterpret_cast<PartStats*>(p.workspace) + r * P;
-    if (tid == 0 && !RETRY) part_publish(ws + h, mx, sm, 0.f);
+    if (tid == 0 && !RETRY) part_publish(ws + h, mb, sm, 0.f);
     if (tid < P) {
-      float om = mx, os = sm, ob;
+      float om = mb, os = sm, ob;
       s.xok[tid] = (tid == h) || part_collect(ws + tid, RETRY ? 0x7fffffff : p.spin_limit, om, os, ob);
       s.xm[tid] = om; s.xs[tid] = os;
     }
@@ -285,31 +287,30 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
     if (top == -INFINITY) {
       for (int j = 0; j < P; ++j) S += s.xs[j];                       // 0, or NaN
     } else {
-      for (int j = 0; j < P; ++j) S += s.xs[j] * fast_exp2((s.xm[j] - top) * a);
+      for (int j = 0; j < P; ++j) S += s.xs[j] * fast_exp2(s.xm[j] - top);
     }
-    mb = top == -INFINITY ? 0.f : top * a;
+    mb = top;
     sm = S;
   }
-  const float b = mb + fast_log2(sm);    // log2 of the rest's sum: -inf where no column outside the list has a finite logit
 
-  // the K outcomes and the rest
-  const bool rest = !(b == -INFINITY);
-  const float top = fmaxf(zmax, b);
-  if (!rest && zmax < LOW && zs == zs) return leave();                // no unmasked logit (nor NaN)
+  // the K outcomes and the rest (none where no column outside the list has an unmasked logit: a sum of 0)
+  const bool rest = !(sm == 0.f);
+  if (!rest && zb < LOW && zs == zs) return leave();                  // no unmasked logit (nor NaN)
   if (!rest && ps == 0.f) return leave();                             // nothing to compare
-  const float lse = top + fast_log2((zmax == -INFINITY ? zs : zs * fast_exp2(zmax - top)) + (rest ? fast_exp2(b - top) : 0.f));
+  const float top = rest ? fmaxf(zb, mb) : zb, lr = fast_log2(sm);    // (lr: log2 of the rest's sum, from mb on)
+  const float lse = fast_log2((zb == -INFINITY ? zs : zs * fast_exp2(zb - top)) + (rest ? sm * fast_exp2(mb - top) : 0.f));      // from top on
   const float p0 = rest ? fmaxf(1.f - ps, p.rest_min) : 0.f, lz = logf(ps + p0);
   float loss = 0.f, slopes = 0.f, slope[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
     if (lp[j] != -INFINITY) {
-      rest_outcome(lp[j] - lz, (z[j] - lse) * LN2, p.beta, loss, slope[j]);
+      rest_outcome(lp[j] - lz, (fmaf(z[j], a, -top) - lse) * LN2, p.beta, loss, slope[j]);
       slopes += slope[j];
     }
   block_sum2<NT>(loss, slopes, s.red);
   float slope0 = 0.f, q0 = 0.f;
   if (rest) {
-    const float lq0 = (b - lse) * LN2;
+    const float lq0 = (mb - top + (lr - lse)) * LN2;
     rest_outcome(logf(p0) - lz, lq0, p.beta, loss, slope0);
     slopes += slope0;
     q0 = expf(lq0);
@@ -320,10 +321,10 @@ __device__ __forceinline__ void rest_part(const RestParams& p, const RestLds& s,
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int k = j * NT + tid;
-    if (lp[j] != -INFINITY) s.lp[k] = (slope[j] - fast_exp2(z[j] - lse) * slopes) * c;
+    if (lp[j] != -INFINITY) s.lp[k] = (slope[j] - fast_exp2(fmaf(z[j], a, -top) - lse) * slopes) * c;
     else if (k < p.K) s.idx[k] = -1;
   }
-  const float kc = !rest || masked ? 0.f : fast_exp2(mb_own - b) * (slope0 - q0 * slopes) * c;      // stashed power -> gradient
+  const float kc = !rest || masked ? 0.f : fast_exp2(mb_own - mb - lr) * (slope0 - q0 * slopes) * c;      // stashed power -> gradient
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {

@@ -325,3 +325,36 @@ def test_rows_of_a_low_finite_mask_count_for_nothing(D, V, dtype, low):
             loss, grad = D.div_topk_rest(beta, logits.to(DEV), tv.to(DEV), ti.to(DEV), T=T)
             assert (loss[[1, 3]] == 0).all() and (grad[[1, 3]] == 0).all()
             assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and (loss[[0, 2]] > 0).all()
+
+
+@pytest.mark.parametrize("V", [600, 70001])
+@pytest.mark.parametrize("shift", [0.0, 2.0 ** 15, -2.0 ** 15])
+@pytest.mark.parametrize("beta", BETAS)
+def test_only_differences_of_logits_count(D, V, shift, beta):
+    """fp32 logits far from 0: what a probability is off by goes with the logits' distances from the largest, not with the logits."""
+    logits, tv, ti = case(3, V, 50, torch.float32, 20)
+    logits = (logits * 256).round() / 256 + shift             # exact in fp32 with and without the shift
+    for T in (1.0, 1.5):
+        loss, grad = D.div_topk_rest(beta, logits.to(DEV), tv.to(DEV), ti.to(DEV), T=T)
+        for r in range(3):
+            ids, lp = entries(tv[r], ti[r], 50, V)
+            z = (logits[r].double() / T).requires_grad_(True)
+            P, Q = outcomes(z, lp, ids, REST_MIN)
+            want = divergence(P, Q, beta)
+            want.backward()
+            g = z.grad / T
+            with torch.no_grad():
+                # log2 of a probability is x a - top, one multiply-add with a off by 2^-23 of itself, less the log2 of a sum of
+                # powers, a few roundings of 2^-22: in all 2^-21 (4 + the largest distance in log2 units), whatever top is.  From
+                # there as in check()
+                E = 2.0 ** -21 * (4 + (z.max() - z.min()).item() * 1.4427)
+                share = (P.exp() + Q.exp()) * (1 + (P - Q).abs())
+                A = share.sum().item()
+                q = torch.softmax(z, 0)
+                others = torch.ones(V, dtype=torch.bool)
+                others[ids] = False
+                bound = q * (2 * A + 1) + torch.where(others, q, 0.0) / q[others].sum() * share[-1]
+                bound[ids] += share[:-1]
+                bound = bound * E / T + HALF_ULP[torch.float32] * g.abs() * (1 + 2.0 ** -6) + STEP[torch.float32]
+                assert abs(loss[r].item() - want.item()) <= E * A
+                assert ((grad[r].cpu().double() - g).abs() <= bound).all()
