@@ -100,13 +100,26 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
 
 @torch.library.custom_op("distillery_amd::embed", mutates_args=())
 def embed(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """`embed_rows` with autograd: differentiable with respect to `table` (a dense gradient, made by `embed_grad`)."""
+    """`embed_rows` with autograd: differentiable with respect to `table` (a dense gradient, made by `embed_grad`), any number of times.
+    A registered operator, as its backward is: torch.compile and FakeTensor tracing see through both."""
     return embed_rows(table, tokens, scale=scale)
 
 
 @embed.register_fake
 def _(table, tokens, scale=1.0):
     return table.new_empty((*tokens.shape, table.shape[1]))
+
+
+# Its gradient as an operator of its own, so that a backward pass is traced as well (shapes alone) and differentiated again: linear in
+# `grad`, with the lookup for its derivative.
+@torch.library.custom_op("distillery_amd::embed_backward", mutates_args=())
+def embed_backward_op(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
+    return embed_grad(grad, tokens, vocab, scale=scale)
+
+
+@embed_backward_op.register_fake
+def _(grad, tokens, vocab, scale):
+    return grad.new_empty((vocab, grad.shape[-1]))
 
 
 def _embed_setup(ctx, inputs, output):
@@ -117,7 +130,19 @@ def _embed_setup(ctx, inputs, output):
 
 def _embed_backward(ctx, grad):
     (tokens,) = ctx.saved_tensors
-    return embed_grad(grad, tokens, ctx.vocab, scale=ctx.scale), None, None
+    return embed_backward_op(grad, tokens, ctx.vocab, ctx.scale), None, None
+
+
+def _embed_backward_setup(ctx, inputs, output):
+    _, tokens, _, scale = inputs
+    ctx.save_for_backward(tokens)
+    ctx.scale = scale
+
+
+def _embed_twice(ctx, grad):
+    (tokens,) = ctx.saved_tensors
+    return embed(grad.contiguous(), tokens, ctx.scale), None, None, None
 
 
 embed.register_autograd(_embed_backward, setup_context=_embed_setup)
+embed_backward_op.register_autograd(_embed_twice, setup_context=_embed_backward_setup)

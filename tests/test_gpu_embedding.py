@@ -205,3 +205,33 @@ def test_refusals(D):
     assert lib.dl_embed_grad(*args[:2], 7, *args[3:], 0, 0, 0) == -3
     assert lib.dl_embed_grad(g.data_ptr(), 0, 8, 3, 8, t.data_ptr(), 1, 1.0, 0, table.data_ptr(), 1, 8, 10, 0, 0, 0) == -2
     assert lib.dl_embed_rows(table.data_ptr(), 0, 8, 10, 8, t.data_ptr() + 4, 1, 3, 1.0, g.data_ptr(), 8, 0) == -6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_gradient_is_differentiated_again(D, dtype):
+    """d/dw of <v, gradient of <w, embed(table)>> is embed(v); v comes dense and as one broadcast number."""
+    gen = torch.Generator().manual_seed(21)
+    table = torch.randn(50, 24, generator=gen).to(dtype).to(DEV).requires_grad_(True)
+    t = _tokens(60, 50, 9, "padded").to(DEV).view(6, 10)
+    w = torch.randn(6, 10, 24, generator=gen).to(dtype).to(DEV).requires_grad_(True)
+    v = torch.randn(50, 24, generator=gen).to(dtype).to(DEV)
+    grad, = torch.autograd.grad(D.embed(table, t, 3.0), table, w, create_graph=True)
+    assert torch.equal(grad.detach(), D.embed_grad(w.detach(), t, 50, scale=3.0))
+    again, = torch.autograd.grad(grad, w, v, retain_graph=True)
+    assert torch.equal(again, D.embed_rows(v, t, scale=3.0))
+    flat, = torch.autograd.grad(grad.sum(), w)
+    assert torch.equal(flat, D.embed_rows(torch.ones_like(v), t, scale=3.0))
+
+
+def test_registered_operators_and_a_compiled_step(D):
+    gen = torch.Generator().manual_seed(22)
+    table = torch.randn(40, 16, generator=gen).to(DEV).requires_grad_(True)
+    t = _tokens(30, 40, 5, "padded").to(DEV).view(5, 6)
+    w = torch.randn(5, 6, 16, generator=gen).to(DEV)
+    from llm_distillery_amd import embedding
+    torch.library.opcheck(embedding.embed, (table, t, 2.0))
+    torch.library.opcheck(embedding.embed_backward_op, (w.clone().requires_grad_(True), t, 40, 2.0))
+    step = lambda table, t, w: (D.embed(table, t, 2.0) * w).sum()  # noqa: E731
+    want, = torch.autograd.grad(step(table, t, w), table)
+    got, = torch.autograd.grad(torch.compile(step, backend="aot_eager", fullgraph=True)(table, t, w), table)
+    assert torch.equal(got, want)

@@ -411,3 +411,18 @@ def test_partial_marginals_are_taken_where_the_tiles_spared_outweigh_them(rows, 
     marginal meets few tiles."""
     n = D._lib.load().dl_rkl_marginalised_workspace_bytes(rows, Vt, columns, tile)
     assert n == (rows * parts * columns * 4 if parts > 1 else 0)
+
+
+def test_embedding_traces_with_fake_tensors_in_both_directions():
+    """The lookup, its gradient and that gradient's derivative have shape-only implementations: a training step is traced without a GPU."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        table = torch.empty(50, 24, dtype=torch.bfloat16, requires_grad=True)
+        tokens = torch.empty(6, 10, dtype=torch.int32)
+        weight = torch.empty(6, 10, 24, dtype=torch.bfloat16, requires_grad=True)
+        rows = D.embed(table, tokens, 3.0)
+        assert rows.shape == (6, 10, 24) and rows.dtype == torch.bfloat16
+        grad, = torch.autograd.grad((rows * weight).sum(), table, create_graph=True)
+        assert grad.shape == table.shape and grad.dtype == torch.bfloat16 and grad.requires_grad
+        again, = torch.autograd.grad(grad.sum(), weight)
+        assert again.shape == weight.shape and again.dtype == torch.bfloat16
