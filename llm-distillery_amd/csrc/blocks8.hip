@@ -151,10 +151,11 @@ __device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, cons
 // half of a's, so that three quarters of the bytes have a step and a half to arrive (what the latency of memory asks for: with
 // one step, waits were a third of the time).
 // Workgroups stay: each walks its tiles as one sequence of steps, so that the next tile's operands arrive while the last one is stored.
-// Measured: 8192 x 128256 x 4096 (bf16 out) 3.80-3.94 ms, 2190-2270 Tflop/s; the matrix units' time alone, at the 1.97 GHz that the card
+// Measured: 8192 x 128256 x 4096 (bf16 out) 3.69-3.94 ms, 2190-2330 Tflop/s; the matrix units' time alone, at the 1.97 GHz that the card
 // holds under this load, is 2.1 ms, the scaling's multiply-adds share the issue slots with them.  (A library product of the same operands
-// with one scale for all: 3.17 ms.)  Few rows are bound by the weights' bytes: 1 x 128256 x 4096 99-116 us (4.5-5.3 TB/s),
-// 61 x 50257 x 2048 18-19 us (5.5 TB/s).
+// with one scale for all: 3.17 ms.)  Few rows are bound by the weights' bytes: 1 x 128256 x 4096 99-117 us (4.5-5.3 TB/s),
+// 61 x 50257 x 2048 25 us (4.1 TB/s), 19 where MALL still has the weights.  (Few rows in a kernel that streams the weights straight into
+// the operands: 107 us for one row of 128256 x 4096, 115 for 4, 147 for 16, but 28 to 40 where these tiles take 17.5 on 50257 x 2048.)
 typedef const unsigned __attribute__((address_space(1))) * global_words;
 typedef unsigned __attribute__((address_space(3))) * lds_words;
 
@@ -418,7 +419,7 @@ static int launch_tiles(const BlocksParams& p, hipStream_t st) {
 
 // The tile of a call: that with the least time by a model of two numbers each, microseconds for a step of a CU -- alone, and what every
 // further tile of the CU adds -- measured over 15 shapes from 64 x 4096 to 4096 x 8000 (64 x 50257 x 2048: 34, 23, 21, 24 us in
-// the order of the list; 128 x 128256 x 4096: 137, 118, 148, 175; 512 x 128256 x 4096: 271, 335, 428, 519; 128 x 8000 x 4096: 51, 34, 21, 18).
+// the order of the list; 128 x 128256 x 4096: 137, 118, 148, 175; 512 x 128256 x 4096: 271, 335, 428, 519; 128 x 8000 x 4096: 51, 34, 21, 17-18).
 struct TileShape { int bm, bn; float alone, each; };
 constexpr TileShape TILE_SHAPES[] = {{256, 256, 1.55f, 1.55f}, {128, 256, 1.05f, 1.25f}, {64, 128, 0.62f, 0.43f}, {64, 64, 0.50f, 0.26f}};
 static int tile_shape(int64_t M, int64_t N) {

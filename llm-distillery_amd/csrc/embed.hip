@@ -10,8 +10,9 @@
 // leaves one fp32 partial sum per tile, which a last launch adds up in tile order.  No float atomics: the same bits
 // every time.  A frequent token is spread over as many workgroups as it has tiles.  The rows of the gradient that no
 // token names are zeroed by workgroups that ride along in the sorting launches, which would leave the card idle
-// otherwise: the sort is a chain of short launches, the zeroes are most of the bytes.  32768 tokens x 2048 bf16 into 128256 rows: 135 us
-// for 525 MB of gradient and 134 MB of g (4.9 TB/s), of them 91 in the sorting launches; 131 x 1024: 14 us in three launches.
+// otherwise: the sort is a chain of short launches, the zeroes are most of the bytes.  32768 tokens x 2048 bf16 into 128256 rows, 525 MB of
+// gradient and 121 MB of g: a call takes 156 us (4.1 TB/s), 134 where g is still in MALL (the sorting launches 92, the sums 33, the
+// join 9).  131 x 1024 fp32 added to a gradient: a call 19 us, its three launches in a graph 13.5.
 #include "distill_common.hpp"
 #include "distill_hip.h"
 
@@ -29,7 +30,8 @@ __device__ __forceinline__ int64_t token_row(const void* tokens, int itype, int6
 // TPR threads share a row: a wave where there are rows enough to fill the card with waves, else a workgroup (bf16, us for 64 / 256
 // threads: 1 x 4096 3.1 / 2.6, 512 x 4096 3.8 / 3.2, 2048 x 4096 4.7 / 4.8, 8192 x 4096 20.4 / 20.4, 8192 x 1024 4.9 / 6.0).  Table
 // rows are read with ordinary loads (frequent tokens then come from L2), the result is streamed out.  Rows may start
-// on any element; the columns behind the last whole 16 bytes go one by one.  Bound by HBM: 32768 x 4096 bf16 69 us.
+// on any element; the columns behind the last whole 16 bytes go one by one.  Bound by HBM: 32768 x 4096 bf16 70-79 us
+// (419 MB; the faster, the more of the rows MALL still has).
 template <class Tag, int TPR>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const char* __restrict__ table, int64_t table_stride, int64_t vocab, int64_t width,
                                                          const void* __restrict__ tokens, int itype, int64_t n_tokens, float scale,

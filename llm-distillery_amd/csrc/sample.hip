@@ -64,7 +64,9 @@ __device__ __forceinline__ float sample_t(const RowScale& s, float x) {
   return fmaxf(d * s.rate, -64.f);
 }
 // 2^(t + 31), every operation rounded by itself.  t plus 1.5 * 2^23 is rint(t) in the lowest bits; the coefficients carry the 2^31 (a
-// power of two changes no rounding), and 2^rint(t) is added to the exponent.
+// power of two changes no rounding), and 2^rint(t) is added to the exponent.  The polynomial is the one of degree 5 with p(0) = 1 whose
+// largest relative error over [-1/2, 1/2] is least (a linear program over a grid), its coefficients rounded to fp32: off by 1.1e-7 of 2^f at
+// most, 1.9e-7 as evaluated here.
 __device__ __forceinline__ float sample_power(float t) {
 #pragma clang fp contract(off)
   const float r = t + 0x1.8p23f, f = t - (r - 0x1.8p23f);
@@ -913,8 +915,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4, 8))) void
 // threads, top-k 50 and top-p 0.95 (T = 1.5 and top-p 0.98): 256 x 128256 35.4 / 34.6 (153 / 102), 300 x 128256 41.7 / 54.7 (166 / 164),
 // 512 x 32000 20.8 / 30.6 (53 / 70), 1024 x 50257 53 / 78 (140 / 193); 2048 x 50257 fp32 139 / 179 (276 / 375).
 // Bound by vector work and additions in LDS where a row is flat (four sweeps over it, the first from HBM, the others from L2 and MALL), by
-// the two sweeps' latency and the barriers between them for single rows: 1 x 32000 14.6 us; 256 x 128256 bf16 with mixed settings 75 us
-// (0.88 TB/s); 2048 x 50257 fp32 without top-k 216 us (1.9 TB/s).
+// the two sweeps' latency and the barriers between them for single rows: 1 x 32000 14.6 us; 256 x 128256 bf16 with mixed settings 75-96 us
+// (0.7-0.9 TB/s, by how flat the flattest row is); 2048 x 50257 fp32 without top-k 209-218 us (1.9 TB/s).
 template <class Tag>
 static int launch_sample(const SampleParams& p, hipStream_t st) {
   if (p.n_rows <= 256) hipLaunchKernelGGL((sample_row_kernel<Tag, 1024>), dim3((unsigned)p.n_rows), dim3(1024), 0, st, p);

@@ -8,8 +8,9 @@
 //   dL/dz_k = s_k - q_k S on a listed id, and softmax over the rest's columns times (s_rest - q_rest S) on those:
 // the rest's columns need one number per row, so the row is read once, written once and costs one exponential per column (two-byte
 // logits: their powers stay in registers as fp16; four-byte ones: as fp32).  Bound by HBM traffic, 2 V bytes x the element size per row:
-// 8192 x 128256 bf16, K = 200: 809-856 us (4.9-5.2 TB/s); 4093 x 50257, K = 100: 185-200 us (a tenth of the rows masked; 50304 columns,
-// whose rows begin on 16 bytes: 15 % less); 131 x 32000 fp32, K = 400: 17 us, the latency of its phases.
+// 8192 x 128256 bf16, K = 200: 799-856 us (4.9-5.3 TB/s); 4093 x 50257, K = 100: 182-204 us (a tenth of the rows masked; 50304 columns,
+// whose rows begin on 16 bytes: 15 % less); 2048 x 128256 fp32 in parts 432 us (4.9 TB/s); 131 x 32000 fp32, K = 400: 17 us, the latency
+// of its phases.
 //
 // Layout as in the forward-KL kernels: a row, or one column part of it, sits in its workgroup's registers; parts exchange
 // (max, sum) of the rest's columns through records in a workspace, with a bounded wait and a second launch for parts

@@ -138,8 +138,9 @@ def matmul_blocks(a: BlockQuantized, b: BlockQuantized, *, dtype: torch.dtype = 
     """a [M, width] times the transpose of b [N, width], both in 8-bit floating point: [M, N] in `dtype` (bf16/fp16/fp32).
 
     `a` has a scale for every 128 values of a row, `b` for every 128 x 128 (`quantize_blocks` with rows = 1 and 128).  A block's
-    128 products are summed by the matrix unit, the scaled sums of the blocks in fp32, and the result is rounded once.  A row's
-    result has the same bits whatever rows it comes with."""
+    128 products are summed by the matrix unit, the scaled sums of the blocks in fp32, and the result is rounded once.  The matrix
+    unit's sums are not fp32 sums: one is off by up to 2^-12 of the sum of its products' magnitudes (normal data: some 2e-5 of it),
+    which fp32 results show.  A row's result has the same bits whatever rows it comes with."""
     dev = a.codes.device
     if dtype not in _DT:
         raise RuntimeError("unsupported dtype")
