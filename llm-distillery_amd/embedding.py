@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _lib
 from .ops import _DT, _IT, _dev, _on, _row_pitch, _share_memory, _stream_ptr
@@ -130,6 +131,10 @@ def _embed_setup(ctx, inputs, output):
 
 def _embed_backward(ctx, grad):
     (tokens,) = ctx.saved_tensors
+    # Neither traced nor to be differentiated again: straight to the kernels (131 x 1024 fp32, forward and back: 115 us,
+    # 142 through the dispatcher).
+    if type(grad) is torch.Tensor and not torch.is_grad_enabled() and not is_in_torch_dispatch_mode():
+        return embed_grad(grad, tokens, ctx.vocab, scale=ctx.scale), None, None
     return embed_backward_op(grad, tokens, ctx.vocab, ctx.scale), None, None
 
 

@@ -235,3 +235,18 @@ def test_registered_operators_and_a_compiled_step(D):
     want, = torch.autograd.grad(step(table, t, w), table)
     got, = torch.autograd.grad(torch.compile(step, backend="aot_eager", fullgraph=True)(table, t, w), table)
     assert torch.equal(got, want)
+
+
+def test_a_traced_backward_pass_has_the_operator(D):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    table = torch.randn(40, 16, device=DEV)
+    t = _tokens(30, 40, 5, "padded").to(DEV)
+    w = torch.randn(30, 16, device=DEV)
+
+    def step(table, w):
+        table = table.detach().requires_grad_(True)
+        return torch.autograd.grad(D.embed(table, t, 2.0), table, w)[0]
+    for mode in ("real", "fake"):
+        graph = make_fx(step, tracing_mode=mode, _allow_non_fake_inputs=True)(table, w)
+        assert any("embed_backward" in str(n.target) for n in graph.graph.nodes)
+        assert torch.equal(graph(2 * table, 3 * w), step(2 * table, 3 * w))
