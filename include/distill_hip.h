@@ -36,7 +36,8 @@ typedef enum {
   DL_ERR_LAUNCH = -5,   /* the HIP runtime refused the launch              */
   DL_ERR_ALIGN = -6,    /* a pointer/stride breaks a stated alignment rule */
   DL_ERR_WORKSPACE = -7, /* a required workspace is too small              */
-  DL_ERR_SCRATCH = -8   /* dl_div_topk_static: the problem needs more scratch than the static array holds */
+  DL_ERR_SCRATCH = -8,  /* dl_div_topk_static: the problem needs more scratch than the static array holds */
+  DL_ERR_OVERLAP = -9   /* buffers that a call writes overlap              */
 } dl_status;
 
 #define DL_MAX_TOPK 2048      /* entries per row a sparse teacher may hold        */
@@ -668,6 +669,79 @@ int64_t dl_embed_grad_workspace_bytes(int64_t n_tokens, int64_t width);
 int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t n_tokens, int64_t width, const void* tokens, int itype,
                   float scale, int accumulate, void* grad, int grad_dtype, int64_t grad_stride, int64_t vocab, void* workspace,
                   int64_t workspace_bytes, void* stream);
+
+/*
+ * Logits made ready for the sampler: penalties for the tokens of a row's text, a bias, a mask of the tokens that are allowed.
+ *   y = x > 0 ? x / repetition : x * repetition    for the tokens among the first lengths[r] of the row's text
+ *   y -= frequency * count + presence              for those from entry prompt[r] on, `count` times there
+ *   y += bias[v];   y = -inf where bit v % 32 of word v / 32 of the row's mask is 0
+ * in this order, in fp32, rounded once to the logits' dtype.  -inf and NaN logits stay what they are, but for masked ones, which are -inf.
+ * tokens     int32 or int64 [n_texts, length] (row stride `token_stride`), NULL: no texts; ids outside [0, V) are padding.  Row r has text
+ *            token_rows[r] (outside [0, n_texts): none); without token_rows text r, or text 0 where there is one only.
+ * lengths    int32 [n_rows]: entries of its text that a row has (at most `length`; 0 or less: none); NULL: `length`.
+ * prompt     int32 [n_rows]: how many of these are the prompt's, which frequency and presence do not count; NULL: prompt_all.
+ * repetition, frequency, presence: fp32 [n_rows], or NULL and the `_all` value counts for every row.  A row with 1, 0, 0 has no penalties.
+ *            repetition should be positive.
+ * bias       [n_rows, V] (`bias_stride`) or, with bias_stride 0, [V] for all rows; fp32 or the logits' dtype; NULL: none.
+ * allowed    [n_masks, words] (`allowed_stride` words a row, at least V / 32 rounded up); NULL: all tokens are.  Row r has mask allowed_rows[r]
+ *            (outside [0, n_masks): none, all tokens are allowed); without allowed_rows mask r, or mask 0 where there is one only.
+ * out        [n_rows, V] of the logits' dtype; it may be the logits themselves (the same address and stride), else they do not overlap.
+ * V and length below 2^31 (DL_ERR_LIMIT); any element-aligned pointers and strides.
+ *
+ * dl_adjust_grad: the gradient.  g: [n_rows, V] of the logits' dtype, by y.
+ *   out[r, v]    = 0 where masked, else g / repetition or g * repetition at the text's tokens by the sign of x, else g     (NULL: not wanted)
+ *   bias_grad[v] = sum over r of g[r, v] where not masked, fp32 or the logits' dtype: of a bias that all rows share       (NULL: not wanted)
+ * out may be g itself.  logits: may be NULL where there is no text.  Sums are fp32 over runs of rows, these in fp64, always in the
+ * same order.  workspace: dl_adjust_grad_workspace_bytes(...) bytes where bias_grad is wanted, 16-byte aligned, contents irrelevant; two calls
+ * that may overlap in time must not share it.
+ */
+int dl_adjust_rows(const void* logits, int dtype, int64_t row_stride, int64_t n_rows, int64_t V, const void* tokens, int itype,
+                   int64_t token_stride, int64_t n_texts, int64_t length, const int32_t* token_rows, const int32_t* lengths,
+                   const int32_t* prompt, int64_t prompt_all, const float* repetition, const float* frequency, const float* presence,
+                   float repetition_all, float frequency_all, float presence_all, const void* bias, int bias_dtype, int64_t bias_stride,
+                   const int32_t* allowed, int64_t allowed_stride, int64_t n_masks, const int32_t* allowed_rows, void* out,
+                   int64_t out_stride, void* stream);
+int64_t dl_adjust_grad_workspace_bytes(int64_t n_rows, int64_t V);
+int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, const void* logits, int64_t row_stride, int64_t n_rows, int64_t V,
+                   const void* tokens, int itype, int64_t token_stride, int64_t n_texts, int64_t length, const int32_t* token_rows,
+                   const int32_t* lengths, const float* repetition, float repetition_all, const int32_t* allowed,
+                   int64_t allowed_stride, int64_t n_masks, const int32_t* allowed_rows, void* out, int64_t out_stride,
+                   void* bias_grad, int bias_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * 8-bit integers with a scale for every row, and the product of two such matrices.
+ *
+ * dl_quantize_rows: x [rows, cols] -> codes [rows, whole blocks of 128 columns] (zeros behind the last column), scales [rows].
+ * scale = max(largest magnitude * r, 2^-100) with r = 1 / 127 in fp32; code = x / scale (fp32), rounded to even, within [-127, 127].  A row
+ * with a NaN or an infinity has NaN for its scale and zeros for its codes.
+ *
+ * dl_matmul_rows: out[m, n] = (sum over the K columns of a[m, k] b[n, k]) * (a_scale[m] * b_scale[n]), out [M, N] of out_dtype.  The sum is exact
+ * (32-bit integers; any codes), one fp32 rounding makes it a float, one each the scales' product and the product with it, and
+ * one the result.  K up to 130944 (DL_ERR_LIMIT), in whole blocks of 128 whose tails hold zeros.
+ *
+ * codes, a and b: 16-byte aligned, strides of whole 16 bytes, at least the whole blocks (DL_ERR_ALIGN, DL_ERR_SHAPE); x and out: any
+ * element-aligned address and stride.
+ */
+int dl_quantize_rows(const void* x, int dtype, int64_t row_stride, int64_t rows, int64_t cols, void* codes, int64_t code_stride,
+                     float* scales, void* stream);
+int dl_matmul_rows(const void* a, int64_t a_stride, const float* a_scale, int64_t M, const void* b, int64_t b_stride, const float* b_scale,
+                   int64_t N, int64_t K, void* out, int out_dtype, int64_t out_stride, void* stream);
+
+/*
+ * The norm of the gradients of all parameters together, and the gradients clipped by it, in place.
+ *   norm = scale * sqrt(sum of the squares of all elements);   element = round(element * (scale * min(1, max_norm / norm)))
+ * tensors, sizes, dtypes: HOST arrays of n_tensors device addresses, numbers of elements (dense, in any order) and dtypes.  They travel with the
+ * launches, 240 tensors each.  Squares are added up in fp64, in the same order on every call.
+ * norm       device, one fp32.  dl_clip_grads writes it, or, with norm_given, takes it (that of more than these tensors: shards on other cards).
+ * A norm that is NaN or infinite leaves every tensor as it is.  So does one within max_norm where scale is 1: nothing is written then.
+ * scale: positive and finite; max_norm: not negative, not NaN (infinite: only scaled).  Tensors that overlap: DL_ERR_OVERLAP (dl_clip_grads).
+ * workspace  dl_grad_norm_workspace_bytes(...) bytes, 8-byte aligned, contents irrelevant; not needed with norm_given.
+ */
+int64_t dl_grad_norm_workspace_bytes(const int64_t* sizes, int64_t n_tensors);
+int dl_grad_norm(const void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t n_tensors, float scale, float* norm,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+int dl_clip_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes, int64_t n_tensors, float scale, float max_norm,
+                  float* norm, int norm_given, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Deterministic sum of n fp32 values times `scale` into out[0] (fixed reduction tree,

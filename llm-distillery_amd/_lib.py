@@ -94,6 +94,16 @@ _SIGNATURES = {
     "dl_embed_grad_workspace_bytes": (c_int64, [c_int64, c_int64]),
     "dl_embed_grad": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int, c_float, c_int, _P, c_int, c_int64, c_int64, _P,
                               c_int64, _P]),
+    "dl_adjust_rows": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P, c_int64, _P, _P, _P,
+                               c_float, c_float, c_float, _P, c_int, c_int64, _P, c_int64, c_int64, _P, _P, c_int64, _P]),
+    "dl_adjust_grad_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "dl_adjust_grad": (c_int, [_P, c_int, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P, c_float,
+                               _P, c_int64, c_int64, _P, _P, c_int64, _P, c_int, _P, c_int64, _P]),
+    "dl_quantize_rows": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int64, _P, _P]),
+    "dl_matmul_rows": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, _P, c_int, c_int64, _P]),
+    "dl_grad_norm_workspace_bytes": (c_int64, [_P, c_int64]),
+    "dl_grad_norm": (c_int, [_P, _P, _P, c_int64, c_float, _P, _P, c_int64, _P]),
+    "dl_clip_grads": (c_int, [_P, _P, _P, c_int64, c_float, c_float, _P, c_int, _P, c_int64, _P]),
     "dl_reduce_sum": (c_int, [_P, c_int64, c_float, _P, _P]),
     "dl_copy16": (c_int, [_P, _P, c_int64, _P]),
     "dl_copy_rows": (c_int, [_P, _P, c_int64, c_int64, c_int, c_int, c_int, _P]),

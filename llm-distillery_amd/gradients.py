@@ -1,0 +1,98 @@
+"""The norm of the gradients of all parameters together, and the gradients clipped by it.  Thin wrappers over the C ABI; all arithmetic runs in
+the HIP kernels."""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable, Optional
+
+import torch
+
+from . import _lib
+from .ops import _DT, _dev, _on, _stream_ptr
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill their stretch of memory, in any order and each place once."""
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class _Tensors:
+    """Tensors as the C ABI takes them: host arrays of addresses, sizes and dtypes."""
+
+    def __init__(self, grads: Iterable[torch.Tensor]):
+        self.all = grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+        if not grads:
+            raise RuntimeError("no gradients")
+        self.dev = grads[0].device
+        for g in grads:
+            if g.device != self.dev or not g.is_cuda or g.dtype not in _DT or g.layout is not torch.strided:
+                _dev(g, "a gradient")
+                if g.device != self.dev:
+                    raise RuntimeError(f"gradients live on {self.dev} and {g.device}: all tensors of a call must share one device")
+                raise RuntimeError("gradients must be dense bf16/fp16/fp32 tensors")
+            if not g.is_contiguous() and g.numel() and not _dense(g):
+                raise RuntimeError("a gradient must fill its memory (a slice or an expanded tensor does not)")
+        n = self.n = len(grads)
+        self.at = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
+        self.sizes = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
+        self.dtypes = (ctypes.c_int32 * n)(*[_DT[g.dtype] for g in grads])
+
+    def args(self):
+        return ctypes.addressof(self.at), ctypes.addressof(self.sizes), ctypes.addressof(self.dtypes), self.n
+
+    def workspace(self, lib) -> torch.Tensor:
+        return torch.empty(lib.dl_grad_norm_workspace_bytes(ctypes.addressof(self.sizes), self.n), dtype=torch.uint8, device=self.dev)
+
+
+def _positive(scale: float) -> float:
+    scale = float(scale)
+    if not 0.0 < scale <= 3.0e38:
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
+def grad_norm(grads: Iterable[torch.Tensor], *, scale: float = 1.0) -> torch.Tensor:
+    """`scale` times the 2-norm of all elements of `grads` (bf16/fp16/fp32 tensors of any shapes on one device) together, an fp32 tensor without
+    dimensions.  Squares are added up in fp64, in an order that does not change between calls."""
+    scale = _positive(scale)
+    t = _Tensors(grads)
+    lib = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=t.dev)
+    ws = t.workspace(lib)
+    with _on(t.dev):
+        st = lib.dl_grad_norm(*t.args(), scale, norm.data_ptr(), ws.data_ptr(), ws.numel(), _stream_ptr(t.dev))
+    _lib.check(st, "dl_grad_norm")
+    return norm
+
+
+def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, scale: float = 1.0, norm: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Multiplies all `grads` in place with `scale` (an average that should be a sum, a loss scale taken out) and, where the norm of what that gives is
+    above `max_norm`, with max_norm / norm as well: one factor, one rounding.  Returns the norm before clipping, an fp32 tensor without dimensions.
+
+    `norm` (fp32, one element, `scale` included): is taken for the norm instead, for gradients of which these are only a part (shards on other
+    cards: the root of the sum of the squares of their `grad_norm`).  A norm that is NaN or infinite leaves all gradients as they are; one within
+    max_norm leaves them unwritten where scale is 1.  The gradients must not overlap.  Nothing waits for the GPU."""
+    scale, max_norm = _positive(scale), float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must not be negative")
+    t = _Tensors(grads)
+    lib = _lib.load()
+    given = norm is not None
+    if given:
+        if norm.device != t.dev or norm.dtype != torch.float32 or norm.numel() != 1:
+            _dev(norm, "norm")
+            raise RuntimeError(f"norm must be one fp32 element on {t.dev}")
+        ws = None
+    else:
+        norm = torch.empty((), dtype=torch.float32, device=t.dev)
+        ws = t.workspace(lib)
+    with _on(t.dev):
+        st = lib.dl_clip_grads(*t.args(), scale, max_norm, norm.data_ptr(), int(given), ws.data_ptr() if ws is not None else 0,
+                               ws.numel() if ws is not None else 0, _stream_ptr(t.dev))
+    _lib.check(st, "dl_clip_grads")
+    return norm

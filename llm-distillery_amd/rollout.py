@@ -1,4 +1,4 @@
-"""What a student needs to write its own continuations: sampling from its logits, and its head in 8-bit floating point.  Thin
+"""What a student needs to write its own continuations: sampling from its logits, and its head in 8-bit floating point or integers.  Thin
 wrappers over the C ABI; all arithmetic runs in the HIP kernels."""
 from __future__ import annotations
 
@@ -159,4 +159,82 @@ def matmul_blocks(a: BlockQuantized, b: BlockQuantized, *, dtype: torch.dtype = 
         with _on(dev):
             st = _lib.load().dl_matmul_blocks(*left, M, *right, N, W, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
         _lib.check(st, "dl_matmul_blocks")
+    return out
+
+
+class RowQuantized(NamedTuple):
+    """A matrix [rows, width] held in 8-bit integers: `codes` int8 [rows, width rounded up to whole blocks of 128] with zeros behind the last
+    column, and `scales` fp32 [rows]; an element is its code times its row's scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    width: int
+
+    def dequantize(self) -> torch.Tensor:
+        """The matrix in fp32 (plain torch; for looking at it)."""
+        return (self.codes.float() * self.scales.unsqueeze(1))[:, :self.width]
+
+
+def quantize_rows(x: torch.Tensor) -> RowQuantized:
+    """x [..., width] (bf16/fp16/fp32, rows evenly strided) in 8-bit integers with one scale for every row: a state, or the weights of an output
+    channel (laid out once).
+
+    A row's scale is its largest magnitude times 1 / 127 (in fp32), at least 2^-100; codes are the values over the scale, rounded to even, within
+    [-127, 127].  A row with a NaN or an infinity has a scale of NaN."""
+    _dev(x, "x")
+    v = x if x.dim() == 2 and x.stride(1) == 1 else _rows_2d(x if x.dim() > 1 else x.unsqueeze(0))
+    if v.dtype not in _DT:
+        raise RuntimeError("unsupported dtype")
+    R, W = v.shape
+    if R > 1 and v.stride(0) < W:
+        raise RuntimeError("x: rows overlap; make them contiguous first")
+    dev = v.device
+    wide = _blocks(W) * 128
+    codes = torch.empty((R, wide), dtype=torch.int8, device=dev)
+    scales = torch.empty(R, dtype=torch.float32, device=dev)
+    if R and W:
+        with _on(dev):
+            st = _lib.load().dl_quantize_rows(v.data_ptr(), _DT[v.dtype], _row_pitch(v), R, W, codes.data_ptr(), wide, scales.data_ptr(),
+                                              _stream_ptr(dev))
+        _lib.check(st, "dl_quantize_rows")
+    return RowQuantized(codes, scales, W)
+
+
+def _check_rows(q: RowQuantized, name: str, wide: int, dev: torch.device):
+    """(address, row stride) of the codes and the address of the scales of an operand."""
+    codes, scales = q.codes, q.scales
+    if codes.device != dev or scales.device != dev:
+        _dev(codes, f"{name}.codes", dev), _dev(scales, f"{name}.scales", dev)
+    rows, columns = codes.shape
+    pitch, one = codes.stride()
+    if codes.dtype != torch.int8 or columns != wide or rows and (one != 1 or rows > 1 and pitch < wide):
+        raise RuntimeError(f"{name}.codes must be an int8 matrix of whole blocks of 128 columns, dense along its rows")
+    if scales.dtype != torch.float32 or scales.shape != (rows,) or rows > 1 and scales.stride(0) != 1:
+        raise RuntimeError(f"{name}.scales must be a contiguous fp32 vector of {rows} entries")
+    return codes.data_ptr(), pitch if rows > 1 else wide, scales.data_ptr()
+
+
+def matmul_rows(a: RowQuantized, b: RowQuantized, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [M, width] times the transpose of b [N, width], both in 8-bit integers with a scale for every row (`quantize_rows`): [M, N] in `dtype`
+    (bf16/fp16/fp32).
+
+    Sums of products are exact; a sum becomes a float, is multiplied with the product of the two scales (each rounded in fp32), and the result is
+    rounded once.  A row's result has the same bits whatever rows it comes with.  Up to 130944 columns."""
+    dev = a.codes.device
+    if dtype not in _DT:
+        raise RuntimeError("unsupported dtype")
+    if a.codes.dim() != 2 or b.codes.dim() != 2:
+        raise RuntimeError("codes must be matrices")
+    M, N, W = a.codes.shape[0], b.codes.shape[0], a.width
+    if W != b.width:
+        raise RuntimeError(f"a has {W} columns, b {b.width}")
+    if W <= 0:
+        raise RuntimeError("the rows have no columns")
+    _dev(a.codes, "a.codes")
+    a_ptr, a_pitch, a_scale = _check_rows(a, "a", _blocks(W) * 128, dev)
+    b_ptr, b_pitch, b_scale = _check_rows(b, "b", _blocks(W) * 128, dev)
+    out = torch.empty((M, N), dtype=dtype, device=dev)
+    if M and N:
+        with _on(dev):
+            st = _lib.load().dl_matmul_rows(a_ptr, a_pitch, a_scale, M, b_ptr, b_pitch, b_scale, N, W, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
+        _lib.check(st, "dl_matmul_rows")
     return out
