@@ -12,13 +12,13 @@
 #include "distill_common.hpp"
 #include "distill_hip.h"
 #include "product_schedule.hpp"
+#include "tiles8.hpp"
 
 #include <algorithm>
 
 namespace dl {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int QB = 128;                       // values that share a scale; bytes of a block of a row
 constexpr float QSCALE = 1.f / 448.f, QSCALE_MIN = 0x1p-100f;
@@ -27,20 +27,6 @@ constexpr float QSCALE = 1.f / 448.f, QSCALE_MIN = 0x1p-100f;
 // scale = max(largest magnitude * (1 / 448 in fp32), 2^-100), code = x / scale (an IEEE division) rounded to e4m3, ties to even.
 // Columns behind the last one are zeros, up to the end of the block.  NaN stays NaN; a block with an infinity has an infinite
 // scale and NaN in the infinity's place.
-template <class Tag>
-__device__ __forceinline__ void load_eight(const char* row, int64_t col, int64_t cols, float* f) {
-  if (col + 8 <= cols) {
-    if constexpr (Tag::bytes == 2) {
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 2), f);
-    } else {
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 4), f);
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 4 + 16), f + 4);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = col + e < cols ? load_as_float(row, Tag::id, col + e) : 0.f;
-  }
-}
 __device__ __forceinline__ float largest_of_eight(const float* f) {
   float m = 0.f;
 #pragma unroll
@@ -121,25 +107,6 @@ __device__ __forceinline__ f32x4 block_product(const i32x8& b, const i32x8& a) {
 __device__ __forceinline__ i32x8 join_pieces(const u32x4& lo, const u32x4& hi) {
   return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
-// Four neighbouring columns of a row, as far as it reaches.
-template <class Tag>
-__device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, const f32x4& v) {
-  if (n + 4 <= N) {
-    if constexpr (Tag::bytes == 4) {
-      store16_unaligned(row + n * 4, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
-    } else {
-      const float f[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
-      const u32x4 c = Chunk<Tag>::pack(f);
-      const u32x2 two = {c[0], c[1]};
-      __builtin_memcpy(row + n * 2, &two, 8);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < N) store_from_float(row, Tag::id, n + i, v[i]);
-  }
-}
-
 // Tiles of BM x BN, a wave WM x WN of it, one block of 128 columns per step.  A step's operands are fetched into LDS by loads
 // that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted by
 // piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in
@@ -156,30 +123,10 @@ __device__ __forceinline__ void store_four(char* row, int64_t n, int64_t N, cons
 // with one scale for all: 3.17 ms.)  Few rows are bound by the weights' bytes: 1 x 128256 x 4096 99-117 us (4.5-5.3 TB/s),
 // 61 x 50257 x 2048 25 us (4.1 TB/s), 19 where MALL still has the weights.  (Few rows in a kernel that streams the weights straight into
 // the operands: 107 us for one row of 128256 x 4096, 115 for 4, 147 for 16, but 28 to 40 where these tiles take 17.5 on 50257 x 2048.)
-typedef const unsigned __attribute__((address_space(1))) * global_words;
-typedef unsigned __attribute__((address_space(3))) * lds_words;
-
 // The operand that begins `lo` / `hi` bytes into LDS for this lane (its two pieces), `rows` (a constant) rows on.
 __device__ __forceinline__ i32x8 tile_operand(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
   return join_pieces(*reinterpret_cast<const u32x4*>(lds + lo + rows * QB), *reinterpret_cast<const u32x4*>(lds + hi + rows * QB));
 }
-
-// The tiles of a launch: consecutive workgroups go round the 8 XCDs; each XCD has a contiguous eighth of the tiles, in bands of 8
-// rows of tiles, so that the tiles it works on at a time share their operands in its L2.
-struct TileWalk {
-  unsigned tiles_m, tiles_n, first, step, end;
-  __device__ TileWalk(unsigned tm, unsigned tn) : tiles_m(tm), tiles_n(tn) {
-    const unsigned total = tm * tn, each = (total + 7) / 8, xcd = blockIdx.x & 7u;
-    first = xcd * each + (blockIdx.x >> 3);
-    end = min(total, (xcd + 1) * each);
-    step = gridDim.x >> 3;
-  }
-  __device__ void origin(unsigned t, int64_t& m, int64_t& n) const {      // in tiles
-    const unsigned band = t / (8u * tiles_n), high = min(8u, tiles_m - band * 8u), in = t - band * 8u * tiles_n;
-    m = band * 8u + in % high;
-    n = in / high;
-  }
-};
 
 template <class Tag, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void tile_kernel(const BlocksParams p, unsigned tiles_m, unsigned tiles_n) {

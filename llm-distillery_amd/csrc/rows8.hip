@@ -7,6 +7,7 @@
 // neighbouring columns n of one row m, and the result is stored in pieces of four.
 #include "distill_common.hpp"
 #include "distill_hip.h"
+#include "tiles8.hpp"
 
 #include <algorithm>
 
@@ -20,20 +21,6 @@ constexpr float ISCALE = 1.f / 127.f, ISCALE_MIN = 0x1p-100f;
 
 // ---- quantise ---------------------------------------------------------------------------------------
 // A workgroup a row, twice: for its largest magnitude, and for the codes.
-template <class Tag>
-__device__ __forceinline__ void load_some(const char* row, int64_t col, int64_t cols, float* f) {      // eight
-  if (col + 8 <= cols) {
-    if constexpr (Tag::bytes == 2) {
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 2), f);
-    } else {
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 4), f);
-      Chunk<Tag>::unpack(load16_unaligned(row + col * 4 + 16), f + 4);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = col + e < cols ? load_as_float(row, Tag::id, col + e) : 0.f;
-  }
-}
 struct RowsQuant {
   const char* x; int64_t row_stride, rows, cols, width;        // width: whole blocks
   signed char* codes; int64_t code_stride;
@@ -48,7 +35,7 @@ __global__ __launch_bounds__(NT) void quantize_whole_rows_kernel(const RowsQuant
     float m = 0.f;
     for (int64_t col = threadIdx.x * 8; col < p.cols; col += NT * 8) {
       float f[8];
-      load_some<Tag>(x, col, p.cols, f);
+      load_eight<Tag>(x, col, p.cols, f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = not_finite(f[e]) ? __builtin_inff() : fmaxf(m, fabsf(f[e]));
     }
@@ -58,7 +45,7 @@ __global__ __launch_bounds__(NT) void quantize_whole_rows_kernel(const RowsQuant
     if (threadIdx.x == 0) p.scales[row] = odd ? __builtin_nanf("") : scale;
     for (int64_t col = threadIdx.x * 8; col < p.width; col += NT * 8) {
       float f[8];
-      load_some<Tag>(x, col, p.cols, f);
+      load_eight<Tag>(x, col, p.cols, f);
       u32x2 c = {0u, 0u};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -77,85 +64,250 @@ struct RowsParams {
   int blocks;
   char* out; int64_t out_stride;
 };
-template <class Tag>
-__device__ __forceinline__ void store_four_columns(char* row, int64_t n, int64_t N, const float* v) {
-  if (n + 4 <= N) {
-    if constexpr (Tag::bytes == 4) {
-      store16_unaligned(row + n * 4, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
-    } else {
-      const float f[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
-      const u32x4 c = Chunk<Tag>::pack(f);
-      const u32x2 two = {c[0], c[1]};
-      __builtin_memcpy(row + n * 2, &two, 8);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < N) store_from_float(row, Tag::id, n + i, v[i]);
-  }
+
+// Tiles of BM x BN, a wave WM x WN of it, a block of 128 columns (two matrix instructions deep) per step.  A step's operands are fetched into LDS by
+// loads that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted
+// by piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in lane
+// order, so it is their source addresses that are permuted.)
+// Within a step a wave goes through its WM / 16 rows of tiles: the operand of the next row is read while the matrix unit works on this one.  A
+// step's last barrier sits ahead of the last row, whose operands are in registers by then, so that the matrix unit is busy across it; another one at
+// half the step frees b's place and half of a's.  Workgroups stay: each walks its tiles as one sequence of steps.
+struct Piece { i32x4 lo, hi; };                                // a lane's 32 bytes of a row: 16 columns of either half of the block
+__device__ __forceinline__ Piece row_piece(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
+  return Piece{*reinterpret_cast<const i32x4*>(lds + lo + rows * KB), *reinterpret_cast<const i32x4*>(lds + hi + rows * KB)};
 }
 
-// Tiles of BM x BN, a wave WM x WN of it, a block of 128 columns at a time through LDS.  A row of a tile is 128 bytes, its eight 16-byte
-// pieces permuted by piece ^ (row % 8).
 template <class Tag, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_kernel(const RowsParams p) {
-  constexpr int NT = (BM / WM) * (BN / WN) * WAVE, TM = WM / 16, TN = WN / 16;
-  __shared__ __align__(16) unsigned char lds[(BM + BN) * KB];
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, i16 = lane % 16, quad = lane / 16;
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(const RowsParams p, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16, NA = BM / 8 / WAVES, NB = BN / 8 / WAVES;
+  static_assert(TM >= 2 && BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole fetches");
+  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes)
+  constexpr int STEP = (BM + BN) * KB;
+  const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), i16 = lane % 16;      // (w: known to be the wave's)
   const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
-  const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
-  i32x4 acc[TM][TN];
+  const TileWalk walk(tiles_m, tiles_n);
+  if (walk.first >= walk.end) return;
+  const unsigned steps = ((walk.end - walk.first + walk.step - 1) / walk.step) * (unsigned)p.blocks;
+
+  // the fetching side: its tile, its block, this thread's places in them
+  unsigned f_tile = walk.first;
+  int f_kb = 0;
+  const unsigned char *f_a, *f_b;
+  unsigned f_ao[NA], f_bo[NB];
+  const auto f_begin = [&]() {
+    int64_t m, n;
+    walk.origin(f_tile, m, n);
+    m *= BM;
+    n *= BN;
+    f_a = p.a + m * p.a_stride;
+    f_b = p.b + n * p.b_stride;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-  for (int kb = 0; kb < p.blocks; ++kb) {
-    for (int c = threadIdx.x; c < (BM + BN) * 8; c += NT) {
-      const int row = c / 8, piece = c % 8;
-      const unsigned char* from = row < BM ? p.a + min(m0 + row, p.M - 1) * p.a_stride : p.b + min(n0 + row - BM, p.N - 1) * p.b_stride;
-      *reinterpret_cast<u32x4*>(lds + row * KB + (piece ^ (row & 7)) * 16) = *reinterpret_cast<const u32x4*>(from + (int64_t)kb * KB + piece * 16);
+    for (int i = 0; i < NA; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_ao[i] = (unsigned)(min((int64_t)row, p.M - 1 - m) * p.a_stride) + piece * 16;
     }
-    __syncthreads();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x4 af[TM], bf[TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) af[i] = *reinterpret_cast<const i32x4*>(lds + (wm + i * 16 + i16) * KB + ((h * 4 + quad) ^ (i16 & 7)) * 16);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) bf[j] = *reinterpret_cast<const i32x4*>(lds + (BM + wn + j * 16 + i16) * KB + ((h * 4 + quad) ^ (i16 & 7)) * 16);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af[i], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < NB; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
     }
-    __syncthreads();
+  };
+  // In two parts, by when their places become free: `early` after half a step (b, whose operands are in registers from a step's
+  // beginning on, and of a the rows that the waves go through first), `late` at its end.
+  constexpr bool HALVES = WM / 2 == WAVES * 8;                 // every other fetch of a: those rows
+  constexpr int EARLY = NB + (HALVES ? NA / 2 : 0);
+  const auto fetch_a = [&](unsigned char* to, int i) {
+    __builtin_amdgcn_global_load_lds((global_words)(f_a + f_ao[i]), (lds_words)(to + (i * WAVES + w) * 1024), 16, 0, 0);
+  };
+  const auto fetch_early = [&](unsigned step) {
+    unsigned char* to = lds + (step & 1u) * STEP;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      __builtin_amdgcn_global_load_lds((global_words)(f_b + f_bo[i]), (lds_words)(to + BM * KB + (i * WAVES + w) * 1024), 16, 0, 0);
+    if (HALVES)
+#pragma unroll
+      for (int i = 0; i < NA; i += 2) fetch_a(to, i);
+  };
+  const auto fetch_late = [&](unsigned step) {
+    unsigned char* to = lds + (step & 1u) * STEP;
+#pragma unroll
+    for (int i = HALVES ? 1 : 0; i < NA; i += HALVES ? 2 : 1) fetch_a(to, i);
+    f_a += KB;
+    f_b += KB;
+    if (++f_kb == p.blocks) {
+      f_kb = 0;
+      f_tile += walk.step;
+      if (f_tile < walk.end) f_begin();
+    }
+  };
+  const auto meet = [&]() {                                    // everyone's reads so far are done
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // This wave's fetches are there but for the last `early` part (loads come back in order; the stores of a tile only add to the count).
+  const auto landed = [&](bool early_under_way) {
+    if (early_under_way) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EARLY) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+
+  f_begin();
+  fetch_early(0);
+  fetch_late(0);
+  landed(false);
+  meet();
+  if (steps > 1) {
+    fetch_early(1);
+    fetch_late(1);
   }
+  // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
+  const unsigned lo = i16 * KB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
+  unsigned a_lo = wm * KB + lo, a_hi = wm * KB + hi, b_lo = (BM + wn) * KB + lo, b_hi = (BM + wn) * KB + hi;
+  unsigned flip = STEP;                                        // from a place in this step's buffer to the other's
+  Piece bf[TN], af[2];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + wm + i * 16 + i16;
-    if (m >= p.M) continue;
-    const float sa = p.sa[m];
+  for (int j = 0; j < TN; ++j) bf[j] = row_piece(lds, b_lo, b_hi, j * 16);
+  af[0] = row_piece(lds, a_lo, a_hi, 0);
+  unsigned step = 0;
+  for (unsigned tile = walk.first; tile < walk.end; tile += walk.step) {
+    int64_t m0, n0;
+    walk.origin(tile, m0, n0);
+    m0 *= BM;
+    n0 *= BN;
+    i32x4 acc[TM][TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int64_t n = n0 + wn + j * 16 + quad * 4;
-      if (n >= p.N) continue;
-      float v[4];
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * (sa * p.sb[min(n + e, p.N - 1)]);
-      store_four_columns<Tag>(p.out + m * p.out_stride * Tag::bytes, n, p.N, v);
+      for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll 1
+    for (int kb = 0; kb < p.blocks; ++kb, ++step) {
+#pragma unroll
+      for (int i = 0; i < TM - 1; ++i) {
+        af[(i + 1) & 1] = row_piece(lds, a_lo, a_hi, (i + 1) * 16);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].lo, af[i & 1].lo, acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[i & 1].hi, acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // the next operand's reads behind the first product
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN - 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == TM / 2 - 1 && step + 2 < steps) {
+          meet();
+          fetch_early(step);                                   // (into this step's buffer)
+        }
+      }
+      landed(step + 2 < steps);
+      meet();
+      if (step + 2 < steps) fetch_late(step);
+      a_lo += flip;
+      a_hi += flip;
+      b_lo += flip;
+      b_hi += flip;
+      flip = 0u - flip;
+      constexpr int L = TM - 1;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].lo, af[L & 1].lo, acc[L][j], 0, 0, 0);
+        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[L & 1].hi, acc[L][j], 0, 0, 0);
+        bf[j] = row_piece(lds, b_lo, b_hi, j * 16);            // (behind the last step: what lies there, unused)
+      }
+      af[0] = row_piece(lds, a_lo, a_hi, 0);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    // The tile's values.  Two-byte results go through 2 KiB of LDS of the wave's own, 16 rows at a time, so that a store writes whole
+    // 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by unit ^ (row % 8).
+    int here = lane;
+    asm volatile("" : "+v"(here));                             // (keeps the stores' addresses out of the steps' registers)
+    const int row = here % 16, quad = here / 16;
+    f32x4 sb[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sb[j][e] = p.sb[min(n0 + wn + j * 16 + quad * 4 + e, p.N - 1)];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const float sa = p.sa[min(m0 + wm + i * 16 + row, p.M - 1)];
+      f32x4 v[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = (float)acc[i][j][e] * (sa * sb[j][e]);
+      if constexpr (Tag::bytes == 2 && WN == 64) {
+        unsigned char* stage = lds + 2 * STEP + w * 2048;
+        const int r8 = here / 8, unit = here % 8;
+        const int64_t n = n0 + wn + unit * 8;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const float f[8] = {v[j][0], v[j][1], v[j][2], v[j][3], 0.f, 0.f, 0.f, 0.f};
+          const u32x4 c = Chunk<Tag>::pack(f);
+          *reinterpret_cast<u32x2*>(stage + row * 128 + ((j * 2 + quad / 2) ^ (row & 7)) * 16 + (quad & 1) * 8) = u32x2{c[0], c[1]};
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int64_t m = m0 + wm + i * 16 + k * 8 + r8;
+          const u32x4 c = *reinterpret_cast<const u32x4*>(stage + (k * 8 + r8) * 128 + (unit ^ r8) * 16);
+          char* to = p.out + (m * p.out_stride + n) * 2;
+          if (m < p.M && n + 8 <= p.N) store16_stream_any(to, c);
+          else if (m < p.M && n < p.N) store_chunk_elementwise<Tag>(to, 0, (int)(p.N - n), c);
+        }
+      } else {
+        const int64_t m = m0 + wm + i * 16 + row;
+        char* to = p.out + m * p.out_stride * Tag::bytes;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int64_t n = n0 + wn + j * 16 + quad * 4;
+          if (m < p.M && n < p.N) store_four<Tag>(to, n, p.N, v[j]);
+        }
+      }
     }
   }
 }
 
 static int rows_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH; }
 
+template <class Tag, int BM, int BN, int WM, int WN>
+static int launch_row_tiles(const RowsParams& p, hipStream_t st) {
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * (BM + BN) * KB + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+  if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
+  if (bytes > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&rows_kernel<Tag, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return DL_ERR_LAUNCH;
+  const unsigned grid = (unsigned)std::min<int64_t>((tm * tn + 7) / 8 * 8, 256 * std::min(per_cu, 4));
+  hipLaunchKernelGGL((rows_kernel<Tag, BM, BN, WM, WN>), dim3(grid), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
+  return rows_status();
+}
+
+// The tile of a call: that with the least time by a model of two numbers each, microseconds for a step of a CU -- alone, and what every
+// further tile of the CU adds.
+struct RowsShape { int bm, bn; float alone, each; };
+constexpr RowsShape ROWS_SHAPES[] = {{256, 256, 1.55f, 1.55f}, {128, 256, 1.05f, 1.25f}, {64, 128, 0.62f, 0.43f}, {64, 64, 0.50f, 0.26f}};
+static int rows_shape(int64_t M, int64_t N) {
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const RowsShape& t = ROWS_SHAPES[i];
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const float time = std::max(t.alone, (float)((tiles + 255) / 256) * t.each);
+    if (i == 0 || time < least) { best = i; least = time; }
+  }
+  return best;
+}
+
 template <class Tag>
 static int launch_rows(const RowsParams& p, hipStream_t st) {
-  constexpr int B = 128;
-  const int64_t tm = (p.M + B - 1) / B, tn = (p.N + B - 1) / B;
-  if (tm * tn * 256 > LAUNCH_THREADS || tn > 65535) return DL_ERR_LIMIT;
-  hipLaunchKernelGGL((rows_kernel<Tag, B, B, 64, 64>), dim3((unsigned)tm, (unsigned)tn), dim3(256), 0, st, p);
-  return rows_status();
+  switch (rows_shape(p.M, p.N)) {
+    case 0: return launch_row_tiles<Tag, 256, 256, 128, 64>(p, st);
+    case 1: return launch_row_tiles<Tag, 128, 256, 64, 64>(p, st);
+    case 2: return launch_row_tiles<Tag, 64, 128, 32, 64>(p, st);
+    default: return launch_row_tiles<Tag, 64, 64, 32, 32>(p, st);
+  }
 }
 
 }  // namespace dl
