@@ -4,10 +4,14 @@
 //   y -= frequency * count + presence                    for those behind the text's prompt, `count` times there
 //   y += bias;   y = -inf where the row's mask has no bit
 //
-// A workgroup has a row, or a part of its columns.  It counts the text's tokens that fall into its columns in LDS -- whole numbers, so
-// the order of the additions does not show -- and then goes through the columns once.  The gradient (by x: g, times what the penalty
-// multiplied with; by a bias that the rows share: the sum of g over the rows, both 0 where the mask has no bit) needs of x only the sign
-// at the text's tokens.
+// A workgroup has a row, or a part of its columns.  A text's tokens are few among these and the row's bytes are what has to move, so nothing is
+// done for a column that the text does not have: the tokens set a bit for their column in LDS, and count themselves (whole numbers: the order of the
+// additions does not show); the columns go from registers to memory in 16-byte pieces, by way of LDS where a piece has a bit: the thread puts its
+// pieces there, works on the elements whose bits are set, one after the other, and takes the pieces back.  Masked ones are taken out by a few bit
+// selects.  Nothing is unpacked unless there is a bias.  Texts are asked for first and the row behind them, so that its loads are under way while
+// tokens are counted; what a mask takes out throughout is not read.
+// The gradient (by x: g over or times the repetition at the text's tokens; by a bias that the rows share: the sum of g over the rows; both 0
+// where the mask has no bit) goes the same way; of x it reads the pieces with a bit alone.
 #include "distill_common.hpp"
 #include "distill_hip.h"
 
@@ -21,190 +25,338 @@ struct AdjustParams {
   char* out; int64_t out_stride;
   int64_t n_rows, V;
   const char* tokens; int itype; int64_t token_stride, n_texts, length;
-  const int32_t *token_rows, *lengths, *prompt; int64_t prompt_all;
+  const int32_t *token_rows, *lengths, *prompt; int prompt_all;
   const float *repetition, *frequency, *presence; float repetition_all, frequency_all, presence_all;
   const char* bias; int bias_dtype; int64_t bias_stride;
   const unsigned* allowed; int64_t allowed_stride, n_masks; const int32_t* allowed_rows;
   unsigned parts, part_columns;
-  int64_t first_row;
+  int64_t first_row, run;                                      // `run` rows a workgroup
 };
 
-// What a row has besides its logits.
+// What a row has besides its logits.  A lane fetches one of its settings each, so that they take one trip to memory; the same in all waves.
 struct AdjustRow {
   const char* text;
-  int64_t length, prompt;                                      // entries that count, and how many of them are the prompt's
-  float repetition, frequency, presence;
+  int length, prompt;                                          // entries that count, and how many of them are the prompt's
+  float repetition, inverse, frequency, presence;
   const unsigned char* bits;                                   // its mask, or nothing
   __device__ __forceinline__ AdjustRow(const AdjustParams& p, int64_t r) {
-    repetition = p.repetition ? p.repetition[r] : p.repetition_all;
-    frequency = p.frequency ? p.frequency[r] : p.frequency_all;
-    presence = p.presence ? p.presence[r] : p.presence_all;
-    int64_t t = p.token_rows ? (int64_t)p.token_rows[r] : p.n_texts == 1 ? 0 : r;
-    length = p.lengths ? min((int64_t)p.lengths[r], p.length) : p.length;
+    const void* const settings[7] = {p.repetition, p.frequency, p.presence, p.token_rows, p.lengths, p.prompt, p.allowed_rows};
+    const int lane = threadIdx.x & (WAVE - 1);
+    const void* mine = nullptr;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) mine = lane == k ? settings[k] : mine;
+    int got = 0;
+    if (mine) got = reinterpret_cast<const int*>(mine)[r];
+    const auto number = [&](int k) { return __builtin_amdgcn_readlane(got, k); };
+    repetition = p.repetition ? __int_as_float(number(0)) : p.repetition_all;
+    frequency = p.frequency ? __int_as_float(number(1)) : p.frequency_all;
+    presence = p.presence ? __int_as_float(number(2)) : p.presence_all;
+    int64_t t = p.token_rows ? (int64_t)number(3) : p.n_texts == 1 ? 0 : r;
+    length = p.lengths ? min(number(4), (int)p.length) : (int)p.length;
+    prompt = p.prompt ? number(5) : p.prompt_all;
     if (t < 0 || t >= p.n_texts || length < 0 || (repetition == 1.f && frequency == 0.f && presence == 0.f)) t = length = 0;
-    prompt = p.prompt ? (int64_t)p.prompt[r] : p.prompt_all;
     text = p.tokens + t * p.token_stride * (p.itype == I64 ? 8 : 4);
-    const int64_t m = p.allowed_rows ? (int64_t)p.allowed_rows[r] : p.n_masks == 1 ? 0 : r;
+    const int64_t m = p.allowed_rows ? (int64_t)number(6) : p.n_masks == 1 ? 0 : r;
     bits = m >= 0 && m < p.n_masks ? reinterpret_cast<const unsigned char*>(p.allowed + m * p.allowed_stride) : nullptr;
+    inverse = 1.f / repetition;
+  }
+  // f / repetition, rounded once: a product with the rounded reciprocal, and what it is off by taken off (the remainder is exact).  Where the product is no
+  // number or infinite, it is the quotient.
+  __device__ __forceinline__ float quotient(float f) const {
+    const float q = f * inverse, better = fmaf(fmaf(-q, repetition, f), inverse, q);
+    return fabsf(q) <= 3.402823466e38f ? better : q;
   }
 };
 
-// The counters of a part's columns: one 32-bit word a column (WIDE), or half a word, whose top bit says that the prompt has the token and
-// whose other bits count up to 32767 tokens behind it.
-template <bool WIDE>
-struct Counters {
-  static constexpr unsigned PROMPT = WIDE ? 0x80000000u : 0x8000u;
-  static constexpr int64_t MOST = WIDE ? 0x7fffffff : 0x7fff;
-  __device__ static __forceinline__ void add(unsigned* words, unsigned column, bool prompt) {
-    unsigned* w = words + (WIDE ? column : column >> 1);
-    const unsigned at = WIDE ? 0u : (column & 1u) * 16u;
-    if (prompt) atomicOr(w, PROMPT << at);
-    else atomicAdd(w, 1u << at);
+// `yes` where the element's bit is set, else `no`.
+template <class Tag>
+__device__ __forceinline__ u32x4 select_bits(unsigned bits, const u32x4& yes, const u32x4& no) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    unsigned m;
+    if constexpr (Tag::bytes == 4) m = (unsigned)__builtin_amdgcn_sbfe((int)bits, k, 1);
+    else m = ((unsigned)__builtin_amdgcn_sbfe((int)bits, 2 * k, 1) & 0xffffu) | ((unsigned)__builtin_amdgcn_sbfe((int)bits, 2 * k + 1, 1) & 0xffff0000u);
+    v[k] = (yes[k] & m) | (no[k] & ~m);
   }
-  // The counters of N neighbouring columns; whether there is any.
-  template <int N>
-  __device__ static __forceinline__ bool load(const unsigned* words, unsigned column, unsigned (&c)[N]) {
-    constexpr int W = WIDE ? N : N / 2;
-    unsigned w[W], any = 0u;
+  return v;
+}
+// The bits of a 16-byte piece's elements, its first at column `col` (a multiple of as many).
+template <class Tag>
+__device__ __forceinline__ unsigned piece_bits(const unsigned char* bits, unsigned col) {
+  return Tag::bytes == 2 ? bits[col >> 3] : (bits[col >> 3] >> (col & 4)) & 15u;
+}
+
+// Four neighbouring tokens of a text, as they lie there.
+template <class Index>
+struct FourTokens {
+  u32x4 v[sizeof(Index) / 4];
+  __device__ __forceinline__ void load(const char* text, int first) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      w[i] = words[(WIDE ? column : column >> 1) + i];
-      any |= w[i];
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) c[i] = WIDE ? w[i % W] : (w[i / 2] >> (i % 2 * 16)) & 0xffffu;
-    return any != 0u;
+    for (int k = 0; k < (int)sizeof(Index) / 4; ++k) v[k] = load16_unaligned(text + (int64_t)first * (int)sizeof(Index) + k * 16);
+  }
+  // No id of 32 bits: 2^32 - 1.
+  __device__ __forceinline__ unsigned get(int e) const {
+    if constexpr (sizeof(Index) == 4) return v[0][e];
+    else return v[e / 2][e % 2 * 2 + 1] ? ~0u : v[e / 2][e % 2 * 2];
   }
 };
+__device__ const unsigned NOTHING[4] = {0u, 0u, 0u, 0u};       // in the place of a row too short for a piece
+typedef const char __attribute__((address_space(1))) * global_bytes;      // (said to be global, so that a choice of two is no load of any kind of memory)
 
-// N values from column `col` on of a row of V (those that are there), as floats.
-template <class Tag>
-__device__ __forceinline__ u32x4 load_columns(const char* row, int64_t col, int64_t V) {
-  if (col + Chunk<Tag>::N <= V) return load16_stream_any(row + col * Tag::bytes);
-  return load_chunk_elementwise<Tag>(row + col * Tag::bytes, 0, (int)(V - col));
-}
-template <class Tag>
-__device__ __forceinline__ void store_columns(char* row, int64_t col, int64_t V, const u32x4& v) {
-  if (col + Chunk<Tag>::N <= V) store16_stream_any(row + col * Tag::bytes, v);
-  else store_chunk_elementwise<Tag>(row + col * Tag::bytes, 0, (int)(V - col), v);
-}
-template <int N>
-__device__ __forceinline__ unsigned mask_bits(const unsigned char* bits, int64_t col) {
-  return N == 8 ? bits[col >> 3] : (bits[col >> 3] >> (col & 4)) & 15u;
-}
-
-template <class Tag, int NT, int NCH, bool WIDE, bool GRAD>
-__global__ __launch_bounds__(NT) void adjust_kernel(const AdjustParams p) {
-  constexpr int N = Chunk<Tag>::N;
-  extern __shared__ __align__(16) unsigned counts[];
-  const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a row on one XCD
-  const int64_t r = p.first_row + (int64_t)group * 8 + (in & 7u);
-  if (r >= p.n_rows) return;
-  const int64_t c0 = (int64_t)(in >> 3) * p.part_columns, columns = min((int64_t)p.part_columns, p.V - c0);
-  const AdjustRow row(p, r);
-  const char* from = (GRAD ? p.g + r * p.g_stride * Tag::bytes : p.x + r * p.x_stride * Tag::bytes) + c0 * Tag::bytes;
-  char* to = p.out + r * p.out_stride * Tag::bytes + c0 * Tag::bytes;
-  u32x4 v[NCH];
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int64_t col = (int64_t)(i * NT + (int)threadIdx.x) * N;
-    if (col < columns) v[i] = load_columns<Tag>(from, col, columns);
-  }
-  if (row.length > 0) {
-    for (unsigned i = threadIdx.x; i < p.part_columns / (WIDE ? 4u : 8u); i += NT) reinterpret_cast<u32x4*>(counts)[i] = u32x4{0u, 0u, 0u, 0u};
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < row.length; i += NT) {
-      const int64_t c = load_index(row.text, p.itype, i) - c0;
-      if (c >= 0 && c < columns) Counters<WIDE>::add(counts, (unsigned)c, GRAD || i < row.prompt);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int64_t col = (int64_t)(i * NT + (int)threadIdx.x) * N;
-    if (col >= columns) break;
-    float f[N];
-    Chunk<Tag>::unpack(v[i], f);
-    unsigned c[N];
-    if (row.length > 0 && Counters<WIDE>::template load<N>(counts, (unsigned)col, c)) {
-      float x[N];
-      if (GRAD) Chunk<Tag>::unpack(load_columns<Tag>(p.x + (r * p.x_stride + c0) * Tag::bytes, col, columns), x);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (c[e]) {
-          f[e] = (GRAD ? x[e] : f[e]) > 0.f ? f[e] / row.repetition : f[e] * row.repetition;
-          const unsigned count = c[e] & (Counters<WIDE>::PROMPT - 1u);
-          if (!GRAD && count) f[e] -= row.frequency * (float)count + row.presence;
-        }
-    }
-    if (!GRAD && p.bias) {
-      const char* b = p.bias + (r * p.bias_stride + c0) * (p.bias_dtype == F32 ? 4 : 2);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (col + e < columns) f[e] += load_as_float(b, p.bias_dtype, col + e);
-    }
-    if (row.bits) {
-      const unsigned m = mask_bits<N>(row.bits, c0 + col);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (!(m >> e & 1u)) f[e] = GRAD ? 0.f : -__builtin_inff();
-    }
-    store_columns<Tag>(to, col, columns, Chunk<Tag>::pack(f));
-  }
-}
-
-// The gradient of a bias that the rows share: sums over `rows` rows at a time in fp32, the sums' in fp64.
-template <class Tag, int NT>
-__global__ __launch_bounds__(NT) void bias_sums_kernel(const AdjustParams p, float* sums, int64_t rows) {
-  constexpr int N = Chunk<Tag>::N;
-  const int64_t col = ((int64_t)blockIdx.x * NT + threadIdx.x) * N, first = (int64_t)blockIdx.y * rows;
-  if (col >= p.V) return;
-  float total[N] = {};
-  for (int64_t r = first; r < min(first + rows, p.n_rows); ++r) {
+// `run` rows, one after the other, of a part of the columns.  SUMS (the gradient's): what they have in common, the gradient by a shared bias, is added
+// up on the way, one row of `sums` for every run.  Count: what a column's counter is held in.
+template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
+__global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, float* sums) {
+  constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = 2;   // (tokens of a thread at a time: four times NTOK)
+  extern __shared__ __align__(16) unsigned lds[];              // for each column a bit, its new value, and a counter or (GRAD) the logit
+  const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a run on one XCD
+  const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + k * p.run, last = min(first + p.run, p.n_rows);
+  const int64_t c0 = (int64_t)(in >> 3) * p.part_columns;
+  if (first >= last || c0 >= p.V) return;                      // (parts are whole blocks of 128 columns: the last may be none)
+  // a wave's pieces are neighbours, NCH KiB of them: all of a thread's lie within the offset of an instruction
+  const unsigned tid = threadIdx.x, mine = tid / WAVE * (WAVE * NCH) + tid % WAVE;
+  const unsigned columns = (unsigned)min((int64_t)p.part_columns, p.V - c0), pieces = columns / N, tail = columns % N;
+  const unsigned char* said = reinterpret_cast<const unsigned char*>(lds);
+  char* values = reinterpret_cast<char*>(lds + p.part_columns / 32);
+  char* beside = values + p.part_columns * B;
+  unsigned* counts = reinterpret_cast<unsigned*>(beside);
+  const u32x4 masked = GRAD ? u32x4{0u, 0u, 0u, 0u} : Chunk<Tag>::neg_inf();
+  float total[SUMS ? NCH : 1][N] = {}, total_tail = 0.f;
+#pragma unroll 1
+  for (int64_t r = first; r < last; ++r) {
     const AdjustRow row(p, r);
-    const unsigned m = row.bits ? mask_bits<N>(row.bits, col) : 255u;
-    float f[N];
-    Chunk<Tag>::unpack(load_columns<Tag>(p.g + r * p.g_stride * Tag::bytes, col, p.V), f);
+    const char* from = (GRAD ? p.g + (r * p.g_stride + c0) * B : p.x + (r * p.x_stride + c0) * B);
+    const char* x = p.x + (r * p.x_stride + c0) * B;
+    char* to = p.out + (r * p.out_stride + c0) * B;
+    const char* bias = GRAD || !p.bias ? nullptr : p.bias + (r * p.bias_stride + c0) * (p.bias_dtype == F32 ? 4 : 2);
+    const unsigned char* bits = row.bits ? row.bits + (c0 >> 3) : nullptr;      // (a part begins at a whole word)
+    const int length = row.length, prompt = row.prompt;
+    const bool counted = !GRAD && (row.frequency != 0.f || row.presence != 0.f);
+    // (All loads are made, those that nobody needs from the part's or the text's beginning: a load that is branched around is waited for before
+    // the next one.)
+    FourTokens<Index> t[NTOK];
+    u32x4 v[NCH];
+    unsigned m[NCH];
+    const auto fetch = [&](int at) {                           // a thread's tokens from `at` on; the text's last four where there are less
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (m >> e & 1u) total[e] += f[e];
+      for (int i = 0; i < NTOK; ++i) t[i].load(row.text, min(at + (i * NT + (int)tid) * 4, length - 4));
+    };
+    if (length >= 4) fetch(0);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) m[i] = 255u;
+    if (bits && pieces) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) m[i] = piece_bits<Tag>(bits, (mine + i * WAVE < pieces ? mine + i * WAVE : 0u) * N);
+    }
+    const global_bytes whole = pieces ? (global_bytes)from : (global_bytes) reinterpret_cast<const char*>(NOTHING);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) v[i] = __builtin_nontemporal_load((const u32x4_on_2 __attribute__((address_space(1)))*)(whole + (mine + i * WAVE < pieces && m[i] ? mine + i * WAVE : 0u) * 16u));
+    if (length > 0) {
+      for (unsigned i = tid; i < p.part_columns / 128; i += NT) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0u, 0u, 0u, 0u};
+      if (counted)
+        for (unsigned i = tid; i < p.part_columns * (unsigned)sizeof(Count) / 16; i += NT) reinterpret_cast<u32x4*>(counts)[i] = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+      const auto take = [&](unsigned token, int i) {
+        const unsigned c = token - (unsigned)c0;               // (no id: beyond any part)
+        if (c >= columns) return;
+        atomicOr(&lds[c >> 5], 1u << (c & 31u));
+        if (counted && i >= prompt) atomicAdd(&counts[c * sizeof(Count) / 4], 1u << (sizeof(Count) == 4 ? 0u : (c & 1u) * 16u));
+      };
+      if (length < 4 && (int)tid < length) {
+        const Index token = reinterpret_cast<const Index*>(row.text)[tid];
+        if (token >= 0 && token <= 0x7fffffff) take((unsigned)token, (int)tid);
+      }
+#pragma unroll 1
+      for (int at = 0; length >= 4;) {
+#pragma unroll
+        for (int i = 0; i < NTOK; ++i) {
+          const int own = at + (i * NT + (int)tid) * 4, first_token = min(own, length - 4);      // (what is ahead of its own is another thread's)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (first_token + e >= own) take(t[i].get(e), first_token + e);
+        }
+        at += NTOK * NT * 4;
+        if (at >= length) break;
+        fetch(at);
+      }
+      __syncthreads();
+    }
+    if (GRAD)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        if (bits) v[i] = select_bits<Tag>(m[i], v[i], masked);
+        if (SUMS) {
+          float f[N];
+          Chunk<Tag>::unpack(v[i], f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) total[i][e] += f[e];
+        }
+      }
+    const auto penalised = [&](float f, float sign, unsigned col) {
+      f = sign > 0.f ? row.quotient(f) : f * row.repetition;
+      if (counted) {
+        const unsigned n = reinterpret_cast<const Count*>(counts)[col];
+        if (n) f -= row.frequency * (float)n + row.presence;
+      }
+      return f;
+    };
+    constexpr bool OVER = B == 2;                              // (two-byte values with a bias: the sum is rounded, not the penalised value)
+    unsigned c[NCH], left = 0u;
+    if (length > 0 && (!SUMS || p.out)) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        c[i] = mine + i * WAVE < pieces ? piece_bits<Tag>(said, (mine + i * WAVE) * N) & m[i] : 0u;      // (no work on masked ones)
+        left |= c[i] << (i * N);
+      }
+      if (GRAD && pieces) {
+        u32x4 xs[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) xs[i] = load16_unaligned(x + (c[i] ? mine + i * WAVE : 0u) * 16u);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (c[i]) *reinterpret_cast<u32x4*>(beside + (mine + i * WAVE) * 16u) = xs[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (c[i]) *reinterpret_cast<u32x4*>(values + (mine + i * WAVE) * 16u) = v[i];
+#pragma unroll 1
+      for (; left; left &= left - 1u) {
+        const unsigned e = (unsigned)__builtin_ctz(left), col = (mine + e / N * WAVE) * N + e % N;
+        const float f = load_as_float(values, Tag::id, col);
+        float y = penalised(f, GRAD ? load_as_float(beside, Tag::id, col) : f, col);
+        if (!GRAD && OVER && bias) y += load_as_float(bias, p.bias_dtype, col);
+        store_from_float(values, Tag::id, col, y);
+      }
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (c[i] && !(OVER && bias)) v[i] = *reinterpret_cast<const u32x4*>(values + (mine + i * WAVE) * 16u);
+    }
+    if (!GRAD && bias && pieces) {
+      const auto add = [&](int i, const float* a) {
+        float f[N];
+        Chunk<Tag>::unpack(v[i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] += a[e];
+        v[i] = Chunk<Tag>::pack(f);
+        if (OVER && length > 0 && c[i]) v[i] = select_bits<Tag>(c[i], *reinterpret_cast<const u32x4*>(values + (mine + i * WAVE) * 16u), v[i]);
+      };
+      const auto place = [&](int i) { return (mine + i * WAVE < pieces ? mine + i * WAVE : 0u) * 16u; };
+      if (OVER && p.bias_dtype == F32) {
+        u32x4 a[NCH][2];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) a[i][h] = load16_unaligned(bias + place(i) * 2u + h * 16);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          float f[8];
+          Chunk<TagF32>::unpack(a[i][0], f);
+          Chunk<TagF32>::unpack(a[i][1], f + 4);
+          add(i, f);
+        }
+      } else {
+        u32x4 a[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) a[i] = load16_unaligned(bias + place(i));
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          float f[N];
+          Chunk<Tag>::unpack(a[i], f);
+          add(i, f);
+        }
+      }
+    }
+    if (!GRAD && bits) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) v[i] = select_bits<Tag>(m[i], v[i], masked);
+    }
+    if (!SUMS || p.out) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (mine + i * WAVE < pieces) store16_stream_any(to + (mine + i * WAVE) * 16u, v[i]);
+    }
+    if (tid < tail) {                                          // the columns behind the last whole piece
+      const unsigned at = pieces * N + tid;
+      const bool open = !bits || (bits[at >> 3] >> (at & 7u) & 1u);
+      float f = open ? load_as_float(from, Tag::id, at) : 0.f;
+      if (SUMS) total_tail += f;
+      if (!SUMS || p.out) {
+        if (length > 0 && open && (said[at >> 3] >> (at & 7u) & 1u)) f = penalised(f, GRAD ? load_as_float(x, Tag::id, at) : f, at);
+        if (!GRAD && bias) f += load_as_float(bias, p.bias_dtype, at);
+        store_from_float(to, Tag::id, at, GRAD || open ? f : -__builtin_inff());
+      }
+    }
+    if (SUMS && length > 0) __syncthreads();                   // the bits are the next row's
   }
+  if (SUMS) {
+    float* at = sums + (first / p.run) * p.V + c0;
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (col + e < p.V) sums[(int64_t)blockIdx.y * p.V + col + e] = total[e];
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (mine + i * WAVE < pieces) at[(mine + i * WAVE) * N + e] = total[i][e];
+    if (tid < tail) at[pieces * N + tid] = total_tail;
+  }
 }
-template <int NT>
-__global__ __launch_bounds__(NT) void bias_join_kernel(const float* sums, int64_t groups, int64_t V, void* out, int dtype) {
-  const int64_t col = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (col >= V) return;
+
+// The runs' sums, added up in fp64: 32 columns a workgroup, eight threads to a column, each every eighth run.
+__global__ __launch_bounds__(256) void bias_join_kernel(const float* sums, int64_t runs, int64_t V, void* out, int dtype) {
+  __shared__ double part[8][32];
+  const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const int64_t col = (int64_t)blockIdx.x * 32 + lane;
   double total = 0.0;
-  for (int64_t k = 0; k < groups; ++k) total += (double)sums[k * V + col];
-  store_from_float(out, dtype, col, (float)total);
+  if (col < V)
+    for (int64_t k = slice; k < runs; k += 8) total += (double)sums[k * V + col];
+  part[slice][lane] = total;
+  __syncthreads();
+  if (slice == 0 && col < V) {
+#pragma unroll
+    for (int s = 1; s < 8; ++s) total += part[s][lane];
+    store_from_float(out, dtype, col, (float)total);
+  }
 }
 
 static int adjust_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH; }
 
-template <class Tag, int NT, int NCH, bool WIDE, bool GRAD>
-static void launch_adjust(AdjustParams p, hipStream_t st) {
-  const int64_t most = (int64_t)NT * NCH * Chunk<Tag>::N;
-  p.parts = (unsigned)((p.V + most - 1) / most);
-  p.part_columns = (unsigned)((p.V + p.parts - 1) / p.parts + 31) / 32 * 32;
-  const size_t lds = p.length > 0 ? p.part_columns * (WIDE ? 4 : 2) : 0;
-  const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8;      // rows of a launch
-  for (p.first_row = 0; p.first_row < p.n_rows; p.first_row += slice) {
-    AdjustParams q = p;
-    q.n_rows = std::min(p.n_rows, p.first_row + slice);
-    hipLaunchKernelGGL((adjust_kernel<Tag, NT, NCH, WIDE, GRAD>), dim3((unsigned)((q.n_rows - q.first_row + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, q);
-  }
-}
-template <class Tag, bool GRAD>
-static void adjust_rows(const AdjustParams& p, hipStream_t st) {
-  if (p.length > Counters<false>::MOST) launch_adjust<Tag, 256, 4, true, GRAD>(p, st);
-  else launch_adjust<Tag, 256, 4, false, GRAD>(p, st);
+constexpr int ADJUST_NT = 256, ADJUST_NCH = 4;
+
+// Rows whose sum goes to the workspace in one piece: enough workgroups, few pieces, no more than 65535 of them.
+static int64_t sums_run(int64_t n_rows, int64_t V) {
+  return std::max(std::max<int64_t>(4, std::min<int64_t>(64, n_rows * ((V + 8191) / 8192) / 2048)), (n_rows + 65534) / 65535);
 }
 
-// Rows that one thread adds up: 64, or as many as leave no more runs than a launch has blocks in y.
-static int64_t bias_rows(int64_t n_rows) { return std::max<int64_t>(64, (n_rows + 65534) / 65535); }
+template <class Tag, class Index, int NT, class Count, bool GRAD, bool SUMS>
+static void launch_adjust(AdjustParams p, float* sums, hipStream_t st) {
+  constexpr int64_t most = (int64_t)NT * ADJUST_NCH * Chunk<Tag>::N;
+  p.parts = (unsigned)((p.V + most - 1) / most);
+  p.part_columns = (unsigned)std::min<int64_t>(most, ((p.V + p.parts - 1) / p.parts + 127) / 128 * 128);      // (whole words of the masks, whole pieces of the bits)
+  p.run = SUMS ? sums_run(p.n_rows, p.V) : 1;
+  const size_t lds = p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (GRAD ? Tag::bytes : sizeof(Count))) : 0;
+  const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8 * p.run, all = p.n_rows;      // rows of a launch
+  for (p.first_row = 0; p.first_row < all; p.first_row += slice) {
+    p.n_rows = std::min(all, p.first_row + slice);
+    const int64_t runs = (p.n_rows - p.first_row + p.run - 1) / p.run;
+    hipLaunchKernelGGL((adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), dim3((unsigned)((runs + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, p, sums);
+  }
+}
+template <class Tag, class Index, bool GRAD, bool SUMS>
+static void adjust_texts(const AdjustParams& p, float* sums, hipStream_t st) {
+  if constexpr (!GRAD)
+    if (p.length > 65535) return launch_adjust<Tag, Index, ADJUST_NT, unsigned, GRAD, SUMS>(p, sums, st);
+  launch_adjust<Tag, Index, ADJUST_NT, unsigned short, GRAD, SUMS>(p, sums, st);
+}
+template <class Tag, bool GRAD, bool SUMS>
+static void adjust_rows(const AdjustParams& p, float* sums, hipStream_t st) {
+  if (p.itype == I64) adjust_texts<Tag, int64_t, GRAD, SUMS>(p, sums, st);
+  else adjust_texts<Tag, int32_t, GRAD, SUMS>(p, sums, st);
+}
+template <bool GRAD, bool SUMS>
+static void adjust_rows(const AdjustParams& p, int dtype, float* sums, hipStream_t st) {
+  if (dtype == DL_F32) adjust_rows<TagF32, GRAD, SUMS>(p, sums, st);
+  else if (dtype == DL_BF16) adjust_rows<TagBF16, GRAD, SUMS>(p, sums, st);
+  else adjust_rows<TagF16, GRAD, SUMS>(p, sums, st);
+}
 
 // What both entry points ask of their common arguments.
 static int adjust_check(const AdjustParams& p, int dtype) {
@@ -233,24 +385,22 @@ extern "C" int dl_adjust_rows(const void* logits, int dtype, int64_t row_stride,
   if (!tokens) n_texts = length = 0;
   if (!allowed) n_masks = 0;
   AdjustParams p{reinterpret_cast<const char*>(logits), row_stride, nullptr, 0, reinterpret_cast<char*>(out), out_stride, n_rows, V,
-                 reinterpret_cast<const char*>(tokens), itype, token_stride, n_texts, n_texts ? length : 0, token_rows, lengths, prompt, prompt_all,
+                 reinterpret_cast<const char*>(tokens), itype, token_stride, n_texts, n_texts ? length : 0, token_rows, lengths, prompt, (int)std::max<int64_t>(0, std::min<int64_t>(prompt_all, 0x7fffffff)),
                  repetition, frequency, presence, repetition_all, frequency_all, presence_all,
                  reinterpret_cast<const char*>(bias), bias_dtype, bias_stride,
-                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0};
+                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 1};
   if (const int bad = adjust_check(p, dtype)) return bad;
   if (n_rows == 0 || V == 0) return DL_OK;
   if (!logits || !out) return DL_ERR_NULL;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == DL_F32) adjust_rows<TagF32, false>(p, st);
-  else if (dtype == DL_BF16) adjust_rows<TagBF16, false>(p, st);
-  else adjust_rows<TagF16, false>(p, st);
+  adjust_rows<false, false>(p, dtype, nullptr, st);
   return adjust_status();
 }
 
 extern "C" int64_t dl_adjust_grad_workspace_bytes(int64_t n_rows, int64_t V) {
   if (n_rows <= 0 || V <= 0) return 0;
-  const int64_t rows = dl::bias_rows(n_rows);
-  return (n_rows + rows - 1) / rows * V * 4;
+  const int64_t run = dl::sums_run(n_rows, V);
+  return (n_rows + run - 1) / run * V * 4;
 }
 
 extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, const void* logits, int64_t row_stride, int64_t n_rows, int64_t V,
@@ -267,7 +417,7 @@ extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, 
   AdjustParams p{reinterpret_cast<const char*>(logits), row_stride, reinterpret_cast<const char*>(grad), grad_stride, reinterpret_cast<char*>(out), out_stride, n_rows, V,
                  reinterpret_cast<const char*>(tokens), itype, token_stride, n_texts, n_texts ? length : 0, token_rows, lengths, nullptr, 0,
                  repetition, nullptr, nullptr, repetition_all, 0.f, 0.f, nullptr, F32, 0,
-                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0};
+                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 1};
   if (grad_stride < V) return DL_ERR_SHAPE;
   if (const int bad = adjust_check(p, dtype)) return bad;
   if (V == 0 || (n_rows == 0 && !bias_grad)) return DL_OK;
@@ -275,23 +425,19 @@ extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, 
   const uintptr_t eb = dtype == DL_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(grad) % eb || reinterpret_cast<uintptr_t>(bias_grad) % (bias_dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return DL_ERR_ALIGN;
-  const int64_t run = bias_rows(n_rows), groups = (n_rows + run - 1) / run;
-  if (bias_grad && groups > 0 && (!workspace || workspace_bytes < dl_adjust_grad_workspace_bytes(n_rows, V))) return DL_ERR_WORKSPACE;
+  if (bias_grad && n_rows > 0 && (!workspace || workspace_bytes < dl_adjust_grad_workspace_bytes(n_rows, V))) return DL_ERR_WORKSPACE;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (bias_grad) {
-    float* sums = reinterpret_cast<float*>(workspace);
-    const dim3 grid((unsigned)((V + 256 * 16 / eb - 1) / (256 * 16 / eb)), (unsigned)groups);
-    if (groups > 0) {
-      if (dtype == DL_F32) hipLaunchKernelGGL((bias_sums_kernel<TagF32, 256>), grid, dim3(256), 0, st, p, sums, run);
-      else if (dtype == DL_BF16) hipLaunchKernelGGL((bias_sums_kernel<TagBF16, 256>), grid, dim3(256), 0, st, p, sums, run);
-      else hipLaunchKernelGGL((bias_sums_kernel<TagF16, 256>), grid, dim3(256), 0, st, p, sums, run);
-    }
-    hipLaunchKernelGGL((bias_join_kernel<256>), dim3((unsigned)((V + 255) / 256)), dim3(256), 0, st, sums, groups, V, bias_grad, bias_dtype);
+  if (!bias_grad) {
+    if (out) adjust_rows<true, false>(p, dtype, nullptr, st);
+    return adjust_status();
   }
-  if (out && n_rows > 0) {
-    if (dtype == DL_F32) adjust_rows<TagF32, true>(p, st);
-    else if (dtype == DL_BF16) adjust_rows<TagBF16, true>(p, st);
-    else adjust_rows<TagF16, true>(p, st);
+  float* sums = reinterpret_cast<float*>(workspace);
+  int64_t runs = 0;
+  if (n_rows > 0) {
+    if (!out) p.length = 0;                                    // the bias does not feel the texts
+    adjust_rows<true, true>(p, dtype, sums, st);
+    runs = (n_rows + sums_run(n_rows, V) - 1) / sums_run(n_rows, V);
   }
+  hipLaunchKernelGGL(bias_join_kernel, dim3((unsigned)((V + 31) / 32)), dim3(256), 0, st, sums, runs, V, bias_grad, bias_dtype);
   return adjust_status();
 }
