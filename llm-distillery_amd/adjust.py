@@ -2,7 +2,7 @@
 that.  Thin wrappers over the C ABI; all arithmetic runs in the HIP kernels."""
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import Optional, Tuple, Union
 
 import torch
 from torch.utils._python_dispatch import is_in_torch_dispatch_mode
@@ -16,10 +16,11 @@ Number = Union[float, torch.Tensor]
 
 def _logit_rows(t: torch.Tensor, name: str, dev: Optional[torch.device] = None) -> torch.Tensor:
     """t [..., V] as [rows, V] without a copy."""
-    _dev(t, name, dev)
+    if dev is None or t.device != dev:
+        _dev(t, name, dev)
     if t.dtype not in _DT:
         raise RuntimeError(f"{name}: unsupported dtype")
-    x = _rows_2d(t if t.dim() > 1 else t.unsqueeze(0))
+    x = t if t.dim() == 2 and t.stride(1) == 1 else _rows_2d(t if t.dim() > 1 else t.unsqueeze(0))
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         raise RuntimeError(f"{name}: rows overlap; make them contiguous first")
     return x
@@ -30,17 +31,12 @@ def _per_row(v: Number, rows: int, name: str, dev: torch.device) -> Tuple[Option
     return (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
 
 
-class _Texts(NamedTuple):
-    """The texts as the C ABI takes them: address, index type, stride, number, length, address of the map; and what has to stay alive."""
-    args: tuple
-    keep: tuple
-
-
-def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], rows: int, dev: torch.device) -> _Texts:
+def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], rows: int, dev: torch.device) -> Tuple[tuple, tuple]:
+    """The texts as the C ABI takes them -- address, index type, stride, number, length, address of the map -- and what has to stay alive."""
     if tokens is None:
         if token_rows is not None:
             raise RuntimeError("token_rows without tokens")
-        return _Texts((0, 0, 0, 0, 0, 0), ())
+        return (0, 0, 0, 0, 0, 0), ()
     _dev(tokens, "tokens", dev)
     if tokens.dtype not in _IT:
         raise RuntimeError("tokens must be int32 or int64")
@@ -54,15 +50,15 @@ def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], r
         token_rows = _row_vector(token_rows, rows, torch.int32, "token_rows", dev)
     elif n not in (1, rows):
         raise RuntimeError(f"{n} texts for {rows} rows and no token_rows")
-    return _Texts((t.data_ptr(), _IT[t.dtype], t.stride(0) if n > 1 else length, n, length, token_rows.data_ptr() if token_rows is not None else 0),
-                  (t, token_rows))
+    return (t.data_ptr(), _IT[t.dtype], t.stride(0) if n > 1 else length, n, length, token_rows.data_ptr() if token_rows is not None else 0), (t, token_rows)
 
 
-def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor], rows: int, V: int, dev: torch.device) -> _Texts:
+def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor], rows: int, V: int, dev: torch.device) -> Tuple[tuple, tuple]:
+    """The masks the same way: address, stride, number, address of the map."""
     if allowed is None:
         if allowed_rows is not None:
             raise RuntimeError("allowed_rows without allowed")
-        return _Texts((0, 0, 0, 0), ())
+        return (0, 0, 0, 0), ()
     _dev(allowed, "allowed", dev)
     words = -(-V // 32)
     m = allowed if allowed.dim() != 1 else allowed.unsqueeze(0)
@@ -77,7 +73,7 @@ def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor]
         allowed_rows = _row_vector(allowed_rows, rows, torch.int32, "allowed_rows", dev)
     elif n not in (1, rows):
         raise RuntimeError(f"{n} masks for {rows} rows and no allowed_rows")
-    return _Texts((m.data_ptr(), m.stride(0) if n > 1 else m.shape[1], n, allowed_rows.data_ptr() if allowed_rows is not None else 0), (m, allowed_rows))
+    return (m.data_ptr(), m.stride(0) if n > 1 else m.shape[1], n, allowed_rows.data_ptr() if allowed_rows is not None else 0), (m, allowed_rows)
 
 
 def _row_lengths(lengths: Optional[torch.Tensor], rows: int, dev: torch.device) -> Optional[torch.Tensor]:
@@ -125,7 +121,7 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     x = _logit_rows(logits, "logits")
     R, V = x.shape
     dev = x.device
-    text, mask = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
+    (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
     lengths = _row_lengths(lengths, R, dev)
     prompt_rows, prompt_all = (_row_vector(prompt, R, torch.int32, "prompt", dev), 0) if isinstance(prompt, torch.Tensor) else (None, int(prompt))
     (rep, rep_all), (freq, freq_all), (pres, pres_all) = (_per_row(v, R, n, dev) for v, n in
@@ -145,11 +141,11 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
         b_ptr, b_dtype, b_stride = b.data_ptr(), _DT[b.dtype], b.stride(0) if b.dim() == 2 and b.shape[0] > 1 else 0
     res = _written(out, x, "out", "the logits")
     with _on(dev):
-        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, *text.args, _address(lengths), _address(prompt_rows),
+        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, *text, _address(lengths), _address(prompt_rows),
                                         prompt_all, _address(rep), _address(freq), _address(pres), rep_all, freq_all, pres_all, b_ptr, b_dtype,
-                                        b_stride, *mask.args, res.data_ptr(), _row_pitch(res), _stream_ptr(dev))
+                                        b_stride, *mask, res.data_ptr(), _row_pitch(res), _stream_ptr(dev))
     _lib.check(st, "dl_adjust_rows")
-    return out if out is not None else res.view(logits.shape)
+    return out if out is not None else res if logits.dim() == 2 else res.view(logits.shape)
 
 
 def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None, *,
@@ -167,7 +163,7 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     g = _logit_rows(grad, "grad")
     R, V = g.shape
     dev = g.device
-    text, mask = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
+    (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
     lengths = _row_lengths(lengths, R, dev)
     rep, rep_all = _per_row(repetition, R, "repetition", dev)
     if rep is None and not rep_all > 0.0:
@@ -189,11 +185,11 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     ws_bytes = lib.dl_adjust_grad_workspace_bytes(R, V) if want_bias else 0
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with _on(dev):
-        st = lib.dl_adjust_grad(g.data_ptr(), _DT[g.dtype], _row_pitch(g), _address(x), 0 if x is None else _row_pitch(x), R, V, *text.args,
-                                _address(lengths), _address(rep), rep_all, *mask.args, _address(res), 0 if res is None else _row_pitch(res),
+        st = lib.dl_adjust_grad(g.data_ptr(), _DT[g.dtype], _row_pitch(g), _address(x), 0 if x is None else _row_pitch(x), R, V, *text,
+                                _address(lengths), _address(rep), rep_all, *mask, _address(res), 0 if res is None else _row_pitch(res),
                                 _address(by_bias), _DT[bias_dtype], _address(ws), ws_bytes, _stream_ptr(dev))
     _lib.check(st, "dl_adjust_grad")
-    return (out if out is not None else res.view(grad.shape) if want_logits else None), by_bias
+    return (out if out is not None else res if not want_logits or grad.dim() == 2 else res.view(grad.shape)), by_bias
 
 
 # ---- autograd.  Registered operators with shape-only forms, so that torch.compile and FakeTensor tracing see through both directions.  The two

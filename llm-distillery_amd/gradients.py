@@ -2,7 +2,7 @@
 the HIP kernels."""
 from __future__ import annotations
 
-import ctypes
+from array import array
 from typing import Iterable, Optional
 
 import torch
@@ -28,25 +28,26 @@ class _Tensors:
         self.all = grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
         if not grads:
             raise RuntimeError("no gradients")
-        self.dev = grads[0].device
+        index = grads[0].get_device()
         for g in grads:
-            if g.device != self.dev or not g.is_cuda or g.dtype not in _DT or g.layout is not torch.strided:
-                _dev(g, "a gradient")
-                if g.device != self.dev:
-                    raise RuntimeError(f"gradients live on {self.dev} and {g.device}: all tensors of a call must share one device")
-                raise RuntimeError("gradients must be dense bf16/fp16/fp32 tensors")
+            if g.get_device() != index or index < 0 or g.layout is not torch.strided:
+                _dev(g, "a gradient", grads[0].device if index >= 0 else None)
+                raise RuntimeError("gradients must be dense tensors")
             if not g.is_contiguous() and g.numel() and not _dense(g):
                 raise RuntimeError("a gradient must fill its memory (a slice or an expanded tensor does not)")
-        n = self.n = len(grads)
-        self.at = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-        self.sizes = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
-        self.dtypes = (ctypes.c_int32 * n)(*[_DT[g.dtype] for g in grads])
+        self.dev = grads[0].device
+        try:
+            self.dtypes = array("i", [_DT[g.dtype] for g in grads])
+        except KeyError:
+            raise RuntimeError("gradients must be bf16/fp16/fp32") from None
+        self.at = array("q", [g.data_ptr() for g in grads])
+        self.sizes = array("q", [g.numel() for g in grads])
 
     def args(self):
-        return ctypes.addressof(self.at), ctypes.addressof(self.sizes), ctypes.addressof(self.dtypes), self.n
+        return self.at.buffer_info()[0], self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], len(self.at)
 
     def workspace(self, lib) -> torch.Tensor:
-        return torch.empty(lib.dl_grad_norm_workspace_bytes(ctypes.addressof(self.sizes), self.n), dtype=torch.uint8, device=self.dev)
+        return torch.empty(lib.dl_grad_norm_workspace_bytes(self.sizes.buffer_info()[0], len(self.at)), dtype=torch.uint8, device=self.dev)
 
 
 def _positive(scale: float) -> float:
