@@ -28,7 +28,7 @@ def _logit_rows(t: torch.Tensor, name: str, dev: Optional[torch.device] = None) 
 
 def _per_row(v: Number, rows: int, name: str, dev: torch.device) -> Tuple[Optional[torch.Tensor], float]:
     """A setting as (one fp32 entry per row, 0) or (nothing, the number for all)."""
-    return (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
+    return (None, v) if type(v) is float else (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
 
 
 def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], rows: int, dev: torch.device) -> Tuple[tuple, tuple]:
@@ -82,9 +82,9 @@ def _row_lengths(lengths: Optional[torch.Tensor], rows: int, dev: torch.device) 
 
 def _written(out: Optional[torch.Tensor], x: torch.Tensor, name: str, over: str, others: tuple = ()) -> torch.Tensor:
     """The matrix that the result goes to: new, or `out` checked -- `x` itself, or memory that neither `x` nor `others` have."""
-    R, V = x.shape
     if out is None:
-        return torch.empty((R, V), dtype=x.dtype, device=x.device)
+        return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    R, V = x.shape
     o = _logit_rows(out, name, x.device)
     if tuple(o.shape) != (R, V) or o.dtype != x.dtype:
         raise RuntimeError(f"{name} must be a [{R}, {V}] {x.dtype} matrix")
@@ -124,8 +124,9 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
     lengths = _row_lengths(lengths, R, dev)
     prompt_rows, prompt_all = (_row_vector(prompt, R, torch.int32, "prompt", dev), 0) if isinstance(prompt, torch.Tensor) else (None, int(prompt))
-    (rep, rep_all), (freq, freq_all), (pres, pres_all) = (_per_row(v, R, n, dev) for v, n in
-                                                         ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")))
+    rep, rep_all = _per_row(repetition, R, "repetition", dev)
+    freq, freq_all = _per_row(frequency, R, "frequency", dev)
+    pres, pres_all = _per_row(presence, R, "presence", dev)
     if rep is None and not rep_all > 0.0:
         raise ValueError("repetition must be positive")
     b_ptr = b_dtype = b_stride = 0

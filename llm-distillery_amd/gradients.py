@@ -28,14 +28,13 @@ class _Tensors:
         self.all = grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
         if not grads:
             raise RuntimeError("no gradients")
-        index = grads[0].get_device()
+        self.dev = dev = grads[0].device
         for g in grads:
-            if g.get_device() != index or index < 0 or g.layout is not torch.strided:
-                _dev(g, "a gradient", grads[0].device if index >= 0 else None)
+            if g.device != dev or not g.is_cuda or g.layout is not torch.strided:
+                _dev(g, "a gradient", dev if dev.type == "cuda" else None)
                 raise RuntimeError("gradients must be dense tensors")
             if not g.is_contiguous() and g.numel() and not _dense(g):
                 raise RuntimeError("a gradient must fill its memory (a slice or an expanded tensor does not)")
-        self.dev = grads[0].device
         try:
             self.dtypes = array("i", [_DT[g.dtype] for g in grads])
         except KeyError:
