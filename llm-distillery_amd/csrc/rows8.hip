@@ -20,39 +20,65 @@ constexpr int64_t K_MOST = 130944;                             // 1023 blocks: 1
 constexpr float ISCALE = 1.f / 127.f, ISCALE_MIN = 0x1p-100f;
 
 // ---- quantise ---------------------------------------------------------------------------------------
-// A workgroup a row, twice: for its largest magnitude, and for the codes.
+// A workgroup a row, which it holds in registers between the maximum and the codes (up to 16384 columns; wider rows are read twice).
+// x / scale, rounded once, is a product with the rounded reciprocal and what that is off by taken off: the remainder is exact but where the code is 0
+// whatever it is (scales are 2^-100 or more).
 struct RowsQuant {
   const char* x; int64_t row_stride, rows, cols, width;        // width: whole blocks
   signed char* codes; int64_t code_stride;
   float* scales;
 };
 __device__ __forceinline__ bool not_finite(float f) { return (__float_as_uint(f) & 0x7f800000u) == 0x7f800000u; }
-template <class Tag, int NT>
+__device__ __forceinline__ u32x2 codes_of_eight(const float* f, float scale, float inverse) {
+  u32x2 c = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = f[e] * inverse, quotient = fmaf(fmaf(-q, scale, f[e]), inverse, q);
+    c[e / 4] |= (unsigned)((int)fminf(fmaxf(rintf(quotient), -127.f), 127.f) & 255) << (e % 4 * 8);
+  }
+  return c;
+}
+__device__ __forceinline__ float largest_finite_of_eight(const float* f, float m) {      // infinite where one is not finite
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = not_finite(f[e]) ? __builtin_inff() : fmaxf(m, fabsf(f[e]));
+  return m;
+}
+template <class Tag, int NT, int NCH>
 __global__ __launch_bounds__(NT) void quantize_whole_rows_kernel(const RowsQuant p) {
   __shared__ float red[NT / WAVE];
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const char* x = p.x + row * p.row_stride * Tag::bytes;
-    float m = 0.f;
-    for (int64_t col = threadIdx.x * 8; col < p.cols; col += NT * 8) {
-      float f[8];
-      load_eight<Tag>(x, col, p.cols, f);
+  const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= p.rows) return;
+  const char* x = p.x + row * p.row_stride * Tag::bytes;
+  signed char* to = p.codes + row * p.code_stride;
+  const int col = (int)threadIdx.x * 8;
+  float f[NCH > 0 ? NCH : 1][8], m = 0.f;
+  if constexpr (NCH > 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = not_finite(f[e]) ? __builtin_inff() : fmaxf(m, fabsf(f[e]));
+    for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+      if (col + i * NT * 8 < p.cols) load_eight<Tag>(x, col + i * NT * 8, p.cols, f[i]);
     }
-    m = block_max<NT>(m, red);
-    const bool odd = not_finite(m);
-    const float scale = fmaxf(m * ISCALE, ISCALE_MIN);
-    if (threadIdx.x == 0) p.scales[row] = odd ? __builtin_nanf("") : scale;
-    for (int64_t col = threadIdx.x * 8; col < p.width; col += NT * 8) {
-      float f[8];
-      load_eight<Tag>(x, col, p.cols, f);
-      u32x2 c = {0u, 0u};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int q = odd ? 0 : (int)fminf(fmaxf(rintf(f[e] / scale), -127.f), 127.f);
-        c[e / 4] |= (unsigned)(q & 255) << (e % 4 * 8);
-      }
-      *reinterpret_cast<u32x2*>(p.codes + row * p.code_stride + col) = c;
+    for (int i = 0; i < NCH; ++i) m = largest_finite_of_eight(f[i], m);
+  } else {
+    for (int64_t c = col; c < p.cols; c += NT * 8) {
+      load_eight<Tag>(x, c, p.cols, f[0]);
+      m = largest_finite_of_eight(f[0], m);
+    }
+  }
+  m = block_max<NT>(m, red);
+  const bool odd = not_finite(m);
+  const float scale = odd ? 1.f : fmaxf(m * ISCALE, ISCALE_MIN), inverse = 1.f / scale;
+  if (threadIdx.x == 0) p.scales[row] = odd ? __builtin_nanf("") : scale;
+  if constexpr (NCH > 0) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+      if (col + i * NT * 8 < p.width) *reinterpret_cast<u32x2*>(to + col + i * NT * 8) = odd ? u32x2{0u, 0u} : codes_of_eight(f[i], scale, inverse);
+  } else {
+    for (int64_t c = col; c < p.width; c += NT * 8) {
+      load_eight<Tag>(x, c, p.cols, f[0]);
+      *reinterpret_cast<u32x2*>(to + c) = odd ? u32x2{0u, 0u} : codes_of_eight(f[0], scale, inverse);
     }
   }
 }
@@ -65,6 +91,15 @@ struct RowsParams {
   char* out; int64_t out_stride;
 };
 
+// 16 bytes a lane from `base` + `offset` into LDS, from `to` on in lane order (base and to: the wave's).  Said to the compiler as something that touches
+// memory and no more: for a load into LDS that it knows it waits before the next access to LDS, and for all that are under way.  (Small tiles then
+// drained their own fetches at every step, 128 x 8000 x 4096 17.8 us and with the ring below 23.6, now 12.9; a tile's values waited for the next
+// tile's operands and for each other's stores, 8192 x 32000 x 1024 297 us, now 283.)  The waits are the kernels' own, by the count of fetches; those of
+// the compiler, which does not count them, can only ask for more.  (m0, which holds the place in LDS, is nobody else's in these kernels.)
+__device__ __forceinline__ void fetch_to_lds(const unsigned char* base, unsigned offset, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+
 // Tiles of BM x BN, a wave WM x WN of it, a block of 128 columns (two matrix instructions deep) per step.  A step's operands are fetched into LDS by
 // loads that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted
 // by piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in lane
@@ -75,6 +110,63 @@ struct RowsParams {
 struct Piece { i32x4 lo, hi; };                                // a lane's 32 bytes of a row: 16 columns of either half of the block
 __device__ __forceinline__ Piece row_piece(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
   return Piece{*reinterpret_cast<const i32x4*>(lds + lo + rows * KB), *reinterpret_cast<const i32x4*>(lds + hi + rows * KB)};
+}
+
+// The block of columns that a tile begins with (sums are exact: any order gives the same bits).  Tiles that share no operand begin at different ones: in
+// step, their rows' places, a row's stride apart, would all lie in the same few channels of memory (1 x 128256 x 4096: 107 us, so 92).  Tiles that
+// share operands stay in step, and find them in the L2.
+__device__ __forceinline__ int first_block(unsigned tile, unsigned tiles_m, int blocks) { return tiles_m == 1 ? (int)(tile % (unsigned)blocks) : 0; }
+
+// A wave's values, from row m0 and column n0 of the result on.  Two-byte results go through 2 KiB of LDS of the wave's own, `stage`, 16 rows at a
+// time, so that a store writes whole 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by
+// unit ^ (row % 8).
+template <class Tag, int TM, int TN>
+__device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int lane, unsigned char* stage) {
+  asm volatile("" : "+v"(lane));                               // (keeps the stores' addresses out of the steps' registers)
+  const int row = lane % 16, quad = lane / 16;
+  f32x4 sb[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sb[j][e] = p.sb[min(n0 + j * 16 + quad * 4 + e, p.N - 1)];
+  float sas[TM];                                               // (all ahead of the first store, which a load behind it would wait for)
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sas[i] = p.sa[min(m0 + i * 16 + row, p.M - 1)];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const float sa = sas[i];
+    f32x4 v[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = (float)acc[i][j][e] * (sa * sb[j][e]);
+    if constexpr (Tag::bytes == 2 && TN == 4) {
+      const int r8 = lane / 8, unit = lane % 8;
+      const int64_t n = n0 + unit * 8;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const float f[8] = {v[j][0], v[j][1], v[j][2], v[j][3], 0.f, 0.f, 0.f, 0.f};
+        const u32x4 c = Chunk<Tag>::pack(f);
+        *reinterpret_cast<u32x2*>(stage + row * 128 + ((j * 2 + quad / 2) ^ (row & 7)) * 16 + (quad & 1) * 8) = u32x2{c[0], c[1]};
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int64_t m = m0 + i * 16 + k * 8 + r8;
+        const u32x4 c = *reinterpret_cast<const u32x4*>(stage + (k * 8 + r8) * 128 + (unit ^ r8) * 16);
+        char* to = p.out + (m * p.out_stride + n) * 2;
+        if (m < p.M && n + 8 <= p.N) store16_stream_any(to, c);
+        else if (m < p.M && n < p.N) store_chunk_elementwise<Tag>(to, 0, (int)(p.N - n), c);
+      }
+    } else {
+      const int64_t m = m0 + i * 16 + row;
+      char* to = p.out + m * p.out_stride * Tag::bytes;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + j * 16 + quad * 4;
+        if (m < p.M && n < p.N) store_four<Tag>(to, n, p.N, v[j]);
+      }
+    }
+  }
 }
 
 template <class Tag, int BM, int BN, int WM, int WN>
@@ -91,7 +183,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
 
   // the fetching side: its tile, its block, this thread's places in them
   unsigned f_tile = walk.first;
-  int f_kb = 0;
+  int f_kb, f_left;                                            // the block to fetch, and how many are
   const unsigned char *f_a, *f_b;
   unsigned f_ao[NA], f_bo[NB];
   const auto f_begin = [&]() {
@@ -99,8 +191,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
     walk.origin(f_tile, m, n);
     m *= BM;
     n *= BN;
-    f_a = p.a + m * p.a_stride;
-    f_b = p.b + n * p.b_stride;
+    f_left = p.blocks;
+    f_kb = first_block(f_tile, tiles_m, p.blocks);
+    f_a = p.a + m * p.a_stride + (int64_t)f_kb * KB;
+    f_b = p.b + n * p.b_stride + (int64_t)f_kb * KB;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
@@ -116,26 +210,29 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
   // beginning on, and of a the rows that the waves go through first), `late` at its end.
   constexpr bool HALVES = WM / 2 == WAVES * 8;                 // every other fetch of a: those rows
   constexpr int EARLY = NB + (HALVES ? NA / 2 : 0);
-  const auto fetch_a = [&](unsigned char* to, int i) {
-    __builtin_amdgcn_global_load_lds((global_words)(f_a + f_ao[i]), (lds_words)(to + (i * WAVES + w) * 1024), 16, 0, 0);
-  };
+  const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((lds_words)lds);
+  const auto fetch_a = [&](unsigned to, int i) { fetch_to_lds(f_a, f_ao[i], to + (i * WAVES + w) * 1024); };
   const auto fetch_early = [&](unsigned step) {
-    unsigned char* to = lds + (step & 1u) * STEP;
+    const unsigned to = lds0 + (step & 1u) * STEP;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      __builtin_amdgcn_global_load_lds((global_words)(f_b + f_bo[i]), (lds_words)(to + BM * KB + (i * WAVES + w) * 1024), 16, 0, 0);
+      fetch_to_lds(f_b, f_bo[i], to + BM * KB + (i * WAVES + w) * 1024);
     if (HALVES)
 #pragma unroll
       for (int i = 0; i < NA; i += 2) fetch_a(to, i);
   };
   const auto fetch_late = [&](unsigned step) {
-    unsigned char* to = lds + (step & 1u) * STEP;
+    const unsigned to = lds0 + (step & 1u) * STEP;
 #pragma unroll
     for (int i = HALVES ? 1 : 0; i < NA; i += HALVES ? 2 : 1) fetch_a(to, i);
     f_a += KB;
     f_b += KB;
     if (++f_kb == p.blocks) {
       f_kb = 0;
+      f_a -= (int64_t)p.blocks * KB;
+      f_b -= (int64_t)p.blocks * KB;
+    }
+    if (--f_left == 0) {
       f_tile += walk.step;
       if (f_tile < walk.end) f_begin();
     }
@@ -220,52 +317,123 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
       }
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
-    // The tile's values.  Two-byte results go through 2 KiB of LDS of the wave's own, 16 rows at a time, so that a store writes whole
-    // 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by unit ^ (row % 8).
-    int here = lane;
-    asm volatile("" : "+v"(here));                             // (keeps the stores' addresses out of the steps' registers)
-    const int row = here % 16, quad = here / 16;
-    f32x4 sb[TN];
+    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + 2 * STEP + w * 2048);
+  }
+}
+
+// The same for small tiles, whose steps are too short to wait for memory with two buffers: a ring of S, S - 1 steps' operands under way, one barrier a step.
+template <class Tag, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_ring_kernel(const RowsParams p, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16, NA = BM / 8 / WAVES, NB = BN / 8 / WAVES;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole fetches");
+  extern __shared__ __align__(1024) unsigned char lds[];      // S of (a: BM rows, b: BN rows of 128 bytes)
+  constexpr int STEP = (BM + BN) * KB;
+  const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), i16 = lane % 16;
+  const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
+  const TileWalk walk(tiles_m, tiles_n);
+  if (walk.first >= walk.end) return;
+  const unsigned steps = ((walk.end - walk.first + walk.step - 1) / walk.step) * (unsigned)p.blocks;
+  unsigned f_tile = walk.first, f_step = 0;
+  int f_kb, f_left, f_place = 0;
+  const unsigned char *f_a, *f_b;
+  unsigned f_ao[NA], f_bo[NB];
+  const auto f_begin = [&]() {
+    int64_t m, n;
+    walk.origin(f_tile, m, n);
+    m *= BM;
+    n *= BN;
+    f_left = p.blocks;
+    f_kb = first_block(f_tile, tiles_m, p.blocks);
+    f_a = p.a + m * p.a_stride + (int64_t)f_kb * KB;
+    f_b = p.b + n * p.b_stride + (int64_t)f_kb * KB;
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sb[j][e] = p.sb[min(n0 + wn + j * 16 + quad * 4 + e, p.N - 1)];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const float sa = p.sa[min(m0 + wm + i * 16 + row, p.M - 1)];
-      f32x4 v[TN];
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = (float)acc[i][j][e] * (sa * sb[j][e]);
-      if constexpr (Tag::bytes == 2 && WN == 64) {
-        unsigned char* stage = lds + 2 * STEP + w * 2048;
-        const int r8 = here / 8, unit = here % 8;
-        const int64_t n = n0 + wn + unit * 8;
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const float f[8] = {v[j][0], v[j][1], v[j][2], v[j][3], 0.f, 0.f, 0.f, 0.f};
-          const u32x4 c = Chunk<Tag>::pack(f);
-          *reinterpret_cast<u32x2*>(stage + row * 128 + ((j * 2 + quad / 2) ^ (row & 7)) * 16 + (quad & 1) * 8) = u32x2{c[0], c[1]};
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int64_t m = m0 + wm + i * 16 + k * 8 + r8;
-          const u32x4 c = *reinterpret_cast<const u32x4*>(stage + (k * 8 + r8) * 128 + (unit ^ r8) * 16);
-          char* to = p.out + (m * p.out_stride + n) * 2;
-          if (m < p.M && n + 8 <= p.N) store16_stream_any(to, c);
-          else if (m < p.M && n < p.N) store_chunk_elementwise<Tag>(to, 0, (int)(p.N - n), c);
-        }
-      } else {
-        const int64_t m = m0 + wm + i * 16 + row;
-        char* to = p.out + m * p.out_stride * Tag::bytes;
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const int64_t n = n0 + wn + j * 16 + quad * 4;
-          if (m < p.M && n < p.N) store_four<Tag>(to, n, p.N, v[j]);
-        }
-      }
+    for (int i = 0; i < NA; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_ao[i] = (unsigned)(min((int64_t)row, p.M - 1 - m) * p.a_stride) + piece * 16;
     }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
+      f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
+    }
+  };
+  const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((lds_words)lds);
+  const auto fetch = [&]() {
+    const unsigned to = lds0 + f_place * STEP;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) fetch_to_lds(f_b, f_bo[i], to + BM * KB + (i * WAVES + w) * 1024);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) fetch_to_lds(f_a, f_ao[i], to + (i * WAVES + w) * 1024);
+    f_place = f_place + 1 == S ? 0 : f_place + 1;
+    f_a += KB;
+    f_b += KB;
+    if (++f_kb == p.blocks) {
+      f_kb = 0;
+      f_a -= (int64_t)p.blocks * KB;
+      f_b -= (int64_t)p.blocks * KB;
+    }
+    ++f_step;
+    if (--f_left == 0) {
+      f_tile += walk.step;
+      if (f_tile < walk.end) f_begin();
+    }
+  };
+  f_begin();
+#pragma unroll 1
+  for (int s = 0; s < S - 1; ++s)
+    if (f_step < steps) fetch();
+  const unsigned lo = i16 * KB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
+  int place = 0;
+  unsigned step = 0;
+  for (unsigned tile = walk.first; tile < walk.end; tile += walk.step) {
+    int64_t m0, n0;
+    walk.origin(tile, m0, n0);
+    m0 *= BM;
+    n0 *= BN;
+    i32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll 1
+    for (int kb = 0; kb < p.blocks; ++kb, ++step) {
+      // this step's operands are there: all but the last S - 2 steps' fetches (they come back in order; a tile's stores only add to the count)
+      if (step + (S - 2) < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * (NA + NB)) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (f_step < steps) fetch();                             // (into the place of the step before, which all have read)
+      const unsigned char* at = lds + place * STEP;
+      place = place + 1 == S ? 0 : place + 1;
+      Piece af[TM], bf[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) bf[j] = row_piece(at, (BM + wn) * KB + lo, (BM + wn) * KB + hi, j * 16);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[i] = row_piece(at, wm * KB + lo, wm * KB + hi, i * 16);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].lo, af[i].lo, acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[i].hi, acc[i][j], 0, 0, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + S * STEP + w * 2048);
+  }
+}
+
+template <class Tag, int NT, int NCH>
+static void launch_quantize(RowsQuant p, hipStream_t st) {
+  constexpr int64_t MOST = LAUNCH_THREADS / NT / 65536 * 65536;      // rows of a launch
+  for (int64_t all = p.rows; all > 0; all -= MOST) {
+    p.rows = std::min(all, MOST);
+    const unsigned x = (unsigned)std::min<int64_t>(p.rows, 65536), y = (unsigned)((p.rows + x - 1) / x);
+    hipLaunchKernelGGL((quantize_whole_rows_kernel<Tag, NT, NCH>), dim3(x, y), dim3(NT), 0, st, p);
+    p.x += MOST * p.row_stride * Tag::bytes;
+    p.codes += MOST * p.code_stride;
+    p.scales += MOST;
   }
 }
 
@@ -284,14 +452,28 @@ static int launch_row_tiles(const RowsParams& p, hipStream_t st) {
   return rows_status();
 }
 
+template <class Tag, int BM, int BN, int WM, int WN, int S>
+static int launch_row_ring(const RowsParams& p, hipStream_t st) {
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = S * (BM + BN) * KB + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+  if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
+  if (bytes > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&rows_ring_kernel<Tag, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return DL_ERR_LAUNCH;
+  const unsigned grid = (unsigned)std::min<int64_t>((tm * tn + 7) / 8 * 8, 256 * std::min(per_cu, 4));
+  hipLaunchKernelGGL((rows_ring_kernel<Tag, BM, BN, WM, WN, S>), dim3(grid), dim3(threads), bytes, st, p, (unsigned)tm, (unsigned)tn);
+  return rows_status();
+}
+
 // The tile of a call: that with the least time by a model of two numbers each, microseconds for a step of a CU -- alone, and what every
-// further tile of the CU adds.
+// further tile of the CU adds -- measured over 21 shapes from 64 x 1000 to 8192 x 32000 (us, in the order of the list: 8192 x 32000 x 1024 283, 336, 424,
+// 631, 797; 512 x 14336 x 4096 53, 36, 58, 62, 81; 61 x 50257 x 2048 34, 28, 26, 29, 33; 128 x 8000 x 4096 46, 30, 16, 12.9, 14; 64 x 4096 x 4096 44, 31, 16, 13, 11).
 struct RowsShape { int bm, bn; float alone, each; };
-constexpr RowsShape ROWS_SHAPES[] = {{256, 256, 1.55f, 1.55f}, {128, 256, 1.05f, 1.25f}, {64, 128, 0.62f, 0.43f}, {64, 64, 0.50f, 0.26f}};
+constexpr RowsShape ROWS_SHAPES[] = {{256, 256, 1.30f, 1.72f}, {128, 256, 0.89f, 1.19f}, {64, 128, 0.37f, 0.43f}, {64, 64, 0.31f, 0.27f}, {64, 32, 0.25f, 0.175f}};
 static int rows_shape(int64_t M, int64_t N) {
   int best = 0;
   float least = 0.f;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 5; ++i) {
     const RowsShape& t = ROWS_SHAPES[i];
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
     const float time = std::max(t.alone, (float)((tiles + 255) / 256) * t.each);
@@ -305,8 +487,9 @@ static int launch_rows(const RowsParams& p, hipStream_t st) {
   switch (rows_shape(p.M, p.N)) {
     case 0: return launch_row_tiles<Tag, 256, 256, 128, 64>(p, st);
     case 1: return launch_row_tiles<Tag, 128, 256, 64, 64>(p, st);
-    case 2: return launch_row_tiles<Tag, 64, 128, 32, 64>(p, st);
-    default: return launch_row_tiles<Tag, 64, 64, 32, 32>(p, st);
+    case 2: return launch_row_ring<Tag, 64, 128, 32, 64, 3>(p, st);
+    case 3: return launch_row_ring<Tag, 64, 64, 32, 32, 4>(p, st);
+    default: return launch_row_ring<Tag, 64, 32, 32, 16, 4>(p, st);
   }
 }
 
@@ -325,10 +508,18 @@ extern "C" int dl_quantize_rows(const void* x, int dtype, int64_t row_stride, in
     return DL_ERR_ALIGN;
   const RowsQuant p{reinterpret_cast<const char*>(x), row_stride, rows, cols, width, reinterpret_cast<signed char*>(codes), code_stride, scales};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)std::min<int64_t>(rows, 65535));
-  if (dtype == DL_F32) hipLaunchKernelGGL((quantize_whole_rows_kernel<TagF32, 256>), grid, dim3(256), 0, st, p);
-  else if (dtype == DL_BF16) hipLaunchKernelGGL((quantize_whole_rows_kernel<TagBF16, 256>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((quantize_whole_rows_kernel<TagF16, 256>), grid, dim3(256), 0, st, p);
+  if (rows > 0xffffffffLL) return DL_ERR_LIMIT;
+#define DL_QUANTIZE_ROWS(TAG, NT, NCH) launch_quantize<TAG, NT, NCH>(p, st)
+#define DL_QUANTIZE_TAG(TAG)                                  \
+  if (width <= 1024) DL_QUANTIZE_ROWS(TAG, 128, 1);           \
+  else if (width <= 2048) DL_QUANTIZE_ROWS(TAG, 256, 1);      \
+  else if (width <= 4096) DL_QUANTIZE_ROWS(TAG, 256, 2);      \
+  else if (width <= 8192) DL_QUANTIZE_ROWS(TAG, 512, 2);      \
+  else if (width <= 16384) DL_QUANTIZE_ROWS(TAG, 512, 4);     \
+  else DL_QUANTIZE_ROWS(TAG, 512, 0);
+  if (dtype == DL_F32) { DL_QUANTIZE_TAG(TagF32) } else if (dtype == DL_BF16) { DL_QUANTIZE_TAG(TagBF16) } else { DL_QUANTIZE_TAG(TagF16) }
+#undef DL_QUANTIZE_TAG
+#undef DL_QUANTIZE_ROWS
   return rows_status();
 }
 
