@@ -302,20 +302,26 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
       b_lo += flip;
       b_hi += flip;
       flip = 0u - flip;
+      // The last row's products, and behind each what the next step begins with, in the order in which that needs it: a's first, b's first
+      // halves, b's second halves.  (Behind the last step: what lies there, unused.)
       constexpr int L = TM - 1;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].lo, af[L & 1].lo, acc[L][j], 0, 0, 0);
-        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[L & 1].hi, acc[L][j], 0, 0, 0);
-        bf[j] = row_piece(lds, b_lo, b_hi, j * 16);            // (behind the last step: what lies there, unused)
-      }
       af[0] = row_piece(lds, a_lo, a_hi, 0);
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].lo, af[L & 1].lo, acc[L][j], 0, 0, 0);
+        bf[j].lo = *reinterpret_cast<const i32x4*>(lds + b_lo + j * 16 * KB);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        acc[L][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[L & 1].hi, acc[L][j], 0, 0, 0);
+        bf[j].hi = *reinterpret_cast<const i32x4*>(lds + b_hi + j * 16 * KB);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int j = 0; j < 2 * TN; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
     store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + 2 * STEP + w * 2048);
   }
