@@ -100,13 +100,22 @@ __device__ __forceinline__ void fetch_to_lds(const unsigned char* base, unsigned
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 
+__device__ __forceinline__ void fetch_word_to_lds(const float* base, unsigned offset, unsigned to) {      // 4 bytes a lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+
 // Tiles of BM x BN, a wave WM x WN of it, a block of 128 columns (two matrix instructions deep) per step.  A step's operands are fetched into LDS by
-// loads that bypass the registers, two steps ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted
+// loads that bypass the registers, a step ahead of their use; a row of a tile is 128 bytes of LDS, its eight 16-byte pieces permuted
 // by piece ^ (row / 2 % 8): the 16 rows x 16 bytes that a quarter of a wave reads then lie on all banks once.  (The loads write LDS in lane
 // order, so it is their source addresses that are permuted.)
-// Within a step a wave goes through its WM / 16 rows of tiles: the operand of the next row is read while the matrix unit works on this one.  A
-// step's last barrier sits ahead of the last row, whose operands are in registers by then, so that the matrix unit is busy across it; another one at
-// half the step frees b's place and half of a's.  Workgroups stay: each walks its tiles as one sequence of steps.
+// Within a step a wave goes through its WM / 16 rows of tiles: the operand of the next row is read while the matrix unit works on this one.  The step's
+// barrier sits ahead of the last row, whose operands are in registers by then: what follows it -- the last row's products, the next step's first
+// operands, the fetches into what has just become free -- keeps the matrix unit busy.  Workgroups stay: each walks its tiles as one sequence of
+// steps, so that the next tile's operands arrive while the last one is stored.
+// Measured: 8192 x 128256 x 4096 (bf16 out) 3.42-3.55 ms, 2430-2520 Top/s (a library product with 32-bit results: 4.0-4.3 ms); without its fetches the
+// same kernel takes 2.80, without reads of LDS as well 2.47: what is left are the matrix units (2.08 at the 1.98 GHz that the card holds under them) and
+// the stores (0.39).  Fetches and reads share LDS with each other.  Tried: 32 x 32 x 32 instructions (3.97 ms), lines asked for ahead into the L2
+// (3.88), four waves of 128 x 128 with the next step's b in registers (3.90), a second barrier for earlier fetches (level).
 struct Piece { i32x4 lo, hi; };                                // a lane's 32 bytes of a row: 16 columns of either half of the block
 __device__ __forceinline__ Piece row_piece(const unsigned char* lds, unsigned lo, unsigned hi, int rows) {
   return Piece{*reinterpret_cast<const i32x4*>(lds + lo + rows * KB), *reinterpret_cast<const i32x4*>(lds + hi + rows * KB)};
@@ -121,17 +130,18 @@ __device__ __forceinline__ int first_block(unsigned tile, unsigned tiles_m, int 
 // time, so that a store writes whole 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by
 // unit ^ (row % 8).
 template <class Tag, int TM, int TN>
-__device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int lane, unsigned char* stage) {
+__device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int lane, unsigned char* stage,
+                                           const float* sa_here = nullptr, const float* sb_here = nullptr) {
   asm volatile("" : "+v"(lane));                               // (keeps the stores' addresses out of the steps' registers)
   const int row = lane % 16, quad = lane / 16;
   f32x4 sb[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sb[j][e] = p.sb[min(n0 + j * 16 + quad * 4 + e, p.N - 1)];
+    for (int e = 0; e < 4; ++e) sb[j][e] = sb_here ? sb_here[j * 16 + quad * 4 + e] : p.sb[min(n0 + j * 16 + quad * 4 + e, p.N - 1)];
   float sas[TM];                                               // (all ahead of the first store, which a load behind it would wait for)
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sas[i] = p.sa[min(m0 + i * 16 + row, p.M - 1)];
+  for (int i = 0; i < TM; ++i) sas[i] = sa_here ? sa_here[i * 16 + row] : p.sa[min(m0 + i * 16 + row, p.M - 1)];
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const float sa = sas[i];
@@ -173,8 +183,8 @@ template <class Tag, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(const RowsParams p, unsigned tiles_m, unsigned tiles_n) {
   constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16, NA = BM / 8 / WAVES, NB = BN / 8 / WAVES;
   static_assert(TM >= 2 && BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole fetches");
-  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes)
-  constexpr int STEP = (BM + BN) * KB;
+  extern __shared__ __align__(1024) unsigned char lds[];      // two of (a: BM rows, b: BN rows of 128 bytes); two tiles' scales; 2 KiB of each wave's own
+  constexpr int STEP = (BM + BN) * KB, SCALES = 2 * STEP, STAGE = SCALES + 2 * (BM + BN) * 4;
   const int lane = threadIdx.x & (WAVE - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), i16 = lane % 16;      // (w: known to be the wave's)
   const int wm = (w / (BN / WN)) * WM, wn = (w % (BN / WN)) * WN;
   const TileWalk walk(tiles_m, tiles_n);
@@ -206,25 +216,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
       f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
     }
   };
-  // In two parts, by when their places become free: `early` after half a step (b, whose operands are in registers from a step's
-  // beginning on, and of a the rows that the waves go through first), `late` at its end.
-  constexpr bool HALVES = WM / 2 == WAVES * 8;                 // every other fetch of a: those rows
-  constexpr int EARLY = NB + (HALVES ? NA / 2 : 0);
   const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((lds_words)lds);
-  const auto fetch_a = [&](unsigned to, int i) { fetch_to_lds(f_a, f_ao[i], to + (i * WAVES + w) * 1024); };
-  const auto fetch_early = [&](unsigned step) {
+  const auto fetch = [&](unsigned step) {
     const unsigned to = lds0 + (step & 1u) * STEP;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-      fetch_to_lds(f_b, f_bo[i], to + BM * KB + (i * WAVES + w) * 1024);
-    if (HALVES)
+    for (int i = 0; i < NB; ++i) fetch_to_lds(f_b, f_bo[i], to + BM * KB + (i * WAVES + w) * 1024);
 #pragma unroll
-      for (int i = 0; i < NA; i += 2) fetch_a(to, i);
-  };
-  const auto fetch_late = [&](unsigned step) {
-    const unsigned to = lds0 + (step & 1u) * STEP;
-#pragma unroll
-    for (int i = HALVES ? 1 : 0; i < NA; i += HALVES ? 2 : 1) fetch_a(to, i);
+    for (int i = 0; i < NA; ++i) fetch_to_lds(f_a, f_ao[i], to + (i * WAVES + w) * 1024);
     f_a += KB;
     f_b += KB;
     if (++f_kb == p.blocks) {
@@ -237,26 +235,30 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
       if (f_tile < walk.end) f_begin();
     }
   };
-  const auto meet = [&]() {                                    // everyone's reads so far are done
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  // A tile's scales, BM of a's and BN of b's, 64 at a time: the waves in turn.
+  const auto fetch_scales = [&](unsigned tile, unsigned which) {
+    int64_t m, n;
+    walk.origin(tile, m, n);
+    m *= BM;
+    n *= BN;
+    const unsigned to = lds0 + SCALES + which * (BM + BN) * 4;
+    for (int k = w; k < (BM + BN) / WAVE; k += WAVES) {
+      const int at = k * WAVE + lane;
+      if (k < BM / WAVE) fetch_word_to_lds(p.sa + m, (unsigned)min((int64_t)at, p.M - 1 - m) * 4, to + k * WAVE * 4);
+      else fetch_word_to_lds(p.sb + n, (unsigned)min((int64_t)at - BM, p.N - 1 - n) * 4, to + k * WAVE * 4);
+    }
+  };
+  const auto meet = [&]() {                                    // this wave's fetches are there and its reads done, and so are everyone's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // This wave's fetches are there but for the last `early` part (loads come back in order; the stores of a tile only add to the count).
-  const auto landed = [&](bool early_under_way) {
-    if (early_under_way) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EARLY) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  };
 
   f_begin();
-  fetch_early(0);
-  fetch_late(0);
-  landed(false);
+  fetch_scales(walk.first, 0);
+  fetch(0);
   meet();
-  if (steps > 1) {
-    fetch_early(1);
-    fetch_late(1);
-  }
+  if (steps > 1) fetch(1);
   // (the permutation of a row depends on its place among 16: the same for all operands of a lane)
   const unsigned lo = i16 * KB + ((lane / 16) ^ (i16 >> 1)) * 16, hi = lo ^ 64u;
   unsigned a_lo = wm * KB + lo, a_hi = wm * KB + hi, b_lo = (BM + wn) * KB + lo, b_hi = (BM + wn) * KB + hi;
@@ -265,8 +267,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
 #pragma unroll
   for (int j = 0; j < TN; ++j) bf[j] = row_piece(lds, b_lo, b_hi, j * 16);
   af[0] = row_piece(lds, a_lo, a_hi, 0);
-  unsigned step = 0;
-  for (unsigned tile = walk.first; tile < walk.end; tile += walk.step) {
+  unsigned step = 0, which = 0;
+  for (unsigned tile = walk.first; tile < walk.end; tile += walk.step, which ^= 1u) {
     int64_t m0, n0;
     walk.origin(tile, m0, n0);
     m0 *= BM;
@@ -289,14 +291,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN - 1, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (i == TM / 2 - 1 && step + 2 < steps) {
-          meet();
-          fetch_early(step);                                   // (into this step's buffer)
-        }
       }
-      landed(step + 2 < steps);
       meet();
-      if (step + 2 < steps) fetch_late(step);
+      if (step + 2 < steps) fetch(step);                       // (into this step's buffer)
+      if (kb == 0 && tile + walk.step < walk.end) fetch_scales(tile + walk.step, which ^ 1u);      // (all have stored the tile before)
       a_lo += flip;
       a_hi += flip;
       b_lo += flip;
@@ -323,7 +321,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
     }
-    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + 2 * STEP + w * 2048);
+    const float* scales = reinterpret_cast<const float*>(lds + SCALES) + which * (BM + BN);
+    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + STAGE + w * 2048, scales + wm, scales + BM + wn);
   }
 }
 
@@ -447,7 +446,7 @@ static int rows_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_E
 
 template <class Tag, int BM, int BN, int WM, int WN>
 static int launch_row_tiles(const RowsParams& p, hipStream_t st) {
-  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * (BM + BN) * KB + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
+  constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = 2 * (BM + BN) * (KB + 4) + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
   if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
   if (bytes > 64 * 1024 &&
