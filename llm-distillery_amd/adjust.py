@@ -2,6 +2,7 @@
 that.  Thin wrappers over the C ABI; all arithmetic runs in the HIP kernels."""
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -127,9 +128,10 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     rep, rep_all = _per_row(repetition, R, "repetition", dev)
     freq, freq_all = _per_row(frequency, R, "frequency", dev)
     pres, pres_all = _per_row(presence, R, "presence", dev)
-    if rep is None and not rep_all > 0.0:
-        raise ValueError("repetition must be positive")
+    if rep is None and not 0.0 < rep_all <= 3.0e38:
+        raise ValueError("repetition must be positive and finite")
     b_ptr = b_dtype = b_stride = 0
+    others = ()
     if bias is not None:
         _dev(bias, "bias", dev)
         if bias.dtype not in (torch.float32, x.dtype):
@@ -140,7 +142,8 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
         if b.dim() == 1 and V > 1 and b.stride(0) != 1:
             b = b.contiguous()
         b_ptr, b_dtype, b_stride = b.data_ptr(), _DT[b.dtype], b.stride(0) if b.dim() == 2 and b.shape[0] > 1 else 0
-    res = _written(out, x, "out", "the logits")
+        others = (b if b.dim() == 2 else b.unsqueeze(0),)
+    res = _written(out, x, "out", "the logits", others)
     with _on(dev):
         st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, *text, _address(lengths), _address(prompt_rows),
                                         prompt_all, _address(rep), _address(freq), _address(pres), rep_all, freq_all, pres_all, b_ptr, b_dtype,
@@ -167,8 +170,8 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
     lengths = _row_lengths(lengths, R, dev)
     rep, rep_all = _per_row(repetition, R, "repetition", dev)
-    if rep is None and not rep_all > 0.0:
-        raise ValueError("repetition must be positive")
+    if rep is None and not 0.0 < rep_all <= 3.0e38:
+        raise ValueError("repetition must be positive and finite")
     if bias_dtype not in (torch.float32, g.dtype):
         raise RuntimeError(f"the bias's gradient is fp32 or {g.dtype}")
     x = None
@@ -238,6 +241,16 @@ def _(grad, allowed, allowed_rows, dtype):
     return torch.empty(grad.shape[-1:], dtype=dtype, device=grad.device)
 
 
+def _even(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it down, expanded or transposed as it may be, with rows as the kernels take them."""
+    if not grad.is_contiguous():
+        s, n = grad.stride(), grad.shape
+        lead = all(n[d] == 1 or s[d] == s[-2] * math.prod(n[d + 1:-1]) for d in range(grad.dim() - 1))
+        if grad.dim() < 2 or s[-1] != 1 or not lead or s[-2] < n[-1]:
+            return grad.contiguous()
+    return grad
+
+
 def _adjust_setup(ctx, inputs, output):
     logits, bias, tokens, token_rows, lengths, allowed, allowed_rows, _, _, repetition_rows, repetition = inputs[:11]
     if repetition_rows is None and repetition == 1.0:
@@ -252,8 +265,7 @@ def _adjust_backward(ctx, grad):
     logits, tokens, token_rows, lengths, allowed, allowed_rows, repetition_rows = ctx.saved_tensors
     want_logits, want_bias = ctx.needs_input_grad[0], ctx.bias is not None and ctx.needs_input_grad[1]
     by_logits = by_bias = None
-    if grad.stride(-1) != 1 or grad.dim() > 1 and grad.shape[-2] > 1 and grad.stride(-2) < grad.shape[-1]:
-        grad = grad.contiguous()                              # an expanded or transposed gradient
+    grad = _even(grad)
     shared = want_bias and ctx.bias[0].numel() == grad.shape[-1]
     if shared and type(grad) is torch.Tensor and not torch.is_grad_enabled() and not is_in_torch_dispatch_mode():
         # Neither traced nor to be differentiated again: both in one sweep.

@@ -61,8 +61,9 @@ struct AdjustRow {
     inverse = 1.f / repetition;
   }
   // f / repetition, rounded once: a product with the rounded reciprocal, and what it is off by taken off (the remainder is exact).  Where the product is no
-  // number or infinite, it is the quotient.
+  // number or infinite, it is the quotient; so far from 1 that the reciprocal loses bits, a division.
   __device__ __forceinline__ float quotient(float f) const {
+    if (!(repetition >= 0x1p-64f && repetition <= 0x1p64f)) return f / repetition;
     const float q = f * inverse, better = fmaf(fmaf(-q, repetition, f), inverse, q);
     return fabsf(q) <= 3.402823466e38f ? better : q;
   }
@@ -300,11 +301,11 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
   }
 }
 
-// The runs' sums, added up in fp64: 32 columns a workgroup, eight threads to a column, each every eighth run.
-__global__ __launch_bounds__(256) void bias_join_kernel(const float* sums, int64_t runs, int64_t V, void* out, int dtype) {
+// The runs' sums, added up in fp64: 32 columns a workgroup, from `first` on, eight threads to a column, each every eighth run.
+__global__ __launch_bounds__(256) void bias_join_kernel(const float* sums, int64_t runs, int64_t first, int64_t V, void* out, int dtype) {
   __shared__ double part[8][32];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t col = first + (int64_t)blockIdx.x * 32 + lane;
   double total = 0.0;
   if (col < V)
     for (int64_t k = slice; k < runs; k += 8) total += (double)sums[k * V + col];
@@ -333,6 +334,9 @@ static void launch_adjust(AdjustParams p, float* sums, hipStream_t st) {
   p.part_columns = (unsigned)std::min<int64_t>(most, ((p.V + p.parts - 1) / p.parts + 127) / 128 * 128);      // (whole words of the masks, whole pieces of the bits)
   p.run = SUMS ? sums_run(p.n_rows, p.V) : 1;
   const size_t lds = p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (GRAD ? Tag::bytes : sizeof(Count))) : 0;
+  if (NT * ADJUST_NCH * 16 > 32768 && lds > 65536 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+    return;                                                    // (the error is the launch's)
   const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8 * p.run, all = p.n_rows;      // rows of a launch
   for (p.first_row = 0; p.first_row < all; p.first_row += slice) {
     p.n_rows = std::min(all, p.first_row + slice);
@@ -444,6 +448,8 @@ extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, 
     adjust_rows<true, true>(p, dtype, sums, st);
     runs = (n_rows + sums_run(n_rows, V) - 1) / sums_run(n_rows, V);
   }
-  hipLaunchKernelGGL(bias_join_kernel, dim3((unsigned)((V + 31) / 32)), dim3(256), 0, st, sums, runs, V, bias_grad, bias_dtype);
+  constexpr int64_t MOST = LAUNCH_THREADS / 256 * 32;          // columns of a launch
+  for (int64_t col = 0; col < V; col += MOST)
+    hipLaunchKernelGGL(bias_join_kernel, dim3((unsigned)((std::min(MOST, V - col) + 31) / 32)), dim3(256), 0, st, sums, runs, col, V, bias_grad, bias_dtype);
   return adjust_status();
 }

@@ -505,3 +505,74 @@ def test_refusals(D):
                  lambda: D.adjust_grad(x.clone(), x, t, out=x), lambda: D.adjust_grad(x, want_logits=False, out=x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("repetition", [2.0 ** -100, 2.0 ** -64, 1e-3, 3.0, 2.0 ** 64, 2.0 ** 101])
+def test_quotients_are_rounded_once(D, repetition):
+    """x / repetition of ordinary numbers is the fp32 quotient bit for bit, whatever the penalty's size."""
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn(1, 5000, generator=g).abs() * (2.0 ** -20 if repetition < 1 else 2.0 ** 20)
+    got = D.adjust_rows(x.to(DEV), torch.arange(5000, device=DEV).unsqueeze(0), repetition=torch.tensor([repetition], device=DEV))
+    assert torch.equal(got.cpu(), x / torch.tensor(repetition))
+
+
+def test_gradients_of_any_layout(D):
+    """What autograd hands down may be transposed over the batch, expanded, or a part of wider rows."""
+    g = torch.Generator().manual_seed(41)
+    x = torch.randn(3, 4, 100, generator=g).to(DEV)
+    t = texts(12, 20, 100, 42).to(DEV)
+    w = torch.randn(3, 4, 100, generator=g).to(DEV)
+    want = None
+    for weigh in (lambda y: (y * w).sum(), lambda y: (y.transpose(0, 1) * w.transpose(0, 1).contiguous()).sum(),
+                  lambda y: (y.permute(2, 0, 1) * w.permute(2, 0, 1).contiguous()).sum(),
+                  lambda y: (torch.nn.functional.pad(y, (3, 5)) * torch.nn.functional.pad(w, (3, 5))).sum()):
+        xs = x.clone().requires_grad_()
+        b = torch.zeros(100, device=DEV).requires_grad_()
+        weigh(D.adjust_logits(xs, t, bias=b, repetition=1.5)).backward()
+        if want is None:
+            want = xs.grad, b.grad
+        assert torch.equal(xs.grad, want[0]) and torch.equal(b.grad, want[1])
+
+
+def test_a_compiled_step(D):
+    g = torch.Generator().manual_seed(43)
+    x, b = torch.randn(6, 80, generator=g).to(DEV).requires_grad_(), torch.randn(80, generator=g).to(DEV).requires_grad_()
+    t = texts(6, 15, 80, 44).to(DEV)
+    w = torch.randn(6, 80, generator=g).to(DEV)
+
+    def step(x, b, t, w):
+        return (torch.softmax(D.adjust_logits(x, t, bias=b, repetition=1.25, presence=0.5), 1) * w).sum()
+
+    want = torch.autograd.grad(step(x, b, t, w), (x, b))
+    got = torch.autograd.grad(torch.compile(step, backend="aot_eager", fullgraph=True)(x, b, t, w), (x, b))
+    assert torch.equal(got[0], want[0]) and torch.allclose(got[1], want[1], rtol=2.0 ** -20, atol=2.0 ** -24)
+
+
+def test_very_wide_rows(D):
+    """More columns than one launch joins; a text at both ends."""
+    V = 540_000_000
+    x = torch.zeros((1, V), dtype=torch.bfloat16, device=DEV)
+    x[0, 0], x[0, V - 1], x[0, V // 2] = 2.0, 3.0, -1.0
+    y = D.adjust_rows(x, torch.tensor([[0, V - 1, V - 1, V // 2, V, -1]], device=DEV), repetition=2.0, frequency=0.25)
+    assert y[0, 0] == 0.75 and y[0, V - 1] == 1.0 and y[0, V // 2] == -2.25 and y.count_nonzero().item() == 3
+    _, by_bias = D.adjust_grad(x, want_logits=False, want_bias=True)
+    assert by_bias[0] == 2.0 and by_bias[V - 1] == 3.0 and by_bias[V // 2] == -1.0 and by_bias.count_nonzero().item() == 3
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sums_of_many_full_rows(D, dtype):
+    """Rows enough, and as wide as the parts of the larger workgroups."""
+    R, V = 2100, 32768 if dtype != torch.float32 else 16384
+    g = torch.Generator(device=DEV).manual_seed(45)
+    grad, x = torch.randn((R, V), generator=g, device=DEV).to(dtype), torch.randn((R, V), generator=g, device=DEV).to(dtype)
+    t = torch.randint(V, (3, 700), generator=g, device=DEV)
+    at = torch.arange(R, device=DEV)
+    kw = dict(token_rows=(at // 700).int(), lengths=(at % 700).int(), repetition=1.5, allowed=torch.randint(-2 ** 31, 2 ** 31 - 1, (1, V // 32), generator=g, device=DEV, dtype=torch.int64).int())
+    got, by_bias = D.adjust_grad(grad, x, t, want_bias=True, **kw)
+    assert torch.equal(got, D.adjust_grad(grad, x, t, **kw)[0])
+    bit = ((kw["allowed"].view(-1, 1) >> torch.arange(32, device=DEV, dtype=torch.int32)) & 1).view(-1)
+    kept = grad.double() * bit
+    assert ((by_bias.double() - kept.sum(0)).abs() <= 2.0 ** -24 * 66 * kept.abs().sum(0)).all()      # (runs of 64 rows, one rounding)
+    some = torch.tensor([0, 1, 699, 700, 1399, 2099], device=DEV)
+    small, _ = D.adjust_grad(grad[some], x[some], t, token_rows=kw["token_rows"][some], lengths=kw["lengths"][some], repetition=1.5, allowed=kw["allowed"])
+    assert torch.equal(got[some], small)

@@ -190,3 +190,14 @@ def test_refusals(D):
     wide = torch.zeros(2, 130944 + 128, dtype=torch.int8, device=DEV)
     with pytest.raises(RuntimeError):
         D.matmul_rows(*[D.RowQuantized(wide, torch.ones(2, device=DEV), 130944 + 1)] * 2)
+
+
+def test_more_rows_than_a_launch_takes(D):
+    n = 33_488_896 + 77
+    g = torch.Generator(device=DEV).manual_seed(13)
+    x = torch.randn((n, 3), generator=g, device=DEV, dtype=torch.bfloat16)
+    q = D.quantize_rows(x)
+    for rows in (slice(0, 2 ** 18), slice(33_488_896 - 2 ** 18, n)):
+        some = D.quantize_rows(x[rows])
+        assert torch.equal(q.codes[rows], some.codes) and torch.equal(q.scales[rows], some.scales)
+    assert torch.equal(some.scales.cpu(), quantised(x[rows].cpu())[1])
