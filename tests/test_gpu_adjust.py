@@ -576,3 +576,34 @@ def test_sums_of_many_full_rows(D, dtype):
     some = torch.tensor([0, 1, 699, 700, 1399, 2099], device=DEV)
     small, _ = D.adjust_grad(grad[some], x[some], t, token_rows=kw["token_rows"][some], lengths=kw["lengths"][some], repetition=1.5, allowed=kw["allowed"])
     assert torch.equal(got[some], small)
+
+
+def test_the_example_writes_and_learns_under_penalties():
+    """It runs with an integer head and penalties, no token twice in a text where a presence penalty forbids it, and its gradients through the
+    adjustment are those of the same formula in torch operations."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "on_policy.py")
+    spec = importlib.util.spec_from_file_location("on_policy_example_too", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    import llm_distillery_amd as D
+    assert all(math.isfinite(v) for v in example.train(steps=3, penalties=dict(repetition=1.2, presence=0.5), integers=True))
+    m = example.Model(200, 64, DEV, 3, 2.0)
+    first = torch.arange(8, device=DEV)
+    u = torch.rand(12, 8, generator=torch.Generator(device=DEV).manual_seed(46), device=DEV)
+    written, _ = m.write(first, 12, u, penalties=dict(presence=1e9), integers=True)
+    for f, row in zip(first.tolist(), written.tolist()):
+        assert len({f, *row}) == 13
+    tokens = torch.cat([first.unsqueeze(1), written[:, :-1]], 1)
+    at = torch.arange(96, device=DEV, dtype=torch.int32)
+    w = torch.randn(96, 200, generator=torch.Generator(device=DEV).manual_seed(47), device=DEV).bfloat16()
+    logits = m.logits(m.states(tokens)).detach().requires_grad_()
+    D.adjust_logits(logits, tokens, token_rows=at // 12, lengths=at % 12 + 1, repetition=1.5, presence=0.25).backward(w)
+    seen = torch.zeros(96, 200, dtype=torch.bool, device=DEV)
+    for r in range(96):
+        seen[r, tokens[r // 12, : r % 12 + 1]] = True
+    want = torch.where(seen, torch.where(logits > 0, w.double() / 1.5, w.double() * 1.5), w.double())
+    # an fp32 rounding, and one to bf16, whose eight significant bits leave at most half a step, 2^-8 of the value
+    bound = (HALF_ULP[torch.bfloat16] + 2.0 ** -24) * want.abs() * (1 + 2.0 ** -20) + STEP[torch.bfloat16]
+    assert ((logits.grad.double() - want).abs() <= bound).all()
