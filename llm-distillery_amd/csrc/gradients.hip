@@ -175,7 +175,7 @@ __global__ __launch_bounds__(GRAD_NT, 4) void scale_kernel(const GradTable t, co
   const double all = sums ? norm_of(sums, n_sums, scale, scratch) : (double)norm[0];
   if (sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
   const float by = (float)(all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale);
-  if (!(all <= 1.7976931348623157e308) || by == 1.f) return;   // NaN or infinite: left as they are
+  if (!((float)all <= 3.402823466e38f) || by == 1.f) return;   // NaN or, as fp32 shows it, infinite: left as they are
   const unsigned q = t.pieces - 1u - blockIdx.x;
   find_entry(t, q, found);
   const GradPiece p = piece_of(found, q);

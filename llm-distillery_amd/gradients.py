@@ -29,7 +29,8 @@ class _Tensors:
         if not grads:
             raise RuntimeError("no gradients")
         self.dev = dev = grads[0].device
-        for g in grads:
+        usual = dev.type == "cuda" and {*map(torch.Tensor.get_device, grads)} == {dev.index} and all(map(torch.Tensor.is_contiguous, grads))
+        for g in grads if not usual else ():
             if g.device != dev or not g.is_cuda or g.layout is not torch.strided:
                 _dev(g, "a gradient", dev if dev.type == "cuda" else None)
                 raise RuntimeError("gradients must be dense tensors")
@@ -39,8 +40,8 @@ class _Tensors:
             self.dtypes = array("i", [_DT[g.dtype] for g in grads])
         except KeyError:
             raise RuntimeError("gradients must be bf16/fp16/fp32") from None
-        self.at = array("q", [g.data_ptr() for g in grads])
-        self.sizes = array("q", [g.numel() for g in grads])
+        self.at = array("q", map(torch.Tensor.data_ptr, grads))
+        self.sizes = array("q", map(torch.Tensor.numel, grads))
 
     def args(self):
         return self.at.buffer_info()[0], self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], len(self.at)

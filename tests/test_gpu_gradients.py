@@ -107,6 +107,16 @@ def test_a_norm_that_is_no_number_leaves_the_gradients(D, odd):
     near(D.clip_grads(grads[2:], 1e9), exact_norm(grads[2:]))
 
 
+@pytest.mark.parametrize("size", [4, 40_000_000])            # (with the sums added up in the launch that scales, and ahead of it)
+def test_a_norm_beyond_fp32_leaves_the_gradients(D, size):
+    """Finite gradients whose norm is infinite in fp32: nothing is written, as with any infinite norm."""
+    grads = [torch.full((size,), 3e38, device=DEV)]
+    before = grads[0].clone()
+    assert D.grad_norm(grads).item() == math.inf
+    assert D.clip_grads(grads, 1.0).item() == math.inf
+    assert torch.equal(grads[0], before)
+
+
 def test_a_norm_that_is_given(D):
     """Two halves of the gradients, as two cards have them, clipped by the norm of both; an infinite bound only scales."""
     grads = some((1000, 70000, 12, 400), 6)
