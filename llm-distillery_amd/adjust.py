@@ -17,12 +17,13 @@ Number = Union[float, torch.Tensor]
 
 def _logit_rows(t: torch.Tensor, name: str, dev: Optional[torch.device] = None) -> torch.Tensor:
     """t [..., V] as [rows, V] without a copy."""
-    if dev is None or t.device != dev:
+    if dev is None or t.get_device() != dev.index:
         _dev(t, name, dev)
     if t.dtype not in _DT:
         raise RuntimeError(f"{name}: unsupported dtype")
     x = t if t.dim() == 2 and t.stride(1) == 1 else _rows_2d(t if t.dim() > 1 else t.unsqueeze(0))
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    (R, V), pitch = x.shape, x.stride(0)
+    if pitch < V and R > 1:
         raise RuntimeError(f"{name}: rows overlap; make them contiguous first")
     return x
 
@@ -38,20 +39,23 @@ def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], r
         if token_rows is not None:
             raise RuntimeError("token_rows without tokens")
         return (0, 0, 0, 0, 0, 0), ()
-    _dev(tokens, "tokens", dev)
-    if tokens.dtype not in _IT:
+    if tokens.get_device() != dev.index:
+        _dev(tokens, "tokens", dev)
+    kind, t = _IT.get(tokens.dtype), tokens
+    if kind is None:
         raise RuntimeError("tokens must be int32 or int64")
-    if tokens.dim() == 0:
-        raise RuntimeError("tokens must be [..., length]")
-    t = tokens if tokens.dim() == 2 else tokens.unsqueeze(0) if tokens.dim() == 1 else tokens.reshape(-1, tokens.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    n, length = t.shape
+    if t.dim() != 2:
+        if t.dim() == 0:
+            raise RuntimeError("tokens must be [..., length]")
+        t = t.unsqueeze(0) if t.dim() == 1 else t.reshape(-1, t.shape[-1])
+    (n, length), (pitch, one) = t.shape, t.stride()
+    if one != 1 and length > 1:
+        t, pitch = t.contiguous(), length
     if token_rows is not None:
         token_rows = _row_vector(token_rows, rows, torch.int32, "token_rows", dev)
     elif n not in (1, rows):
         raise RuntimeError(f"{n} texts for {rows} rows and no token_rows")
-    return (t.data_ptr(), _IT[t.dtype], t.stride(0) if n > 1 else length, n, length, token_rows.data_ptr() if token_rows is not None else 0), (t, token_rows)
+    return (t.data_ptr(), kind, pitch if n > 1 else length, n, length, token_rows.data_ptr() if token_rows is not None else 0), (t, token_rows)
 
 
 def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor], rows: int, V: int, dev: torch.device) -> Tuple[tuple, tuple]:
@@ -60,21 +64,22 @@ def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor]
         if allowed_rows is not None:
             raise RuntimeError("allowed_rows without allowed")
         return (0, 0, 0, 0), ()
-    _dev(allowed, "allowed", dev)
+    if allowed.get_device() != dev.index:
+        _dev(allowed, "allowed", dev)
     words = -(-V // 32)
     m = allowed if allowed.dim() != 1 else allowed.unsqueeze(0)
     if m.dtype != torch.int32 or m.dim() < 2 or m.shape[-1] < words:
         raise RuntimeError(f"allowed must be int32 [masks, {words}], one bit for each of the {V} tokens")
     if m.dim() > 2:
         m = m.reshape(-1, m.shape[-1])
-    if m.shape[1] > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < words:
-        m = m.contiguous()
-    n = m.shape[0]
+    (n, held), (pitch, one) = m.shape, m.stride()
+    if one != 1 and held > 1 or pitch < words and n > 1:
+        m, pitch = m.contiguous(), held
     if allowed_rows is not None:
         allowed_rows = _row_vector(allowed_rows, rows, torch.int32, "allowed_rows", dev)
     elif n not in (1, rows):
         raise RuntimeError(f"{n} masks for {rows} rows and no allowed_rows")
-    return (m.data_ptr(), m.stride(0) if n > 1 else m.shape[1], n, allowed_rows.data_ptr() if allowed_rows is not None else 0), (m, allowed_rows)
+    return (m.data_ptr(), pitch if n > 1 else held, n, allowed_rows.data_ptr() if allowed_rows is not None else 0), (m, allowed_rows)
 
 
 def _row_lengths(lengths: Optional[torch.Tensor], rows: int, dev: torch.device) -> Optional[torch.Tensor]:
@@ -133,7 +138,8 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     b_ptr = b_dtype = b_stride = 0
     others = ()
     if bias is not None:
-        _dev(bias, "bias", dev)
+        if bias.get_device() != dev.index:
+            _dev(bias, "bias", dev)
         if bias.dtype not in (torch.float32, x.dtype):
             raise RuntimeError(f"bias must be fp32 or {x.dtype}")
         b = bias if bias.dim() == 1 else _logit_rows(bias, "bias", dev)
@@ -145,10 +151,11 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
         others = (b if b.dim() == 2 else b.unsqueeze(0),)
     res = _written(out, x, "out", "the logits", others)
     with _on(dev):
-        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], _row_pitch(x), R, V, *text, _address(lengths), _address(prompt_rows),
+        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], x.stride(0) if R > 1 else V, R, V, *text, _address(lengths), _address(prompt_rows),
                                         prompt_all, _address(rep), _address(freq), _address(pres), rep_all, freq_all, pres_all, b_ptr, b_dtype,
-                                        b_stride, *mask, res.data_ptr(), _row_pitch(res), _stream_ptr(dev))
-    _lib.check(st, "dl_adjust_rows")
+                                        b_stride, *mask, res.data_ptr(), res.stride(0) if R > 1 else V, _stream_ptr(dev))
+    if st:
+        _lib.check(st, "dl_adjust_rows")
     return out if out is not None else res if logits.dim() == 2 else res.view(logits.shape)
 
 

@@ -21,7 +21,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(dev: torch.device):
     """`torch.cuda.device(dev)` where that changes anything: entering and leaving it costs a microsecond a launch."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _stream_ptr(dev: torch.device) -> int:

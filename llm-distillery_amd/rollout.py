@@ -12,7 +12,7 @@ from .ops import _DT, _dev, _on, _row_pitch, _rows_2d, _stream_ptr
 
 def _row_vector(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, dev: torch.device) -> torch.Tensor:
     """`t`, one entry per row, as a contiguous vector."""
-    if t.device != dev or t.dtype != dtype or t.numel() != n:
+    if t.get_device() != dev.index or t.dtype != dtype or t.numel() != n:
         _dev(t, name, dev)
         raise RuntimeError(f"{name} must be a {dtype} tensor with one entry for each of the {n} rows")
     return t if t.is_contiguous() else t.contiguous()
@@ -184,16 +184,18 @@ def quantize_rows(x: torch.Tensor) -> RowQuantized:
     v = x if x.dim() == 2 and x.stride(1) == 1 else _rows_2d(x if x.dim() > 1 else x.unsqueeze(0))
     if v.dtype not in _DT:
         raise RuntimeError("unsupported dtype")
-    R, W = v.shape
-    if R > 1 and v.stride(0) < W:
+    (R, W), pitch = v.shape, v.stride(0)
+    if R <= 1:
+        pitch = W
+    elif pitch < W:
         raise RuntimeError("x: rows overlap; make them contiguous first")
     dev = v.device
     wide = _blocks(W) * 128
-    codes = torch.empty((R, wide), dtype=torch.int8, device=dev)
-    scales = torch.empty(R, dtype=torch.float32, device=dev)
+    codes = v.new_empty(R, wide, dtype=torch.int8)
+    scales = v.new_empty(R, dtype=torch.float32)
     if R and W:
         with _on(dev):
-            st = _lib.load().dl_quantize_rows(v.data_ptr(), _DT[v.dtype], _row_pitch(v), R, W, codes.data_ptr(), wide, scales.data_ptr(),
+            st = _lib.load().dl_quantize_rows(v.data_ptr(), _DT[v.dtype], pitch, R, W, codes.data_ptr(), wide, scales.data_ptr(),
                                               _stream_ptr(dev))
         _lib.check(st, "dl_quantize_rows")
     return RowQuantized(codes, scales, W)
@@ -202,13 +204,12 @@ def quantize_rows(x: torch.Tensor) -> RowQuantized:
 def _check_rows(q: RowQuantized, name: str, wide: int, dev: torch.device):
     """(address, row stride) of the codes and the address of the scales of an operand."""
     codes, scales = q.codes, q.scales
-    if codes.device != dev or scales.device != dev:
+    if codes.get_device() != dev.index or scales.get_device() != dev.index:
         _dev(codes, f"{name}.codes", dev), _dev(scales, f"{name}.scales", dev)
-    rows, columns = codes.shape
-    pitch, one = codes.stride()
+    (rows, columns), (pitch, one) = codes.shape, codes.stride()
     if codes.dtype != torch.int8 or columns != wide or rows and (one != 1 or rows > 1 and pitch < wide):
         raise RuntimeError(f"{name}.codes must be an int8 matrix of whole blocks of 128 columns, dense along its rows")
-    if scales.dtype != torch.float32 or scales.shape != (rows,) or rows > 1 and scales.stride(0) != 1:
+    if scales.dtype != torch.float32 or scales.dim() != 1 or scales.numel() != rows or rows > 1 and not scales.is_contiguous():
         raise RuntimeError(f"{name}.scales must be a contiguous fp32 vector of {rows} entries")
     return codes.data_ptr(), pitch if rows > 1 else wide, scales.data_ptr()
 
@@ -219,8 +220,8 @@ def matmul_rows(a: RowQuantized, b: RowQuantized, *, dtype: torch.dtype = torch.
 
     Sums of products are exact; a sum becomes a float, is multiplied with the product of the two scales (each rounded in fp32), and the result is
     rounded once.  A row's result has the same bits whatever rows it comes with.  Up to 130944 columns."""
-    dev = a.codes.device
-    if dtype not in _DT:
+    dev, kind = a.codes.device, _DT.get(dtype)
+    if kind is None:
         raise RuntimeError("unsupported dtype")
     if a.codes.dim() != 2 or b.codes.dim() != 2:
         raise RuntimeError("codes must be matrices")
@@ -232,9 +233,9 @@ def matmul_rows(a: RowQuantized, b: RowQuantized, *, dtype: torch.dtype = torch.
     _dev(a.codes, "a.codes")
     a_ptr, a_pitch, a_scale = _check_rows(a, "a", _blocks(W) * 128, dev)
     b_ptr, b_pitch, b_scale = _check_rows(b, "b", _blocks(W) * 128, dev)
-    out = torch.empty((M, N), dtype=dtype, device=dev)
+    out = a.codes.new_empty(M, N, dtype=dtype)
     if M and N:
         with _on(dev):
-            st = _lib.load().dl_matmul_rows(a_ptr, a_pitch, a_scale, M, b_ptr, b_pitch, b_scale, N, W, out.data_ptr(), _DT[dtype], N, _stream_ptr(dev))
+            st = _lib.load().dl_matmul_rows(a_ptr, a_pitch, a_scale, M, b_ptr, b_pitch, b_scale, N, W, out.data_ptr(), kind, N, _stream_ptr(dev))
         _lib.check(st, "dl_matmul_rows")
     return out
