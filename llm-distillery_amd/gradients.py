@@ -3,12 +3,16 @@ the HIP kernels."""
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 from typing import Iterable, Optional
 
 import torch
 
 from . import _lib
 from .ops import _DT, _dev, _on, _stream_ptr
+
+
+_DTYPE = attrgetter("dtype")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -37,11 +41,12 @@ class _Tensors:
             if not g.is_contiguous() and g.numel() and not _dense(g):
                 raise RuntimeError("a gradient must fill its memory (a slice or an expanded tensor does not)")
         try:
-            self.dtypes = array("i", [_DT[g.dtype] for g in grads])
+            kinds = [*{*map(_DTYPE, grads)}]                   # (most often one)
+            self.dtypes = array("i", [_DT[kinds[0]]]) * len(grads) if len(kinds) == 1 else array("i", [_DT[g.dtype] for g in grads])
         except KeyError:
             raise RuntimeError("gradients must be bf16/fp16/fp32") from None
-        self.at = array("q", map(torch.Tensor.data_ptr, grads))
-        self.sizes = array("q", map(torch.Tensor.numel, grads))
+        self.at = array("q", [*map(torch.Tensor.data_ptr, grads)])
+        self.sizes = array("q", [*map(torch.Tensor.numel, grads)])
 
     def args(self):
         return self.at.buffer_info()[0], self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], len(self.at)
