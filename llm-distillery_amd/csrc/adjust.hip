@@ -15,7 +15,7 @@
 //
 // Bound by HBM where there are rows enough: 4096 x 50257 fp32, 512-token texts, a shared bias, 303 us (1.65 GB: 5.4 TB/s); 256 x 128256 bf16, texts of
 // 4096, masks that allow 30 %, 29 us (134 MB: 4.6 TB/s, the first tokens and the last pieces with nothing beside them); 8192 x 128256 bf16 with a bias's
-// gradient 900 us (4.2 GB and 0.27 GB of texts' logits: 5.0 TB/s).  One row of 32000 takes 4.6 us, the depth of its loads.  Tried at the second of these:
+// gradient 900 us (4.2 GB, 0.2 of logits at the texts' tokens, 0.13 of sums: 5.0 TB/s).  One row of 32000 takes 4.6 us, the depth of its loads.  Tried at the second of these:
 // the penalty computed in all columns and selected 54 us, a list of the text's columns that were claimed, gathered and scattered 70 (texts of
 // 16384: 1036 against 290), new values picked into registers by comparisons 34, 512 or 1024 threads with one or two pieces each level to 35.  Several rows
 // a workgroup for texts that rows share, so that a row adds only its own tokens' bits, is slower (the third 874 to 992 traced, as it is
