@@ -89,6 +89,7 @@ struct RowsParams {
   const unsigned char* b; int64_t b_stride; const float* sb; int64_t N;
   int blocks;
   char* out; int64_t out_stride;
+  int wide;                                                    // columns of the result that a small tile has, at most its BN
 };
 
 // 16 bytes a lane from `base` + `offset` into LDS, from `to` on in lane order (base and to: the wave's).  Said to the compiler as something that touches
@@ -126,11 +127,11 @@ __device__ __forceinline__ Piece row_piece(const unsigned char* lds, unsigned lo
 // share operands stay in step, and find them in the L2.
 __device__ __forceinline__ int first_block(unsigned tile, unsigned tiles_m, int blocks) { return tiles_m == 1 ? (int)(tile % (unsigned)blocks) : 0; }
 
-// A wave's values, from row m0 and column n0 of the result on.  Two-byte results go through 2 KiB of LDS of the wave's own, `stage`, 16 rows at a
+// A wave's values, from row m0 and column n0 of the result on, as far as column N.  Two-byte results go through 2 KiB of LDS of the wave's own, `stage`, 16 rows at a
 // time, so that a store writes whole 128-byte stretches of 8 rows instead of 32 bytes of 16; a row's 16-byte units are permuted by
 // unit ^ (row % 8).
 template <class Tag, int TM, int TN>
-__device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int lane, unsigned char* stage,
+__device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int64_t N, int lane, unsigned char* stage,
                                            const float* sa_here = nullptr, const float* sb_here = nullptr) {
   asm volatile("" : "+v"(lane));                               // (keeps the stores' addresses out of the steps' registers)
   const int row = lane % 16, quad = lane / 16;
@@ -142,6 +143,12 @@ __device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&ac
   float sas[TM];                                               // (all ahead of the first store, which a load behind it would wait for)
 #pragma unroll
   for (int i = 0; i < TM; ++i) sas[i] = sa_here ? sa_here[i * 16 + row] : p.sa[min(m0 + i * 16 + row, p.M - 1)];
+  // (Waited for here, and in all lanes: loads that one without anything to store left unused would be waited for in the next tile's steps, as soon as their
+  // registers are written again, and with them the steps' fetches: 64 x 8000 x 4096 11.6 us, so 24.)
+#pragma unroll
+  for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(sas[i]));
+#pragma unroll
+  for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(sb[j]));
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const float sa = sas[i];
@@ -164,8 +171,8 @@ __device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&ac
         const int64_t m = m0 + i * 16 + k * 8 + r8;
         const u32x4 c = *reinterpret_cast<const u32x4*>(stage + (k * 8 + r8) * 128 + (unit ^ r8) * 16);
         char* to = p.out + (m * p.out_stride + n) * 2;
-        if (m < p.M && n + 8 <= p.N) store16_stream_any(to, c);
-        else if (m < p.M && n < p.N) store_chunk_elementwise<Tag>(to, 0, (int)(p.N - n), c);
+        if (m < p.M && n + 8 <= N) store16_stream_any(to, c);
+        else if (m < p.M && n < N) store_chunk_elementwise<Tag>(to, 0, (int)(N - n), c);
       }
     } else {
       const int64_t m = m0 + i * 16 + row;
@@ -173,7 +180,7 @@ __device__ __forceinline__ void store_tile(const RowsParams& p, const i32x4 (&ac
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int64_t n = n0 + j * 16 + quad * 4;
-        if (m < p.M && n < p.N) store_four<Tag>(to, n, p.N, v[j]);
+        if (m < p.M && n < N) store_four<Tag>(to, n, N, v[j]);
       }
     }
   }
@@ -322,7 +329,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE, 2) void rows_kernel(c
       }
     }
     const float* scales = reinterpret_cast<const float*>(lds + SCALES) + which * (BM + BN);
-    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + STAGE + w * 2048, scales + wm, scales + BM + wn);
+    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, p.N, lane, lds + STAGE + w * 2048, scales + wm, scales + BM + wn);
   }
 }
 
@@ -346,7 +353,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_ring_kernel
     int64_t m, n;
     walk.origin(f_tile, m, n);
     m *= BM;
-    n *= BN;
+    n *= p.wide;
     f_left = p.blocks;
     f_kb = first_block(f_tile, tiles_m, p.blocks);
     f_a = p.a + m * p.a_stride + (int64_t)f_kb * KB;
@@ -359,7 +366,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_ring_kernel
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int row = (i * WAVES + w) * 8 + lane / 8, piece = (lane & 7) ^ ((row >> 1) & 7);
-      f_bo[i] = (unsigned)(min((int64_t)row, p.N - 1 - n) * p.b_stride) + piece * 16;
+      f_bo[i] = (unsigned)(min((int64_t)row, min((int64_t)p.wide, p.N - n) - 1) * p.b_stride) + piece * 16;
     }
   };
   const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((lds_words)lds);
@@ -394,7 +401,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_ring_kernel
     int64_t m0, n0;
     walk.origin(tile, m0, n0);
     m0 *= BM;
-    n0 *= BN;
+    n0 *= p.wide;
     i32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -425,7 +432,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * WAVE) void rows_ring_kernel
         for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j].hi, af[i].hi, acc[i][j], 0, 0, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, lane, lds + S * STEP + w * 2048);
+    store_tile<Tag, TM, TN>(p, acc, m0 + wm, n0 + wn, min(p.N, n0 + p.wide), lane, lds + S * STEP + w * 2048);
   }
 }
 
@@ -457,10 +464,20 @@ static int launch_row_tiles(const RowsParams& p, hipStream_t st) {
   return rows_status();
 }
 
+// Columns of a small tile: as many tiles a CU as whole ones make, all of a width, so that no CU has more weights to fetch than others (61 rows, from memory,
+// us for whole tiles / even ones: x 32896 x 2048 21.0 / 19.8, x 50257 x 2048 25.4 / 24.0, x 65664 x 2048 34.4 / 30.4; 33 x 40000 x 4096 37.0 / 33.5; 8 x 14336 x 4096 14.6 /
+// 13.6).  The places behind them are filled with the last row again: leaving them out costs branches and waits by count (64 x 8000 x 4096 11.5, so 14).
+static int ring_wide(int64_t tm, int64_t N, int BN) {
+  const int64_t each = (tm * ((N + BN - 1) / BN) + 255) / 256, across = std::max<int64_t>(1, 256 * each / tm);
+  return (int)std::min<int64_t>(BN, ((N + across - 1) / across + 7) / 8 * 8);
+}
+
 template <class Tag, int BM, int BN, int WM, int WN, int S>
-static int launch_row_ring(const RowsParams& p, hipStream_t st) {
+static int launch_row_ring(RowsParams p, hipStream_t st) {
   constexpr int threads = (BM / WM) * (BN / WN) * WAVE, bytes = S * (BM + BN) * KB + threads / WAVE * (WN == 64 && Tag::bytes == 2 ? 2048 : 0), per_cu = 160 * 1024 / bytes;
-  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+  const int64_t tm = (p.M + BM - 1) / BM;
+  p.wide = ring_wide(tm, p.N, BN);
+  const int64_t tn = (p.N + p.wide - 1) / p.wide;
   if (tm * tn > 0x7ffffff0LL || p.a_stride * BM > 0xffffffffLL || p.b_stride * BN > 0xffffffffLL) return DL_ERR_LIMIT;
   if (bytes > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(&rows_ring_kernel<Tag, BM, BN, WM, WN, S>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)

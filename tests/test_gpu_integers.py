@@ -86,6 +86,15 @@ def test_large_tiles_bit_for_bit(D, M, N, W):
     assert torch.equal(got, want.half())
 
 
+@pytest.mark.parametrize("M,N,W", [(61, 32896, 128), (61, 50257, 256), (1, 65664, 130), (33, 20011, 300), (8, 14337, 128), (130, 9001, 640), (64, 4099, 1000), (299, 5391, 257)])
+def test_even_small_tiles_bit_for_bit(D, M, N, W):
+    """Small tiles of fewer columns than they have room for, several a compute unit."""
+    a, b = codes(M, W, M), codes(N, W, N)
+    for dtype in (torch.float32, torch.bfloat16):
+        got, want = product(D, a, b, W, dtype)
+        assert torch.equal(got, want.to(dtype))
+
+
 @pytest.mark.parametrize("M,N", [(1, 7), (40, 200), (300, 300)])
 def test_the_largest_sums(D, M, N):
     """The widest rows of the largest codes, -128 among them: sums of up to 2^31 - 2^21."""
