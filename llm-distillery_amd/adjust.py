@@ -9,7 +9,7 @@ import torch
 from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _lib
-from .ops import _DT, _IT, _dev, _on, _row_pitch, _rows_2d, _share_memory, _stream_ptr
+from .ops import _DT, _IT, _dev, _on, _rows_2d, _share_memory, _stream_ptr
 from .rollout import _row_vector
 
 Number = Union[float, torch.Tensor]
@@ -30,7 +30,7 @@ def _logit_rows(t: torch.Tensor, name: str, dev: Optional[torch.device] = None) 
 
 def _per_row(v: Number, rows: int, name: str, dev: torch.device) -> Tuple[Optional[torch.Tensor], float]:
     """A setting as (one fp32 entry per row, 0) or (nothing, the number for all)."""
-    return (None, v) if type(v) is float else (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
+    return (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
 
 
 def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], rows: int, dev: torch.device) -> Tuple[tuple, tuple]:
@@ -82,10 +82,6 @@ def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor]
     return (m.data_ptr(), pitch if n > 1 else held, n, allowed_rows.data_ptr() if allowed_rows is not None else 0), (m, allowed_rows)
 
 
-def _row_lengths(lengths: Optional[torch.Tensor], rows: int, dev: torch.device) -> Optional[torch.Tensor]:
-    return None if lengths is None else _row_vector(lengths, rows, torch.int32, "lengths", dev)
-
-
 def _written(out: Optional[torch.Tensor], x: torch.Tensor, name: str, over: str, others: tuple = ()) -> torch.Tensor:
     """The matrix that the result goes to: new, or `out` checked -- `x` itself, or memory that neither `x` nor `others` have."""
     if out is None:
@@ -98,10 +94,6 @@ def _written(out: Optional[torch.Tensor], x: torch.Tensor, name: str, over: str,
     if not same and _share_memory(o, x) or any(_share_memory(o, t) for t in others):
         raise RuntimeError(f"{name} must be {over} itself or share no memory with the arguments")
     return o
-
-
-def _address(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
 
 
 def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, token_rows: Optional[torch.Tensor] = None,
@@ -128,11 +120,12 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     R, V = x.shape
     dev = x.device
     (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
-    lengths = _row_lengths(lengths, R, dev)
+    if lengths is not None:
+        lengths = _row_vector(lengths, R, torch.int32, "lengths", dev)
     prompt_rows, prompt_all = (_row_vector(prompt, R, torch.int32, "prompt", dev), 0) if isinstance(prompt, torch.Tensor) else (None, int(prompt))
-    rep, rep_all = _per_row(repetition, R, "repetition", dev)
-    freq, freq_all = _per_row(frequency, R, "frequency", dev)
-    pres, pres_all = _per_row(presence, R, "presence", dev)
+    rep, rep_all = (None, repetition) if type(repetition) is float else _per_row(repetition, R, "repetition", dev)
+    freq, freq_all = (None, frequency) if type(frequency) is float else _per_row(frequency, R, "frequency", dev)
+    pres, pres_all = (None, presence) if type(presence) is float else _per_row(presence, R, "presence", dev)
     if rep is None and not 0.0 < rep_all <= 3.0e38:
         raise ValueError("repetition must be positive and finite")
     b_ptr = b_dtype = b_stride = 0
@@ -151,9 +144,10 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
         others = (b if b.dim() == 2 else b.unsqueeze(0),)
     res = _written(out, x, "out", "the logits", others)
     with _on(dev):
-        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], x.stride(0) if R > 1 else V, R, V, *text, _address(lengths), _address(prompt_rows),
-                                        prompt_all, _address(rep), _address(freq), _address(pres), rep_all, freq_all, pres_all, b_ptr, b_dtype,
-                                        b_stride, *mask, res.data_ptr(), res.stride(0) if R > 1 else V, _stream_ptr(dev))
+        st = _lib.load().dl_adjust_rows(x.data_ptr(), _DT[x.dtype], x.stride(0) if R > 1 else V, R, V, *text, 0 if lengths is None else lengths.data_ptr(),
+                                        0 if prompt_rows is None else prompt_rows.data_ptr(), prompt_all, 0 if rep is None else rep.data_ptr(),
+                                        0 if freq is None else freq.data_ptr(), 0 if pres is None else pres.data_ptr(), rep_all, freq_all, pres_all,
+                                        b_ptr, b_dtype, b_stride, *mask, res.data_ptr(), res.stride(0) if R > 1 else V, _stream_ptr(dev))
     if st:
         _lib.check(st, "dl_adjust_rows")
     return out if out is not None else res if logits.dim() == 2 else res.view(logits.shape)
@@ -175,8 +169,9 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     R, V = g.shape
     dev = g.device
     (text, alive), (mask, alive_too) = _texts(tokens, token_rows, R, dev), _masks(allowed, allowed_rows, R, V, dev)
-    lengths = _row_lengths(lengths, R, dev)
-    rep, rep_all = _per_row(repetition, R, "repetition", dev)
+    if lengths is not None:
+        lengths = _row_vector(lengths, R, torch.int32, "lengths", dev)
+    rep, rep_all = (None, repetition) if type(repetition) is float else _per_row(repetition, R, "repetition", dev)
     if rep is None and not 0.0 < rep_all <= 3.0e38:
         raise ValueError("repetition must be positive and finite")
     if bias_dtype not in (torch.float32, g.dtype):
@@ -196,10 +191,13 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     ws_bytes = lib.dl_adjust_grad_workspace_bytes(R, V) if want_bias else 0
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with _on(dev):
-        st = lib.dl_adjust_grad(g.data_ptr(), _DT[g.dtype], _row_pitch(g), _address(x), 0 if x is None else _row_pitch(x), R, V, *text,
-                                _address(lengths), _address(rep), rep_all, *mask, _address(res), 0 if res is None else _row_pitch(res),
-                                _address(by_bias), _DT[bias_dtype], _address(ws), ws_bytes, _stream_ptr(dev))
-    _lib.check(st, "dl_adjust_grad")
+        st = lib.dl_adjust_grad(g.data_ptr(), _DT[g.dtype], g.stride(0) if R > 1 else V, 0 if x is None else x.data_ptr(),
+                                0 if x is None else x.stride(0) if R > 1 else V, R, V, *text, 0 if lengths is None else lengths.data_ptr(),
+                                0 if rep is None else rep.data_ptr(), rep_all, *mask, 0 if res is None else res.data_ptr(),
+                                0 if res is None else res.stride(0) if R > 1 else V, 0 if by_bias is None else by_bias.data_ptr(),
+                                _DT[bias_dtype], 0 if ws is None else ws.data_ptr(), ws_bytes, _stream_ptr(dev))
+    if st:
+        _lib.check(st, "dl_adjust_grad")
     return (out if out is not None else res if not want_logits or grad.dim() == 2 else res.view(grad.shape)), by_bias
 
 
