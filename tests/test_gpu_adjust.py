@@ -439,6 +439,33 @@ def test_captured_calls_replay(D):
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+def test_a_captured_training_step_replays(D):
+    """`adjust_logits` and its backward pass in one graph, as a training loop captures them: warmed up on a side stream, no eager graph alive."""
+    R, V, L = 40, 5003, 30
+    g = torch.Generator(device=DEV).manual_seed(37)
+    x, b = torch.randn(R, V, generator=g, device=DEV, requires_grad=True), torch.randn(V, generator=g, device=DEV, requires_grad=True)
+    t, up = torch.randint(V, (R, L), generator=g, device=DEV), torch.randn(R, V, generator=g, device=DEV)
+
+    def step():
+        y = D.adjust_logits(x, t, repetition=1.3, presence=0.5, bias=b)
+        return (y.detach(), *torch.autograd.grad(y, (x, b), up))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.normal_(generator=g), b.normal_(generator=g), t.random_(0, V, generator=g), up.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(outs, step()))
+
+
 def test_another_stream(D):
     x, t = torch.randn(20, 9000, device=DEV), torch.randint(9000, (20, 100), device=DEV)
     want = D.adjust_rows(x, t, repetition=1.2)
