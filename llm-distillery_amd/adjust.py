@@ -47,7 +47,7 @@ def _texts(tokens: Optional[torch.Tensor], token_rows: Optional[torch.Tensor], r
     if t.dim() != 2:
         if t.dim() == 0:
             raise RuntimeError("tokens must be [..., length]")
-        t = t.unsqueeze(0) if t.dim() == 1 else t.reshape(-1, t.shape[-1])
+        t = t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
     (n, length), (pitch, one) = t.shape, t.stride()
     if one != 1 and length > 1:
         t, pitch = t.contiguous(), length
@@ -71,7 +71,7 @@ def _masks(allowed: Optional[torch.Tensor], allowed_rows: Optional[torch.Tensor]
     if m.dtype != torch.int32 or m.dim() < 2 or m.shape[-1] < words:
         raise RuntimeError(f"allowed must be int32 [masks, {words}], one bit for each of the {V} tokens")
     if m.dim() > 2:
-        m = m.reshape(-1, m.shape[-1])
+        m = m.flatten(0, -2)
     (n, held), (pitch, one) = m.shape, m.stride()
     if one != 1 and held > 1 or pitch < words and n > 1:
         m, pitch = m.contiguous(), held

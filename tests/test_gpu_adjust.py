@@ -634,3 +634,15 @@ def test_the_example_writes_and_learns_under_penalties():
     # an fp32 rounding, and one to bf16, whose eight significant bits leave at most half a step, 2^-8 of the value
     bound = (HALF_ULP[torch.bfloat16] + 2.0 ** -24) * want.abs() * (1 + 2.0 ** -20) + STEP[torch.bfloat16]
     assert ((logits.grad.double() - want).abs() <= bound).all()
+
+
+def test_empty_texts_and_rows(D):
+    """Texts of no tokens, in any shape, and logits of no rows."""
+    x = torch.randn(2, 3, 100, device=DEV)
+    for t in (torch.empty((2, 3, 0), dtype=torch.int64, device=DEV), torch.empty((6, 0), dtype=torch.int32, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV)):
+        assert torch.equal(D.adjust_rows(x, t, repetition=2.0, presence=1.0), x)
+        assert torch.equal(D.adjust_grad(x, x, t, repetition=2.0)[0], x)
+    none = torch.empty((0, 100), device=DEV)
+    assert D.adjust_rows(none, torch.empty((0, 5), dtype=torch.int64, device=DEV), repetition=2.0).shape == (0, 100)
+    rows, by_bias = D.adjust_grad(none, want_bias=True)
+    assert rows.shape == (0, 100) and by_bias.count_nonzero().item() == 0 and by_bias.shape == (100,)
