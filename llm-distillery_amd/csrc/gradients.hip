@@ -144,14 +144,28 @@ __device__ __forceinline__ double norm_of(const double* sums, unsigned n, float 
   for (; i < n; i += GRAD_NT) v += sums[i];
   return sqrt(block_total(v, scratch)) * (double)scale;
 }
-__global__ __launch_bounds__(GRAD_NT) void norm_kernel(const double* sums, unsigned n, float scale, float* norm) {
+// `keep`: where the norm goes as it is, over the sums.
+__global__ __launch_bounds__(GRAD_NT) void norm_kernel(double* sums, unsigned n, float scale, float* norm, bool keep) {
   __shared__ double scratch[GRAD_NT / WAVE];
-  const double v = norm_of(sums, n, scale, scratch);
-  if (threadIdx.x == 0) norm[0] = (float)v;
+  const double v = norm_of(sums, n, scale, scratch);           // (all have read theirs)
+  if (threadIdx.x == 0) {
+    norm[0] = (float)v;
+    if (keep) sums[0] = v;
+  }
 }
 
+// f times a factor of 64 bits, held as the sum of two of 32: the one rounding that shows is the result's (a factor rounded to 32 bits would be off by up to
+// 2^-24 in all elements alike).
+struct GradFactor {
+  float hi, lo;
+  __device__ __forceinline__ explicit GradFactor(double by) : hi((float)by), lo((float)(by - (double)(float)by)) {}
+  __device__ __forceinline__ float times(float f) const {
+    const float rest = f * lo;
+    return fmaf(f, hi, fabsf(rest) <= 3.402823466e38f ? rest : 0.f);
+  }
+};
 template <class Tag>
-__device__ __forceinline__ void scale_piece(const GradPiece& p, float by) {
+__device__ __forceinline__ void scale_piece(const GradPiece& p, const GradFactor& by) {
   constexpr int N = Chunk<Tag>::N;
   u32x4 v[GRAD_NCH];
 #pragma unroll
@@ -164,23 +178,24 @@ __device__ __forceinline__ void scale_piece(const GradPiece& p, float by) {
     float f[N];
     Chunk<Tag>::unpack(v[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] *= by;
+    for (int e = 0; e < N; ++e) f[e] = by.times(f[e]);
     if (grad_chunk(i) < p.chunks) store16_stream(p.body + grad_chunk(i) * 16, Chunk<Tag>::pack(f));
   }
   for (int side = 0; side < 2; ++side)
     if ((int)threadIdx.x < (side ? p.n_behind : p.n_ahead)) {
       char* at = side ? p.behind : p.ahead;
-      store_from_float(at, Tag::id, threadIdx.x, load_as_float(at, Tag::id, threadIdx.x) * by);
+      store_from_float(at, Tag::id, threadIdx.x, by.times(load_as_float(at, Tag::id, threadIdx.x)));
     }
 }
-// `sums`: the norm is theirs, and is written; else it is there.
+// The norm: of `n_sums` sums, and is written; or (none) the first of them; or (no `sums`) given.
 __global__ __launch_bounds__(GRAD_NT, 4) void scale_kernel(const GradTable t, const double* sums, unsigned n_sums, float scale, float max_norm, float* norm) {
   __shared__ GradFind found;
   __shared__ double scratch[GRAD_NT / WAVE];
-  const double all = sums ? norm_of(sums, n_sums, scale, scratch) : (double)norm[0];
-  if (sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
-  const float by = (float)(all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale);
-  if (!((float)all <= 3.402823466e38f) || by == 1.f) return;   // NaN or, as fp32 shows it, infinite: left as they are
+  const double all = !sums ? (double)norm[0] : n_sums ? norm_of(sums, n_sums, scale, scratch) : sums[0];
+  if (n_sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
+  const double factor = all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale;
+  if (!((float)all <= 3.402823466e38f) || factor == 1.0) return;      // NaN or, as fp32 shows it, infinite: left as they are
+  const GradFactor by(factor);
   const unsigned q = t.pieces - 1u - blockIdx.x;
   find_entry(t, q, found);
   const GradPiece p = piece_of(found, q);
@@ -275,7 +290,7 @@ extern "C" int dl_grad_norm(const void* const* tensors, const int64_t* sizes, co
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   double* sums = reinterpret_cast<double*>(workspace);
   const unsigned n = launch_squares(tensors, sizes, dtypes, n_tensors, sums, st);
-  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(GRAD_NT), 0, st, sums, n, scale, norm);
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(GRAD_NT), 0, st, sums, n, scale, norm, false);
   return gradients_status();
 }
 
@@ -293,8 +308,8 @@ extern "C" int dl_clip_grads(void* const* tensors, const int64_t* sizes, const i
   if (!norm_given) {
     n = launch_squares(tensors, sizes, dtypes, n_tensors, sums, st);
     if (n == 0 || n > FEW_SUMS) {
-      hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(GRAD_NT), 0, st, sums, n, scale, norm);
-      sums = nullptr;
+      hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(GRAD_NT), 0, st, sums, n, scale, norm, n > 0);
+      n = 0;
     }
   }
   for_tables(tensors, sizes, dtypes, n_tensors, [&](const GradTable& t, unsigned) {

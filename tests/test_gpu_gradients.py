@@ -96,6 +96,22 @@ def test_large_and_small_values(D):
     assert D.clip_grads(ones, 0.0).item() == 10 and (ones[0] == 0).all()      # nothing is allowed
 
 
+@pytest.mark.parametrize("sizes", [(1000, 77), (40_000_001,)])
+def test_the_one_rounding_is_the_results(D, sizes):
+    """fp32 gradients by a factor of 64 bits: half a step of the result.  (What the factor, held in two floats, and the sum of the parts leave off
+    is some 2^-46 of it; the sums of squares in 64 bits, pairwise here and there, agree to some 2^-48: together below 2^-24 * 2^-16.)"""
+    grads = some(sizes, 9, (torch.float32,))
+    for share, scale in ((0.3, 1.0), (1 / 7, 3.3), (2.0, 0.7)):
+        scale = torch.tensor(scale).item()                    # (as fp32 has it)
+        norm = exact_norm(grads) * scale
+        most = torch.tensor(norm * share).item()
+        now = [g.clone() for g in grads]
+        D.clip_grads(now, most, scale=scale)
+        for a, b in zip(now, grads):
+            want = b.double() * (scale * min(1.0, most / norm))
+            assert ((a.double() - want).abs() <= 2.0 ** -24 * want.abs() * (1 + 2.0 ** -16) + 2.0 ** -149).all()
+
+
 @pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
 def test_a_norm_that_is_no_number_leaves_the_gradients(D, odd):
     grads = some((100, 20000, 3), 5)
