@@ -9,7 +9,7 @@
 // The second pass has a workgroup for every piece, the last piece first: what was read last may still be in MALL.
 // Bound by HBM: 1.2 billion bf16 elements (2.4 GB) 1165 us, of it the squares 353 (6.8 TB/s), their sum 5, the product 805 (5.9 TB/s read and written: a
 // copy of the size by the library reaches 4.9); 203 million fp32 elements of odd sizes, only read, 128 us, the squares 119 to 124.  Few small tensors
-// (1 million elements in 11): 4.5 and 2.4 us on the card, and what the host needs for two launches.  Tried at the first of these: every workgroup
+// (1 million elements in 11): 5 and 8 us on the card, less than the host needs for two launches.  Tried at the first of these: every workgroup
 // a contiguous share of all 1261 us, long-lived workgroups that take every so many-th piece in the second pass 1245, its stores kept in the caches 1322, half
 // as many chunks a thread 1361.
 #include "distill_common.hpp"
@@ -194,7 +194,8 @@ __global__ __launch_bounds__(GRAD_NT, 4) void scale_kernel(const GradTable t, co
   const double all = !sums ? (double)norm[0] : n_sums ? norm_of(sums, n_sums, scale, scratch) : sums[0];
   if (n_sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
   const double factor = all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale;
-  if (!((float)all <= 3.402823466e38f) || factor == 1.0) return;      // NaN or, as fp32 shows it, infinite: left as they are
+  if (!((float)all <= 3.402823466e38f)) return;                // NaN or, as fp32 shows it, infinite: left as they are
+  if (fabs(factor - 1.0) <= 0x1p-25) return;                   // less than half a step of any element: they would stay what they are
   const GradFactor by(factor);
   const unsigned q = t.pieces - 1u - blockIdx.x;
   find_entry(t, q, found);
