@@ -32,8 +32,11 @@ class _Tensors:
         self.all = grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
         if not grads:
             raise RuntimeError("no gradients")
-        self.dev = dev = grads[0].device
-        usual = dev.type == "cuda" and {*map(torch.Tensor.get_device, grads)} == {dev.index} and all(map(torch.Tensor.is_contiguous, grads))
+        try:
+            self.dev = dev = grads[0].device
+            usual = {*map(torch.Tensor.get_device, grads)} == {dev.index} and all(map(torch.Tensor.is_contiguous, grads))
+        except (AttributeError, TypeError):
+            raise RuntimeError("gradients must be tensors (leave out parameters that have none)") from None
         for g in grads if not usual else ():
             if g.device != dev or not g.is_cuda or g.layout is not torch.strided:
                 _dev(g, "a gradient", dev if dev.type == "cuda" else None)

@@ -99,6 +99,13 @@ def test_no_cpu_path():
             call()
 
 
+def test_parameters_without_a_gradient_are_refused():
+    import pytest
+    for grads in ([None], [torch.ones(3), None], [], ()):
+        with pytest.raises(RuntimeError, match="no gradients|must be tensors"):
+            D.clip_grads(grads, 1.0)
+
+
 def test_adjusted_logits_trace_with_fake_tensors_in_both_directions():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
