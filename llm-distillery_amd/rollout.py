@@ -182,7 +182,8 @@ def quantize_rows(x: torch.Tensor) -> RowQuantized:
     [-127, 127].  A row with a NaN or an infinity has a scale of NaN."""
     _dev(x, "x")
     v = x if x.dim() == 2 and x.stride(1) == 1 else _rows_2d(x if x.dim() > 1 else x.unsqueeze(0))
-    if v.dtype not in _DT:
+    kind = _DT.get(v.dtype)
+    if kind is None:
         raise RuntimeError("unsupported dtype")
     (R, W), pitch = v.shape, v.stride(0)
     if R <= 1:
@@ -190,28 +191,28 @@ def quantize_rows(x: torch.Tensor) -> RowQuantized:
     elif pitch < W:
         raise RuntimeError("x: rows overlap; make them contiguous first")
     dev = v.device
-    wide = _blocks(W) * 128
+    wide = (W + 127) // 128 * 128
     codes = v.new_empty(R, wide, dtype=torch.int8)
     scales = v.new_empty(R, dtype=torch.float32)
     if R and W:
         with _on(dev):
-            st = _lib.load().dl_quantize_rows(v.data_ptr(), _DT[v.dtype], pitch, R, W, codes.data_ptr(), wide, scales.data_ptr(),
-                                              _stream_ptr(dev))
-        _lib.check(st, "dl_quantize_rows")
+            st = _lib.load().dl_quantize_rows(v.data_ptr(), kind, pitch, R, W, codes.data_ptr(), wide, scales.data_ptr(), _stream_ptr(dev))
+        if st:
+            _lib.check(st, "dl_quantize_rows")
     return RowQuantized(codes, scales, W)
 
 
-def _check_rows(q: RowQuantized, name: str, wide: int, dev: torch.device):
-    """(address, row stride) of the codes and the address of the scales of an operand."""
-    codes, scales = q.codes, q.scales
-    if codes.get_device() != dev.index or scales.get_device() != dev.index:
+def _check_rows(codes: torch.Tensor, scales: torch.Tensor, name: str, wide: int, dev: torch.device):
+    """(address, row stride) of the codes and the address of the scales of an operand, and how many rows it has."""
+    here = dev.index
+    if codes.get_device() != here or scales.get_device() != here:
         _dev(codes, f"{name}.codes", dev), _dev(scales, f"{name}.scales", dev)
     (rows, columns), (pitch, one) = codes.shape, codes.stride()
     if codes.dtype != torch.int8 or columns != wide or rows and (one != 1 or rows > 1 and pitch < wide):
         raise RuntimeError(f"{name}.codes must be an int8 matrix of whole blocks of 128 columns, dense along its rows")
     if scales.dtype != torch.float32 or scales.dim() != 1 or scales.numel() != rows or rows > 1 and not scales.is_contiguous():
         raise RuntimeError(f"{name}.scales must be a contiguous fp32 vector of {rows} entries")
-    return codes.data_ptr(), pitch if rows > 1 else wide, scales.data_ptr()
+    return codes.data_ptr(), pitch if rows > 1 else wide, scales.data_ptr(), rows
 
 
 def matmul_rows(a: RowQuantized, b: RowQuantized, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -220,22 +221,23 @@ def matmul_rows(a: RowQuantized, b: RowQuantized, *, dtype: torch.dtype = torch.
 
     Sums of products are exact; a sum becomes a float, is multiplied with the product of the two scales (each rounded in fp32), and the result is
     rounded once.  A row's result has the same bits whatever rows it comes with.  Up to 130944 columns."""
-    dev, kind = a.codes.device, _DT.get(dtype)
+    (a_codes, a_scales, W), (b_codes, b_scales, b_width), kind = a, b, _DT.get(dtype)
     if kind is None:
         raise RuntimeError("unsupported dtype")
-    if a.codes.dim() != 2 or b.codes.dim() != 2:
+    if a_codes.dim() != 2 or b_codes.dim() != 2:
         raise RuntimeError("codes must be matrices")
-    M, N, W = a.codes.shape[0], b.codes.shape[0], a.width
-    if W != b.width:
-        raise RuntimeError(f"a has {W} columns, b {b.width}")
+    if W != b_width:
+        raise RuntimeError(f"a has {W} columns, b {b_width}")
     if W <= 0:
         raise RuntimeError("the rows have no columns")
-    _dev(a.codes, "a.codes")
-    a_ptr, a_pitch, a_scale = _check_rows(a, "a", _blocks(W) * 128, dev)
-    b_ptr, b_pitch, b_scale = _check_rows(b, "b", _blocks(W) * 128, dev)
-    out = a.codes.new_empty(M, N, dtype=dtype)
+    _dev(a_codes, "a.codes")
+    dev, wide = a_codes.device, (W + 127) // 128 * 128
+    *left, M = _check_rows(a_codes, a_scales, "a", wide, dev)
+    *right, N = _check_rows(b_codes, b_scales, "b", wide, dev)
+    out = a_codes.new_empty(M, N, dtype=dtype)
     if M and N:
         with _on(dev):
-            st = _lib.load().dl_matmul_rows(a_ptr, a_pitch, a_scale, M, b_ptr, b_pitch, b_scale, N, W, out.data_ptr(), kind, N, _stream_ptr(dev))
-        _lib.check(st, "dl_matmul_rows")
+            st = _lib.load().dl_matmul_rows(*left, M, *right, N, W, out.data_ptr(), kind, N, _stream_ptr(dev))
+        if st:
+            _lib.check(st, "dl_matmul_rows")
     return out
