@@ -686,7 +686,7 @@ int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t n_tokens, 
  * allowed    [n_masks, words] (`allowed_stride` words a row, at least V / 32 rounded up); NULL: all tokens are.  Row r has mask allowed_rows[r]
  *            (outside [0, n_masks): none, all tokens are allowed); without allowed_rows mask r, or mask 0 where there is one only.
  * out        [n_rows, V] of the logits' dtype; it may be the logits themselves (the same address and stride), else they do not overlap.
- * V and length below 2^31 (DL_ERR_LIMIT); any element-aligned pointers and strides.
+ * V below 2^31, length up to 2^31 - 8192 (DL_ERR_LIMIT); any element-aligned pointers and strides.
  *
  * dl_adjust_grad: the gradient.  g: [n_rows, V] of the logits' dtype, by y.
  *   out[r, v]    = 0 where masked, else g / repetition or g * repetition at the text's tokens by the sign of x, else g     (NULL: not wanted)

@@ -110,6 +110,10 @@ struct FourTokens {
     else return v[e / 2][e % 2 * 2 + 1] ? ~0u : v[e / 2][e % 2 * 2];
   }
 };
+// A thread has as many of these at a time.  A text's places are 32-bit numbers, and the last step of the largest workgroup passes its end by
+// less than a step: beyond LENGTH_MOST tokens that would pass 2^31 - 1.
+constexpr int NTOK = 2;
+constexpr int64_t LENGTH_MOST = (1LL << 31) - 1024 * NTOK * 4;
 __device__ const unsigned NOTHING[4] = {0u, 0u, 0u, 0u};       // in the place of a row too short for a piece
 typedef const char __attribute__((address_space(1))) * global_bytes;      // (said to be global, so that a choice of two is no load of any kind of memory)
 
@@ -119,7 +123,8 @@ typedef const char __attribute__((address_space(1))) * global_bytes;      // (sa
 // spill).
 template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
 __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, float* sums) {
-  constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = 2;   // (tokens of a thread at a time: four times NTOK)
+  static_assert(NT <= 1024, "LENGTH_MOST");
+  constexpr int N = Chunk<Tag>::N, B = Tag::bytes;
   extern __shared__ __align__(16) unsigned lds[];              // for each column a bit, its new value, and a counter or (GRAD) the logit
   const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a run on one XCD
   const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + k * p.run, last = min(first + p.run, p.n_rows);
@@ -385,7 +390,7 @@ static int adjust_check(const AdjustParams& p, int dtype) {
   if (p.n_texts > 0 && (p.token_stride < 0 || (p.n_texts > 1 && !p.token_rows && p.n_texts < p.n_rows))) return DL_ERR_SHAPE;
   if (p.n_masks > 0 && (p.allowed_stride < (p.V + 31) / 32 || (p.n_masks > 1 && !p.allowed_rows && p.n_masks < p.n_rows))) return DL_ERR_SHAPE;
   if (p.bias && p.bias_stride != 0 && p.bias_stride < p.V) return DL_ERR_SHAPE;
-  if (p.V > 0x7fffffffLL || p.length > 0x7fffffffLL) return DL_ERR_LIMIT;
+  if (p.V > 0x7fffffffLL || p.length > LENGTH_MOST) return DL_ERR_LIMIT;
   const uintptr_t eb = dtype == DL_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out)) % eb || reinterpret_cast<uintptr_t>(p.tokens) % (p.itype == I64 ? 8 : 4) ||
       reinterpret_cast<uintptr_t>(p.allowed) % 4 || reinterpret_cast<uintptr_t>(p.bias) % (p.bias_dtype == F32 ? 4 : 2))

@@ -52,6 +52,15 @@ def test_their_gradient():
     assert adjust_grad(V=0) == 0 and adjust_grad(n_rows=0, bias_grad=0) == 0
 
 
+def test_texts_whose_last_place_is_beyond_32_bits():
+    """The kernels count a text's places in 32 bits and step past its end by up to 8192: longer texts than 2^31 - 8192 are refused.  (Without logits: a
+    call whose length is accepted is refused for them.)"""
+    for length, status in ((2 ** 31 - 8192, -1), (2 ** 31 - 8191, -4), (2 ** 31 - 2048, -4), (2 ** 31 - 1, -4)):
+        for itype in (0, 1):
+            assert adjust(logits=0, itype=itype, n_texts=1, token_stride=length, length=length) == status
+            assert adjust_grad(logits=0, itype=itype, n_texts=1, token_stride=length, length=length) == status
+
+
 def test_integer_products():
     lib = D._lib.load()
     assert lib.dl_quantize_rows(P, 3, 256, 4, 256, P, 256, P, 0) == -2
