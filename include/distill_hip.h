@@ -691,8 +691,8 @@ int dl_embed_grad(const void* g, int dtype, int64_t g_stride, int64_t n_tokens, 
  * dl_adjust_grad: the gradient.  g: [n_rows, V] of the logits' dtype, by y.
  *   out[r, v]    = 0 where masked, else g / repetition or g * repetition at the text's tokens by the sign of x, else g     (NULL: not wanted)
  *   bias_grad[v] = sum over r of g[r, v] where not masked, fp32 or the logits' dtype: of a bias that all rows share       (NULL: not wanted)
- * out may be g itself.  logits: may be NULL where there is no text.  Sums are fp32 over runs of rows, these in fp64, always in the
- * same order.  workspace: dl_adjust_grad_workspace_bytes(...) bytes where bias_grad is wanted, 16-byte aligned, contents irrelevant; two calls
+ * out may be g itself.  logits: may be NULL where there is no text.  Sums are fp64, always in the same order, rounded once
+ * (through fp32 where bias_grad is of 16 bits).  workspace: dl_adjust_grad_workspace_bytes(...) bytes where bias_grad is wanted, 16-byte aligned, contents irrelevant; two calls
  * that may overlap in time must not share it.
  */
 int dl_adjust_rows(const void* logits, int dtype, int64_t row_stride, int64_t n_rows, int64_t V, const void* tokens, int itype,

@@ -110,21 +110,22 @@ struct FourTokens {
     else return v[e / 2][e % 2 * 2 + 1] ? ~0u : v[e / 2][e % 2 * 2];
   }
 };
-// A thread has as many of these at a time.  A text's places are 32-bit numbers, and the last step of the largest workgroup passes its end by
-// less than a step: beyond LENGTH_MOST tokens that would pass 2^31 - 1.
-constexpr int NTOK = 2;
-constexpr int64_t LENGTH_MOST = (1LL << 31) - 1024 * NTOK * 4;
+// A text's places are 32-bit numbers, and a workgroup's last step passes its end by less than STEP_MOST, the most tokens of a step: beyond LENGTH_MOST
+// tokens that would pass 2^31 - 1.
+constexpr int STEP_MOST = 8192;
+constexpr int64_t LENGTH_MOST = (1LL << 31) - STEP_MOST;
 __device__ const unsigned NOTHING[4] = {0u, 0u, 0u, 0u};       // in the place of a row too short for a piece
 typedef const char __attribute__((address_space(1))) * global_bytes;      // (said to be global, so that a choice of two is no load of any kind of memory)
 
 // `run` rows, one after the other, of a part of the columns.  SUMS (the gradient's): what they have in common, the gradient by a shared bias, is added
-// up on the way in fp32, one row of `sums` for every run.  Count: what a column's counter is held in, 16 bits where no text has more tokens than these count.
-// 16 KiB of a row a workgroup, four 16-byte pieces a thread; LDS and registers leave room for four such workgroups on a CU (asked for six or eight, values
-// spill).
+// up on the way, one row of `sums` for every run, in fp64: what shows is the result's rounding, and a sum on the way may be larger than fp32 holds.
+// Count: what a column's counter is held in, 16 bits where no text has more tokens than these count.
+// 16 KiB of a row a workgroup, four 16-byte pieces a thread (three where two-byte rows are added up); LDS and registers leave room for four such workgroups
+// on a CU (asked for six or eight, values spill).
 template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
-__global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, float* sums) {
-  static_assert(NT <= 1024, "LENGTH_MOST");
-  constexpr int N = Chunk<Tag>::N, B = Tag::bytes;
+__global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, double* sums) {
+  constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = SUMS ? 1 : 2;      // (tokens of a thread at a time: four times NTOK)
+  static_assert(NT * NTOK * 4 <= STEP_MOST, "places of 32 bits");
   extern __shared__ __align__(16) unsigned lds[];              // for each column a bit, its new value, and a counter or (GRAD) the logit
   const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a run on one XCD
   const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + k * p.run, last = min(first + p.run, p.n_rows);
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
   char* beside = values + p.part_columns * B;
   unsigned* counts = reinterpret_cast<unsigned*>(beside);
   const u32x4 masked = GRAD ? u32x4{0u, 0u, 0u, 0u} : Chunk<Tag>::neg_inf();
-  float total[SUMS ? NCH : 1][N] = {}, total_tail = 0.f;
+  double total[SUMS ? NCH : 1][N] = {}, total_tail = 0.0;
 #pragma unroll 1
   for (int64_t r = first; r < last; ++r) {
     const AdjustRow row(p, r);
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
           float f[N];
           Chunk<Tag>::unpack(v[i], f);
 #pragma unroll
-          for (int e = 0; e < N; ++e) total[i][e] += f[e];
+          for (int e = 0; e < N; ++e) total[i][e] += (double)f[e];
         }
       }
     const auto penalised = [&](float f, float sign, unsigned col) {
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
       const unsigned at = pieces * N + tid;
       const bool open = !bits || (bits[at >> 3] >> (at & 7u) & 1u);
       float f = open ? load_as_float(from, Tag::id, at) : 0.f;
-      if (SUMS) total_tail += f;
+      if (SUMS) total_tail += (double)f;
       if (!SUMS || p.out) {
         if (length > 0 && open && (said[at >> 3] >> (at & 7u) & 1u)) f = penalised(f, GRAD ? load_as_float(x, Tag::id, at) : f, at);
         if (!GRAD && bias) f += load_as_float(bias, p.bias_dtype, at);
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
     if (SUMS && length > 0) __syncthreads();                   // the bits are the next row's
   }
   if (SUMS) {
-    float* at = sums + (first / p.run) * p.V + c0;
+    double* at = sums + (first / p.run) * p.V + c0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
@@ -317,13 +318,13 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, flo
 }
 
 // The runs' sums, added up in fp64: 32 columns a workgroup, from `first` on, eight threads to a column, each every eighth run.
-__global__ __launch_bounds__(256) void bias_join_kernel(const float* sums, int64_t runs, int64_t first, int64_t V, void* out, int dtype) {
+__global__ __launch_bounds__(256) void bias_join_kernel(const double* sums, int64_t runs, int64_t first, int64_t V, void* out, int dtype) {
   __shared__ double part[8][32];
   const int lane = threadIdx.x % 32, slice = threadIdx.x / 32;
   const int64_t col = first + (int64_t)blockIdx.x * 32 + lane;
   double total = 0.0;
   if (col < V)
-    for (int64_t k = slice; k < runs; k += 8) total += (double)sums[k * V + col];
+    for (int64_t k = slice; k < runs; k += 8) total += sums[k * V + col];
   part[slice][lane] = total;
   __syncthreads();
   if (slice == 0 && col < V) {
@@ -336,49 +337,65 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* sums, int64
 static int adjust_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL_ERR_LAUNCH; }
 
 constexpr int ADJUST_NT = 256, ADJUST_NCH = 4;
+constexpr int SUMS_NT = 1024;
 
-// Rows whose sum goes to the workspace in one piece: enough workgroups, few pieces, no more than 65535 of them.  (64 rows of 8192 x 128256: 66 MB of
-// sums written and read again beside 4.2 GB, the join 13 us.)
-static int64_t sums_run(int64_t n_rows, int64_t V) {
-  return std::max(std::max<int64_t>(4, std::min<int64_t>(64, n_rows * ((V + 8191) / 8192) / 2048)), (n_rows + 65534) / 65535);
-}
+// What a call that adds up rows is cut into: the threads of a workgroup and their pieces, and the rows whose sums go to the workspace together.
+//
+// Totals in fp64 take two registers a column: two-byte rows have three pieces a thread (four spill: 8192 x 128256 bf16 1040 us, so 975).  Four-byte rows whose columns
+// fill the parts of 1024 threads take these (4096 x 128256 fp32 825 us, with 256 threads 850), not few rows or parts three quarters full.
+// Runs are as long as leaves every CU its workgroups -- one round of these, or up to four while a run is longer than SUMS_ROWS rows, whose texts differ
+// in length: 512 x 128256 bf16 in one round 83 us, in two 96, in four 107, of its bytes more and more sums; 8192 x 128256 1000, 972, 989.
+struct SumsCut {
+  bool wide;
+  int64_t run;
+  SumsCut(int64_t n_rows, int64_t V, int bytes) {
+    constexpr int64_t WIDE = (int64_t)SUMS_NT * ADJUST_NCH * 4, SUMS_ROWS = 100;
+    wide = bytes == 4 && n_rows >= 2048 && V * 10 >= (V + WIDE - 1) / WIDE * WIDE * 9;
+    const int64_t columns = wide ? WIDE : (int64_t)ADJUST_NT * pieces(bytes) * 16 / bytes, parts = (V + columns - 1) / columns;
+    const int64_t at_once = 32 * (wide ? 1 : 4);               // workgroups of an XCD, which has all parts of a run
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+      const int64_t runs = 8 * std::max<int64_t>(1, at_once * rounds / parts);
+      run = std::max<int64_t>(4, (n_rows + runs - 1) / runs);
+      if (run <= SUMS_ROWS) break;
+    }
+  }
+  static constexpr int pieces(int bytes) { return bytes == 2 ? 3 : ADJUST_NCH; }
+  int64_t runs(int64_t n_rows) const { return (n_rows + run - 1) / run; }
+};
 
 template <class Tag, class Index, int NT, class Count, bool GRAD, bool SUMS>
-static void launch_adjust(AdjustParams p, float* sums, hipStream_t st) {
-  constexpr int64_t most = (int64_t)NT * ADJUST_NCH * Chunk<Tag>::N;
+static void launch_adjust(AdjustParams p, double* sums, hipStream_t st) {
+  constexpr int NCH = SUMS ? SumsCut::pieces(Tag::bytes) : ADJUST_NCH;
+  constexpr int64_t most = (int64_t)NT * NCH * Chunk<Tag>::N;
   p.parts = (unsigned)((p.V + most - 1) / most);
   p.part_columns = (unsigned)std::min<int64_t>(most, ((p.V + p.parts - 1) / p.parts + 127) / 128 * 128);      // (whole words of the masks, whole pieces of the bits)
-  p.run = SUMS ? sums_run(p.n_rows, p.V) : 1;
+  p.run = SUMS ? SumsCut(p.n_rows, p.V, Tag::bytes).run : 1;
   const size_t lds = p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (GRAD ? Tag::bytes : sizeof(Count))) : 0;
-  if (NT * ADJUST_NCH * 16 > 32768 && lds > 65536 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+  if (NT * NCH * 16 > 32768 && lds > 65536 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return;                                                    // (the error is the launch's)
   const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8 * p.run, all = p.n_rows;      // rows of a launch
   for (p.first_row = 0; p.first_row < all; p.first_row += slice) {
     p.n_rows = std::min(all, p.first_row + slice);
     const int64_t runs = (p.n_rows - p.first_row + p.run - 1) / p.run;
-    hipLaunchKernelGGL((adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), dim3((unsigned)((runs + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, p, sums);
+    hipLaunchKernelGGL((adjust_kernel<Tag, Index, NT, NCH, Count, GRAD, SUMS>), dim3((unsigned)((runs + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, p, sums);
   }
 }
 template <class Tag, class Index, bool GRAD, bool SUMS>
-static void adjust_texts(const AdjustParams& p, float* sums, hipStream_t st) {
-  // Sums of many rows whose columns fill the parts of 1024 threads: 8192 x 128256 bf16 905 us (256 threads: 943), 4096 x 128256 fp32 843 (882); parts three
-  // quarters full, 8192 x 50257 bf16, 647 (547), few rows, 512 x 128256 bf16, 81 (74).
-  if constexpr (SUMS) {
-    constexpr int64_t MOST = 1024 * ADJUST_NCH * Chunk<Tag>::N;
-    if (p.n_rows >= 2048 && p.V * 10 >= (p.V + MOST - 1) / MOST * MOST * 9) return launch_adjust<Tag, Index, 1024, unsigned short, GRAD, SUMS>(p, sums, st);
-  }
+static void adjust_texts(const AdjustParams& p, double* sums, hipStream_t st) {
+  if constexpr (SUMS && Tag::bytes == 4)
+    if (SumsCut(p.n_rows, p.V, Tag::bytes).wide) return launch_adjust<Tag, Index, SUMS_NT, unsigned short, GRAD, SUMS>(p, sums, st);
   if constexpr (!GRAD)
     if (p.length > 65535) return launch_adjust<Tag, Index, ADJUST_NT, unsigned, GRAD, SUMS>(p, sums, st);
   launch_adjust<Tag, Index, ADJUST_NT, unsigned short, GRAD, SUMS>(p, sums, st);
 }
 template <class Tag, bool GRAD, bool SUMS>
-static void adjust_rows(const AdjustParams& p, float* sums, hipStream_t st) {
+static void adjust_rows(const AdjustParams& p, double* sums, hipStream_t st) {
   if (p.itype == I64) adjust_texts<Tag, int64_t, GRAD, SUMS>(p, sums, st);
   else adjust_texts<Tag, int32_t, GRAD, SUMS>(p, sums, st);
 }
 template <bool GRAD, bool SUMS>
-static void adjust_rows(const AdjustParams& p, int dtype, float* sums, hipStream_t st) {
+static void adjust_rows(const AdjustParams& p, int dtype, double* sums, hipStream_t st) {
   if (dtype == DL_F32) adjust_rows<TagF32, GRAD, SUMS>(p, sums, st);
   else if (dtype == DL_BF16) adjust_rows<TagBF16, GRAD, SUMS>(p, sums, st);
   else adjust_rows<TagF16, GRAD, SUMS>(p, sums, st);
@@ -425,8 +442,7 @@ extern "C" int dl_adjust_rows(const void* logits, int dtype, int64_t row_stride,
 
 extern "C" int64_t dl_adjust_grad_workspace_bytes(int64_t n_rows, int64_t V) {
   if (n_rows <= 0 || V <= 0) return 0;
-  const int64_t run = dl::sums_run(n_rows, V);
-  return (n_rows + run - 1) / run * V * 4;
+  return std::max(dl::SumsCut(n_rows, V, 2).runs(n_rows), dl::SumsCut(n_rows, V, 4).runs(n_rows)) * V * 8;      // (of either width)
 }
 
 extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, const void* logits, int64_t row_stride, int64_t n_rows, int64_t V,
@@ -457,12 +473,12 @@ extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, 
     if (out) adjust_rows<true, false>(p, dtype, nullptr, st);
     return adjust_status();
   }
-  float* sums = reinterpret_cast<float*>(workspace);
+  double* sums = reinterpret_cast<double*>(workspace);
   int64_t runs = 0;
   if (n_rows > 0) {
     if (!out) p.length = 0;                                    // the bias does not feel the texts
     adjust_rows<true, true>(p, dtype, sums, st);
-    runs = (n_rows + sums_run(n_rows, V) - 1) / sums_run(n_rows, V);
+    runs = SumsCut(n_rows, V, dtype == DL_F32 ? 4 : 2).runs(n_rows);
   }
   constexpr int64_t MOST = LAUNCH_THREADS / 256 * 32;          // columns of a launch
   for (int64_t col = 0; col < V; col += MOST)

@@ -646,3 +646,33 @@ def test_empty_texts_and_rows(D):
     assert D.adjust_rows(none, torch.empty((0, 5), dtype=torch.int64, device=DEV), repetition=2.0).shape == (0, 100)
     rows, by_bias = D.adjust_grad(none, want_bias=True)
     assert rows.shape == (0, 100) and by_bias.count_nonzero().item() == 0 and by_bias.shape == (100,)
+
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V", [(1, 5), (7, 33), (512, 9001), (2100, 32768), (4096, 16384), (9000, 40)])
+def test_the_sum_of_rows_is_rounded_once(D, dtype, R, V):
+    """The gradient by a shared bias: a sum in 64 bits, off by at most R - 1 roundings of 2^-53 of the magnitudes' sum (as the one here is), and one
+    rounding to fp32, or that and one more to a type of 16 bits."""
+    grad = torch.randn((R, V), generator=torch.Generator(device=DEV).manual_seed(R), device=DEV).to(dtype)
+    want, size = grad.double().sum(0), grad.double().abs().sum(0)
+    for bias_dtype in {torch.float32, dtype}:
+        _, by_bias = D.adjust_grad(grad, want_logits=False, want_bias=True, bias_dtype=bias_dtype)
+        half = 2.0 ** -24 + (HALF_ULP[bias_dtype] if bias_dtype != torch.float32 else 0.0)
+        assert ((by_bias.double() - want).abs() <= half * want.abs() * (1 + 2.0 ** -7) + 2 * R * 2.0 ** -53 * size + STEP[bias_dtype]).all()
+        assert torch.equal(by_bias, D.adjust_grad(grad, want_bias=True, bias_dtype=bias_dtype)[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [4, 8, 96, 4096])
+def test_sums_on_the_way_may_leave_fp32(D, dtype, R):
+    """Finite sums of values near the type's largest, the positive ones first: within a run of rows, and whole runs of them."""
+    big = torch.finfo(dtype).max / 2
+    grad = torch.zeros((R, 20000), dtype=dtype, device=DEV)
+    grad[: R // 2, ::3], grad[R // 2:, ::3] = big, -big
+    grad[::4, 1::3], grad[1::4, 1::3], grad[2::4, 1::3] = 1.5 * big, 1.5 * big, -3 * big / 2
+    grad[3::4, 1::3] = -1.5 * big
+    grad[0, 2::3], grad[R - 1, 2::3] = big, 0.5 * big
+    want = grad.double().sum(0)
+    _, by_bias = D.adjust_grad(grad, want_logits=False, want_bias=True)
+    assert want.abs().max() == 1.5 * big and torch.equal(by_bias, want.float())
