@@ -6,6 +6,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.graph import increment_version
 from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _lib
@@ -86,6 +87,8 @@ def _written(out: Optional[torch.Tensor], x: torch.Tensor, name: str, over: str,
     """The matrix that the result goes to: new, or `out` checked -- `x` itself, or memory that neither `x` nor `others` have."""
     if out is None:
         return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient and the call records none: detach it, or call under torch.no_grad()")
     R, V = x.shape
     o = _logit_rows(out, name, x.device)
     if tuple(o.shape) != (R, V) or o.dtype != x.dtype:
@@ -115,7 +118,8 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     row r has number `allowed_rows`[r] (int32; negative: every token is allowed).  A masked token is -inf whatever its logit was; a row whose mask
     allows nothing is -inf throughout, and `sample_rows` gives it token -1.
 
-    Arithmetic is fp32, rounded once to the logits' dtype.  Returns a new tensor, or `out`, which may be the logits themselves."""
+    Arithmetic is fp32, rounded once to the logits' dtype.  Returns a new tensor, or `out`, which may be the logits themselves.  Autograd knows of the
+    write into `out`: a backward pass that needs what was there raises.  `out` must not require a gradient unless recording is off."""
     x = _logit_rows(logits, "logits")
     R, V = x.shape
     dev = x.device
@@ -150,6 +154,8 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
                                         b_ptr, b_dtype, b_stride, *mask, res.data_ptr(), res.stride(0) if R > 1 else V, _stream_ptr(dev))
     if st:
         _lib.check(st, "dl_adjust_rows")
+    if out is not None:
+        increment_version(out)
     return out if out is not None else res if logits.dim() == 2 else res.view(logits.shape)
 
 
@@ -164,7 +170,7 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     `grad` and not needed without tokens), 0 where the mask does not allow the token, whatever `grad` has there.  By the bias: the sum of the rows of
     `grad` over what their masks allow, fp32 or in the dtype of `grad`, in an order that does not change between calls.  (A bias of each row's own has
     the gradient that the logits have without tokens.)  Texts, masks and `repetition` as for `adjust_rows`.  `out`, for the first, may be
-    `grad` itself.  Returns (by the logits or None, by the bias or None)."""
+    `grad` itself (and is written as by `adjust_rows`).  Returns (by the logits or None, by the bias or None)."""
     g = _logit_rows(grad, "grad")
     R, V = g.shape
     dev = g.device
@@ -198,6 +204,8 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
                                 _DT[bias_dtype], 0 if ws is None else ws.data_ptr(), ws_bytes, _stream_ptr(dev))
     if st:
         _lib.check(st, "dl_adjust_grad")
+    if out is not None:
+        increment_version(out)
     return (out if out is not None else res if not want_logits or grad.dim() == 2 else res.view(grad.shape)), by_bias
 
 

@@ -7,6 +7,7 @@ from operator import attrgetter
 from typing import Iterable, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _DT, _dev, _on, _stream_ptr
@@ -85,7 +86,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, scale: float =
 
     `norm` (fp32, one element, `scale` included): is taken for the norm instead, for gradients of which these are only a part (shards on other
     cards: the root of the sum of the squares of their `grad_norm`).  A norm that is NaN or infinite leaves all gradients as they are; one within
-    max_norm leaves them unwritten where scale is 1.  The gradients must not overlap.  Nothing waits for the GPU."""
+    max_norm leaves them unwritten where scale is 1.  The gradients must not overlap.  Autograd takes all of them for written: a backward pass that needs
+    what was there raises.  Nothing waits for the GPU."""
     scale, max_norm = _positive(scale), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative")
@@ -104,4 +106,5 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, scale: float =
         st = lib.dl_clip_grads(*t.args(), scale, max_norm, norm.data_ptr(), int(given), ws.data_ptr() if ws is not None else 0,
                                ws.numel() if ws is not None else 0, _stream_ptr(t.dev))
     _lib.check(st, "dl_clip_grads")
+    increment_version(t.all)
     return norm

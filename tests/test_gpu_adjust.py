@@ -676,3 +676,44 @@ def test_sums_on_the_way_may_leave_fp32(D, dtype, R):
     want = grad.double().sum(0)
     _, by_bias = D.adjust_grad(grad, want_logits=False, want_bias=True)
     assert want.abs().max() == 1.5 * big and torch.equal(by_bias, want.float())
+
+
+def test_autograd_sees_what_is_written_in_place(D):
+    """A backward pass that needs values which a later call has overwritten raises, and none that does not need them."""
+    g = torch.Generator(device=DEV).manual_seed(50)
+    x = torch.randn(4, 100, generator=g, device=DEV).requires_grad_()
+    t, w = torch.randint(100, (4, 30), generator=g, device=DEV), torch.randn(4, 100, generator=g, device=DEV).requires_grad_()
+    kw = dict(repetition=1.5, presence=3.0)
+    y = D.adjust_logits(x, t, **kw)                           # (whose gradient goes by the logits' signs)
+    want, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    over = y.detach()
+    assert D.adjust_rows(over, t, out=over, **kw) is over and y._version == 1
+    assert torch.equal(torch.autograd.grad(y.sum(), x, retain_graph=True)[0], want)
+    into = torch.empty_like(over)
+    D.adjust_rows(x.detach(), t, out=into, **kw)
+    assert into._version == 1 and x._version == 0
+    D.adjust_rows(x.detach(), t, out=x.detach(), **kw)
+    assert x._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z = (w * x).sum()
+    D.adjust_grad(w.detach(), x.detach(), t, repetition=1.5, out=w.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():                              # (a tensor without a version)
+        into = torch.zeros(4, 100, device=DEV)
+        D.adjust_rows(into, bias=torch.ones(100, device=DEV), out=into)
+    assert (into == 1).all()
+
+
+def test_a_result_that_would_need_a_gradient_is_refused(D):
+    x = torch.randn(4, 100, device=DEV, requires_grad=True)
+    y, bias = x * 1, torch.ones(100, device=DEV)
+    before = y.detach().clone()
+    for call in (lambda: D.adjust_rows(y, bias=bias, out=y), lambda: D.adjust_rows(before, bias=bias, out=x), lambda: D.adjust_grad(before, out=y)):
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call()
+    assert torch.equal(y, before) and y._version == 0
+    with torch.no_grad():
+        assert D.adjust_rows(y, bias=bias, out=y) is y
+    assert torch.equal(y, before + 1) and y._version == 1

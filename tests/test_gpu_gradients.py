@@ -224,3 +224,16 @@ def test_refusals(D):
             call()
     assert (a == 1).all()
     near(D.grad_norm([a, a]), math.sqrt(200))                 # only read: the same one twice counts twice
+
+
+def test_autograd_sees_that_gradients_are_clipped(D):
+    """Gradients that are to be differentiated again and were clipped in between: an error, no derivative of what they were not."""
+    w = torch.randn(50, generator=torch.Generator(device=DEV).manual_seed(10), device=DEV).requires_grad_()
+    grad, = torch.autograd.grad(w.pow(3).sum(), w, create_graph=True)
+    z, parts = grad.square().sum(), torch.ones(30, device=DEV)
+    D.grad_norm([grad])
+    assert grad._version == 0
+    D.clip_grads([grad, parts[:10], parts[10:]], 1e-3)
+    assert grad._version == 1 and parts._version == 2
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
