@@ -96,13 +96,13 @@ struct RowsParams {
 // memory and no more: for a load into LDS that it knows it waits before the next access to LDS, and for all that are under way.  (Small tiles then
 // drained their own fetches at every step, 128 x 8000 x 4096 17.8 us and with the ring below 23.6, now 12.9; a tile's values waited for the next
 // tile's operands and for each other's stores, 8192 x 32000 x 1024 297 us, now 283.)  The waits are the kernels' own, by the count of fetches; those of
-// the compiler, which does not count them, can only ask for more.  (m0, which holds the place in LDS, is nobody else's in these kernels.)
+// the compiler, which does not count them, can only ask for more.  (m0 holds the place in LDS: it is the operand's register, which the compiler writes ahead of each.)
 __device__ __forceinline__ void fetch_to_lds(const unsigned char* base, unsigned offset, unsigned to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(base) : "memory");
 }
 
 __device__ __forceinline__ void fetch_word_to_lds(const float* base, unsigned offset, unsigned to) {      // 4 bytes a lane
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(to), "v"(offset), "s"(base) : "memory");
 }
 
 // Tiles of BM x BN, a wave WM x WN of it, a block of 128 columns (two matrix instructions deep) per step.  A step's operands are fetched into LDS by
