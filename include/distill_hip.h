@@ -712,7 +712,7 @@ int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, const void*
  * 8-bit integers with a scale for every row, and the product of two such matrices.
  *
  * dl_quantize_rows: x [rows, cols] -> codes [rows, whole blocks of 128 columns] (zeros behind the last column), scales [rows].
- * scale = max(largest magnitude * r, 2^-100) with r = 1 / 127 in fp32; code = x / scale (fp32), rounded to even, within [-127, 127].  A row
+ * scale = max(largest magnitude * r, 2^-100) with r = 1 / 127 in fp32 (rows of no columns: 2^-100); code = x / scale (fp32), rounded to even, within [-127, 127].  A row
  * with a NaN or an infinity has NaN for its scale and zeros for its codes.
  *
  * dl_matmul_rows: out[m, n] = (sum over the K columns of a[m, k] b[n, k]) * (a_scale[m] * b_scale[n]), out [M, N] of out_dtype.  The sum is exact

@@ -523,8 +523,8 @@ extern "C" int dl_quantize_rows(const void* x, int dtype, int64_t row_stride, in
   if ((unsigned)dtype > DL_F16) return DL_ERR_DTYPE;
   const int64_t width = (cols + KB - 1) / KB * KB;
   if (rows < 0 || cols < 0 || row_stride < cols || code_stride < width) return DL_ERR_SHAPE;
-  if (rows == 0 || cols == 0) return DL_OK;
-  if (!x || !codes || !scales) return DL_ERR_NULL;
+  if (rows == 0) return DL_OK;
+  if (!scales || (cols > 0 && (!x || !codes))) return DL_ERR_NULL;      // (rows of no columns have a scale too)
   if (reinterpret_cast<uintptr_t>(x) % (dtype == DL_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(codes) % 16 || code_stride % 16 ||
       reinterpret_cast<uintptr_t>(scales) % 4)
     return DL_ERR_ALIGN;

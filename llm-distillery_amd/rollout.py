@@ -194,7 +194,7 @@ def quantize_rows(x: torch.Tensor) -> RowQuantized:
     wide = (W + 127) // 128 * 128
     codes = v.new_empty(R, wide, dtype=torch.int8)
     scales = v.new_empty(R, dtype=torch.float32)
-    if R and W:
+    if R:
         with _on(dev):
             st = _lib.load().dl_quantize_rows(v.data_ptr(), kind, pitch, R, W, codes.data_ptr(), wide, scales.data_ptr(), _stream_ptr(dev))
         if st:

@@ -210,3 +210,13 @@ def test_more_rows_than_a_launch_takes(D):
         some = D.quantize_rows(x[rows])
         assert torch.equal(q.codes[rows], some.codes) and torch.equal(q.scales[rows], some.scales)
     assert torch.equal(some.scales.cpu(), quantised(x[rows].cpu())[1])
+
+
+def test_rows_of_no_columns_have_the_least_scale(D):
+    """As rows of zeros have it, and no memory as it was found."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        found = torch.full((5,), math.nan, device=DEV)
+        del found                                             # (what the scales are likely to get)
+        q = D.quantize_rows(torch.empty(5, 0, dtype=dtype, device=DEV))
+        assert q.codes.shape == (5, 0) and q.width == 0 and (q.scales == 2.0 ** -100).all()
+        assert torch.equal(q.scales, D.quantize_rows(torch.zeros(5, 3, dtype=dtype, device=DEV)).scales)

@@ -74,6 +74,11 @@ def test_integer_products():
     assert mul(K=130945, sa=131072, sb=131072) == -4
 
 
+def test_rows_of_no_columns():
+    lib = D._lib.load()
+    assert lib.dl_quantize_rows(0, 0, 0, 4, 0, 0, 0, 0, 0) == -1 and lib.dl_quantize_rows(0, 0, 0, 0, 0, 0, 0, 0, 0) == 0      # (their scales are wanted)
+
+
 def test_clipped_gradients():
     lib = D._lib.load()
 
