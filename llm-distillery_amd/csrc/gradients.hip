@@ -154,18 +154,10 @@ __global__ __launch_bounds__(GRAD_NT) void norm_kernel(double* sums, unsigned n,
   }
 }
 
-// f times a factor of 64 bits, held as the sum of two of 32: the one rounding that shows is the result's (a factor rounded to 32 bits would be off by up to
-// 2^-24 in all elements alike).
-struct GradFactor {
-  float hi, lo;
-  __device__ __forceinline__ explicit GradFactor(double by) : hi((float)by), lo((float)(by - (double)(float)by)) {}
-  __device__ __forceinline__ float times(float f) const {
-    const float rest = f * lo;
-    return fmaf(f, hi, fabsf(rest) <= 3.402823466e38f ? rest : 0.f);
-  }
-};
+// f times a factor of 64 bits, which may be smaller than fp32 holds: a product in 64 bits, so that the one rounding that shows is the result's.
+__device__ __forceinline__ float scaled(float f, double by) { return (float)((double)f * by); }
 template <class Tag>
-__device__ __forceinline__ void scale_piece(const GradPiece& p, const GradFactor& by) {
+__device__ __forceinline__ void scale_piece(const GradPiece& p, double by) {
   constexpr int N = Chunk<Tag>::N;
   u32x4 v[GRAD_NCH];
 #pragma unroll
@@ -178,13 +170,13 @@ __device__ __forceinline__ void scale_piece(const GradPiece& p, const GradFactor
     float f[N];
     Chunk<Tag>::unpack(v[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = by.times(f[e]);
+    for (int e = 0; e < N; ++e) f[e] = scaled(f[e], by);
     if (grad_chunk(i) < p.chunks) store16_stream(p.body + grad_chunk(i) * 16, Chunk<Tag>::pack(f));
   }
   for (int side = 0; side < 2; ++side)
     if ((int)threadIdx.x < (side ? p.n_behind : p.n_ahead)) {
       char* at = side ? p.behind : p.ahead;
-      store_from_float(at, Tag::id, threadIdx.x, by.times(load_as_float(at, Tag::id, threadIdx.x)));
+      store_from_float(at, Tag::id, threadIdx.x, scaled(load_as_float(at, Tag::id, threadIdx.x), by));
     }
 }
 // The norm: of `n_sums` sums, and is written; or (none) the first of them; or (no `sums`) given.
@@ -193,10 +185,9 @@ __global__ __launch_bounds__(GRAD_NT, 4) void scale_kernel(const GradTable t, co
   __shared__ double scratch[GRAD_NT / WAVE];
   const double all = !sums ? (double)norm[0] : n_sums ? norm_of(sums, n_sums, scale, scratch) : sums[0];
   if (n_sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
-  const double factor = all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale;
+  const double by = all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale;
   if (!((float)all <= 3.402823466e38f)) return;                // NaN or, as fp32 shows it, infinite: left as they are
-  if (fabs(factor - 1.0) <= 0x1p-25) return;                   // less than half a step of any element: they would stay what they are
-  const GradFactor by(factor);
+  if (fabs(by - 1.0) <= 0x1p-25) return;                   // less than half a step of any element: they would stay what they are
   const unsigned q = t.pieces - 1u - blockIdx.x;
   find_entry(t, q, found);
   const GradPiece p = piece_of(found, q);

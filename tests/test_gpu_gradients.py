@@ -237,3 +237,41 @@ def test_autograd_sees_that_gradients_are_clipped(D):
     assert grad._version == 1 and parts._version == 2
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.backward()
+
+
+def check_rounded_once(after, before, by):
+    """By a factor of 64 bits: half a step of an fp32 result (what the norm and the factor leave off is below 2^-16 of that, as above); half a
+    step of a type of 16 bits behind that of the fp32 number that it is rounded from."""
+    for a, b in zip(after, before):
+        want = b.double() * by
+        half = 2.0 ** -24 if b.dtype == torch.float32 else 2.0 ** -24 * (1 + 2.0 ** -7) + HALF_ULP[b.dtype]
+        assert ((a.double() - want).abs() <= half * want.abs() * (1 + 2.0 ** -16) + STEP[b.dtype]).all()
+
+
+@pytest.mark.parametrize("most", [1.0, 1e-6, 3e-38])
+def test_factors_smaller_than_fp32_holds(D, most):
+    """Norms above 1e38: the factor is subnormal or 0 in fp32, the results are not."""
+    most, given = torch.tensor(most).item(), torch.tensor(2e38, device=DEV)
+    grads = some((1001, 12, 70_000), 11, (torch.float32, torch.bfloat16), std=4e35)
+    norm = exact_norm(grads)
+    assert 0.9e38 < norm < 3e38
+    for kw, by in (({}, most / norm), (dict(norm=given), most / given.item())):
+        now = [g.clone() for g in grads]
+        D.clip_grads(now, most, **kw)
+        check_rounded_once(now, grads, by)
+
+
+def test_one_rounding_at_any_offset_and_in_any_number(D):
+    """Three tables of tensors of all types and of odd sizes, parts of one buffer, a norm that is given."""
+    grads = some((*range(1, 600), 100_003, 64, 1_000_000, 17), 12)
+    flat, = some((90_001,), 13, (torch.float32,))
+    grads += [flat[1:4], flat[5:50_000], flat[50_002:]]
+    norm = exact_norm(grads)
+    most = torch.tensor(norm / 3).item()
+    for kw, by in (({}, most / norm), (dict(norm=torch.tensor(7.0, device=DEV), scale=0.75), 0.75 * min(1.0, most / 7.0))):
+        now = [g.clone() for g in grads[:-3]]
+        whole = flat.clone()
+        now += [whole[1:4], whole[5:50_000], whole[50_002:]]
+        D.clip_grads(now, most, **kw)
+        check_rounded_once(now, grads, by)
+        assert whole[0] == flat[0] and whole[4] == flat[4] and torch.equal(whole[50_000:50_002], flat[50_000:50_002])
