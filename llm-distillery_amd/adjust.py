@@ -29,6 +29,12 @@ def _logit_rows(t: torch.Tensor, name: str, dev: Optional[torch.device] = None) 
     return x
 
 
+def _check_repetition(v: float) -> None:
+    """Of a number for all rows: what the kernels take is its fp32 form, which is 0 below half the smallest subnormal."""
+    if not 2.0 ** -149 <= v <= 3.0e38:
+        raise ValueError("repetition must be positive and finite in fp32")
+
+
 def _per_row(v: Number, rows: int, name: str, dev: torch.device) -> Tuple[Optional[torch.Tensor], float]:
     """A setting as (one fp32 entry per row, 0) or (nothing, the number for all)."""
     return (_row_vector(v, rows, torch.float32, name, dev), 0.0) if isinstance(v, torch.Tensor) else (None, float(v))
@@ -130,8 +136,8 @@ def adjust_rows(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, 
     rep, rep_all = (None, repetition) if type(repetition) is float else _per_row(repetition, R, "repetition", dev)
     freq, freq_all = (None, frequency) if type(frequency) is float else _per_row(frequency, R, "frequency", dev)
     pres, pres_all = (None, presence) if type(presence) is float else _per_row(presence, R, "presence", dev)
-    if rep is None and not 0.0 < rep_all <= 3.0e38:
-        raise ValueError("repetition must be positive and finite")
+    if rep is None:
+        _check_repetition(rep_all)
     b_ptr = b_dtype = b_stride = 0
     others = ()
     if bias is not None:
@@ -178,8 +184,8 @@ def adjust_grad(grad: torch.Tensor, logits: Optional[torch.Tensor] = None, token
     if lengths is not None:
         lengths = _row_vector(lengths, R, torch.int32, "lengths", dev)
     rep, rep_all = (None, repetition) if type(repetition) is float else _per_row(repetition, R, "repetition", dev)
-    if rep is None and not 0.0 < rep_all <= 3.0e38:
-        raise ValueError("repetition must be positive and finite")
+    if rep is None:
+        _check_repetition(rep_all)
     if bias_dtype not in (torch.float32, g.dtype):
         raise RuntimeError(f"the bias's gradient is fp32 or {g.dtype}")
     x = None

@@ -717,3 +717,12 @@ def test_a_result_that_would_need_a_gradient_is_refused(D):
     with torch.no_grad():
         assert D.adjust_rows(y, bias=bias, out=y) is y
     assert torch.equal(y, before + 1) and y._version == 1
+
+
+def test_a_repetition_that_is_zero_in_fp32_is_refused(D):
+    x, t = torch.zeros(2, 9, device=DEV), torch.zeros((2, 3), dtype=torch.int64, device=DEV)
+    for repetition in (1e-46, 2.0 ** -150, 1e-300):
+        for call in (lambda: D.adjust_rows(x, t, repetition=repetition), lambda: D.adjust_grad(x, x, t, repetition=repetition)):
+            with pytest.raises(ValueError, match="positive"):
+                call()
+    assert torch.equal(D.adjust_rows(x, t, repetition=2.0 ** -149), x)      # (0 / 2^-149)
