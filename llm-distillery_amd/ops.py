@@ -69,7 +69,7 @@ def _rows_2d(logits: torch.Tensor) -> torch.Tensor:
         return logits
     V = logits.shape[-1]
     try:
-        return logits.view(-1, V)
+        return logits.view(logits.shape[:-1].numel(), V)
     except RuntimeError:
         flat = logits.as_strided((logits.numel() // V, V), (logits.stride(-2), 1), logits.storage_offset())
         lead = 1

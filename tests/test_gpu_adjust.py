@@ -726,3 +726,13 @@ def test_a_repetition_that_is_zero_in_fp32_is_refused(D):
             with pytest.raises(ValueError, match="positive"):
                 call()
     assert torch.equal(D.adjust_rows(x, t, repetition=2.0 ** -149), x)      # (0 / 2^-149)
+
+
+def test_rows_without_columns(D):
+    """In any shape: nothing to adjust, gradients of no columns, rows of no codes."""
+    x = torch.empty((2, 3, 0), device=DEV)
+    assert D.adjust_rows(x, torch.zeros((6, 4), dtype=torch.int64, device=DEV), repetition=2.0).shape == (2, 3, 0)
+    rows, by_bias = D.adjust_grad(x, want_bias=True)
+    assert rows.shape == (2, 3, 0) and by_bias.shape == (0,)
+    q = D.quantize_rows(x)
+    assert q.codes.shape == (6, 0) and (q.scales == 2.0 ** -100).all()

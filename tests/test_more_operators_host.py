@@ -134,3 +134,9 @@ def test_adjusted_logits_trace_with_fake_tensors_in_both_directions():
             assert gx.shape == x.shape and gx.dtype == torch.bfloat16 and gb.shape == shape and gb.dtype == torch.float32
             again, = torch.autograd.grad(gx.sum() + gb.sum(), weight)
             assert again.shape == weight.shape
+
+
+def test_rows_without_columns_in_any_shape():
+    """Their view is the one that rows with columns have: as many of them, none dropped."""
+    for shape, rows in (((2, 3, 0), 6), ((4, 0), 4), ((0, 3, 0), 0), ((2, 0, 5), 0), ((2, 3, 5), 6)):
+        assert D.ops._rows_2d(torch.empty(shape)).shape == (rows, shape[-1])
