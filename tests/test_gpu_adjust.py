@@ -736,3 +736,33 @@ def test_rows_without_columns(D):
     assert rows.shape == (2, 3, 0) and by_bias.shape == (0,)
     q = D.quantize_rows(x)
     assert q.codes.shape == (6, 0) and (q.scales == 2.0 ** -100).all()
+
+
+def test_a_captured_backward_pass_into_the_leaves(D):
+    """`.backward()` in a graph: the leaves have been in no graph of eager calls, their gradients are the capture's own."""
+    R, V, L = 40, 5003, 30
+    g = torch.Generator(device=DEV).manual_seed(51)
+    leaves = lambda: (torch.zeros(R, V, device=DEV, requires_grad=True), torch.zeros(V, device=DEV, requires_grad=True))  # noqa: E731
+    t, up = torch.zeros((R, L), dtype=torch.int64, device=DEV), torch.zeros(R, V, device=DEV)
+
+    def step(x, b):
+        D.adjust_logits(x, t, repetition=1.3, presence=0.5, bias=b).backward(up)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    x, b = leaves()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(x, b)
+    for _ in range(3):
+        with torch.no_grad():
+            x.normal_(generator=g), b.normal_(generator=g), t.random_(0, V, generator=g), up.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = [v.detach().clone().requires_grad_() for v in (x, b)]
+        step(*eager)
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, eager[0].grad) and torch.equal(b.grad, eager[1].grad)
