@@ -38,7 +38,7 @@ struct AdjustParams {
   const char* bias; int bias_dtype; int64_t bias_stride;
   const unsigned* allowed; int64_t allowed_stride, n_masks; const int32_t* allowed_rows;
   unsigned parts, part_columns;
-  int64_t first_row, run;                                      // `run` rows a workgroup
+  int64_t first_row, first_run, runs;                          // of a launch; every `runs`-th pair of rows is a workgroup's (SUMS)
 };
 
 // What a row has besides its logits.  A lane fetches one of its settings each, so that they take one trip to memory; the same in all waves.
@@ -115,33 +115,45 @@ struct FourTokens {
 constexpr int STEP_MOST = 8192;
 constexpr int64_t LENGTH_MOST = (1LL << 31) - STEP_MOST;
 __device__ const unsigned NOTHING[4] = {0u, 0u, 0u, 0u};       // in the place of a row too short for a piece
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef const char __attribute__((address_space(1))) * global_bytes;      // (said to be global, so that a choice of two is no load of any kind of memory)
 
-// `run` rows, one after the other, of a part of the columns.  SUMS (the gradient's): what they have in common, the gradient by a shared bias, is added
-// up on the way, one row of `sums` for every run, in fp64: what shows is the result's rounding, and a sum on the way may be larger than fp32 holds.
+// A part of the columns of a row, or (SUMS, the gradient's) of a run of rows, one after the other: what these have in common, the gradient by a shared bias,
+// is added up on the way, one row of `sums` for every run, in fp64: what shows is the result's rounding, and a sum on the way may be larger than fp32 holds.
+// A run is every so many-th pair of rows: the texts of neighbouring rows are of a length, those of runs of neighbours would not be (4096 x 50257 fp32,
+// texts of 2048, 400 us, so 429); a pair shares the line in which one row ends and the next begins (8192 x 50257 bf16 472 us, single rows 552).
 // Count: what a column's counter is held in, 16 bits where no text has more tokens than these count.
-// 16 KiB of a row a workgroup, four 16-byte pieces a thread (three where two-byte rows are added up); LDS and registers leave room for four such workgroups
-// on a CU (asked for six or eight, values spill).
+// 16 KiB of a row a workgroup, four 16-byte pieces a thread; LDS and registers leave room for four such workgroups on a CU (asked for six or eight, values
+// spill).  The totals of two-byte rows, 64 registers, do not fit beside the rest: those of a thread's last piece are in LDS.
 template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
 __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, double* sums) {
   constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = SUMS ? 1 : 2;      // (tokens of a thread at a time: four times NTOK)
   static_assert(NT * NTOK * 4 <= STEP_MOST, "places of 32 bits");
-  extern __shared__ __align__(16) unsigned lds[];              // for each column a bit, its new value, and a counter or (GRAD) the logit
+  constexpr int KEPT = SUMS && B == 2 ? NCH - 1 : NCH;         // pieces whose totals are in registers
+  constexpr bool SIGNS = KEPT < NCH;                           // (which leaves no room for the logits in LDS: a bit of a register each)
+  extern __shared__ __align__(16) unsigned all_lds[];          // the other totals; for each column a bit, its new value, and a counter or (GRAD) the logit
+  f64x2* const last_totals = reinterpret_cast<f64x2*>(all_lds) + threadIdx.x;      // this thread's, NT apart
+  unsigned* const lds = all_lds + (KEPT < NCH ? NT * N * 2 : 0);
   const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a run on one XCD
-  const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + k * p.run, last = min(first + p.run, p.n_rows);
+  const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + (SUMS ? 2 * k : k), last = SUMS ? p.n_rows : min(first + 1, p.n_rows);
   const int64_t c0 = (int64_t)(in >> 3) * p.part_columns;
-  if (first >= last || c0 >= p.V) return;                      // (parts are whole blocks of 128 columns: the last may be none)
+  if (k >= p.runs || c0 >= p.V) return;                      // (parts are whole blocks of 128 columns: the last may be none)
   // a wave's pieces are neighbours, NCH KiB of them: all of a thread's lie within the offset of an instruction
-  const unsigned tid = threadIdx.x, mine = tid / WAVE * (WAVE * NCH) + tid % WAVE;
+  const unsigned tid = threadIdx.x, place = tid / WAVE * (WAVE * NCH) + tid % WAVE;
   const unsigned columns = (unsigned)min((int64_t)p.part_columns, p.V - c0), pieces = columns / N, tail = columns % N;
   const unsigned char* said = reinterpret_cast<const unsigned char*>(lds);
   char* values = reinterpret_cast<char*>(lds + p.part_columns / 32);
   char* beside = values + p.part_columns * B;
   unsigned* counts = reinterpret_cast<unsigned*>(beside);
   const u32x4 masked = GRAD ? u32x4{0u, 0u, 0u, 0u} : Chunk<Tag>::neg_inf();
-  double total[SUMS ? NCH : 1][N] = {}, total_tail = 0.0;
+  double total[SUMS ? KEPT : 1][N] = {}, total_tail = 0.0;
+  if (KEPT < NCH)
+#pragma unroll
+    for (int e = 0; e < N; e += 2) last_totals[e / 2 * NT] = f64x2{0.0, 0.0};
 #pragma unroll 1
-  for (int64_t r = first; r < last; ++r) {
+  for (int64_t r = first; r < last; r += (SUMS && (r & 1)) ? 2 * p.runs - 1 : 1) {
+    unsigned mine = place;
+    if (SUMS) asm("" : "+v"(mine) : "s"((int)r));              // (said to change: offsets made from it would take registers from row to row, and spill)
     const AdjustRow row(p, r);
     const char* from = (GRAD ? p.g + (r * p.g_stride + c0) * B : p.x + (r * p.x_stride + c0) * B);
     const char* x = p.x + (r * p.x_stride + c0) * B;
@@ -207,7 +219,15 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
           float f[N];
           Chunk<Tag>::unpack(v[i], f);
 #pragma unroll
-          for (int e = 0; e < N; ++e) total[i][e] += (double)f[e];
+          for (int e = 0; e < N; e += 2) {
+            const f64x2 more = {(double)f[e], (double)f[e + 1]};
+            if (i < KEPT) {
+              total[i < KEPT ? i : 0][e] += more[0];
+              total[i < KEPT ? i : 0][e + 1] += more[1];
+            } else {
+              last_totals[e / 2 * NT] += more;
+            }
+          }
         }
       }
     const auto penalised = [&](float f, float sign, unsigned col) {
@@ -219,7 +239,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
       return f;
     };
     constexpr bool OVER = B == 2;                              // (two-byte values with a bias: the sum is rounded, not the penalised value)
-    unsigned c[NCH], left = 0u;
+    unsigned c[NCH], left = 0u, positive = 0u;                 // (bits of the text's elements; SIGNS: of these the ones with a logit above 0)
     if (length > 0 && (!SUMS || p.out)) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
@@ -231,8 +251,17 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
 #pragma unroll
         for (int i = 0; i < NCH; ++i) xs[i] = load16_unaligned(x + (c[i] ? mine + i * WAVE : 0u) * 16u);
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (c[i]) *reinterpret_cast<u32x4*>(beside + (mine + i * WAVE) * 16u) = xs[i];
+        for (int i = 0; i < NCH; ++i) {
+          if (!c[i]) continue;
+          if (!SIGNS) {
+            *reinterpret_cast<u32x4*>(beside + (mine + i * WAVE) * 16u) = xs[i];
+            continue;
+          }
+          float f[N];
+          Chunk<Tag>::unpack(xs[i], f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) positive |= (f[e] > 0.f ? 1u : 0u) << (i * N + e);
+        }
       }
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
@@ -241,7 +270,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
       for (; left; left &= left - 1u) {
         const unsigned e = (unsigned)__builtin_ctz(left), col = (mine + e / N * WAVE) * N + e % N;
         const float f = load_as_float(values, Tag::id, col);
-        float y = penalised(f, GRAD ? load_as_float(beside, Tag::id, col) : f, col);
+        float y = penalised(f, SIGNS ? (float)(positive >> e & 1u) : GRAD ? load_as_float(beside, Tag::id, col) : f, col);
         if (!GRAD && OVER && bias) y += load_as_float(bias, p.bias_dtype, col);
         store_from_float(values, Tag::id, col, y);
       }
@@ -307,12 +336,12 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
     if (SUMS && length > 0) __syncthreads();                   // the bits are the next row's
   }
   if (SUMS) {
-    double* at = sums + (first / p.run) * p.V + c0;
+    double* at = sums + (p.first_run + k) * p.V + c0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (mine + i * WAVE < pieces) at[(mine + i * WAVE) * N + e] = total[i][e];
+        if (place + i * WAVE < pieces) at[(place + i * WAVE) * N + e] = i < KEPT ? total[i < KEPT ? i : 0][e] : last_totals[e / 2 * NT][e % 2];
     if (tid < tail) at[pieces * N + tid] = total_tail;
   }
 }
@@ -339,51 +368,44 @@ static int adjust_status() { return hipGetLastError() == hipSuccess ? DL_OK : DL
 constexpr int ADJUST_NT = 256, ADJUST_NCH = 4;
 constexpr int SUMS_NT = 1024;
 
-// What a call that adds up rows is cut into: the threads of a workgroup and their pieces, and the rows whose sums go to the workspace together.
-//
-// Totals in fp64 take two registers a column: two-byte rows have three pieces a thread (four spill: 8192 x 128256 bf16 1040 us, so 975).  Four-byte rows whose columns
-// fill the parts of 1024 threads take these (4096 x 128256 fp32 825 us, with 256 threads 850), not few rows or parts three quarters full.
-// Runs are as long as leaves every CU its workgroups -- one round of these, or up to four while a run is longer than SUMS_ROWS rows, whose texts differ
-// in length: 512 x 128256 bf16 in one round 83 us, in two 96, in four 107, of its bytes more and more sums; 8192 x 128256 1000, 972, 989.
+// What a call that adds up rows is cut into: whether its workgroups are the large ones, and the rows whose sum goes to the workspace in one piece.
+// Rows enough whose columns fill the parts of 1024 threads take these, which go through a text less often (8192 x 128256 bf16, texts of 8192, 1113 us, with
+// 256 threads 1291; 4096 x 128256 fp32 793, 813), not few rows (512 x 128256 bf16 86, 83) or parts three quarters full (8192 x 50257 bf16 542, 479).  Runs are as long as
+// leaves every CU its workgroups, all at once: 8192 x 128256 bf16 943 us, in two rounds of workgroups 965, in four 1025, of their bytes more and more sums.
 struct SumsCut {
   bool wide;
   int64_t run;
   SumsCut(int64_t n_rows, int64_t V, int bytes) {
-    constexpr int64_t WIDE = (int64_t)SUMS_NT * ADJUST_NCH * 4, SUMS_ROWS = 100;
-    wide = bytes == 4 && n_rows >= 2048 && V * 10 >= (V + WIDE - 1) / WIDE * WIDE * 9;
-    const int64_t columns = wide ? WIDE : (int64_t)ADJUST_NT * pieces(bytes) * 16 / bytes, parts = (V + columns - 1) / columns;
-    const int64_t at_once = 32 * (wide ? 1 : 4);               // workgroups of an XCD, which has all parts of a run
-    for (int rounds = 1; rounds <= 4; ++rounds) {
-      const int64_t runs = 8 * std::max<int64_t>(1, at_once * rounds / parts);
-      run = std::max<int64_t>(4, (n_rows + runs - 1) / runs);
-      if (run <= SUMS_ROWS) break;
-    }
+    const int64_t most = (int64_t)SUMS_NT * ADJUST_NCH * 16 / bytes;
+    wide = n_rows >= 2048 && V * 10 >= (V + most - 1) / most * most * 9;
+    const int64_t columns = wide ? most : most / SUMS_NT * ADJUST_NT, parts = (V + columns - 1) / columns;
+    const int64_t runs = 8 * std::max<int64_t>(1, 32 * (wide ? 1 : 4) / parts);      // (an XCD has all parts of a run, and 32 CUs)
+    run = std::max<int64_t>(4, (n_rows + 2 * runs - 1) / (2 * runs) * 2);
   }
-  static constexpr int pieces(int bytes) { return bytes == 2 ? 3 : ADJUST_NCH; }
   int64_t runs(int64_t n_rows) const { return (n_rows + run - 1) / run; }
 };
 
 template <class Tag, class Index, int NT, class Count, bool GRAD, bool SUMS>
 static void launch_adjust(AdjustParams p, double* sums, hipStream_t st) {
-  constexpr int NCH = SUMS ? SumsCut::pieces(Tag::bytes) : ADJUST_NCH;
-  constexpr int64_t most = (int64_t)NT * NCH * Chunk<Tag>::N;
+  constexpr int64_t most = (int64_t)NT * ADJUST_NCH * Chunk<Tag>::N;
   p.parts = (unsigned)((p.V + most - 1) / most);
   p.part_columns = (unsigned)std::min<int64_t>(most, ((p.V + p.parts - 1) / p.parts + 127) / 128 * 128);      // (whole words of the masks, whole pieces of the bits)
-  p.run = SUMS ? SumsCut(p.n_rows, p.V, Tag::bytes).run : 1;
-  const size_t lds = p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (GRAD ? Tag::bytes : sizeof(Count))) : 0;
-  if (NT * NCH * 16 > 32768 && lds > 65536 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+  const int64_t run = SUMS ? SumsCut(p.n_rows, p.V, Tag::bytes).run : 1;
+  const size_t lds = (SUMS && Tag::bytes == 2 ? NT * 64 : 0) + (p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (SUMS && Tag::bytes == 2 ? 0 : GRAD ? Tag::bytes : sizeof(Count))) : 0);
+  if (NT * ADJUST_NCH * 16 > 32768 && lds > 65536 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return;                                                    // (the error is the launch's)
-  const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8 * p.run, all = p.n_rows;      // rows of a launch
+  const int64_t slice = LAUNCH_THREADS / NT / p.parts / 8 * 8 * run, all = p.n_rows;      // rows of a launch
   for (p.first_row = 0; p.first_row < all; p.first_row += slice) {
     p.n_rows = std::min(all, p.first_row + slice);
-    const int64_t runs = (p.n_rows - p.first_row + p.run - 1) / p.run;
-    hipLaunchKernelGGL((adjust_kernel<Tag, Index, NT, NCH, Count, GRAD, SUMS>), dim3((unsigned)((runs + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, p, sums);
+    p.first_run = p.first_row / run;
+    p.runs = (p.n_rows - p.first_row + run - 1) / run;
+    hipLaunchKernelGGL((adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), dim3((unsigned)((p.runs + 7) / 8 * 8) * p.parts), dim3(NT), lds, st, p, sums);
   }
 }
 template <class Tag, class Index, bool GRAD, bool SUMS>
 static void adjust_texts(const AdjustParams& p, double* sums, hipStream_t st) {
-  if constexpr (SUMS && Tag::bytes == 4)
+  if constexpr (SUMS)
     if (SumsCut(p.n_rows, p.V, Tag::bytes).wide) return launch_adjust<Tag, Index, SUMS_NT, unsigned short, GRAD, SUMS>(p, sums, st);
   if constexpr (!GRAD)
     if (p.length > 65535) return launch_adjust<Tag, Index, ADJUST_NT, unsigned, GRAD, SUMS>(p, sums, st);
@@ -431,7 +453,7 @@ extern "C" int dl_adjust_rows(const void* logits, int dtype, int64_t row_stride,
                  reinterpret_cast<const char*>(tokens), itype, token_stride, n_texts, n_texts ? length : 0, token_rows, lengths, prompt, (int)std::max<int64_t>(0, std::min<int64_t>(prompt_all, 0x7fffffff)),
                  repetition, frequency, presence, repetition_all, frequency_all, presence_all,
                  reinterpret_cast<const char*>(bias), bias_dtype, bias_stride,
-                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 1};
+                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 0, 0};
   if (const int bad = adjust_check(p, dtype)) return bad;
   if (n_rows == 0 || V == 0) return DL_OK;
   if (!logits || !out) return DL_ERR_NULL;
@@ -459,7 +481,7 @@ extern "C" int dl_adjust_grad(const void* grad, int dtype, int64_t grad_stride, 
   AdjustParams p{reinterpret_cast<const char*>(logits), row_stride, reinterpret_cast<const char*>(grad), grad_stride, reinterpret_cast<char*>(out), out_stride, n_rows, V,
                  reinterpret_cast<const char*>(tokens), itype, token_stride, n_texts, n_texts ? length : 0, token_rows, lengths, nullptr, 0,
                  repetition, nullptr, nullptr, repetition_all, 0.f, 0.f, nullptr, F32, 0,
-                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 1};
+                 reinterpret_cast<const unsigned*>(allowed), allowed_stride, n_masks, allowed_rows, 0, 0, 0, 0, 0};
   if (grad_stride < V) return DL_ERR_SHAPE;
   if (const int bad = adjust_check(p, dtype)) return bad;
   if (V == 0 || (n_rows == 0 && !bias_grad)) return DL_OK;
