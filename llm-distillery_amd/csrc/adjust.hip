@@ -124,7 +124,7 @@ typedef const char __attribute__((address_space(1))) * global_bytes;      // (sa
 // texts of 2048, 400 us, so 429); a pair shares the line in which one row ends and the next begins (8192 x 50257 bf16 472 us, single rows 552).
 // Count: what a column's counter is held in, 16 bits where no text has more tokens than these count.
 // 16 KiB of a row a workgroup, four 16-byte pieces a thread; LDS and registers leave room for four such workgroups on a CU (asked for six or eight, values
-// spill).  The totals of two-byte rows, 64 registers, do not fit beside the rest: those of a thread's last piece are in LDS.
+// spill; two-byte logits to be adjusted by 64-bit tokens hold 12 or 16 bytes a thread in scratch as it is).  The totals of two-byte rows, 64 registers, do not fit beside the rest: those of a thread's last piece are in LDS.
 template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
 __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, double* sums) {
   constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = SUMS ? 1 : 2;      // (tokens of a thread at a time: four times NTOK)
