@@ -15,11 +15,11 @@
 //
 // Bound by HBM where there are rows enough: 4096 x 50257 fp32, 512-token texts, a shared bias, 303 us (1.65 GB: 5.4 TB/s); 256 x 128256 bf16, texts of
 // 4096, masks that allow 30 %, 29 us (134 MB: 4.6 TB/s, the first tokens and the last pieces with nothing beside them); 8192 x 128256 bf16 with a bias's
-// gradient 900 us (4.2 GB, 0.2 of logits at the texts' tokens, 0.13 of sums: 5.0 TB/s).  One row of 32000 takes 4.6 us, the depth of its loads.  Tried at the second of these:
-// the penalty computed in all columns and selected 54 us, a list of the text's columns that were claimed, gathered and scattered 70 (texts of
+// gradient 950 us (4.2 GB, 0.2 of logits at the texts' tokens, 0.13 of sums: 4.8 TB/s).  One row of 32000 takes 4.6 us, the depth of its loads.  Tried at
+// the second of these: the penalty computed in all columns and selected 54 us, a list of the text's columns that were claimed, gathered and scattered 70 (texts of
 // 16384: 1036 against 290), new values picked into registers by comparisons 34, 512 or 1024 threads with one or two pieces each level to 35.  Several rows
-// a workgroup for texts that rows share, so that a row adds only its own tokens' bits, is slower (the third 874 to 992 traced, as it is
-// 846): a workgroup that goes on to another row waits for the stores of the row before.
+// a workgroup for texts that rows share, so that a row adds only its own tokens' bits, is slower (the third 874 to 992 traced, without
+// 846, both with totals in 32 bits): a workgroup that goes on to another row waits for the stores of the row before.
 #include "distill_common.hpp"
 #include "distill_hip.h"
 
@@ -124,7 +124,8 @@ typedef const char __attribute__((address_space(1))) * global_bytes;      // (sa
 // texts of 2048, 400 us, so 429); a pair shares the line in which one row ends and the next begins (8192 x 50257 bf16 472 us, single rows 552).
 // Count: what a column's counter is held in, 16 bits where no text has more tokens than these count.
 // 16 KiB of a row a workgroup, four 16-byte pieces a thread; LDS and registers leave room for four such workgroups on a CU (asked for six or eight, values
-// spill; two-byte logits to be adjusted by 64-bit tokens hold 12 or 16 bytes a thread in scratch as it is).  The totals of two-byte rows, 64 registers, do not fit beside the rest: those of a thread's last piece are in LDS.
+// spill; two-byte logits to be adjusted by 64-bit tokens hold 12 or 16 bytes a thread in scratch as it is).  The totals of two-byte rows, 64 registers, do
+// not fit beside the rest: those of a thread's last piece are in LDS.
 template <class Tag, class Index, int NT, int NCH, class Count, bool GRAD, bool SUMS>
 __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, double* sums) {
   constexpr int N = Chunk<Tag>::N, B = Tag::bytes, NTOK = SUMS ? 1 : 2;      // (tokens of a thread at a time: four times NTOK)
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(NT, 4) void adjust_kernel(const AdjustParams p, dou
   const unsigned group = blockIdx.x / (8u * p.parts), in = blockIdx.x % (8u * p.parts);      // the parts of a run on one XCD
   const int64_t k = (int64_t)group * 8 + (in & 7u), first = p.first_row + (SUMS ? 2 * k : k), last = SUMS ? p.n_rows : min(first + 1, p.n_rows);
   const int64_t c0 = (int64_t)(in >> 3) * p.part_columns;
-  if (k >= p.runs || c0 >= p.V) return;                      // (parts are whole blocks of 128 columns: the last may be none)
+  if (k >= p.runs || c0 >= p.V) return;                        // (parts are whole blocks of 128 columns: the last may be none)
   // a wave's pieces are neighbours, NCH KiB of them: all of a thread's lie within the offset of an instruction
   const unsigned tid = threadIdx.x, place = tid / WAVE * (WAVE * NCH) + tid % WAVE;
   const unsigned columns = (unsigned)min((int64_t)p.part_columns, p.V - c0), pieces = columns / N, tail = columns % N;
@@ -391,7 +392,9 @@ static void launch_adjust(AdjustParams p, double* sums, hipStream_t st) {
   p.parts = (unsigned)((p.V + most - 1) / most);
   p.part_columns = (unsigned)std::min<int64_t>(most, ((p.V + p.parts - 1) / p.parts + 127) / 128 * 128);      // (whole words of the masks, whole pieces of the bits)
   const int64_t run = SUMS ? SumsCut(p.n_rows, p.V, Tag::bytes).run : 1;
-  const size_t lds = (SUMS && Tag::bytes == 2 ? NT * 64 : 0) + (p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + (SUMS && Tag::bytes == 2 ? 0 : GRAD ? Tag::bytes : sizeof(Count))) : 0);
+  constexpr bool SIGNS = SUMS && Tag::bytes == 2;
+  constexpr size_t beside = SIGNS ? 0 : GRAD ? (size_t)Tag::bytes : sizeof(Count);
+  const size_t lds = (SIGNS ? NT * 64 : 0) + (p.length > 0 ? p.part_columns / 8 + p.part_columns * (Tag::bytes + beside) : 0);
   if (NT * ADJUST_NCH * 16 > 32768 && lds > 65536 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(&adjust_kernel<Tag, Index, NT, ADJUST_NCH, Count, GRAD, SUMS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return;                                                    // (the error is the launch's)

@@ -7,7 +7,7 @@
 // Squares are added up in fp64 (no sum overflows, none of a billion elements loses anything that fp32 shows) by workgroups that stay and take every
 // so many-th piece, one sum per workgroup goes to the workspace, and these are added up in their order: no atomics, the same bits on every call.
 // The second pass has a workgroup for every piece, the last piece first: what was read last may still be in MALL.
-// Bound by HBM: 1.2 billion bf16 elements (2.4 GB) 1165 us, of it the squares 353 (6.8 TB/s), their sum 5, the product 805 (5.9 TB/s read and written: a
+// Bound by HBM: 1.2 billion bf16 elements (2.4 GB) 1176 us, of it the squares 353 (6.8 TB/s), their sum 5, the product 818 (5.8 TB/s read and written: a
 // copy of the size by the library reaches 4.9); 203 million fp32 elements of odd sizes, only read, 128 us, the squares 119 to 124.  Few small tensors
 // (1 million elements in 11): 5 and 8 us on the card, less than the host needs for two launches.  Tried at the first of these: every workgroup
 // a contiguous share of all 1261 us, long-lived workgroups that take every so many-th piece in the second pass 1245, its stores kept in the caches 1322, half
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(GRAD_NT, 4) void scale_kernel(const GradTable t, co
   if (n_sums && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)all;
   const double by = all > (double)max_norm ? (double)max_norm / all * (double)scale : (double)scale;
   if (!((float)all <= 3.402823466e38f)) return;                // NaN or, as fp32 shows it, infinite: left as they are
-  if (fabs(by - 1.0) <= 0x1p-25) return;                   // less than half a step of any element: they would stay what they are
+  if (fabs(by - 1.0) <= 0x1p-25) return;                       // less than half a step of any element: they would stay what they are
   const unsigned q = t.pieces - 1u - blockIdx.x;
   find_entry(t, q, found);
   const GradPiece p = piece_of(found, q);
